@@ -2,6 +2,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "serve.cuh"
 
 namespace b2k {
 
@@ -249,6 +250,8 @@ int b2k_stream_sync(b2k_ctx *ctx, void *stream) {
   if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "error flag readback");
   if (flag) {
     cudaMemset(ctx->error_flag, 0, sizeof(unsigned int) * 4);
+    if (flag == serve::kErrIndex)
+      return b2k::fail(ctx, B2K_EINDEX, "a kernel met a page, length or row count outside its bounds");
     return b2k::fail(ctx, B2K_ETIMEOUT, "a kernel's bounded wait expired (code 0x%x)", flag);
   }
   return B2K_OK;

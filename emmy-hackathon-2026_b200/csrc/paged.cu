@@ -1,0 +1,431 @@
+// Attention over a paged key / value cache: the plan of a call (which kernel
+// takes the shared prefix and which the sequences' own keys, and how the keys
+// are split), the FP32 kernel, and the merge of the parts (paged.cuh has the
+// mathematics).
+//
+// paged_rows_kernel: FP32 arithmetic on the plain cores, for f32 operands and
+// for any layout that the tensor-core kernels do not read (element strides
+// and bases off 16 bytes, head dims off 8).  A block of four warps holds R = 4
+// RW rows (query heads of one cache head, tokens side by side) and streams 32
+// keys at a time through shared memory as FP32.  Scores: lane = key, each
+// warp its own RW rows, so a key is read once for RW rows and the softmax of a
+// tile is one butterfly.  P V: lane = four dims, the probabilities shuffled
+// from their lanes; a probability of exactly zero skips its key, so what a
+// masked place of the cache holds (infinities and NaN too) has no effect.
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace {
+
+using paged::Args;
+
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTile = 32;  // keys
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// DV: float4s of a head that a lane holds (head dim up to 128 DV).
+// V: elements of one access to the cache (16 bytes, or 1).
+template <typename T, int RW, int DV, int V>
+__global__ void __launch_bounds__(kThreads) paged_rows_kernel(const __grid_constant__ Args a, bool prefix, int row_blocks) {
+  constexpr int R = RW * kWarps;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ int64_t k_at[kTile], v_at[kTile];
+  const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4;
+  float *qs = smem, *ks = qs + R * dp, *vs = ks + kTile * ldk;
+  grid_dependency_wait();
+  grid_dependents_launch();
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.y, head = blockIdx.x / row_blocks, block = blockIdx.x % row_blocks, b = blockIdx.z;
+  const int q_heads = a.kv_heads * a.group;
+  paged::Sequence s = {0, 0, 0};
+  if (prefix) s.n = paged::used_tokens(a);
+  else s = paged::sequence(a, b);
+  const int rows = s.n * a.group, row0 = block * R;
+  if (row0 >= rows) return;
+  const int last_token = (min(row0 + R, rows) - 1) / a.group;
+  const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
+  const int key0 = split * chunk;
+  const int key_end = min(prefix ? a.prefix_len : paged::own_limit(a, s, last_token), key0 + chunk);
+  const bool direct = a.own_splits + a.prefix_splits == 1;
+  if (key0 >= key_end && !(direct && key0 == 0)) return;
+
+  // this block's queries, FP32, times log2(e) / scale
+  for (int i = threadIdx.x; i < R * dp; i += kThreads) {
+    const int r = i / dp, c = i % dp, row = row0 + r;
+    float x = 0.0f;
+    if (row < rows && c < a.d)
+      x = serve::to_f32(static_cast<const T *>(a.q)[(int64_t)(s.first + row / a.group) * a.q_token +
+                                                     (head * a.group + row % a.group) * a.q_head + c]);
+    qs[i] = x * a.scale_log2;
+  }
+  int limit[RW];
+  float m[RW], l[RW];
+  float4 o[RW][DV];
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int row = row0 + warp * RW + i;
+    limit[i] = row >= rows ? 0 : prefix ? a.prefix_len : paged::own_limit(a, s, row / a.group);
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DV; ++c) o[i][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+
+  for (int key = key0; key < key_end; key += kTile) {
+    __syncthreads();  // the last tile's readers are done (and qs is written)
+    if (threadIdx.x < kTile) {
+      const int at = key + threadIdx.x;
+      int64_t ko = -1, vo = -1;
+      if (at < key_end) {
+        int r;
+        const int64_t page = paged::key_page(a, prefix, b, at, r);
+        if (page >= 0) {
+          ko = page * a.k_page + r * a.k_row + head * a.k_head;
+          vo = page * a.v_page + r * a.v_row + head * a.v_head;
+        }
+      }
+      k_at[threadIdx.x] = ko;
+      v_at[threadIdx.x] = vo;
+    }
+    __syncthreads();
+    const int per_row = dp / V;
+    for (int i = threadIdx.x; i < kTile * per_row; i += kThreads) {
+      const int r = i / per_row, c = (i % per_row) * V;
+      serve::Pack<T, V> kx = {}, vx = {};
+      if (k_at[r] >= 0 && c < a.d) {
+        kx = *reinterpret_cast<const serve::Pack<T, V> *>(static_cast<const T *>(a.k) + k_at[r] + c);
+        vx = *reinterpret_cast<const serve::Pack<T, V> *>(static_cast<const T *>(a.v) + v_at[r] + c);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        ks[r * ldk + c + e] = serve::to_f32(kx.v[e]);
+        vs[r * dp + c + e] = serve::to_f32(vx.v[e]);
+      }
+    }
+    __syncthreads();
+
+    float p[RW];
+    {
+      float acc[RW];
+#pragma unroll
+      for (int i = 0; i < RW; ++i) acc[i] = 0.0f;
+      for (int c = 0; c < dp; c += 4) {
+        const float4 kv = *reinterpret_cast<const float4 *>(ks + lane * ldk + c);
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+          const float4 qv = *reinterpret_cast<const float4 *>(qs + (warp * RW + i) * dp + c);
+          acc[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, acc[i]))));
+        }
+      }
+      const bool there = k_at[lane] >= 0;
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const float sc = there && key + lane < limit[i] ? acc[i] : -INFINITY;
+        const float mx = fmaxf(m[i], warp_max(sc));
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        const float alpha = exp2_fast(m[i] - base);
+        p[i] = exp2_fast(sc - base);
+        l[i] = l[i] * alpha + p[i];  // this lane's keys; the lanes are added at the end
+        m[i] = mx;
+#pragma unroll
+        for (int c = 0; c < DV; ++c) {
+          o[i][c].x *= alpha;
+          o[i][c].y *= alpha;
+          o[i][c].z *= alpha;
+          o[i][c].w *= alpha;
+        }
+      }
+    }
+    const int keys = min(kTile, key_end - key);
+    for (int t = 0; t < keys; ++t) {
+      float4 vv[DV];
+#pragma unroll
+      for (int c = 0; c < DV; ++c) {
+        const int at = 4 * lane + 128 * c;
+        vv[c] = at < dp ? *reinterpret_cast<const float4 *>(vs + t * dp + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const float pt = __shfl_sync(0xffffffffu, p[i], t);
+        if (pt != 0.0f) {
+#pragma unroll
+          for (int c = 0; c < DV; ++c) {
+            o[i][c].x = fmaf(pt, vv[c].x, o[i][c].x);
+            o[i][c].y = fmaf(pt, vv[c].y, o[i][c].y);
+            o[i][c].z = fmaf(pt, vv[c].z, o[i][c].z);
+            o[i][c].w = fmaf(pt, vv[c].w, o[i][c].w);
+          }
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int row = row0 + warp * RW + i;
+    const float total = warp_sum(l[i]);
+    if (row >= rows) continue;
+    const int64_t token = s.first + row / a.group;
+    const int qh = head * a.group + row % a.group;
+    if (direct) {
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      T *out = static_cast<T *>(a.o) + token * a.o_token + qh * a.o_head;
+#pragma unroll
+      for (int c = 0; c < DV; ++c) {
+        const float x[4] = {o[i][c].x, o[i][c].y, o[i][c].z, o[i][c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * lane + 128 * c + e < a.d) out[4 * lane + 128 * c + e] = serve::from_f32<T>(x[e] * inv);
+      }
+    } else {
+      const int64_t at = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
+      if (lane == 0) a.part_ml[at] = make_float2(m[i], total);
+#pragma unroll
+      for (int c = 0; c < DV; ++c) {
+        const float x[4] = {o[i][c].x, o[i][c].y, o[i][c].z, o[i][c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * lane + 128 * c + e < a.d) a.part_o[at * a.d + 4 * lane + 128 * c + e] = x[e];
+      }
+    }
+  }
+}
+
+// Joins a row's parts: one warp a row (token, query head), lanes over the dims,
+// parts in order, so the result does not depend on which part ended first.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_constant__ Args a) {
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int lane = threadIdx.x & 31;
+  const int q_heads = a.kv_heads * a.group;
+  const paged::Sequence s = paged::sequence(a, blockIdx.x);
+  const int64_t stride = a.tokens * q_heads;
+  for (int64_t row = (int64_t)blockIdx.y * kWarps + (threadIdx.x >> 5); row < (int64_t)s.n * q_heads;
+       row += (int64_t)gridDim.y * kWarps) {
+    const int j = (int)(row / q_heads), qh = (int)(row % q_heads);
+    const int64_t at = (int64_t)(s.first + j) * q_heads + qh;
+    const int own = (paged::own_limit(a, s, j) + a.own_chunk - 1) / a.own_chunk;
+    const int parts = own + a.prefix_splits;
+    auto slot = [&](int i) { return (int64_t)(i < own ? i : a.own_splits + i - own) * stride + at; };
+    float mx = -INFINITY;
+    for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, a.part_ml[slot(i)].x);
+    mx = warp_max(mx);
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    float total = 0.0f;
+    for (int i = lane; i < parts; i += 32) {
+      const float2 ml = a.part_ml[slot(i)];
+      total += ml.y * exp2_fast(ml.x - base);
+    }
+    total = warp_sum(total);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    T *out = static_cast<T *>(a.o) + (int64_t)(s.first + j) * a.o_token + qh * a.o_head;
+    for (int c = lane; c < a.d; c += 32) {
+      float x = 0.0f;
+      for (int i = 0; i < parts; ++i) {
+        const int64_t p = slot(i);
+        x = fmaf(a.part_o[p * a.d + c], exp2_fast(a.part_ml[p].x - base), x);
+      }
+      out[c] = serve::from_f32<T>(x * inv);
+    }
+  }
+}
+
+// What a call launches, from its host values alone.
+struct Plan {
+  int own_splits, own_chunk, prefix_splits, prefix_chunk, joined;
+  int own_rw, prefix_rw;  // rows a warp of paged_rows_kernel
+  size_t bytes;           // workspace
+};
+
+// Bytes of the parts' (m, l), which the sums follow on a 16-byte boundary.
+size_t ml_bytes(size_t slots, int64_t tokens, int q_heads) {
+  return (slots * (size_t)tokens * q_heads * sizeof(float2) + 15) / 16 * 16;
+}
+
+int rows_per_warp(int64_t rows) { return rows <= 4 ? 1 : rows <= 8 ? 2 : 8; }
+
+// Splits of `keys` keys so that `units` independent blocks become about two
+// waves of the GPU's resident blocks, at least `least` keys each.
+void split_keys(int64_t keys, int64_t units, int sms, int least, int &splits, int &chunk) {
+  const int64_t want = std::max<int64_t>(1, (int64_t)sms * 6 / std::max<int64_t>(1, units));
+  int64_t c = std::max<int64_t>(least, (keys + want - 1) / want);
+  c = (c + kTile - 1) / kTile * kTile;
+  splits = (int)std::max<int64_t>(1, (keys + c - 1) / c);
+  chunk = (int)c;
+}
+
+Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, int sms) {
+  Plan p = {};
+  const int64_t group = q_heads / c.heads;
+  const int64_t own_rows = b.max_new * group, prefix_rows = b.tokens * group;
+  p.own_rw = rows_per_warp(own_rows);
+  p.prefix_rw = rows_per_warp(prefix_rows);
+  // Sequences whose own rows fill a block read the prefix with their own keys:
+  // stacking the rows of several sequences would save no reads of it.
+  p.joined = b.prefix_len > 0 && own_rows >= 128;
+  const int64_t own_blocks = (own_rows + 4 * p.own_rw - 1) / (4 * p.own_rw);
+  split_keys((int64_t)b.max_len + (p.joined ? b.prefix_len : 0), own_blocks * c.heads * b.sequences, sms, 128, p.own_splits,
+             p.own_chunk);
+  if (b.prefix_len > 0 && !p.joined)
+    split_keys(b.prefix_len, (prefix_rows + 4 * p.prefix_rw - 1) / (4 * p.prefix_rw) * c.heads, sms, 128,
+               p.prefix_splits, p.prefix_chunk);
+  const size_t slots = (size_t)p.own_splits + p.prefix_splits;
+  if (slots > 1) p.bytes = ml_bytes(slots, b.tokens, q_heads) + slots * (size_t)b.tokens * q_heads * c.d * sizeof(float);
+  return p;
+}
+
+template <typename T, int RW, int DV>
+cudaError_t launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, dim3 grid, int row_blocks, cudaStream_t s) {
+  const int dp = (a.d + 3) / 4 * 4;
+  const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + kTile * (dp + 4) + kTile * dp);
+  constexpr int kFull = 16 / sizeof(T);
+  auto kernel = vec ? paged_rows_kernel<T, RW, DV, kFull> : paged_rows_kernel<T, RW, DV, 1>;
+  constexpr int most = sizeof(float) * (RW * kWarps * 128 * DV + kTile * (128 * DV + 4) + kTile * 128 * DV);
+  cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
+  if (err != cudaSuccess) return err;
+  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), smem, s, a, prefix, row_blocks);
+}
+
+template <typename T>
+cudaError_t rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int rw, cudaStream_t s) {
+  const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
+  const int row_blocks = (int)((rows + 4 * rw - 1) / (4 * rw));
+  const dim3 grid((unsigned)(row_blocks * a.kv_heads), prefix ? a.prefix_splits : a.own_splits, prefix ? 1 : a.sequences);
+  const size_t size = sizeof(T);
+  const bool vec = a.d % (16 / (int)size) == 0 && serve::vec_ok(a.k, a.k_page, a.k_row, a.k_head, size, 16) &&
+                   serve::vec_ok(a.v, a.v_page, a.v_row, a.v_head, size, 16);
+  if (a.d <= 128) {
+    if (rw == 1) return launch_rows<T, 1, 1>(ctx, a, prefix, vec, grid, row_blocks, s);
+    if (rw == 2) return launch_rows<T, 2, 1>(ctx, a, prefix, vec, grid, row_blocks, s);
+    return launch_rows<T, 8, 1>(ctx, a, prefix, vec, grid, row_blocks, s);
+  }
+  if (rw == 1) return launch_rows<T, 1, 2>(ctx, a, prefix, vec, grid, row_blocks, s);
+  if (rw == 2) return launch_rows<T, 2, 2>(ctx, a, prefix, vec, grid, row_blocks, s);
+  return launch_rows<T, 8, 2>(ctx, a, prefix, vec, grid, row_blocks, s);
+}
+
+template <typename T>
+int run(b2k_ctx *ctx, const Args &a, const Plan &p, cudaStream_t s) {
+  int launches = 1;
+  cudaError_t err = cudaSuccess;
+  if (a.prefix_splits > 0) {
+    err = rows_part<T>(ctx, a, true, p.prefix_rw, s);
+    ++launches;
+  }
+  if (err == cudaSuccess) err = rows_part<T>(ctx, a, false, p.own_rw, s);
+  if (err == cudaSuccess && a.own_splits + a.prefix_splits > 1) {
+    const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
+    const dim3 grid(a.sequences, (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, 65535));
+    err = b2k::launch_kernel(b2k::pdl_enabled(), paged_merge_kernel<T>, grid, dim3(kThreads), 0, s, a);
+    ++launches;
+  }
+  if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "paged_attention launch");
+  return b2k::check_launch(ctx, "paged_attention launch", launches);
+}
+
+int check_call(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch, int32_t q_heads) {
+  int status = serve::check_cache(ctx, "paged_attention", cache);
+  if (status == B2K_OK) status = serve::check_batch(ctx, "paged_attention", cache, batch);
+  if (status != B2K_OK) return status;
+  if (q_heads < 1 || q_heads > 65535 || q_heads % cache->heads)
+    return b2k::fail(ctx, B2K_EINVAL, "paged_attention: %d query heads for %d cache heads", q_heads, cache->heads);
+  // the limits of a launch's grid, and of a row's 32-bit number
+  if (batch->sequences > 65535 || batch->tokens * q_heads > INT32_MAX || (int64_t)batch->max_new * q_heads > INT32_MAX ||
+      (int64_t)batch->max_len + batch->prefix_len > INT32_MAX - 65536)
+    return b2k::fail(ctx, B2K_EUNSUPPORTED, "paged_attention: a batch of %d sequences, %lld rows is too large",
+                     batch->sequences, (long long)(batch->tokens * q_heads));
+  return B2K_OK;
+}
+
+}  // namespace
+
+extern "C" int b2k_paged_attention_workspace(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
+                                             int32_t q_heads, size_t *bytes) {
+  if (!ctx) return B2K_EINVAL;
+  if (!bytes) return b2k::fail(ctx, B2K_EINVAL, "paged_attention_workspace: null result");
+  int status = check_call(ctx, cache, batch, q_heads);
+  if (status != B2K_OK) return status;
+  *bytes = make_plan(*cache, *batch, q_heads, ctx->sm_count).bytes;
+  return B2K_OK;
+}
+
+extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
+                                   const b2k_heads *q, const b2k_heads *o, float scale_div, void *workspace,
+                                   size_t workspace_bytes, void *stream) {
+  B2K_CHECK_CTX(ctx);
+  const char *what = "paged_attention";
+  if (!q) return b2k::fail(ctx, B2K_EINVAL, "%s: no q", what);
+  int status = check_call(ctx, cache, batch, q->heads);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "o", o, batch->tokens, cache->d);
+  if (status != B2K_OK) return status;
+  if (q->heads != o->heads) return b2k::fail(ctx, B2K_EINVAL, "%s: %d heads in, %d out", what, q->heads, o->heads);
+  if (q->data == o->data && batch->tokens > 0) return b2k::fail(ctx, B2K_EINVAL, "%s: o is q", what);
+  if (!(scale_div > 0.0f) || !isfinite(scale_div)) return b2k::fail(ctx, B2K_EINVAL, "%s: scale %g", what, scale_div);
+  if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
+  const Plan p = make_plan(*cache, *batch, q->heads, ctx->sm_count);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+    return b2k::fail(ctx, B2K_EINVAL, "%s: a workspace of %zu bytes where %zu are needed", what,
+                     workspace ? workspace_bytes : (size_t)0, p.bytes);
+  if (p.bytes > 0 && !b2k::aligned16(workspace))
+    return b2k::fail(ctx, B2K_EINVAL, "%s: the workspace is not 16-byte aligned", what);
+  Args a = {};
+  a.q = q->data;
+  a.o = o->data;
+  a.q_token = q->stride_token;
+  a.q_head = q->stride_head;
+  a.o_token = o->stride_token;
+  a.o_head = o->stride_head;
+  a.k = cache->k;
+  a.v = cache->v;
+  a.k_page = cache->k_page;
+  a.k_row = cache->k_row;
+  a.k_head = cache->k_head;
+  a.v_page = cache->v_page;
+  a.v_row = cache->v_row;
+  a.v_head = cache->v_head;
+  a.pages = cache->pages;
+  a.page_size = cache->page_size;
+  a.kv_heads = cache->heads;
+  a.group = q->heads / cache->heads;
+  a.d = cache->d;
+  a.sequences = batch->sequences;
+  a.tokens = batch->tokens;
+  a.first = batch->first;
+  a.lengths = batch->lengths;
+  a.table = batch->table;
+  a.prefix_table = batch->prefix_table;
+  a.table_stride = batch->table_stride;
+  a.table_width = batch->table_width;
+  a.prefix_len = batch->prefix_len;
+  a.max_new = batch->max_new;
+  a.max_len = batch->max_len;
+  a.scale_log2 = (float)(1.4426950408889634074 / scale_div);
+  a.err = ctx->error_flag;
+  a.own_splits = p.own_splits;
+  a.own_chunk = p.own_chunk;
+  a.prefix_splits = p.prefix_splits;
+  a.prefix_chunk = p.prefix_chunk;
+  a.joined = p.joined;
+  if (p.bytes > 0) {
+    const size_t slots = (size_t)(p.own_splits + p.prefix_splits);
+    a.part_ml = static_cast<float2 *>(workspace);
+    a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + ml_bytes(slots, batch->tokens, q->heads));
+  }
+  cudaStream_t s = (cudaStream_t)stream;
+  b2k::PhaseTimer timer(ctx, B2K_PHASE_PAGED, s);
+  if (cache->dtype == B2K_F32) return run<float>(ctx, a, p, s);
+  if (cache->dtype == B2K_F16) return run<__half>(ctx, a, p, s);
+  return run<__nv_bfloat16>(ctx, a, p, s);
+}

@@ -1,0 +1,89 @@
+// Shared by the kernels of attention over a paged cache: what a launch of one
+// part of the keys gets, and the partial sums that parts leave for the merge.
+//
+// Mathematics.  A row's softmax over a set of keys is (m, l, o): the largest
+// score, the sum of exp(s - m) and the sum of exp(s - m) v.  Two disjoint sets
+// join exactly: m = max(m1, m2), l and o each the sum of both sides' times
+// exp(m_i - m).  So the keys are cut into parts -- the shared prefix, once for
+// all sequences, and every sequence's own keys, each again into splits where
+// the rows alone would not fill the GPU -- and a last kernel joins a row's
+// parts.  Scores are kept times log2(e) / scale, exponentials are base 2.
+#pragma once
+
+#include "serve.cuh"
+
+namespace paged {
+
+struct Args {
+  const void *q;
+  void *o;
+  int64_t q_token, q_head, o_token, o_head;  // strides, elements
+  const void *k, *v;
+  int64_t k_page, k_row, k_head, v_page, v_row, v_head;
+  int64_t pages;
+  int page_size, kv_heads, group, d;  // group: query heads of a cache head
+  int sequences;
+  int64_t tokens;
+  const int32_t *first, *lengths, *table, *prefix_table;
+  int64_t table_stride;
+  int table_width, prefix_len, max_new, max_len;
+  float scale_log2;  // log2(e) / scale
+  unsigned *err;
+  // the parts: own keys in `own_splits` splits of `own_chunk`, the prefix in
+  // prefix_splits of prefix_chunk behind them (0: there is none, or own parts
+  // begin with it: `joined`)
+  int own_splits, own_chunk, prefix_splits, prefix_chunk;
+  int joined;
+  float *part_o;   // [own_splits + prefix_splits][tokens * q heads][d]
+  float2 *part_ml; // [own_splits + prefix_splits][tokens * q heads]: m, l
+};
+
+// A sequence's rows as its device-side numbers give them; n = 0 (and the error
+// word set) where they leave the bounds the launch was sized by.
+struct Sequence {
+  int first, n, own0;  // own0: own position of its first new token
+};
+__device__ __forceinline__ Sequence sequence(const Args &a, int b) {
+  Sequence s;
+  s.first = a.first[b];
+  s.n = a.first[b + 1] - s.first;
+  const int len = a.lengths[b];
+  s.own0 = len - s.n;
+  if (s.first < 0 || s.n < 0 || (int64_t)s.first + s.n > a.tokens || s.n > a.max_new || len > a.max_len || len < 0) {
+    atomicOr(a.err, serve::kErrIndex);
+    s.n = 0;
+  }
+  return s;
+}
+// Packed rows in use.
+__device__ __forceinline__ int used_tokens(const Args &a) {
+  const int n = a.first[a.sequences];
+  return (int)min((int64_t)max(n, 0), a.tokens);
+}
+
+// Keys of an own part that new token j may see: its prefix (joined) and own
+// positions up to its own.
+__device__ __forceinline__ int own_limit(const Args &a, const Sequence &s, int j) {
+  return max(0, s.own0 + j + 1) + (a.joined ? a.prefix_len : 0);
+}
+
+// Offsets (elements) of a key's rows in the cache, for cache head 0; -1 for a page
+// outside the cache.  `at` counts from the start of the part: the prefix's
+// keys, or the own keys behind the prefix's where the part is joined.
+__device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, int at, int &row) {
+  const int32_t *table = a.prefix_table;
+  if (!prefix) {
+    if (!a.joined || at >= a.prefix_len) {
+      table = a.table + (int64_t)b * a.table_stride;
+      at -= a.joined ? a.prefix_len : 0;
+    }
+  }
+  const int i = (int)((unsigned)at / (unsigned)a.page_size);
+  row = at - i * a.page_size;
+  const int64_t page = table[i];
+  if (page >= 0 && page < a.pages) return page;
+  atomicOr(a.err, serve::kErrIndex);
+  return -1;
+}
+
+}  // namespace paged

@@ -1,0 +1,435 @@
+// Rotary positions, and the append of rotated keys (and values) to a paged
+// cache: one kernel, since both move each element once and differ in where
+// the result goes.
+//
+// Mathematics.  A pair (a, b) of a head turns by position * f_i.  The plan
+// holds f_i / 2 pi as a 64-bit fraction of a turn, so position * turn_i in
+// wrapping 64-bit integer arithmetic IS the angle modulo one turn; its top 32
+// bits, as a signed number, give the angle in half turns for sincospif.  The
+// angle's error is 2^-33 turns plus the rounding of that number to FP32 (at
+// most 2^-25 half turns), at any position: no table of cosines is read, kept
+// or outgrown, and no FP32 product position * f loses the far positions.
+//
+// Bound: HBM (each element read and written once).  A block takes 1 or 4
+// tokens; its cosines and sines are computed once into shared memory while
+// the first heads' loads are in flight, then every thread keeps one place of
+// the head (16 bytes of each half of its pairs) and walks the heads, four
+// loads of two vectors ahead.
+#include <math.h>
+
+#include <algorithm>
+
+#include "serve.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kAhead = 4;       // heads a thread has in flight
+constexpr int kMaxTokens = 4;   // tokens of a block
+constexpr int kMaxPairs = B2K_ROPE_MAX_PAIRS;
+
+enum Target : int { kLinear = 0, kKeys = 1, kValues = 2 };
+
+// One tensor of the call: source, destination, and whether it is rotated.
+struct Segment {
+  const char *x;
+  char *y;
+  int64_t xt, xh;      // source strides in bytes: token, head
+  int64_t yp, yt, yh;  // destination strides in bytes: page, token or row, head
+  int head0;           // first of its heads among the call's
+  int target, rotate;
+};
+
+struct RotaryArgs {
+  Segment seg[3];
+  int heads, d, rot, interleaved;
+  float magnitude, sine;  // sine: +magnitude, or -magnitude for the transpose
+  int items;              // places of a head: a thread keeps one
+  int tokens_per_block;
+  int64_t tokens;
+  const int64_t *positions;  // unpaged
+  // paged
+  const int32_t *first, *lengths, *table;
+  int64_t table_stride, pages;
+  int table_width, page_size, prefix_len, max_new;
+  unsigned *err;
+  uint64_t turn[kMaxPairs];
+};
+
+template <typename T, int V, bool PAGED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  using P = serve::Pack<T, V>;
+  __shared__ float cs[kMaxTokens][kMaxPairs], sn[kMaxTokens][kMaxPairs];
+  grid_dependency_wait();
+  grid_dependents_launch();
+
+  const int tpb = a.tokens_per_block;
+  const int slots = kThreads / a.items;  // (token, head) places of the block
+  const int head_step = slots / tpb;
+  const int j = threadIdx.x % a.items, slot = threadIdx.x / a.items;
+  const int t = slot % tpb, h_first = slot / tpb;
+  const bool mine = h_first < head_step;
+  // The two vectors of the head this thread moves: the two halves of V pairs
+  // (half layout, rotated part), or neighbours.
+  int e0, e1;
+  const int half_items = a.interleaved ? 0 : a.rot / 2 / V;
+  if (j < half_items) {
+    e0 = j * V;
+    e1 = e0 + a.rot / 2;
+  } else {
+    e0 = (a.interleaved ? 0 : a.rot) + (j - half_items) * 2 * V;
+    e1 = e0 + V < a.d ? e0 + V : -1;
+  }
+  const int pairs = a.rot / 2;
+
+  // tokens of this block: global rows row0 .. row0 + count - 1
+  int64_t row_begin, row_end, first_row = 0, own0 = 0;
+  if (PAGED) {
+    const int b = blockIdx.x;
+    first_row = a.first[b];
+    const int64_t n = (int64_t)a.first[b + 1] - first_row;
+    own0 = (int64_t)a.lengths[b] - n;
+    if (first_row < 0 || first_row + n > a.tokens || n > a.max_new) {
+      if (threadIdx.x == 0) atomicOr(a.err, serve::kErrIndex);
+      return;
+    }
+    row_begin = first_row;
+    row_end = first_row + n;
+  } else {
+    row_begin = 0;
+    row_end = a.tokens;
+  }
+  const int64_t chunk0 = PAGED ? blockIdx.y : blockIdx.x, chunk_step = PAGED ? gridDim.y : gridDim.x;
+  for (int64_t row0 = row_begin + chunk0 * tpb; row0 < row_end; row0 += chunk_step * tpb) {
+    const int64_t row = row0 + t;
+    const bool on = mine && row < row_end;
+    P va[kAhead], vb[kAhead];
+    auto segment = [&](int h) { return (h >= a.seg[1].head0) + (h >= a.seg[2].head0); };
+    auto load = [&](int hb) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int h = hb + u * head_step;
+        if (!on || h >= a.heads) continue;
+        const Segment &s = a.seg[segment(h)];
+        const T *x = reinterpret_cast<const T *>(s.x + row * s.xt + (h - s.head0) * s.xh);
+        va[u] = *reinterpret_cast<const P *>(x + e0);
+        if (e1 >= 0) vb[u] = *reinterpret_cast<const P *>(x + e1);
+      }
+    };
+    load(h_first);
+    // where this token's keys and values go
+    int64_t page = -1, page_row = 0;
+    if (PAGED && on) {
+      const int64_t own = own0 + (row - first_row);
+      page = serve::page_of(a.table + blockIdx.x * a.table_stride, a.table_width, a.pages, a.page_size, own);
+      page_row = (uint32_t)own % (uint32_t)a.page_size;
+      if (page < 0) atomicOr(a.err, serve::kErrIndex);
+    }
+    for (int i = threadIdx.x; i < tpb * pairs; i += kThreads) {
+      const int ti = i / pairs, p = i % pairs;
+      if (row0 + ti < row_end) {
+        const int64_t pos = PAGED ? a.prefix_len + own0 + (row0 + ti - first_row) : a.positions[row0 + ti];
+        const uint64_t turns = a.turn[p] * (uint64_t)pos;
+        float s, c;
+        sincospif((float)(int32_t)(turns >> 32) * 4.656612873077392578125e-10f, &s, &c);  // 2^-31
+        cs[ti][p] = c * a.magnitude;
+        sn[ti][p] = s * a.sine;
+      }
+    }
+    __syncthreads();
+    if (on) {
+      for (int hb = h_first; hb < a.heads; hb += kAhead * head_step) {
+        if (hb != h_first) load(hb);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int h = hb + u * head_step;
+          if (h >= a.heads) break;
+          const Segment &s = a.seg[segment(h)];
+          T *y;
+          if (PAGED && s.target != kLinear) {
+            if (page < 0) continue;
+            y = reinterpret_cast<T *>(s.y + page * s.yp + page_row * s.yt + (h - s.head0) * s.yh);
+          } else {
+            y = reinterpret_cast<T *>(s.y + row * s.yt + (h - s.head0) * s.yh);
+          }
+          if (s.rotate) {
+            if (a.interleaved) {
+              T r[2 * V];
+#pragma unroll
+              for (int i = 0; i < V; ++i) r[i] = va[u].v[i], r[V + i] = e1 >= 0 ? vb[u].v[i] : va[u].v[i];
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                const int p = j * V + i;
+                if (p < pairs) {
+                  const float c = cs[t][p], sv = sn[t][p];
+                  const float xa = serve::to_f32(r[2 * i]), xb = serve::to_f32(r[2 * i + 1]);
+                  r[2 * i] = serve::from_f32<T>(xa * c - xb * sv);
+                  r[2 * i + 1] = serve::from_f32<T>(xb * c + xa * sv);
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < V; ++i) va[u].v[i] = r[i], vb[u].v[i] = r[V + i];
+            } else if (j < half_items) {
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                const float c = cs[t][j * V + i], sv = sn[t][j * V + i];
+                const float xa = serve::to_f32(va[u].v[i]), xb = serve::to_f32(vb[u].v[i]);
+                va[u].v[i] = serve::from_f32<T>(xa * c - xb * sv);
+                vb[u].v[i] = serve::from_f32<T>(xb * c + xa * sv);
+              }
+            }
+          }
+          *reinterpret_cast<P *>(y + e0) = va[u];
+          if (e1 >= 0) *reinterpret_cast<P *>(y + e1) = vb[u];
+        }
+      }
+    }
+    __syncthreads();  // the next tokens' cosines overwrite these
+  }
+}
+
+// Widest vector (elements) that every tensor of the call and the layout of
+// its heads allow: 16 bytes, 8 bytes or single elements.
+int pick_vector(const RotaryArgs &a, int count, size_t size) {
+  for (int bytes = 16; bytes >= 8; bytes /= 2) {
+    const int v = bytes / (int)size;
+    bool ok = a.d % v == 0 && (a.interleaved || a.rot % (2 * v) == 0);
+    for (int i = 0; ok && i < count; ++i) {
+      const Segment &s = a.seg[i];
+      ok = serve::vec_ok(s.x, s.xt, s.xh, 0, 1, bytes) && serve::vec_ok(s.y, s.yp, s.yt, s.yh, 1, bytes);
+    }
+    if (ok) return v;
+  }
+  return 1;
+}
+
+template <typename T, bool PAGED>
+cudaError_t launch(const RotaryArgs &a, int v, dim3 grid, cudaStream_t s) {
+  constexpr int kFull = 16 / sizeof(T);
+  const bool pdl = b2k::pdl_enabled();
+  if (v == kFull) return b2k::launch_kernel(pdl, rotary_kernel<T, kFull, PAGED>, grid, dim3(kThreads), 0, s, a);
+  if (v == kFull / 2) return b2k::launch_kernel(pdl, rotary_kernel<T, kFull / 2, PAGED>, grid, dim3(kThreads), 0, s, a);
+  return b2k::launch_kernel(pdl, rotary_kernel<T, 1, PAGED>, grid, dim3(kThreads), 0, s, a);
+}
+
+// Fill in the vector width and the block shape, and launch.  `tokens_each`:
+// tokens of one blockIdx.x (paged: of a sequence).
+template <bool PAGED>
+int run(b2k_ctx *ctx, RotaryArgs &a, int count, int32_t dtype, int64_t tokens_each, unsigned sequences, int phase,
+        cudaStream_t s, const char *what) {
+  for (int i = count; i < 3; ++i) a.seg[i].head0 = INT32_MAX;
+  const size_t size = serve::type_size(dtype);
+  const int v = pick_vector(a, count, size);
+  a.items = a.interleaved ? (a.d + 2 * v - 1) / (2 * v) : a.rot / 2 / v + (a.d - a.rot + 2 * v - 1) / (2 * v);
+  // Four tokens share a block's set-up once there are blocks enough for the
+  // GPU without that; fewer tokens spread one to a block.
+  const int64_t all = PAGED ? tokens_each * sequences : tokens_each;
+  a.tokens_per_block = all >= (int64_t)ctx->sm_count * 16 ? std::min(kMaxTokens, kThreads / a.items) : 1;
+  if (PAGED && tokens_each < a.tokens_per_block) a.tokens_per_block = 1;
+  const int64_t chunks = (tokens_each + a.tokens_per_block - 1) / a.tokens_per_block;
+  const dim3 grid = PAGED ? dim3(sequences, (unsigned)std::min<int64_t>(chunks, 65535))
+                          : dim3((unsigned)std::min<int64_t>(chunks, INT32_MAX));
+  b2k::PhaseTimer timer(ctx, phase, s);
+  cudaError_t err = dtype == B2K_F32   ? launch<float, PAGED>(a, v, grid, s)
+                    : dtype == B2K_F16 ? launch<__half, PAGED>(a, v, grid, s)
+                                       : launch<__nv_bfloat16, PAGED>(a, v, grid, s);
+  if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, what);
+  return b2k::check_launch(ctx, what);
+}
+
+int use_rope(b2k_ctx *ctx, const char *what, const b2k_rope *rope, int32_t d, int transpose, RotaryArgs &a) {
+  if (rope->rot < 2 || rope->rot > 2 * kMaxPairs || rope->rot % 2 || rope->rot > d)
+    return b2k::fail(ctx, B2K_EINVAL, "%s: %d rotated elements of a head of %d", what, rope->rot, d);
+  a.rot = rope->rot;
+  a.interleaved = rope->interleaved != 0;
+  a.magnitude = rope->magnitude;
+  a.sine = transpose ? -rope->magnitude : rope->magnitude;
+  for (int i = 0; i < rope->rot / 2; ++i) a.turn[i] = rope->turn[i];
+  return B2K_OK;
+}
+
+}  // namespace
+
+namespace serve {
+
+int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d) {
+  if (!x) return b2k::fail(ctx, B2K_EINVAL, "%s: no %s", what, name);
+  if (x->heads < 1 || x->heads > 65535) return b2k::fail(ctx, B2K_EINVAL, "%s: %s has %d heads", what, name, x->heads);
+  if (tokens > 0 && !x->data) return b2k::fail(ctx, B2K_EINVAL, "%s: null %s", what, name);
+  if (x->stride_token < 0 || x->stride_head < 0 || (x->heads > 1 && x->stride_head < d))
+    return b2k::fail(ctx, B2K_EINVAL, "%s: %s has strides %lld, %lld", what, name, (long long)x->stride_token,
+                     (long long)x->stride_head);
+  return B2K_OK;
+}
+
+int check_cache(b2k_ctx *ctx, const char *what, const b2k_paged_cache *c) {
+  if (!c) return b2k::fail(ctx, B2K_EINVAL, "%s: no cache", what);
+  if (!type_ok(c->dtype)) return b2k::fail(ctx, B2K_EINVAL, "%s: unknown element type %d", what, c->dtype);
+  if (c->page_size < 1 || c->pages < 1 || c->heads < 1 || c->heads > 65535)
+    return b2k::fail(ctx, B2K_EINVAL, "%s: a cache of %lld pages of %d tokens, %d heads", what, (long long)c->pages,
+                     c->page_size, c->heads);
+  if (c->d < 1 || c->d > B2K_MAX_HEAD_DIM) return b2k::fail(ctx, B2K_EINVAL, "%s: head dim %d", what, c->d);
+  if (!c->k || !c->v) return b2k::fail(ctx, B2K_EINVAL, "%s: null cache", what);
+  if (c->k_page < c->d || c->k_row < c->d || c->k_head < c->d || c->v_page < c->d || c->v_row < c->d ||
+      c->v_head < c->d)
+    return b2k::fail(ctx, B2K_EINVAL, "%s: a cache stride is below the head dim", what);
+  return B2K_OK;
+}
+
+int check_batch(b2k_ctx *ctx, const char *what, const b2k_paged_cache *c, const b2k_paged_batch *b) {
+  if (!b) return b2k::fail(ctx, B2K_EINVAL, "%s: no batch", what);
+  if (b->sequences < 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->prefix_len < 0 || b->table_width < 0)
+    return b2k::fail(ctx, B2K_EINVAL, "%s: negative extent", what);
+  if (b->tokens > INT32_MAX) return b2k::fail(ctx, B2K_EINVAL, "%s: too many tokens", what);
+  if (b->sequences == 0) return B2K_OK;
+  if (!b->first || !b->lengths) return b2k::fail(ctx, B2K_EINVAL, "%s: null first or lengths", what);
+  if (b->max_len > 0 && (!b->table || b->table_width < 1)) return b2k::fail(ctx, B2K_EINVAL, "%s: no page table", what);
+  if (b->table_stride < b->table_width) return b2k::fail(ctx, B2K_EINVAL, "%s: table stride below its width", what);
+  if (b->max_len > (int64_t)b->table_width * c->page_size)
+    return b2k::fail(ctx, B2K_EINVAL, "%s: max_len %d is beyond the table's %d pages of %d", what, b->max_len,
+                     b->table_width, c->page_size);
+  if (b->prefix_len > 0 && !b->prefix_table) return b2k::fail(ctx, B2K_EINVAL, "%s: no prefix table", what);
+  return B2K_OK;
+}
+
+}  // namespace serve
+
+extern "C" {
+
+int b2k_rope_plan(const b2k_rope_params *p, b2k_rope *out) {
+  if (!p || !out) return B2K_EINVAL;
+  const int r = p->rot;
+  const bool ramp = p->scaling == B2K_ROPE_RAMP || p->scaling == B2K_ROPE_LOG_RAMP;
+  if (r < 2 || r > 2 * kMaxPairs || r % 2 || p->scaling < B2K_ROPE_NONE || p->scaling > B2K_ROPE_LOG_RAMP)
+    return B2K_EINVAL;
+  if (!(p->theta > 0) || !isfinite(p->theta) || !isfinite(p->magnitude)) return B2K_EINVAL;
+  if (p->scaling != B2K_ROPE_NONE && (!(p->factor > 0) || !isfinite(p->factor))) return B2K_EINVAL;
+  if (p->scaling == B2K_ROPE_BASE && r == 2) return B2K_EINVAL;
+  if (ramp && (!(p->context > 0) || !isfinite(p->context) || !(p->low < p->high) || !isfinite(p->low) ||
+               !isfinite(p->high) || (p->scaling == B2K_ROPE_LOG_RAMP && !(p->low > 0))))
+    return B2K_EINVAL;
+  // long double: 64 significant bits on this platform, so a turn is good to
+  // about 2^-63 of itself
+  const long double two_pi = 2.0L * acosl(-1.0L);
+  const long double s = p->factor;
+  long double theta = p->theta;
+  if (p->scaling == B2K_ROPE_BASE) theta *= powl(s, (long double)r / (r - 2));
+  b2k_rope rope = {};
+  for (int i = 0; i < r / 2; ++i) {
+    long double f = powl(theta, -2.0L * i / r);
+    if (p->scaling == B2K_ROPE_LINEAR) f /= s;
+    if (ramp) {
+      const long double t = p->context * f / two_pi;
+      long double w = p->scaling == B2K_ROPE_RAMP
+                          ? (t - p->low) / ((long double)p->high - p->low)
+                          : (logl(t) - logl(p->low)) / (logl(p->high) - logl(p->low));
+      w = std::min(1.0L, std::max(0.0L, w));
+      f = f * w + f * (1.0L - w) / s;
+    }
+    const long double turns = f / two_pi;
+    if (!isfinite(turns)) return B2K_EINVAL;
+    // the fraction of a turn, in units of 2^-64; 1 - 2^-65 and above is a whole turn
+    const long double units = ldexpl(turns - floorl(turns), 64);
+    rope.turn[i] = units >= 18446744073709551615.5L ? 0 : (uint64_t)(units + 0.5L);
+  }
+  rope.rot = r;
+  rope.interleaved = p->interleaved != 0;
+  rope.magnitude = (float)p->magnitude;
+  *out = rope;
+  return B2K_OK;
+}
+
+int64_t b2k_paged_slot(const int32_t *table_row, int32_t table_width, int64_t pages, int32_t page_size,
+                       int64_t position) {
+  if (!table_row || table_width < 0 || page_size < 1) return -1;
+  const int64_t page = serve::page_of(table_row, table_width, pages, page_size, position);
+  return page < 0 ? -1 : page * page_size + position % page_size;
+}
+
+int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count, const b2k_heads *x,
+               const b2k_heads *y, const int64_t *positions, int64_t tokens, int32_t d, int32_t transpose,
+               void *stream) {
+  B2K_CHECK_CTX(ctx);
+  if (!rope || !x || !y) return b2k::fail(ctx, B2K_EINVAL, "rotary: null argument");
+  if (!serve::type_ok(dtype)) return b2k::fail(ctx, B2K_EINVAL, "rotary: unknown element type %d", dtype);
+  if (count < 1 || count > 3) return b2k::fail(ctx, B2K_EINVAL, "rotary: %d tensors", count);
+  if (tokens < 0 || d < 1 || d > B2K_MAX_HEAD_DIM || (transpose != 0 && transpose != 1))
+    return b2k::fail(ctx, B2K_EINVAL, "rotary: %lld tokens of head dim %d, transpose %d", (long long)tokens, d, transpose);
+  RotaryArgs a = {};
+  int status = use_rope(ctx, "rotary", rope, d, transpose, a);
+  if (status != B2K_OK) return status;
+  const int64_t size = (int64_t)serve::type_size(dtype);
+  for (int i = 0; i < count; ++i) {
+    if ((status = serve::check_heads(ctx, "rotary", "input", &x[i], tokens, d)) != B2K_OK) return status;
+    if ((status = serve::check_heads(ctx, "rotary", "output", &y[i], tokens, d)) != B2K_OK) return status;
+    if (x[i].heads != y[i].heads)
+      return b2k::fail(ctx, B2K_EINVAL, "rotary: tensor %d has %d heads in and %d out", i, x[i].heads, y[i].heads);
+    if (x[i].data == y[i].data && (x[i].stride_token != y[i].stride_token || x[i].stride_head != y[i].stride_head))
+      return b2k::fail(ctx, B2K_EINVAL, "rotary: tensor %d is rotated in place with other strides", i);
+    a.seg[i] = {static_cast<const char *>(x[i].data), static_cast<char *>(y[i].data), x[i].stride_token * size,
+                x[i].stride_head * size, 0, y[i].stride_token * size, y[i].stride_head * size, a.heads, kLinear, 1};
+    a.heads += x[i].heads;
+  }
+  if (tokens == 0) return B2K_OK;
+  if (!positions) return b2k::fail(ctx, B2K_EINVAL, "rotary: null positions");
+  a.d = d;
+  a.tokens = tokens;
+  a.positions = positions;
+  return run<false>(ctx, a, count, dtype, tokens, 1, B2K_PHASE_ROTARY, (cudaStream_t)stream, "rotary launch");
+}
+
+int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
+                     const b2k_heads *k, const b2k_heads *v, const b2k_heads *q, const b2k_heads *q_out,
+                     void *stream) {
+  B2K_CHECK_CTX(ctx);
+  const char *what = "paged_append";
+  int status = serve::check_cache(ctx, what, cache);
+  if (status == B2K_OK) status = serve::check_batch(ctx, what, cache, batch);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "k", k, batch->tokens, cache->d);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "v", v, batch->tokens, cache->d);
+  if (status != B2K_OK) return status;
+  if (k->heads != cache->heads || v->heads != cache->heads)
+    return b2k::fail(ctx, B2K_EINVAL, "%s: %d key and %d value heads for a cache of %d", what, k->heads, v->heads,
+                     cache->heads);
+  if (!q != !q_out || (q && !rope)) return b2k::fail(ctx, B2K_EINVAL, "%s: q needs q_out and a rope", what);
+  RotaryArgs a = {};
+  a.d = cache->d;
+  if (rope && (status = use_rope(ctx, what, rope, cache->d, 0, a)) != B2K_OK) return status;
+  if (!rope) a.rot = 0, a.interleaved = 1;  // nothing turns: plain copies of neighbouring vectors
+  const int64_t size = (int64_t)serve::type_size(cache->dtype);
+  int count = 0;
+  if (q) {
+    if ((status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d)) != B2K_OK) return status;
+    if ((status = serve::check_heads(ctx, what, "q_out", q_out, batch->tokens, cache->d)) != B2K_OK) return status;
+    if (q->heads != q_out->heads ||
+        (q->data == q_out->data && (q->stride_token != q_out->stride_token || q->stride_head != q_out->stride_head)))
+      return b2k::fail(ctx, B2K_EINVAL, "%s: q and q_out differ in heads, or in strides in place", what);
+    a.seg[count++] = {static_cast<const char *>(q->data), static_cast<char *>(q_out->data), q->stride_token * size,
+                      q->stride_head * size, 0, q_out->stride_token * size, q_out->stride_head * size, 0, kLinear, 1};
+    a.heads += q->heads;
+  }
+  a.seg[count++] = {static_cast<const char *>(k->data), static_cast<char *>(cache->k), k->stride_token * size,
+                    k->stride_head * size, cache->k_page * size, cache->k_row * size, cache->k_head * size, a.heads,
+                    kKeys, rope != nullptr};
+  a.heads += k->heads;
+  a.seg[count++] = {static_cast<const char *>(v->data), static_cast<char *>(cache->v), v->stride_token * size,
+                    v->stride_head * size, cache->v_page * size, cache->v_row * size, cache->v_head * size, a.heads,
+                    kValues, 0};
+  a.heads += v->heads;
+  if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
+  a.tokens = batch->tokens;
+  a.first = batch->first;
+  a.lengths = batch->lengths;
+  a.table = batch->table;
+  a.table_stride = batch->table_stride;
+  a.table_width = batch->table_width;
+  a.pages = cache->pages;
+  a.page_size = cache->page_size;
+  a.prefix_len = batch->prefix_len;
+  a.max_new = batch->max_new;
+  a.err = ctx->error_flag;
+  return run<true>(ctx, a, count, cache->dtype, batch->max_new, (unsigned)batch->sequences, B2K_PHASE_APPEND,
+                   (cudaStream_t)stream, "paged_append launch");
+}
+
+}  // extern "C"

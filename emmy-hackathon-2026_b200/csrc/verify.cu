@@ -1,0 +1,242 @@
+// Verification of drafted tokens: how many of a sequence's drafts the target
+// takes, and the token drawn behind them.
+//
+// Mathematics.  A draft x with drafter's probability q(x) is taken with
+// probability min(1, p(x) / q(x)): u q(x) < p(x), a comparison of two
+// products of FP32 numbers, exact in FP64.  The draw from the rest r =
+// max(p - q, 0) is the inverse of its cumulative sum; FP64 sums of at most
+// 2^31 FP32 terms leave an error near 1e-13 of the total, far below the
+// spacing of the steps, so the order of the summation does not show.
+//
+// Bound: HBM, one row of p and one of q a sequence (2 * 4 * vocab bytes), in
+// one launch: a cluster of eight CTAs takes a sequence, each an eighth of the
+// row, each warp a contiguous run of that.  The runs' sums meet through
+// distributed shared memory, every CTA finds the run that holds the
+// threshold, and the one warp that owns it reads it again (from L2) in order.
+// Few sequences then still use eight SMs each, and nothing is kept in global
+// memory between the two passes.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int kCluster = 8;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kAhead = 8;   // elements a lane has in flight in the first pass
+constexpr int kRun = 8;     // consecutive elements of a lane in the second
+
+struct VerifyArgs {
+  b2k_drafts d;
+  int32_t *accepted, *tokens;
+};
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The rest that the token is drawn from: max(p - q, 0), p where q is not
+// there, and nothing of the rejected draft where that was certain.
+struct Rest {
+  const float *p, *q;
+  int64_t without;
+  __device__ __forceinline__ float at(int64_t i) const {
+    const float pi = __ldg(p + i);
+    const float qi = q ? __ldg(q + i) : 0.0f;
+    return pi > qi && i != without ? pi : 0.0f;  // the difference is taken in FP64
+  }
+  __device__ __forceinline__ double value(int64_t i) const {
+    const float pi = at(i);
+    return pi > 0.0f ? (double)pi - (q ? (double)__ldg(q + i) : 0.0) : 0.0;
+  }
+};
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ double run_sum[kWarps], slice_sum;
+  __shared__ int taken_s;
+  grid_dependency_wait();
+  grid_dependents_launch();
+
+  const b2k_drafts &d = a.d;
+  const int rank = (int)cluster.block_rank();
+  const int64_t b = blockIdx.x / kCluster;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = d.counts ? min(max(d.counts[b], 0), d.drafts) : d.drafts;
+  const int32_t *drafted = d.drafted + b * d.drafts;
+
+  if (warp == 0) {
+    int taken = n;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      bool ok = true;
+      if (i < n) {
+        const int64_t x = drafted[i];
+        ok = x >= 0 && x < d.vocab;
+        if (ok) {
+          const double p = d.target[(b * (d.drafts + 1) + i) * d.ld_target + x];
+          const double q = d.draft ? (double)d.draft[(b * d.drafts + i) * d.ld_draft + x] : 1.0;
+          ok = (double)d.u_accept[b * d.drafts + i] * q < p;
+        }
+      }
+      const unsigned refused = __ballot_sync(0xffffffffu, !ok);
+      if (refused) {
+        taken = i0 + __ffs(refused) - 1;
+        break;
+      }
+    }
+    if (lane == 0) taken_s = taken;
+  }
+  __syncthreads();
+  const int taken = taken_s;
+  Rest rest;
+  rest.p = d.target + (b * (d.drafts + 1) + taken) * d.ld_target;
+  rest.q = taken < n && d.draft ? d.draft + (b * d.drafts + taken) * d.ld_draft : nullptr;
+  rest.without = taken < n && !d.draft ? (int64_t)drafted[taken] : -1;
+
+  // this warp's run [lo, hi) of the row
+  const int64_t run = (d.vocab + kCluster * kWarps - 1) / (kCluster * kWarps);
+  const int64_t lo = min(d.vocab, (rank * kWarps + warp) * run), hi = min(d.vocab, lo + run);
+
+  int64_t token = -1;
+  bool owner = false;
+  for (int pass = 0; pass < 2; ++pass) {  // the second only where the rest is zero everywhere
+    double sum = 0.0;
+    for (int64_t i = lo + lane; i < hi; i += 32 * kAhead) {
+      float pv[kAhead], qv[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const bool in = i + 32 * u < hi;
+        pv[u] = in ? __ldg(rest.p + i + 32 * u) : 0.0f;
+        qv[u] = in && rest.q ? __ldg(rest.q + i + 32 * u) : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (pv[u] > qv[u] && i + 32 * u != rest.without) sum += (double)pv[u] - (double)qv[u];
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) run_sum[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double s = 0.0;
+      for (int w = 0; w < kWarps; ++w) s += run_sum[w];
+      slice_sum = s;
+    }
+    cluster.sync();
+    double slice[kCluster], total = 0.0;
+#pragma unroll
+    for (int r = 0; r < kCluster; ++r) {
+      slice[r] = *cluster.map_shared_rank(&slice_sum, r);
+      total += slice[r];
+    }
+    cluster.sync();  // every CTA has read: the sums may be written again, or the CTA leave
+    if (!(total > 0.0) && pass == 0 && taken < n) {
+      rest.q = nullptr;
+      rest.without = -1;
+      continue;
+    }
+    // the slice, then the run in it, whose cumulative sum first passes the
+    // threshold; rounding may leave none, then the last one that holds anything
+    const double threshold = (double)d.u_sample[b] * total;
+    double before = 0.0, start = 0.0;
+    int slice_at = -1;
+    bool over = false;
+#pragma unroll
+    for (int r = 0; r < kCluster; ++r) {
+      if (!over && slice[r] > 0.0) {
+        slice_at = r;
+        start = before;
+        over = before + slice[r] > threshold;
+      }
+      before += slice[r];
+    }
+    if (slice_at == rank) {
+      int run_at = -1;
+      double at = start, run_start = start;
+      bool found = false;
+      for (int w = 0; w < kWarps; ++w) {
+        if (!found && run_sum[w] > 0.0) {
+          run_at = w;
+          run_start = at;
+          found = at + run_sum[w] > threshold;
+        }
+        at += run_sum[w];
+      }
+      if (run_at == warp) {
+        owner = true;
+        double base = run_start;
+        for (int64_t i0 = lo; i0 < hi; i0 += 32 * kRun) {
+          double v[kRun], mine = 0.0;
+          const int64_t i = i0 + lane * kRun;
+#pragma unroll
+          for (int u = 0; u < kRun; ++u) {
+            v[u] = i + u < hi ? rest.value(i + u) : 0.0;
+            mine += v[u];
+          }
+          double upto = mine;  // inclusive scan over the lanes
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double other = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += other;
+          }
+          double c = base + (upto - mine);
+          int64_t hit = -1, last = -1;
+#pragma unroll
+          for (int u = 0; u < kRun; ++u) {
+            c += v[u];
+            if (v[u] > 0.0) {
+              last = i + u;
+              if (hit < 0 && c > threshold) hit = i + u;
+            }
+          }
+          const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0);
+          if (hits) {
+            token = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+            break;
+          }
+          const unsigned lasts = __ballot_sync(0xffffffffu, last >= 0);
+          if (lasts) token = __shfl_sync(0xffffffffu, last, 31 - __clz(lasts));
+          base += __shfl_sync(0xffffffffu, upto, 31);
+        }
+      }
+    } else if (slice_at < 0) {
+      owner = rank == 0 && warp == 0;  // nothing above zero: token -1
+    }
+    break;
+  }
+  if (owner && lane == 0) a.tokens[b * (d.drafts + 1) + taken] = (int32_t)token;
+  if (rank == 0 && warp == 1) {
+    if (lane == 0) a.accepted[b] = taken;
+    for (int i = lane; i <= d.drafts; i += 32)
+      if (i != taken) a.tokens[b * (d.drafts + 1) + i] = i < taken ? drafted[i] : -1;
+  }
+}
+
+}  // namespace
+
+extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *accepted, int32_t *tokens, void *stream) {
+  B2K_CHECK_CTX(ctx);
+  if (!d) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: null drafts");
+  if (d->batch < 0 || d->drafts < 0 || d->vocab < 1 || d->vocab > INT32_MAX)
+    return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: batch %lld, %d drafts, vocab %lld", (long long)d->batch, d->drafts,
+                     (long long)d->vocab);
+  if (d->batch > INT32_MAX / kCluster) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: too many sequences");
+  if (d->ld_target < d->vocab || (d->draft && d->ld_draft < d->vocab))
+    return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: a row stride is below vocab");
+  if (d->batch == 0) return B2K_OK;
+  if (!d->target || !d->u_sample || !accepted || !tokens || (d->drafts > 0 && (!d->drafted || !d->u_accept)))
+    return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: null buffer");
+  cudaStream_t s = (cudaStream_t)stream;
+  b2k::PhaseTimer timer(ctx, B2K_PHASE_VERIFY, s);
+  const VerifyArgs a{*d, accepted, tokens};
+  cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), verify_kernel, dim3((unsigned)(d->batch * kCluster)),
+                                       dim3(kThreads), 0, s, a);
+  if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "verify_drafts launch");
+  return b2k::check_launch(ctx, "verify_drafts launch");
+}

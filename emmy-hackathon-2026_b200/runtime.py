@@ -13,11 +13,12 @@ from pathlib import Path
 LIBRARY_PATH = Path(__file__).resolve().parent / "libb200k.so"
 
 B2K_OK, B2K_EINVAL, B2K_EUNSUPPORTED, B2K_ECUDA, B2K_ETIMEOUT, B2K_ESCRATCH = 0, 1, 2, -1, -2, 3
-B2K_ENCCL = -3
+B2K_ENCCL, B2K_EINDEX = -3, -4
 NOALLOC_SCRATCH_BYTES = 32 << 20
 MGPU_ID_BYTES = 128
 STATUS_NAMES = {B2K_EINVAL: "EINVAL", B2K_EUNSUPPORTED: "EUNSUPPORTED", B2K_ECUDA: "ECUDA",
-                B2K_ETIMEOUT: "ETIMEOUT", B2K_ESCRATCH: "ESCRATCH", B2K_ENCCL: "ENCCL"}
+                B2K_ETIMEOUT: "ETIMEOUT", B2K_ESCRATCH: "ESCRATCH", B2K_ENCCL: "ENCCL",
+                B2K_EINDEX: "EINDEX"}
 
 PW_MAX_INPUTS, PW_MAX_INSNS = 8, 48
 B_KN, B_NK, A_KM = 0, 1, 2   # A_KM is a flag or-ed into b_layout: A stored [k, m]
@@ -93,6 +94,50 @@ class GemmPlan(C.Structure):
                 ("chunks", C.c_int32)]
 
 
+F32, F16, BF16 = 0, 1, 2   # element types of the serving operators
+ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "log_ramp": 4}
+ROPE_MAX_PAIRS = 128
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("rot", C.c_int32), ("interleaved", C.c_int32), ("scaling", C.c_int32), ("theta", C.c_double),
+                ("factor", C.c_double), ("context", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("magnitude", C.c_double)]
+
+
+class Rope(C.Structure):
+    """b2k_rope: a plan of rotary positions (:func:`rope_plan`)."""
+    _fields_ = [("rot", C.c_int32), ("interleaved", C.c_int32), ("magnitude", C.c_float), ("reserved", C.c_int32),
+                ("turn", C.c_uint64 * ROPE_MAX_PAIRS)]
+
+
+class Heads(C.Structure):
+    """b2k_heads: a [tokens][heads][d] tensor (:func:`heads`)."""
+    _fields_ = [("data", C.c_void_p), ("stride_token", C.c_int64), ("stride_head", C.c_int64), ("heads", C.c_int32)]
+
+
+class PagedCache(C.Structure):
+    """b2k_paged_cache: keys and values in pages (:func:`paged_cache`)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("page_size", C.c_int32),
+                ("pages", C.c_int64), ("heads", C.c_int32), ("d", C.c_int32), ("k_page", C.c_int64),
+                ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_page", C.c_int64), ("v_row", C.c_int64),
+                ("v_head", C.c_int64)]
+
+
+class PagedBatch(C.Structure):
+    """b2k_paged_batch: the sequences of a call and their pages (:func:`paged_batch`)."""
+    _fields_ = [("sequences", C.c_int32), ("table_width", C.c_int32), ("tokens", C.c_int64), ("first", C.c_void_p),
+                ("lengths", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64), ("max_new", C.c_int32),
+                ("max_len", C.c_int32), ("prefix_len", C.c_int32), ("prefix_table", C.c_void_p)]
+
+
+class Drafts(C.Structure):
+    """b2k_drafts: drafted tokens, both models' probabilities and the random numbers."""
+    _fields_ = [("target", C.c_void_p), ("draft", C.c_void_p), ("ld_target", C.c_int64), ("ld_draft", C.c_int64),
+                ("drafted", C.c_void_p), ("counts", C.c_void_p), ("u_accept", C.c_void_p), ("u_sample", C.c_void_p),
+                ("batch", C.c_int64), ("vocab", C.c_int64), ("drafts", C.c_int32)]
+
+
 _P, _I32, _I64, _SZ, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float
 
 # name -> (argtypes without the leading context pointer, or None for no ctx)
@@ -140,6 +185,17 @@ SIGNATURES: dict[str, tuple] = {
     "b2k_kernel_launches": ([C.c_void_p, C.POINTER(_I64)], C.c_int),
     "b2k_selftest_wait_timeout": ([C.c_void_p, _I64, C.c_void_p], C.c_int),
     "b2k_launch": ([C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p), C.c_int32, C.c_void_p], C.c_int),
+    "b2k_rope_plan": ([C.POINTER(RopeParams), C.POINTER(Rope)], C.c_int),
+    "b2k_rotary": ([_P, C.POINTER(Rope), _I32, _I32, C.POINTER(Heads), C.POINTER(Heads), _P, _I64, _I32, _I32, _P],
+                   C.c_int),
+    "b2k_paged_slot": ([C.POINTER(_I32), _I32, _I64, _I32, _I64], _I64),
+    "b2k_paged_append": ([_P, C.POINTER(Rope), C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(Heads),
+                          C.POINTER(Heads), C.POINTER(Heads), C.POINTER(Heads), _P], C.c_int),
+    "b2k_paged_attention_workspace": ([_P, C.POINTER(PagedCache), C.POINTER(PagedBatch), _I32, C.POINTER(_SZ)],
+                                      C.c_int),
+    "b2k_paged_attention": ([_P, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(Heads), C.POINTER(Heads), _F,
+                             _P, _SZ, _P], C.c_int),
+    "b2k_verify_drafts": ([_P, C.POINTER(Drafts), _P, _P, _P], C.c_int),
     "b2k_mgpu_partition": ([_I64, _I32, _I32, _I64, C.POINTER(_I64), C.POINTER(_I64)], C.c_int),
     "b2k_mgpu_unique_id": ([_P], C.c_int),
     "b2k_mgpu_init": ([_P, _I32, _I32, _P, _I64, C.POINTER(_P)], C.c_int),
@@ -151,7 +207,8 @@ SIGNATURES: dict[str, tuple] = {
     "b2k_mgpu_attention_tf32x3": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _I32, _P], C.c_int),
 }
 
-PHASES = {"split": 0, "mma": 1, "pointwise": 2, "softmax": 3, "attention": 4, "rows": 5, "flash": 6}
+PHASES = {"split": 0, "mma": 1, "pointwise": 2, "softmax": 3, "attention": 4, "rows": 5, "flash": 6,
+          "rotary": 7, "append": 8, "paged": 9, "verify": 10}
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None
@@ -207,6 +264,53 @@ def make_program(n_inputs: int, insns: list[tuple], result: int, broadcast=(), o
     return prog
 
 
+def rope_plan(rot: int, *, theta: float = 10000.0, interleaved: bool = False, scaling: str = "none",
+              factor: float = 1.0, context: float = 0.0, low: float = 1.0, high: float = 32.0,
+              magnitude: float = 1.0) -> Rope:
+    """Rotary positions of the first `rot` elements of a head (b2k_rope_plan; host arithmetic).
+
+    ``scaling`` for contexts beyond the trained one: "none", "linear" (f / factor), "base" (theta such that the
+    slowest pair is slowed by `factor`), "ramp" and "log_ramp" (pairs that make at most `low` turns over
+    `context` tokens are slowed by `factor`, those that make `high` or more are kept, linearly in the turns or
+    in their logarithm between)."""
+    params = RopeParams(rot, int(interleaved), ROPE_SCALINGS[scaling], theta, factor, context, low, high, magnitude)
+    out = Rope()
+    status = library().b2k_rope_plan(C.byref(params), C.byref(out))
+    if status != B2K_OK:
+        raise B2KError(status, "rotary parameters outside their ranges", "b2k_rope_plan")
+    return out
+
+
+def heads(data: int, count: int, stride_token: int, stride_head: int) -> Heads:
+    """A [tokens][count][d] tensor at device address `data`, strides in elements."""
+    return Heads(data or None, stride_token, stride_head, count)
+
+
+def paged_cache(k: int, v: int, dtype: int, pages: int, page_size: int, heads: int, d: int, *,
+                head_major: bool = False, k_strides: tuple | None = None, v_strides: tuple | None = None) -> PagedCache:
+    """Contiguous pages [pages][page_size][heads][d], or [pages][heads][page_size][d] when `head_major`;
+    k_strides / v_strides = (page, row, head) in elements for any other layout."""
+    whole = page_size * heads * d
+    plain = (whole, d, page_size * d) if head_major else (whole, heads * d, d)
+    return PagedCache(k or None, v or None, dtype, page_size, pages, heads, d, *(k_strides or plain),
+                      *(v_strides or plain))
+
+
+def paged_batch(sequences: int, tokens: int, first: int, lengths: int, table: int, table_width: int, *, max_new: int,
+                max_len: int, table_stride: int | None = None, prefix_len: int = 0,
+                prefix_table: int = 0) -> PagedBatch:
+    """The sequences of a call (include/b200k.h); first, lengths, table and prefix_table are device addresses."""
+    return PagedBatch(sequences, table_width, tokens, first or None, lengths or None, table or None,
+                      table_width if table_stride is None else table_stride, max_new, max_len, prefix_len,
+                      prefix_table or None)
+
+
+def paged_slot(table_row, pages: int, page_size: int, position: int) -> int:
+    """Cache row of a position under a table row (b2k_paged_slot; host arithmetic), -1 where there is none."""
+    row = (C.c_int32 * max(1, len(table_row)))(*table_row)
+    return library().b2k_paged_slot(row, len(table_row), pages, page_size, position)
+
+
 class BoundCall:
     """One library call with its arguments converted to C types once.
 
@@ -220,7 +324,7 @@ class BoundCall:
     def __init__(self, ctx: "Context", name: str, args: tuple, keep: tuple = ()):
         fn = getattr(ctx.lib, name)
         converted = [a if isinstance(a, (C._SimpleCData, C._Pointer, C.Array)) or type(a).__name__ == "CArgObject"
-                     else t(a) for t, a in zip(fn.argtypes, args)]
+                     else t() if a is None else t(a) for t, a in zip(fn.argtypes, args)]
         self._fn, self._args, self._keep = fn, tuple(converted), keep
         self._ctx, self._name = ctx, name
 
@@ -365,6 +469,86 @@ class Context:
         arr = (_P * max(1, len(inputs)))(*inputs)
         return BoundCall(self, "b2k_pointwise_f32", (self.handle, C.byref(program), arr, out, n, stream),
                          keep=(program, arr))
+
+    # --- serving: rotary positions, paged cache, drafted tokens ------------------------
+    def _rotary_args(self, rope, dtype, pairs, positions, tokens, d, transpose=False, stream=0) -> tuple:
+        x, y = ((Heads * len(pairs))(*side) for side in zip(*pairs))
+        return (self.handle, C.byref(rope), dtype, len(pairs), x, y, positions or None, tokens, d, int(transpose),
+                stream)
+
+    def rotary(self, rope: Rope, dtype: int, pairs: list, positions: int, tokens: int, d: int, *,
+               transpose: bool = False, stream: int = 0) -> None:
+        """y = rotary(x) for each (x, y) of `pairs` (:func:`heads`); `transpose` gives the inputs' gradients
+        from the outputs'."""
+        self.check(self.lib.b2k_rotary(*self._rotary_args(rope, dtype, pairs, positions, tokens, d, transpose,
+                                                          stream)), "b2k_rotary")
+
+    def rotary_call(self, rope: Rope, dtype: int, pairs: list, positions: int, tokens: int, d: int, **kw) -> "BoundCall":
+        """:meth:`rotary` with its arguments converted once (see :class:`BoundCall`)."""
+        return BoundCall(self, "b2k_rotary", self._rotary_args(rope, dtype, pairs, positions, tokens, d, **kw),
+                         keep=(rope, pairs))
+
+    def _append_args(self, cache, batch, k, v, q=None, q_out=None, rope=None, stream=0) -> tuple:
+        ref = lambda x: None if x is None else C.byref(x)  # noqa: E731
+        return (self.handle, ref(rope), C.byref(cache), C.byref(batch), C.byref(k), C.byref(v), ref(q), ref(q_out),
+                stream)
+
+    def paged_append(self, cache: PagedCache, batch: PagedBatch, k: Heads, v: Heads, *, q: Heads | None = None,
+                     q_out: Heads | None = None, rope: Rope | None = None, stream: int = 0) -> None:
+        """The batch's new keys and values into the cache; with a rope, keys (and q into q_out) are rotated."""
+        self.check(self.lib.b2k_paged_append(*self._append_args(cache, batch, k, v, q, q_out, rope, stream)),
+                   "b2k_paged_append")
+
+    def paged_append_call(self, cache: PagedCache, batch: PagedBatch, k: Heads, v: Heads, **kw) -> "BoundCall":
+        """:meth:`paged_append` with its arguments converted once."""
+        return BoundCall(self, "b2k_paged_append", self._append_args(cache, batch, k, v, **kw),
+                         keep=(cache, batch, k, v, kw))
+
+    def paged_attention_workspace(self, cache: PagedCache, batch: PagedBatch, q_heads: int) -> int:
+        """Bytes of device memory :meth:`paged_attention` needs for these sizes."""
+        out = C.c_size_t()
+        self.check(self.lib.b2k_paged_attention_workspace(self.handle, C.byref(cache), C.byref(batch), q_heads,
+                                                          C.byref(out)), "b2k_paged_attention_workspace")
+        return out.value
+
+    def _paged_attention_args(self, cache, batch, q, o, workspace, nbytes, scale=None, stream=0) -> tuple:
+        div = float(cache.d) ** 0.5 if scale is None else float(scale)
+        return (self.handle, C.byref(cache), C.byref(batch), C.byref(q), C.byref(o), div, workspace or None, nbytes,
+                stream)
+
+    def paged_attention(self, cache: PagedCache, batch: PagedBatch, q: Heads, o: Heads, workspace: int = 0,
+                        nbytes: int = 0, *, scale: float | None = None, stream: int = 0) -> None:
+        """o = softmax(q K^T / scale) V of the new tokens over prefix and own cached keys; scale defaults to
+        sqrt(d).  `workspace` is device memory of the caller's, `nbytes` at least
+        :meth:`paged_attention_workspace`."""
+        self.check(self.lib.b2k_paged_attention(*self._paged_attention_args(cache, batch, q, o, workspace, nbytes,
+                                                                            scale, stream)), "b2k_paged_attention")
+
+    def paged_attention_call(self, cache: PagedCache, batch: PagedBatch, q: Heads, o: Heads, workspace: int = 0,
+                             nbytes: int = 0, **kw) -> "BoundCall":
+        """:meth:`paged_attention` with its arguments converted once."""
+        return BoundCall(self, "b2k_paged_attention", self._paged_attention_args(cache, batch, q, o, workspace,
+                                                                                 nbytes, **kw),
+                         keep=(cache, batch, q, o))
+
+    def _verify_args(self, target, drafted, u_accept, u_sample, accepted, tokens, batch, drafts, vocab, draft=0,
+                     counts=0, ld_target=None, ld_draft=None, stream=0) -> tuple:
+        d = Drafts(target or None, draft or None, ld_target or vocab, ld_draft or vocab, drafted or None,
+                   counts or None, u_accept or None, u_sample or None, batch, vocab, drafts)
+        return (self.handle, C.byref(d), accepted or None, tokens or None, stream)
+
+    def verify_drafts(self, target: int, drafted: int, u_accept: int, u_sample: int, accepted: int, tokens: int,
+                      batch: int, drafts: int, vocab: int, **kw) -> None:
+        """How many drafted tokens the target takes, and the token drawn behind them (b2k_verify_drafts);
+        keywords: draft, counts (device addresses), ld_target, ld_draft, stream."""
+        self.check(self.lib.b2k_verify_drafts(*self._verify_args(target, drafted, u_accept, u_sample, accepted, tokens,
+                                                                 batch, drafts, vocab, **kw)), "b2k_verify_drafts")
+
+    def verify_drafts_call(self, target: int, drafted: int, u_accept: int, u_sample: int, accepted: int, tokens: int,
+                           batch: int, drafts: int, vocab: int, **kw) -> "BoundCall":
+        """:meth:`verify_drafts` with its arguments converted once."""
+        return BoundCall(self, "b2k_verify_drafts", self._verify_args(target, drafted, u_accept, u_sample, accepted,
+                                                                      tokens, batch, drafts, vocab, **kw))
 
     # --- pipelined host-array calls: the same operations on HOST pointers, with
     # the copies in, the kernels and the copies out overlapped slab by slab.

@@ -36,6 +36,7 @@ extern "C" {
 #define B2K_ETIMEOUT (-2)  /* a device-side bounded wait expired (kernel error flag) */
 #define B2K_ESCRATCH 3     /* problem needs more than the fixed no-alloc scratch array */
 #define B2K_ENCCL (-3)     /* NCCL error; the multi-GPU handle is aborted and must be destroyed */
+#define B2K_EINDEX (-4)    /* a kernel met an index from device memory outside its bounds */
 
 typedef struct b2k_ctx b2k_ctx;
 
@@ -90,7 +91,11 @@ int b2k_selftest_wait_timeout(b2k_ctx *ctx, int64_t budget_cycles, void *stream)
 #define B2K_PHASE_ATTENTION 4 /* attention (all of its passes) */
 #define B2K_PHASE_ROWS 5      /* row reductions / norms */
 #define B2K_PHASE_FLASH 6     /* fused attention kernel */
-#define B2K_PHASE_COUNT 7
+#define B2K_PHASE_ROTARY 7    /* rotary positions */
+#define B2K_PHASE_APPEND 8    /* append to a paged cache */
+#define B2K_PHASE_PAGED 9     /* attention over a paged cache (all of its kernels) */
+#define B2K_PHASE_VERIFY 10   /* verification of drafted tokens */
+#define B2K_PHASE_COUNT 11
 int b2k_timing_enable(b2k_ctx *ctx, int on);
 /* Restrict timing to the phases whose bit (1 << B2K_PHASE_*) is set in
  * `phase_mask` (default: all).  Each timed phase costs two event records
@@ -299,6 +304,170 @@ int b2k_attention_tf32x3(b2k_ctx *ctx, const float *q, const float *k, const flo
  * kernel: 1 (default) the fused kernel with one CTA per query tile; 0 the
  * three-pass path (for comparisons).  Other values return B2K_EINVAL. */
 int b2k_attention_set_fused(int mode);
+
+/* --- rotary positions ----------------------------------------------------------
+ * Rotates pairs (a, b) of a head's first `rot` elements by position * f_i:
+ *   y_a = g (x_a cos - x_b sin),  y_b = g (x_b cos + x_a sin),  i < rot / 2,
+ * with (a, b) = (i, i + rot / 2), or (2i, 2i + 1) when interleaved; the other
+ * d - rot elements are copied.  f_i = theta^(-2i / rot) radians a position,
+ * changed for contexts longer than the one a model was trained on by
+ *   B2K_ROPE_NONE      nothing
+ *   B2K_ROPE_LINEAR    f / factor
+ *   B2K_ROPE_BASE      theta * factor^(rot / (rot - 2)) for theta: the slowest
+ *                      pair is slowed by `factor`, the fastest not at all
+ *   B2K_ROPE_RAMP      f (w + (1 - w) / factor), w = (t - low) / (high - low)
+ *                      held to [0, 1], t = context * f / 2 pi: the turns the
+ *                      pair makes over the trained context
+ *   B2K_ROPE_LOG_RAMP  the same with log t, log low and log high
+ * and g = magnitude.  Angles are exact for every 64-bit position: the plan
+ * holds f_i / 2 pi as a 64-bit binary fraction of a turn, so position * turn
+ * modulo 2^64 is the angle, with an error of position * 2^-65 turns, and no
+ * table bounds the positions.  No counterpart in the reference. */
+#define B2K_F32 0 /* element types of the operators below */
+#define B2K_F16 1
+#define B2K_BF16 2
+#define B2K_ROPE_NONE 0
+#define B2K_ROPE_LINEAR 1
+#define B2K_ROPE_BASE 2
+#define B2K_ROPE_RAMP 3
+#define B2K_ROPE_LOG_RAMP 4
+#define B2K_ROPE_MAX_PAIRS 128
+#define B2K_MAX_HEAD_DIM 256
+typedef struct b2k_rope_params {
+  int32_t rot;         /* rotated elements of a head: even, 2 .. 256 */
+  int32_t interleaved; /* 0: pairs (i, i + rot / 2); 1: pairs (2i, 2i + 1) */
+  int32_t scaling;     /* B2K_ROPE_* */
+  double theta;        /* > 0 */
+  double factor;       /* > 0; unused by B2K_ROPE_NONE */
+  double context;      /* ramps: trained context, tokens, > 0 */
+  double low, high;    /* ramps: turns at or below `low` are slowed, at or above `high` kept; low < high */
+  double magnitude;    /* g */
+} b2k_rope_params;
+typedef struct b2k_rope {
+  int32_t rot, interleaved;
+  float magnitude;
+  int32_t reserved;
+  uint64_t turn[B2K_ROPE_MAX_PAIRS]; /* f_i / 2 pi * 2^64, modulo 2^64 */
+} b2k_rope;
+/* Fill `out` from `params`: host arithmetic only (no device, no context).
+ * B2K_EINVAL for parameters outside the ranges above. */
+int b2k_rope_plan(const b2k_rope_params *params, b2k_rope *out);
+
+/* A tensor [tokens][heads][d] whose d elements are contiguous: strides in elements. */
+typedef struct b2k_heads {
+  void *data;
+  int64_t stride_token, stride_head;
+  int32_t heads;
+} b2k_heads;
+/* y[i] = rotary(x[i]) for i < count (1 .. 3) tensors of the same tokens, one
+ * launch (queries and keys, say); positions [tokens], any sign.  transpose
+ * = 1 applies the transposed rotation, with the same g: given the gradient
+ * of the outputs it returns the gradient of the inputs.  y[i] may be x[i]
+ * (the same data and strides), but may not overlap it otherwise.  Products
+ * and sums are FP32, rounded once to `dtype`.  tokens may be 0. */
+int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count, const b2k_heads *x,
+               const b2k_heads *y, const int64_t *positions, int64_t tokens, int32_t d, int32_t transpose,
+               void *stream);
+
+/* --- paged key / value cache -----------------------------------------------------
+ * Keys and values live in pages of `page_size` tokens; element (page, row,
+ * head, i) of k is at k + page * k_page + row * k_row + head * k_head + i
+ * (strides in elements), so pages may be token-major [pages][page_size][heads][d],
+ * head-major [pages][heads][page_size][d] or part of a larger buffer.
+ *
+ * A batch is `sequences` sequences whose new tokens are packed one after the
+ * other: sequence b's are rows first[b] .. first[b + 1] - 1 (first does not
+ * fall; none is allowed).  lengths[b] counts its own cached tokens with the
+ * new ones, so new token j of n has own position lengths[b] - n + j, which
+ * lies in page table[b * table_stride + position / page_size], row position %
+ * page_size.  All sequences may share a prefix of prefix_len tokens, cached
+ * once, in the pages of prefix_table in order; own positions follow it.
+ * first, lengths, table and prefix_table are device memory, read when the
+ * kernels run (a captured graph sees their values at replay); the other
+ * members are host values.
+ *
+ * Indexes from device memory are checked on the device: a page outside [0,
+ * pages), a position outside the table, a sequence with more new tokens than
+ * max_new or a length above max_len touches no memory (the token is not
+ * written, the key is left out, the row not computed) and the next
+ * b2k_stream_sync of the context returns B2K_EINDEX.  No counterpart in the
+ * reference. */
+typedef struct b2k_paged_cache {
+  void *k, *v;
+  int32_t dtype;     /* B2K_F32, B2K_F16 or B2K_BF16; every operand's */
+  int32_t page_size; /* tokens, >= 1 */
+  int64_t pages;
+  int32_t heads, d;  /* key / value heads; head dim, 1 .. B2K_MAX_HEAD_DIM */
+  int64_t k_page, k_row, k_head;
+  int64_t v_page, v_row, v_head;
+} b2k_paged_cache;
+typedef struct b2k_paged_batch {
+  int32_t sequences;
+  int32_t table_width;         /* pages in a row of the table */
+  int64_t tokens;              /* rows of the packed tensors; rows from first[sequences] on are left alone */
+  const int32_t *first;        /* [sequences + 1] */
+  const int32_t *lengths;      /* [sequences] */
+  const int32_t *table;        /* [sequences][table_width] */
+  int64_t table_stride;        /* >= table_width */
+  int32_t max_new, max_len;    /* upper bounds of the new tokens and of lengths[b]; sizes of the launches */
+  int32_t prefix_len;
+  const int32_t *prefix_table; /* [ceil(prefix_len / page_size)] */
+} b2k_paged_batch;
+/* The cache row of own position `position` under a table row of `table_width`
+ * pages: page * page_size + row, or -1 where the kernels would refuse it.
+ * Host arithmetic on host memory, by the kernels' own function. */
+int64_t b2k_paged_slot(const int32_t *table_row, int32_t table_width, int64_t pages, int32_t page_size,
+                       int64_t position);
+/* Write the batch's new keys and values k, v [tokens][cache heads][d] into
+ * the cache.  With a rope, keys are rotated on the way to position prefix_len
+ * + own position, and, when q is not NULL, q [tokens][heads][d] is rotated
+ * into q_out (which may be q) by the same launch.  Without one, k is copied
+ * (q must be NULL).  No two new tokens may share a cache row. */
+int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
+                     const b2k_heads *k, const b2k_heads *v, const b2k_heads *q, const b2k_heads *q_out,
+                     void *stream);
+/* Attention of the new tokens over the cache, with the prefix read once for
+ * all sequences: new token j of sequence b sees the whole prefix and own
+ * positions up to its own,
+ *   o = sum_s softmax_s(q . k_s / scale_div) v_s.
+ * Query head h reads cache head h / (q heads / cache heads).  A row that sees
+ * no key is zero.  FP32 softmax and sums; f16 and bf16 operands run on the
+ * tensor cores, with the probabilities rounded to the operands' type.
+ * `workspace` (device memory of the caller's, `workspace_bytes` at least what
+ * b2k_paged_attention_workspace says, 16-byte aligned; may be NULL when that
+ * is 0) holds what parts of one row's keys have summed; calls that may run at
+ * the same time need one each.  o may not overlap q. */
+int b2k_paged_attention_workspace(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
+                                  int32_t q_heads, size_t *bytes);
+int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch, const b2k_heads *q,
+                        const b2k_heads *o, float scale_div, void *workspace, size_t workspace_bytes, void *stream);
+
+/* --- verification of drafted tokens ------------------------------------------------
+ * For each of `batch` sequences with `drafts` drafted tokens x_0 .. x_{n-1},
+ * the target's probabilities p_0 .. p_n ([batch][drafts + 1][vocab]) and the
+ * drafter's q_0 .. q_{n-1} ([batch][drafts][vocab]), contiguous FP32 as
+ * b2k_row_softmax_f32 writes them (row strides ld_target, ld_draft >= vocab):
+ * x_i is taken while u_accept[b][i] * q_i(x_i) < p_i(x_i); at the first i
+ * that is not, one token is drawn from max(p_i - q_i, 0) (from p_i should
+ * that be zero everywhere), and with all taken one from p_n.  Drawn from r:
+ * the smallest t with r_0 + .. + r_t > u_sample[b] * sum(r), in 64 bits (the
+ * last t with r_t > 0 should rounding leave none).  draft == NULL: the drafts
+ * were certain (q_i(x_i) = 1, 0 elsewhere).  counts (may be NULL) holds each
+ * sequence's own number of drafts, 0 .. drafts.  accepted [batch]; tokens
+ * [batch][drafts + 1]: the taken drafts, the drawn token, then -1.  A drafted
+ * token outside [0, vocab) is never taken.  Every draw follows its target
+ * distribution exactly.  No counterpart in the reference. */
+typedef struct b2k_drafts {
+  const float *target, *draft;
+  int64_t ld_target, ld_draft;
+  const int32_t *drafted;      /* [batch][drafts] */
+  const int32_t *counts;       /* [batch] or NULL */
+  const float *u_accept;       /* [batch][drafts], in [0, 1) */
+  const float *u_sample;       /* [batch], in [0, 1) */
+  int64_t batch, vocab;
+  int32_t drafts;
+} b2k_drafts;
+int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *drafts, int32_t *accepted, int32_t *tokens, void *stream);
 
 /* --- launch by descriptor ----------------------------------------------------
  * The reference's runner launches a compiled kernel with
