@@ -244,8 +244,9 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
 // What a call launches, from its host values alone.
 struct Plan {
   int own_splits, own_chunk, prefix_splits, prefix_chunk, joined;
-  int own_rw, prefix_rw;  // rows a warp of paged_rows_kernel
-  size_t bytes;           // workspace
+  bool mma;
+  int own_rows, prefix_rows;  // rows of a block
+  size_t bytes;               // workspace
 };
 
 // Bytes of the parts' (m, l), which the sums follow on a 16-byte boundary.
@@ -253,33 +254,44 @@ size_t ml_bytes(size_t slots, int64_t tokens, int q_heads) {
   return (slots * (size_t)tokens * q_heads * sizeof(float2) + 15) / 16 * 16;
 }
 
-int rows_per_warp(int64_t rows) { return rows <= 4 ? 1 : rows <= 8 ? 2 : 8; }
+int plain_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 32; }
 
-// Splits of `keys` keys so that `units` independent blocks become about two
-// waves of the GPU's resident blocks, at least `least` keys each.
-void split_keys(int64_t keys, int64_t units, int sms, int least, int &splits, int &chunk) {
-  const int64_t want = std::max<int64_t>(1, (int64_t)sms * 6 / std::max<int64_t>(1, units));
+// Whether the tensor-core kernels can read the cache: 16-byte pieces throughout.
+bool cache_pieces(const b2k_paged_cache &c) {
+  return c.dtype != B2K_F32 && c.d % 8 == 0 && serve::vec_ok(c.k, c.k_page, c.k_row, c.k_head, 2, 16) &&
+         serve::vec_ok(c.v, c.v_page, c.v_row, c.v_head, 2, 16);
+}
+// Queries and outputs move in pairs of elements there.
+bool rows_pairs(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_token, x.stride_head, 0, 2, 4); }
+
+// Splits of `keys` keys so that `units` independent row blocks become `want`
+// blocks, each at least `least` keys long.
+void split_keys(int64_t keys, int64_t units, int64_t want, int least, int &splits, int &chunk) {
+  want = std::max<int64_t>(1, want / std::max<int64_t>(1, units));
   int64_t c = std::max<int64_t>(least, (keys + want - 1) / want);
-  c = (c + kTile - 1) / kTile * kTile;
+  c = (c + 63) / 64 * 64;
   splits = (int)std::max<int64_t>(1, (keys + c - 1) / c);
   chunk = (int)c;
 }
 
-Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, int sms) {
+Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, int sms, bool tensor) {
   Plan p = {};
   const int64_t group = q_heads / c.heads;
-  const int64_t own_rows = b.max_new * group, prefix_rows = b.tokens * group;
-  p.own_rw = rows_per_warp(own_rows);
-  p.prefix_rw = rows_per_warp(prefix_rows);
+  const int64_t own = b.max_new * group, prefix = b.tokens * group;
+  p.mma = tensor;
+  p.own_rows = tensor ? paged::mma_rows(c.d, own) : plain_rows(own);
+  p.prefix_rows = tensor ? paged::mma_rows(c.d, prefix) : plain_rows(prefix);
   // Sequences whose own rows fill a block read the prefix with their own keys:
   // stacking the rows of several sequences would save no reads of it.
-  p.joined = b.prefix_len > 0 && own_rows >= 128;
-  const int64_t own_blocks = (own_rows + 4 * p.own_rw - 1) / (4 * p.own_rw);
-  split_keys((int64_t)b.max_len + (p.joined ? b.prefix_len : 0), own_blocks * c.heads * b.sequences, sms, 128, p.own_splits,
-             p.own_chunk);
+  p.joined = b.prefix_len > 0 && own >= 128;
+  // blocks that a wave of the GPU holds, and keys that make a block worth its start
+  const int64_t wave = (int64_t)sms * (!tensor ? 6 : c.d > 128 ? 1 : 2);
+  const int least = tensor ? 256 : 128;
+  split_keys((int64_t)b.max_len + (p.joined ? b.prefix_len : 0),
+             (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, wave, least, p.own_splits, p.own_chunk);
   if (b.prefix_len > 0 && !p.joined)
-    split_keys(b.prefix_len, (prefix_rows + 4 * p.prefix_rw - 1) / (4 * p.prefix_rw) * c.heads, sms, 128,
-               p.prefix_splits, p.prefix_chunk);
+    split_keys(b.prefix_len, (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads, wave, least, p.prefix_splits,
+               p.prefix_chunk);
   const size_t slots = (size_t)p.own_splits + p.prefix_splits;
   if (slots > 1) p.bytes = ml_bytes(slots, b.tokens, q_heads) + slots * (size_t)b.tokens * q_heads * c.d * sizeof(float);
   return p;
@@ -298,8 +310,9 @@ cudaError_t launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, dim3
 }
 
 template <typename T>
-cudaError_t rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int rw, cudaStream_t s) {
+cudaError_t rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, cudaStream_t s) {
   const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
+  const int rw = block_rows / kWarps;
   const int row_blocks = (int)((rows + 4 * rw - 1) / (4 * rw));
   const dim3 grid((unsigned)(row_blocks * a.kv_heads), prefix ? a.prefix_splits : a.own_splits, prefix ? 1 : a.sequences);
   const size_t size = sizeof(T);
@@ -316,14 +329,22 @@ cudaError_t rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int rw, cudaStre
 }
 
 template <typename T>
-int run(b2k_ctx *ctx, const Args &a, const Plan &p, cudaStream_t s) {
+int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
   int launches = 1;
   cudaError_t err = cudaSuccess;
-  if (a.prefix_splits > 0) {
-    err = rows_part<T>(ctx, a, true, p.prefix_rw, s);
-    ++launches;
+  const bool prefix = a.prefix_splits > 0;
+  if (p.mma && (!prefix || p.prefix_rows == p.own_rows)) {
+    err = paged::mma_parts(ctx, a, dtype, prefix, true, p.own_rows, s);
+  } else {
+    if (prefix) {
+      err = p.mma ? paged::mma_parts(ctx, a, dtype, true, false, p.prefix_rows, s)
+                  : rows_part<T>(ctx, a, true, p.prefix_rows, s);
+      ++launches;
+    }
+    if (err == cudaSuccess)
+      err = p.mma ? paged::mma_parts(ctx, a, dtype, false, true, p.own_rows, s)
+                  : rows_part<T>(ctx, a, false, p.own_rows, s);
   }
-  if (err == cudaSuccess) err = rows_part<T>(ctx, a, false, p.own_rw, s);
   if (err == cudaSuccess && a.own_splits + a.prefix_splits > 1) {
     const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
     const dim3 grid(a.sequences, (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, 65535));
@@ -356,7 +377,9 @@ extern "C" int b2k_paged_attention_workspace(b2k_ctx *ctx, const b2k_paged_cache
   if (!bytes) return b2k::fail(ctx, B2K_EINVAL, "paged_attention_workspace: null result");
   int status = check_call(ctx, cache, batch, q_heads);
   if (status != B2K_OK) return status;
-  *bytes = make_plan(*cache, *batch, q_heads, ctx->sm_count).bytes;
+  // queries or outputs off their pairs take the plain kernel, which splits otherwise
+  *bytes = make_plan(*cache, *batch, q_heads, ctx->sm_count, false).bytes;
+  if (cache_pieces(*cache)) *bytes = std::max(*bytes, make_plan(*cache, *batch, q_heads, ctx->sm_count, true).bytes);
   return B2K_OK;
 }
 
@@ -374,7 +397,8 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   if (q->data == o->data && batch->tokens > 0) return b2k::fail(ctx, B2K_EINVAL, "%s: o is q", what);
   if (!(scale_div > 0.0f) || !isfinite(scale_div)) return b2k::fail(ctx, B2K_EINVAL, "%s: scale %g", what, scale_div);
   if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
-  const Plan p = make_plan(*cache, *batch, q->heads, ctx->sm_count);
+  const Plan p = make_plan(*cache, *batch, q->heads, ctx->sm_count,
+                           cache_pieces(*cache) && rows_pairs(*q) && rows_pairs(*o));
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return b2k::fail(ctx, B2K_EINVAL, "%s: a workspace of %zu bytes where %zu are needed", what,
                      workspace ? workspace_bytes : (size_t)0, p.bytes);
@@ -425,7 +449,7 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   }
   cudaStream_t s = (cudaStream_t)stream;
   b2k::PhaseTimer timer(ctx, B2K_PHASE_PAGED, s);
-  if (cache->dtype == B2K_F32) return run<float>(ctx, a, p, s);
-  if (cache->dtype == B2K_F16) return run<__half>(ctx, a, p, s);
-  return run<__nv_bfloat16>(ctx, a, p, s);
+  if (cache->dtype == B2K_F32) return run<float>(ctx, a, p, cache->dtype, s);
+  if (cache->dtype == B2K_F16) return run<__half>(ctx, a, p, cache->dtype, s);
+  return run<__nv_bfloat16>(ctx, a, p, cache->dtype, s);
 }

@@ -86,4 +86,9 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
   return -1;
 }
 
+// paged_mma.cu: rows of a block (16 or 32) for `rows` rows of one cache head, and
+// the launch of the prefix part, the sequences' own parts or both.
+int mma_rows(int d, int64_t rows);
+cudaError_t mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s);
+
 }  // namespace paged
