@@ -241,10 +241,14 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
   }
 }
 
+// The kernel of a part: paged_rows_kernel, warp MMAs (paged_mma.cu) or the
+// tensor-memory kernel (paged_umma.cu).
+enum Path { kPlain, kMma, kUmma };
+
 // What a call launches, from its host values alone.
 struct Plan {
   int own_splits, own_chunk, prefix_splits, prefix_chunk, joined;
-  bool mma;
+  Path own_path, prefix_path;
   int own_rows, prefix_rows;  // rows of a block
   size_t bytes;               // workspace
 };
@@ -261,8 +265,18 @@ bool cache_pieces(const b2k_paged_cache &c) {
   return c.dtype != B2K_F32 && c.d % 8 == 0 && serve::vec_ok(c.k, c.k_page, c.k_row, c.k_head, 2, 16) &&
          serve::vec_ok(c.v, c.v_page, c.v_row, c.v_head, 2, 16);
 }
-// Queries and outputs move in pairs of elements there.
-bool rows_pairs(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_token, x.stride_head, 0, 2, 4); }
+bool rows_pieces(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_token, x.stride_head, 0, 2, 16); }
+
+// Kernel for a part with `rows` rows a cache head.  Up to 32 rows fit one block
+// of the warp kernel, which then reads the keys once as well, two blocks an
+// SM; above that the tensor-memory kernel's 256 rows save re-reading them.
+// Head dims above 128 do not fit its tensor memory twice.
+Path pick_path(bool tensor, int d, int64_t rows) {
+  return !tensor ? kPlain : rows > 32 && d <= 128 ? kUmma : kMma;
+}
+int block_rows(Path path, int d, int64_t rows) {
+  return path == kPlain ? plain_rows(rows) : path == kMma ? paged::mma_rows(d, rows) : paged::kUmmaRows;
+}
 
 // Splits of `keys` keys so that `units` independent row blocks become `want`
 // blocks, each at least `least` keys long.
@@ -278,20 +292,23 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   Plan p = {};
   const int64_t group = q_heads / c.heads;
   const int64_t own = b.max_new * group, prefix = b.tokens * group;
-  p.mma = tensor;
-  p.own_rows = tensor ? paged::mma_rows(c.d, own) : plain_rows(own);
-  p.prefix_rows = tensor ? paged::mma_rows(c.d, prefix) : plain_rows(prefix);
+  p.own_path = pick_path(tensor, c.d, own);
+  p.own_rows = block_rows(p.own_path, c.d, own);
   // Sequences whose own rows fill a block read the prefix with their own keys:
   // stacking the rows of several sequences would save no reads of it.
   p.joined = b.prefix_len > 0 && own >= 128;
-  // blocks that a wave of the GPU holds, and keys that make a block worth its start
-  const int64_t wave = (int64_t)sms * (!tensor ? 6 : c.d > 128 ? 1 : 2);
-  const int least = tensor ? 256 : 128;
+  // blocks that the GPU holds at once, and keys that make a block worth its start
+  auto wave = [&](Path path) { return (int64_t)sms * (path == kPlain ? 6 : path == kUmma || c.d > 128 ? 1 : 2); };
+  auto least = [](Path path) { return path == kPlain ? 128 : path == kMma ? 256 : 512; };
   split_keys((int64_t)b.max_len + (p.joined ? b.prefix_len : 0),
-             (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, wave, least, p.own_splits, p.own_chunk);
-  if (b.prefix_len > 0 && !p.joined)
-    split_keys(b.prefix_len, (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads, wave, least, p.prefix_splits,
-               p.prefix_chunk);
+             (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, wave(p.own_path), least(p.own_path),
+             p.own_splits, p.own_chunk);
+  if (b.prefix_len > 0 && !p.joined) {
+    p.prefix_path = pick_path(tensor, c.d, prefix);
+    p.prefix_rows = block_rows(p.prefix_path, c.d, prefix);
+    split_keys(b.prefix_len, (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads, wave(p.prefix_path),
+               least(p.prefix_path), p.prefix_splits, p.prefix_chunk);
+  }
   const size_t slots = (size_t)p.own_splits + p.prefix_splits;
   if (slots > 1) p.bytes = ml_bytes(slots, b.tokens, q_heads) + slots * (size_t)b.tokens * q_heads * c.d * sizeof(float);
   return p;
@@ -333,17 +350,19 @@ int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t 
   int launches = 1;
   cudaError_t err = cudaSuccess;
   const bool prefix = a.prefix_splits > 0;
-  if (p.mma && (!prefix || p.prefix_rows == p.own_rows)) {
+  if (p.own_path == kMma && (!prefix || (p.prefix_path == kMma && p.prefix_rows == p.own_rows))) {
     err = paged::mma_parts(ctx, a, dtype, prefix, true, p.own_rows, s);
   } else {
+    auto part = [&](bool pre, Path path, int rows) {
+      return path == kPlain ? rows_part<T>(ctx, a, pre, rows, s)
+             : path == kMma ? paged::mma_parts(ctx, a, dtype, pre, !pre, rows, s)
+                            : paged::umma_part(ctx, a, dtype, pre, s);
+    };
     if (prefix) {
-      err = p.mma ? paged::mma_parts(ctx, a, dtype, true, false, p.prefix_rows, s)
-                  : rows_part<T>(ctx, a, true, p.prefix_rows, s);
+      err = part(true, p.prefix_path, p.prefix_rows);
       ++launches;
     }
-    if (err == cudaSuccess)
-      err = p.mma ? paged::mma_parts(ctx, a, dtype, false, true, p.own_rows, s)
-                  : rows_part<T>(ctx, a, false, p.own_rows, s);
+    if (err == cudaSuccess) err = part(false, p.own_path, p.own_rows);
   }
   if (err == cudaSuccess && a.own_splits + a.prefix_splits > 1) {
     const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
@@ -377,7 +396,7 @@ extern "C" int b2k_paged_attention_workspace(b2k_ctx *ctx, const b2k_paged_cache
   if (!bytes) return b2k::fail(ctx, B2K_EINVAL, "paged_attention_workspace: null result");
   int status = check_call(ctx, cache, batch, q_heads);
   if (status != B2K_OK) return status;
-  // queries or outputs off their pairs take the plain kernel, which splits otherwise
+  // queries or outputs off 16 bytes take the plain kernel, which splits otherwise
   *bytes = make_plan(*cache, *batch, q_heads, ctx->sm_count, false).bytes;
   if (cache_pieces(*cache)) *bytes = std::max(*bytes, make_plan(*cache, *batch, q_heads, ctx->sm_count, true).bytes);
   return B2K_OK;
@@ -398,7 +417,7 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   if (!(scale_div > 0.0f) || !isfinite(scale_div)) return b2k::fail(ctx, B2K_EINVAL, "%s: scale %g", what, scale_div);
   if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
   const Plan p = make_plan(*cache, *batch, q->heads, ctx->sm_count,
-                           cache_pieces(*cache) && rows_pairs(*q) && rows_pairs(*o));
+                           cache_pieces(*cache) && rows_pieces(*q) && rows_pieces(*o));
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return b2k::fail(ctx, B2K_EINVAL, "%s: a workspace of %zu bytes where %zu are needed", what,
                      workspace ? workspace_bytes : (size_t)0, p.bytes);

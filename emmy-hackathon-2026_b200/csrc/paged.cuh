@@ -91,4 +91,8 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
 int mma_rows(int d, int64_t rows);
 cudaError_t mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s);
 
+// paged_umma.cu: rows of a block, and the launch of one part.
+constexpr int kUmmaRows = 256;
+cudaError_t umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s);
+
 }  // namespace paged

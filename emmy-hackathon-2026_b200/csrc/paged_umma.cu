@@ -1,0 +1,505 @@
+// Attention over a paged cache for f16 and bf16 operands and many rows a cache
+// head -- the shared prefix under the stacked rows of a batch, prompt chunks --
+// on the 5th-generation tensor cores.
+//
+// One block per SM holds two tiles of 128 rows (A and B), so keys and values
+// are read once for 256 rows, and the tensor core works on one tile while the
+// softmax works on the other:
+//
+//   warps 0-3   softmax of tile A, one thread a row: S_j from tensor memory,
+//   warps 4-7   (tile B the same) running maximum, P_j back into S_j's columns
+//               in the operands' type, where the second product reads it;
+//               at the end the rows' output
+//   warps 8-9   loads: keys and values page by page with 16-byte asynchronous
+//               copies into 128-byte-swizzled tiles of 128 keys, in the order
+//               K_0, V_0, K_1, V_1 ... through one ring; keys outside the part
+//               and in bad pages arrive as zeros
+//   warp 10     MMA issuer: S_j = Q K_j^T (128 x 128), then O += P_j V_j with P
+//               from tensor memory and V as it lies (N-major)
+//
+// Mathematics: O stays in tensor memory over all tiles.  The exponents' base is
+// the running maximum of the time when it was last moved: it moves only when a
+// row's maximum has risen by more than 2^kSlack over it, and then the row's sums
+// in tensor memory are scaled (a rare step after the first tiles).  Until
+// then probabilities may exceed one; FP32 sums and the operands' range carry
+// 2^kSlack.  f16 probabilities are lifted by 2^kLift, so that small ones keep
+// their bits.
+//
+// Bound: tensor core and exponentials alike: a pair of 128 x 128 tiles takes
+// 2 x 1024 tensor cycles at head dim 128 and 2 x 1024 of the special-function unit.
+// All mbarrier waits are bounded (sm100.cuh).
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged.cuh"
+#include "sm100.cuh"
+
+namespace {
+
+using paged::Args;
+
+constexpr int kRows = 128;    // rows of a tile
+constexpr int kKeys = 128;    // keys of a tile
+constexpr int kSoftmaxWarps = 8, kLoadWarps = 2;
+constexpr int kThreads = 32 * (kSoftmaxWarps + kLoadWarps + 1);
+constexpr int kHalf = kKeys * 128;  // bytes of a tile's 64 columns: 128 rows of 128 bytes
+constexpr int kBehind = 2;    // copies in flight behind the one being issued
+constexpr int kMarks = 8;     // tiles whose key marks are kept
+
+template <int DP>
+constexpr int tile_bytes() { return kHalf * (DP / 64); }
+template <int DP>
+constexpr int stages() { return DP == 64 ? 8 : 5; }
+template <int DP>
+constexpr int smem_bytes() { return 2 * tile_bytes<DP>() + stages<DP>() * tile_bytes<DP>(); }
+
+// Tensor-memory columns.
+constexpr uint32_t kColS = 0, kColO = 256;  // S (then P) of tile A, B: 128 each; O of A, B: 128 each
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {
+  const int bytes = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T>
+struct Type;
+template <>
+struct Type<__half> {
+  static constexpr uint32_t kFormat = 0;
+  static constexpr float kLift = 6.0f, kSlack = 8.0f;  // 2^14 at most: within f16
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+template <>
+struct Type<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = 1;
+  static constexpr float kLift = 0.0f, kSlack = 8.0f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+
+// Instruction descriptor, kind::f16, FP32 accumulate (fields as idesc_tf32).
+template <typename T>
+__device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
+  return (1u << 4) | (Type<T>::kFormat << 7) | (Type<T>::kFormat << 10) | (b_mn_major ? (1u << 16) : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+}
+
+// MN-major 16-bit operand with the 128-byte swizzle: atoms of 64 MN-consecutive
+// elements (128 bytes) by 8 K rows (1024 bytes); bits 16-29 the stride between
+// atoms along MN, bits 32-45 along K.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t mn_stride, uint32_t k_stride) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>((mn_stride >> 4) & 0x3FFFu) << 16 |
+         static_cast<uint64_t>((k_stride >> 4) & 0x3FFFu) << 32 | static_cast<uint64_t>(1u) << 46 |
+         static_cast<uint64_t>(2u) << 61;
+}
+
+// D (+)= A B, both operands in shared memory / A in tensor memory; warp-wide.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(accumulate)
+      : "memory");
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_umma_kernel(const __grid_constant__ Args a, const bool prefix, const int row_blocks) {
+  constexpr int kStages = stages<DP>();
+  constexpr int kTile = tile_bytes<DP>();
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2], drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ uint32_t marks[kMarks][4];  // keys of a tile that are there
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int *abort = &abort_word;
+  if (threadIdx.x == 0) {
+    // swizzled tiles need 1024-byte alignment: refuse to run (error word, no
+    // work) rather than compute garbage
+    abort_word = (sm100::smem_addr(smem) & 1023u) ? 1 : 0;
+    if (abort_word) atomicOr(a.err, sm100::kSiteAttention);
+    for (int i = 0; i < kStages; ++i) {
+      sm100::mbar_init(&full[i], kLoadWarps);
+      sm100::mbar_init(&empty[i], 1);
+    }
+    sm100::mbar_init(&q_full, kSoftmaxWarps);
+    for (int i = 0; i < 2; ++i) {
+      sm100::mbar_init(&s_full[i], 1);
+      sm100::mbar_init(&p_full[i], 4);
+      sm100::mbar_init(&o_full[i], 1);
+    }
+    sm100::mbar_init(&drain, 1);
+    sm100::fence_barrier_init();
+  }
+  if (warp == kSoftmaxWarps + kLoadWarps) sm100::tmem_alloc(&tmem_slot, 512);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  grid_dependency_wait();
+  grid_dependents_launch();
+
+  // --- this block's rows and keys ------------------------------------------------
+  unsigned at = blockIdx.x;
+  const int block = row_blocks - 1 - at % row_blocks;  // the longest of a causal part first
+  at /= row_blocks;
+  const int head = at % a.kv_heads;
+  at /= a.kv_heads;
+  const int splits = prefix ? a.prefix_splits : a.own_splits;
+  const int split = at % splits, b = at / splits;
+  paged::Sequence s = {0, 0, 0};
+  if (prefix) s.n = paged::used_tokens(a);
+  else s = paged::sequence(a, b);
+  const int rows = s.n * a.group, row0 = block * 2 * kRows;
+  const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
+  const int key0 = split * chunk;
+  // keys of a tile's rows [first, first + 128): up to its last row's
+  auto keys_of = [&](int first) {
+    if (first >= rows) return 0;
+    const int last = (min(first + kRows, rows) - 1) / a.group;
+    return max(0, min(prefix ? a.prefix_len : paged::own_limit(a, s, last), key0 + chunk) - key0);
+  };
+  const int keys_a = keys_of(row0), keys_b = keys_of(row0 + kRows);
+  const int tiles_a = (keys_a + kKeys - 1) / kKeys, tiles_b = (keys_b + kKeys - 1) / kKeys;
+  const int key_end = key0 + max(keys_a, keys_b), tiles = max(tiles_a, tiles_b);
+  const bool direct = a.own_splits + a.prefix_splits == 1;
+  const bool work = row0 < rows && (tiles > 0 || (direct && key0 == 0));
+
+  uint8_t *const qs = smem, *const ring = smem + 2 * kTile;
+
+  if (work && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kLoadWarps) {
+    // ---------------- loads: warp w takes rows 64 w .. of every tile
+    const int w = warp - kSoftmaxWarps;
+    const T *kc = static_cast<const T *>(a.k) + (int64_t)head * a.k_head;
+    const T *vc = static_cast<const T *>(a.v) + (int64_t)head * a.v_head;
+    const int32_t *own_table = a.table + (int64_t)b * a.table_stride;
+    // page and row of the two keys this lane looks up (64 w + lane, + 32)
+    int page[2], row[2], next_page[2], next_row[2];
+    auto look_up = [&](int j, int (&pg)[2], int (&rw)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int k = key0 + j * kKeys + 64 * w + 32 * h + lane;
+        pg[h] = -1;
+        rw[h] = -1;
+        if (k < key_end) {
+          const int32_t *table = prefix ? a.prefix_table : own_table;
+          if (!prefix && a.joined) {
+            if (k < a.prefix_len) table = a.prefix_table;
+            else k -= a.prefix_len;
+          }
+          const int i = (int)((unsigned)k / (unsigned)a.page_size);
+          rw[h] = k - i * a.page_size;
+          pg[h] = table[i];
+        }
+      }
+    };
+    int n = 0;
+    bool ok = true;
+    auto issue = [&](bool keys, int j) {
+      const int stage = n % kStages;
+      if (n >= kStages)
+        ok = __all_sync(0xffffffffu, sm100::mbar_wait(&empty[stage], ((n / kStages) - 1) & 1, a.err,
+                                                      sm100::kSiteProducerEmpty, abort));
+      if (!ok) return;
+      const uint32_t to = sm100::smem_addr(ring + stage * kTile);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        bool there = page[h] >= 0 && page[h] < a.pages;
+        if (!there && row[h] >= 0) atomicOr(a.err, serve::kErrIndex);
+        const int64_t off = !there ? -1 : keys ? page[h] * a.k_page + row[h] * a.k_row : page[h] * a.v_page + row[h] * a.v_row;
+        if (keys) {
+          const uint32_t mark = __ballot_sync(0xffffffffu, there);
+          if (lane == 0) marks[j % kMarks][2 * w + h] = mark;
+        }
+        const T *from = keys ? kc : vc;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3);           // row of these 32
+          const int64_t o = __shfl_sync(0xffffffffu, off, r);
+          const int rr = 64 * w + 32 * h + r;
+#pragma unroll
+          for (int half = 0; half < DP / 64; ++half) {
+            const int c = lane & 7;
+            const bool on = o >= 0 && half * 64 + c * 8 < a.d;
+            copy16(to + half * kHalf + rr * 128 + ((c ^ (rr & 7)) << 4), from + (on ? o + half * 64 + c * 8 : 0), on);
+          }
+        }
+      }
+      copy_commit();
+      ++n;
+      if (n > kBehind) {
+        copy_wait<kBehind>();
+        sm100::fence_proxy_async_smem();  // the MMAs read through the async proxy
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&full[(n - 1 - kBehind) % kStages]);
+      }
+    };
+    look_up(0, page, row);
+    for (int j = 0; ok && j < tiles; ++j) {
+      issue(true, j);
+      if (j + 1 < tiles) look_up(j + 1, next_page, next_row);
+      if (ok) issue(false, j);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) page[h] = next_page[h], row[h] = next_row[h];
+    }
+    copy_wait<0>();
+    sm100::fence_proxy_async_smem();
+    __syncwarp();
+    if (ok && lane == 0)
+      for (int i = max(0, n - kBehind); i < n; ++i) sm100::mbar_arrive(&full[i % kStages]);
+  } else if (work && warp == kSoftmaxWarps + kLoadWarps) {
+    // ---------------- MMA issuer
+    const uint32_t id_s = idesc<T>(kKeys, false), id_o = idesc<T>(DP, true);
+    const uint32_t q_addr = sm100::smem_addr(qs);
+    bool ok = tiles == 0 || sm100::mbar_wait_warp(&q_full, 0, a.err, sm100::kSiteMmaFull, abort);
+    auto wait_item = [&](int i) {  // K_j is item 2 j, V_j 2 j + 1
+      ok = ok && sm100::mbar_wait_warp(&full[i % kStages], (i / kStages) & 1, a.err, sm100::kSiteMmaFull, abort);
+      sm100::tc_fence_after();
+    };
+    auto item_addr = [&](int i) { return sm100::smem_addr(ring + (i % kStages) * kTile); };
+    auto issue_s = [&](int x, int j) {
+      const uint32_t k = item_addr(2 * j), q = q_addr + x * kTile, d = tmem + kColS + x * 128;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
+        mma_ss(d, sm100::desc_kmajor<128>(q + off), sm100::desc_kmajor<128>(k + off), id_s, kk != 0);
+      }
+      sm100::mma_commit(&s_full[x]);
+    };
+    auto issue_o = [&](int x, int j, bool last) {
+      ok = ok && sm100::mbar_wait_warp(&p_full[x], j & 1, a.err, sm100::kSiteMmaFull, abort);
+      if (!ok) return;
+      sm100::tc_fence_after();
+      const uint32_t v = item_addr(2 * j + 1), p = tmem + kColS + x * 128, d = tmem + kColO + x * 128;
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        mma_ts(d, p + kk * 8, desc_mn(v + kk * 2048, kHalf, 1024), id_o, j != 0 || kk != 0);
+      if (last) sm100::mma_commit(&o_full[x]);
+    };
+    if (ok && tiles > 0) {
+      wait_item(0);
+      if (ok && tiles_a > 0) issue_s(0, 0);
+      if (ok && tiles_b > 0) issue_s(1, 0);
+      if (ok) sm100::mma_commit(&empty[0]);
+      for (int j = 0; ok && j < tiles; ++j) {
+        wait_item(2 * j + 1);
+        if (ok && j < tiles_a) issue_o(0, j, j + 1 == tiles_a);
+        if (ok && j + 1 < tiles) wait_item(2 * j + 2);
+        if (ok && j + 1 < tiles_a) issue_s(0, j + 1);
+        if (ok && j < tiles_b) issue_o(1, j, j + 1 == tiles_b);
+        if (ok) sm100::mma_commit(&empty[(2 * j + 1) % kStages]);
+        if (ok && j + 1 < tiles_b) issue_s(1, j + 1);
+        if (ok && j + 1 < tiles) sm100::mma_commit(&empty[(2 * j + 2) % kStages]);
+      }
+    }
+    sm100::mma_commit(&drain);
+    int never = 0;
+    sm100::mbar_wait(&drain, 0, a.err, sm100::kSiteDrain, &never);
+  } else if (work) {
+    // ---------------- softmax, one thread a row
+    const int x = warp >> 2;  // tile
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    {
+      // both tiles' queries into shared memory, 16 bytes at a time
+      constexpr int kPieces = DP / 8;
+      for (int i = threadIdx.x; i < 2 * kRows * kPieces; i += 32 * kSoftmaxWarps) {
+        const int qr = i / kPieces, c = i % kPieces, row = row0 + qr;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < rows && c * 8 < a.d) {
+          const int j = row / a.group;
+          v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (int64_t)(s.first + j) * a.q_token +
+                                               (int64_t)(head * a.group + row - j * a.group) * a.q_head + c * 8);
+        }
+        const int tr = qr & 127;
+        *reinterpret_cast<uint4 *>(qs + (qr >> 7) * kTile + (c >> 3) * kHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = v;
+      }
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&q_full);
+    }
+    const int row = row0 + x * kRows + r;
+    const int j_row = row / a.group;
+    const int limit = row >= rows ? 0 : min(prefix ? a.prefix_len : paged::own_limit(a, s, j_row), key_end);
+    // keys below this are seen by every row of the warp
+    int free_end = limit;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) free_end = min(free_end, __shfl_xor_sync(0xffffffffu, free_end, o));
+    const int mine = x == 0 ? tiles_a : tiles_b;
+    const float c = a.scale_log2;
+    const uint32_t s_at = tmem + lane_base + kColS + x * 128, o_at = tmem + lane_base + kColO + x * 128;
+    float base = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      ok = ok && sm100::mbar_wait_warp(&s_full[x], j & 1, a.err, sm100::kSiteAttention, abort);
+      if (!ok) break;
+      sm100::tc_fence_after();
+      uint32_t sr[kKeys];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sm100::tmem_ld_32x32b_x32(s_at + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * i]));
+      sm100::tmem_ld_wait();
+      const int key = key0 + j * kKeys;
+      const uint32_t *mk = marks[j % kMarks];
+      const uint32_t m0 = mk[0], m1 = mk[1], m2 = mk[2], m3 = mk[3];
+      if (key + kKeys > free_end || (m0 & m1 & m2 & m3) != 0xffffffffu) {
+        const int lim = limit - key;
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) {
+          const uint32_t word = i < 32 ? m0 : i < 64 ? m1 : i < 96 ? m2 : m3;
+          if (i >= lim || !((word >> (i & 31)) & 1u)) sr[i] = __float_as_uint(-INFINITY);
+        }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < kKeys; i += 4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(sr[i + e]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c - Type<T>::kLift;
+      if (__any_sync(0xffffffffu, top > base + Type<T>::kSlack || (base == -INFINITY && top > base))) {
+        const float moved = fmaxf(base, top);
+        const float alpha = moved == -INFINITY ? 1.0f : exp2_fast(base - moved);
+        base = moved;
+        l *= alpha;
+        if (j > 0) {
+          // S_j is complete, so is the product before it: O holds still
+#pragma unroll
+          for (int i = 0; i < DP; i += 16) {
+            uint32_t ov[16];
+            sm100::tmem_ld_32x32b_x16(o_at + i, ov);
+            sm100::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+            sm100::tmem_st_32x32b_x16(o_at + i, ov);
+          }
+        }
+      }
+      const float from = base == -INFINITY ? 0.0f : base;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint32_t pk[32];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          const float p0 = exp2_fast(fmaf(__uint_as_float(sr[64 * h + i]), c, -from));
+          const float p1 = exp2_fast(fmaf(__uint_as_float(sr[64 * h + i + 1]), c, -from));
+          sum[i & 2] += p0;
+          sum[(i & 2) + 1] += p1;
+          pk[i / 2] = Type<T>::pack(p0, p1);
+        }
+        sm100::tmem_st_32x32b_x32(s_at + 32 * h, pk);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      sm100::tmem_st_wait();
+      sm100::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&p_full[x]);
+    }
+    // ---------------- the row's output
+    if (mine > 0) ok = ok && sm100::mbar_wait_warp(&o_full[x], 0, a.err, sm100::kSiteEpilogueAccum, abort);
+    if (ok && row0 + x * kRows < rows) {
+      sm100::tc_fence_after();
+      const int q_heads = a.kv_heads * a.group;
+      const int64_t token = s.first + j_row;
+      const int qh = head * a.group + row - j_row * a.group;
+      const bool on = row < rows;
+      const bool some = l != 0.0f;  // (NaN too)
+      const float inv = !direct ? 1.0f : some ? 1.0f / l : 0.0f;
+      const int64_t part = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
+      // rows of a split that see none of its keys are not read by the merge
+      if (!direct && on) a.part_ml[part] = make_float2(base, l);
+#pragma unroll
+      for (int i = 0; i < DP; i += 32) {
+        if (i >= a.d) break;
+        uint32_t ov[32];
+        if (mine > 0) {
+          sm100::tmem_ld_32x32b_x32(o_at + i, ov);
+          sm100::tmem_ld_wait();
+        }
+        if (!on) continue;
+        if (direct) {
+          T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + i;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              w[u] = some && mine > 0 ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
+            if (i + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          float *out = a.part_o + part * a.d + i;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (i + e < a.d)
+              *reinterpret_cast<float4 *>(out + e) =
+                  some && mine > 0 ? make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
+                                                 __uint_as_float(ov[e + 3]))
+                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftmaxWarps + kLoadWarps) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int DP>
+cudaError_t launch(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned blocks, cudaStream_t s) {
+  auto kernel = paged_umma_kernel<T, DP>;
+  cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, smem_bytes<DP>());
+  if (err != cudaSuccess) return err;
+  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP>(), s, a, prefix,
+                            row_blocks);
+}
+
+}  // namespace
+
+namespace paged {
+
+cudaError_t umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s) {
+  const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
+  const int64_t row_blocks = (rows + kUmmaRows - 1) / kUmmaRows;
+  const int64_t blocks = row_blocks * a.kv_heads * (prefix ? a.prefix_splits : (int64_t)a.own_splits * a.sequences);
+  if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const unsigned n = (unsigned)blocks;
+  const int rb = (int)row_blocks;
+  if (dtype == B2K_F16)
+    return a.d <= 64 ? launch<__half, 64>(ctx, a, prefix, rb, n, s) : launch<__half, 128>(ctx, a, prefix, rb, n, s);
+  return a.d <= 64 ? launch<__nv_bfloat16, 64>(ctx, a, prefix, rb, n, s)
+                   : launch<__nv_bfloat16, 128>(ctx, a, prefix, rb, n, s);
+}
+
+}  // namespace paged
