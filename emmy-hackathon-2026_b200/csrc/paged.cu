@@ -247,7 +247,7 @@ enum Path { kPlain, kMma, kUmma };
 
 // What a call launches, from its host values alone.
 struct Plan {
-  int own_splits, own_chunk, prefix_splits, prefix_chunk, joined;
+  int own_splits, own_chunk, prefix_splits, prefix_chunk, joined, joined_keys;
   Path own_path, prefix_path;
   int own_rows, prefix_rows;  // rows of a block
   size_t bytes;               // workspace
@@ -283,7 +283,7 @@ int block_rows(Path path, int d, int64_t rows) {
 void split_keys(int64_t keys, int64_t units, int64_t want, int least, int &splits, int &chunk) {
   want = std::max<int64_t>(1, want / std::max<int64_t>(1, units));
   int64_t c = std::max<int64_t>(least, (keys + want - 1) / want);
-  c = (c + 63) / 64 * 64;
+  c = (c + 127) / 128 * 128;  // whole tiles of every kernel
   splits = (int)std::max<int64_t>(1, (keys + c - 1) / c);
   chunk = (int)c;
 }
@@ -300,7 +300,9 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   // blocks that the GPU holds at once, and keys that make a block worth its start
   auto wave = [&](Path path) { return (int64_t)sms * (path == kPlain ? 6 : path == kUmma || c.d > 128 ? 1 : 2); };
   auto least = [](Path path) { return path == kPlain ? 128 : path == kMma ? 256 : 512; };
-  split_keys((int64_t)b.max_len + (p.joined ? b.prefix_len : 0),
+  // the tensor-memory kernel's tiles end with the prefix
+  p.joined_keys = !p.joined ? 0 : p.own_path == kUmma ? (b.prefix_len + 127) / 128 * 128 : b.prefix_len;
+  split_keys((int64_t)b.max_len + p.joined_keys,
              (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, wave(p.own_path), least(p.own_path),
              p.own_splits, p.own_chunk);
   if (b.prefix_len > 0 && !p.joined) {
@@ -315,19 +317,20 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
 }
 
 template <typename T, int RW, int DV>
-cudaError_t launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, dim3 grid, int row_blocks, cudaStream_t s) {
+int launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, dim3 grid, int row_blocks, cudaStream_t s) {
   const int dp = (a.d + 3) / 4 * 4;
   const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + kTile * (dp + 4) + kTile * dp);
   constexpr int kFull = 16 / sizeof(T);
   auto kernel = vec ? paged_rows_kernel<T, RW, DV, kFull> : paged_rows_kernel<T, RW, DV, 1>;
   constexpr int most = sizeof(float) * (RW * kWarps * 128 * DV + kTile * (128 * DV + 4) + kTile * 128 * DV);
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
-  if (err != cudaSuccess) return err;
-  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), smem, s, a, prefix, row_blocks);
+  if (err == cudaSuccess)
+    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), smem, s, a, prefix, row_blocks);
+  return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }
 
 template <typename T>
-cudaError_t rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, cudaStream_t s) {
+int rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, cudaStream_t s) {
   const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
   const int rw = block_rows / kWarps;
   const int row_blocks = (int)((rows + 4 * rw - 1) / (4 * rw));
@@ -347,11 +350,10 @@ cudaError_t rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, 
 
 template <typename T>
 int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
-  int launches = 1;
-  cudaError_t err = cudaSuccess;
+  int launches = 1, status = B2K_OK;
   const bool prefix = a.prefix_splits > 0;
   if (p.own_path == kMma && (!prefix || (p.prefix_path == kMma && p.prefix_rows == p.own_rows))) {
-    err = paged::mma_parts(ctx, a, dtype, prefix, true, p.own_rows, s);
+    status = paged::mma_parts(ctx, a, dtype, prefix, true, p.own_rows, s);
   } else {
     auto part = [&](bool pre, Path path, int rows) {
       return path == kPlain ? rows_part<T>(ctx, a, pre, rows, s)
@@ -359,18 +361,19 @@ int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t 
                             : paged::umma_part(ctx, a, dtype, pre, s);
     };
     if (prefix) {
-      err = part(true, p.prefix_path, p.prefix_rows);
+      status = part(true, p.prefix_path, p.prefix_rows);
       ++launches;
     }
-    if (err == cudaSuccess) err = part(false, p.own_path, p.own_rows);
+    if (status == B2K_OK) status = part(false, p.own_path, p.own_rows);
   }
-  if (err == cudaSuccess && a.own_splits + a.prefix_splits > 1) {
+  if (status != B2K_OK) return status;
+  if (a.own_splits + a.prefix_splits > 1) {
     const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
     const dim3 grid(a.sequences, (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, 65535));
-    err = b2k::launch_kernel(b2k::pdl_enabled(), paged_merge_kernel<T>, grid, dim3(kThreads), 0, s, a);
+    const cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), paged_merge_kernel<T>, grid, dim3(kThreads), 0, s, a);
+    if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "paged_attention launch");
     ++launches;
   }
-  if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "paged_attention launch");
   return b2k::check_launch(ctx, "paged_attention launch", launches);
 }
 
@@ -461,6 +464,7 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   a.prefix_splits = p.prefix_splits;
   a.prefix_chunk = p.prefix_chunk;
   a.joined = p.joined;
+  a.joined_keys = p.joined_keys;
   if (p.bytes > 0) {
     const size_t slots = (size_t)(p.own_splits + p.prefix_splits);
     a.part_ml = static_cast<float2 *>(workspace);

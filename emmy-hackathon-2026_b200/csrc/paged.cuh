@@ -34,6 +34,7 @@ struct Args {
   // begin with it: `joined`)
   int own_splits, own_chunk, prefix_splits, prefix_chunk;
   int joined;
+  int joined_keys;   // where a joined part's own keys begin in its numbering: prefix_len, or that rounded up to whole tiles
   float *part_o;   // [own_splits + prefix_splits][tokens * q heads][d]
   float2 *part_ml; // [own_splits + prefix_splits][tokens * q heads]: m, l
 };
@@ -61,15 +62,18 @@ __device__ __forceinline__ int used_tokens(const Args &a) {
   return (int)min((int64_t)max(n, 0), a.tokens);
 }
 
-// Keys of an own part that new token j may see: its prefix (joined) and own
+// Keys of an own part that new token j may see, as the part numbers them: its
+// prefix (joined; numbers from prefix_len to joined_keys name none) and own
 // positions up to its own.
 __device__ __forceinline__ int own_limit(const Args &a, const Sequence &s, int j) {
-  return max(0, s.own0 + j + 1) + (a.joined ? a.prefix_len : 0);
+  const int own = max(0, s.own0 + j + 1);
+  return !a.joined ? own : own > 0 ? a.joined_keys + own : a.prefix_len;
 }
 
 // Offsets (elements) of a key's rows in the cache, for cache head 0; -1 for a page
 // outside the cache.  `at` counts from the start of the part: the prefix's
-// keys, or the own keys behind the prefix's where the part is joined.
+// keys, or the own keys behind the prefix's where the part is joined
+// (joined_keys = prefix_len).
 __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, int at, int &row) {
   const int32_t *table = a.prefix_table;
   if (!prefix) {
@@ -89,10 +93,10 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
 // paged_mma.cu: rows of a block (16 or 32) for `rows` rows of one cache head, and
 // the launch of the prefix part, the sequences' own parts or both.
 int mma_rows(int d, int64_t rows);
-cudaError_t mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s);
+int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s);
 
 // paged_umma.cu: rows of a block, and the launch of one part.
 constexpr int kUmmaRows = 256;
-cudaError_t umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s);
+int umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s);
 
 }  // namespace paged

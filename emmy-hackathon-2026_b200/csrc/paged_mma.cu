@@ -414,17 +414,20 @@ namespace paged {
 
 int mma_rows(int d, int64_t rows) { return d <= 128 && rows > 16 ? 32 : 16; }
 
-cudaError_t mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s) {
+int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s) {
   Grid g = {};
   g.prefix_row_blocks = (int)((a.tokens * a.group + rows - 1) / rows);
   g.own_row_blocks = (int)(((int64_t)a.max_new * a.group + rows - 1) / rows);
   const int64_t prefix = with_prefix ? (int64_t)g.prefix_row_blocks * a.kv_heads * a.prefix_splits : 0;
   const int64_t own = with_own ? (int64_t)g.own_row_blocks * a.kv_heads * a.own_splits * a.sequences : 0;
-  if (prefix + own > INT32_MAX) return cudaErrorInvalidConfiguration;
+  if (prefix + own > INT32_MAX)
+    return b2k::fail(ctx, B2K_EUNSUPPORTED, "paged_attention: %lld blocks", (long long)(prefix + own));
   g.prefix_blocks = (unsigned)prefix;
   const unsigned blocks = (unsigned)(prefix + own);
   const int mt = rows / 16;
-  return dtype == B2K_F16 ? pick<__half>(ctx, a, g, blocks, mt, s) : pick<__nv_bfloat16>(ctx, a, g, blocks, mt, s);
+  const cudaError_t err =
+      dtype == B2K_F16 ? pick<__half>(ctx, a, g, blocks, mt, s) : pick<__nv_bfloat16>(ctx, a, g, blocks, mt, s);
+  return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }
 
 }  // namespace paged

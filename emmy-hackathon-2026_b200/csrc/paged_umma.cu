@@ -10,12 +10,17 @@
 //   warps 4-7   (tile B the same) running maximum, P_j back into S_j's columns
 //               in the operands' type, where the second product reads it;
 //               at the end the rows' output
-//   warps 8-9   loads: keys and values page by page with 16-byte asynchronous
-//               copies into 128-byte-swizzled tiles of 128 keys, in the order
-//               K_0, V_0, K_1, V_1 ... through one ring; keys outside the part
-//               and in bad pages arrive as zeros
+//   warp 8      loads: keys and values into 128-byte-swizzled tiles of 128 keys, in
+//               the order K_0, V_0, K_1, V_1 ... through one ring, by TMA boxes
+//               of a page (or 128 rows of one); pages outside the cache are
+//               outside the tensor map and arrive as zeros
 //   warp 10     MMA issuer: S_j = Q K_j^T (128 x 128), then O += P_j V_j with P
 //               from tensor memory and V as it lies (N-major)
+//   warp 11     (pages that no box fits: sizes that neither divide 128 nor are a
+//               multiple of it, or below 8) passes on what has landed: there, warps 8
+//               and 9 copy row by row, 16 bytes a lane, and the tensor core sees
+//               such copies behind a proxy fence alone.  Those copies' issue
+//               bounds the kernel then: 7000 cycles a pair of tiles
 //
 // Mathematics: O stays in tensor memory over all tiles.  The exponents' base is
 // the running maximum of the time when it was last moved: it moves only when a
@@ -34,6 +39,7 @@
 
 #include "paged.cuh"
 #include "sm100.cuh"
+#include "tmap.cuh"
 
 namespace {
 
@@ -42,9 +48,8 @@ using paged::Args;
 constexpr int kRows = 128;    // rows of a tile
 constexpr int kKeys = 128;    // keys of a tile
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 2;
-constexpr int kThreads = 32 * (kSoftmaxWarps + kLoadWarps + 1);
+constexpr int kThreads = 32 * (kSoftmaxWarps + kLoadWarps + 2);
 constexpr int kHalf = kKeys * 128;  // bytes of a tile's 64 columns: 128 rows of 128 bytes
-constexpr int kBehind = 2;    // copies in flight behind the one being issued
 constexpr int kMarks = 8;     // tiles whose key marks are kept
 
 template <int DP>
@@ -53,6 +58,14 @@ template <int DP>
 constexpr int stages() { return DP == 64 ? 8 : 5; }
 template <int DP>
 constexpr int smem_bytes() { return 2 * tile_bytes<DP>() + stages<DP>() * tile_bytes<DP>(); }
+
+// 4-D tile load: (element, row of the page, head, page).
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 
 // Tensor-memory columns.
 constexpr uint32_t kColS = 0, kColO = 256;  // S (then P) of tile A, B: 128 each; O of A, B: 128 each
@@ -67,9 +80,11 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {
   const int bytes = on ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Arrive on `bar` once every copy of this thread so far has landed.
+__device__ __forceinline__ void copy_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sm100::smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <typename T>
 struct Type;
@@ -128,13 +143,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_umma_kernel(const __grid_constant__ Args a, const bool prefix, const int row_blocks) {
+    paged_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ Args a, const bool prefix, const int row_blocks) {
   constexpr int kStages = stages<DP>();
   constexpr int kTile = tile_bytes<DP>();
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2], drain;
+  __shared__ __align__(8) uint64_t landed[kStages], full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2], drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ uint32_t marks[kMarks][4];  // keys of a tile that are there
@@ -147,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     abort_word = (sm100::smem_addr(smem) & 1023u) ? 1 : 0;
     if (abort_word) atomicOr(a.err, sm100::kSiteAttention);
     for (int i = 0; i < kStages; ++i) {
-      sm100::mbar_init(&full[i], kLoadWarps);
+      sm100::mbar_init(&landed[i], 32 * kLoadWarps);
+      sm100::mbar_init(&full[i], 1);  // TMA: the bytes; else warp 11
       sm100::mbar_init(&empty[i], 1);
     }
     sm100::mbar_init(&q_full, kSoftmaxWarps);
@@ -195,8 +212,63 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   uint8_t *const qs = smem, *const ring = smem + 2 * kTile;
 
-  if (work && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kLoadWarps) {
-    // ---------------- loads: warp w takes rows 64 w .. of every tile
+  const int tile0 = key0 / kKeys;                                         // of the part
+  const int prefix_tiles = !prefix && a.joined ? a.joined_keys / kKeys : 0;  // of those, the prefix's
+  // keys of the block's tile j
+  auto valid = [&](int j) {
+    const int key = key0 + j * kKeys;
+    return min(kKeys, (tile0 + j < prefix_tiles ? min(key_end, a.prefix_len) : key_end) - key);
+  };
+
+  if (TMA && work && warp == kSoftmaxWarps) {
+    // ---------------- loads: lane i the tile's i-th box
+    const int box = min(a.page_size, kKeys), boxes = kKeys / box;
+    const int32_t *own_table = a.table + (int64_t)b * a.table_stride;
+    auto look_up = [&](int j) {  // page of this lane's box, -1 behind the last key
+      const bool pre = prefix || tile0 + j < prefix_tiles;
+      const int key = (tile0 + j - (pre ? 0 : prefix_tiles)) * kKeys + lane * box;
+      return lane < boxes && lane * box < valid(j) ? (pre ? a.prefix_table : own_table)[(unsigned)key / (unsigned)a.page_size] : -1;
+    };
+    bool ok = true;
+    int page = look_up(0);
+    for (int j = 0; ok && j < tiles; ++j) {
+      const bool pre = prefix || tile0 + j < prefix_tiles;
+      const int key = (tile0 + j - (pre ? 0 : prefix_tiles)) * kKeys + lane * box;
+      const int row = (int)((unsigned)key % (unsigned)a.page_size);
+      const bool wanted = lane < boxes && lane * box < valid(j), there = wanted && page >= 0 && page < a.pages;
+      if (wanted && !there) atomicOr(a.err, serve::kErrIndex);
+      const uint32_t have = __ballot_sync(0xffffffffu, there);
+      if (lane < 4) {
+        uint32_t mark = 0;
+        for (int i = 0; i < 32; i += min(box, 32))
+          if ((have >> ((32 * lane + i) / box)) & 1u) mark |= (box >= 32 ? 0xffffffffu : ((1u << box) - 1u) << i);
+        marks[j % kMarks][lane] = mark;
+      }
+      const int at_page = there ? page : -1;
+      if (j + 1 < tiles) page = look_up(j + 1);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int n = 2 * j + kv, stage = n % kStages;
+        if (n >= kStages)
+          ok = ok && sm100::mbar_wait_warp(&empty[stage], ((n / kStages) - 1) & 1, a.err, sm100::kSiteProducerEmpty, abort);
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive_expect_tx(&full[stage], kTile);
+        __syncwarp();
+        if (lane < boxes) {
+          const uint32_t to = sm100::smem_addr(ring + stage * kTile) + lane * box * 128;
+#pragma unroll
+          for (int half = 0; half < DP / 64; ++half)
+            tma_load_4d(to + half * kHalf, kv ? &map_v : &map_k, &full[stage], 64 * half, row, head, at_page);
+        }
+      }
+    }
+    // loads in flight must land before the block leaves (budget only)
+    int never = 0;
+    if (!ok)
+      for (int i = 0; i < kStages; ++i) sm100::mbar_wait(&full[i], 0, a.err, sm100::kSiteDrain, &never, 1000000);
+  } else if (!TMA && work && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kLoadWarps) {
+    // ---------------- loads row by row: warp w takes rows 64 w .. of every tile
     const int w = warp - kSoftmaxWarps;
     const T *kc = static_cast<const T *>(a.k) + (int64_t)head * a.k_head;
     const T *vc = static_cast<const T *>(a.v) + (int64_t)head * a.v_head;
@@ -206,15 +278,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto look_up = [&](int j, int (&pg)[2], int (&rw)[2]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        int k = key0 + j * kKeys + 64 * w + 32 * h + lane;
+        const bool pre = prefix || tile0 + j < prefix_tiles;
+        const int in = 64 * w + 32 * h + lane, k = (tile0 + j - (pre ? 0 : prefix_tiles)) * kKeys + in;
         pg[h] = -1;
         rw[h] = -1;
-        if (k < key_end) {
-          const int32_t *table = prefix ? a.prefix_table : own_table;
-          if (!prefix && a.joined) {
-            if (k < a.prefix_len) table = a.prefix_table;
-            else k -= a.prefix_len;
-          }
+        if (in < valid(j)) {
+          const int32_t *table = pre ? a.prefix_table : own_table;
           const int i = (int)((unsigned)k / (unsigned)a.page_size);
           rw[h] = k - i * a.page_size;
           pg[h] = table[i];
@@ -253,14 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      copy_commit();
+      copy_arrive(&landed[stage]);
       ++n;
-      if (n > kBehind) {
-        copy_wait<kBehind>();
-        sm100::fence_proxy_async_smem();  // the MMAs read through the async proxy
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&full[(n - 1 - kBehind) % kStages]);
-      }
     };
     look_up(0, page, row);
     for (int j = 0; ok && j < tiles; ++j) {
@@ -270,11 +333,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int h = 0; h < 2; ++h) page[h] = next_page[h], row[h] = next_row[h];
     }
-    copy_wait<0>();
-    sm100::fence_proxy_async_smem();
-    __syncwarp();
-    if (ok && lane == 0)
-      for (int i = max(0, n - kBehind); i < n; ++i) sm100::mbar_arrive(&full[i % kStages]);
+    copy_wait_all();
+  } else if (!TMA && work && warp == kSoftmaxWarps + kLoadWarps + 1) {
+    // ---------------- what has landed becomes visible to the tensor core
+    bool ok = true;
+    for (int i = 0; ok && i < 2 * tiles; ++i) {
+      ok = sm100::mbar_wait_warp(&landed[i % kStages], (i / kStages) & 1, a.err, sm100::kSiteConvert, abort);
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (ok && lane == 0) sm100::mbar_arrive(&full[i % kStages]);
+    }
   } else if (work && warp == kSoftmaxWarps + kLoadWarps) {
     // ---------------- MMA issuer
     const uint32_t id_s = idesc<T>(kKeys, false), id_o = idesc<T>(DP, true);
@@ -311,6 +379,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) sm100::mma_commit(&empty[0]);
       for (int j = 0; ok && j < tiles; ++j) {
         wait_item(2 * j + 1);
+        if (TMA && ok && valid(j) < kKeys) {
+          // the values behind the last key (of the prefix, or of all) become
+          // zeros: a page's unused rows may hold anything, and 0 x NaN is NaN
+          uint8_t *v = ring + ((2 * j + 1) % kStages) * kTile;
+          for (int i = 8 * valid(j) + lane; i < 8 * kKeys; i += 32)
+#pragma unroll
+            for (int half = 0; half < DP / 64; ++half)
+              *reinterpret_cast<uint4 *>(v + half * kHalf + 16 * i) = make_uint4(0, 0, 0, 0);
+          sm100::fence_proxy_async_smem();
+          __syncwarp();
+        }
         if (ok && j < tiles_a) issue_o(0, j, j + 1 == tiles_a);
         if (ok && j + 1 < tiles) wait_item(2 * j + 2);
         if (ok && j + 1 < tiles_a) issue_s(0, j + 1);
@@ -323,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm100::mma_commit(&drain);
     int never = 0;
     sm100::mbar_wait(&drain, 0, a.err, sm100::kSiteDrain, &never);
-  } else if (work) {
+  } else if (work && warp < kSoftmaxWarps) {
     // ---------------- softmax, one thread a row
     const int x = warp >> 2;  // tile
     const int r = (warp & 3) * 32 + lane;
@@ -367,11 +446,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 4; ++i)
         sm100::tmem_ld_32x32b_x32(s_at + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * i]));
       sm100::tmem_ld_wait();
-      const int key = key0 + j * kKeys;
+      const int key = key0 + j * kKeys, part_end = tile0 + j < prefix_tiles ? a.prefix_len : INT32_MAX;
       const uint32_t *mk = marks[j % kMarks];
       const uint32_t m0 = mk[0], m1 = mk[1], m2 = mk[2], m3 = mk[3];
-      if (key + kKeys > free_end || (m0 & m1 & m2 & m3) != 0xffffffffu) {
-        const int lim = limit - key;
+      if (key + kKeys > min(free_end, part_end) || (m0 & m1 & m2 & m3) != 0xffffffffu) {
+        const int lim = min(limit, part_end) - key;
 #pragma unroll
         for (int i = 0; i < kKeys; ++i) {
           const uint32_t word = i < 32 ? m0 : i < 64 ? m1 : i < 96 ? m2 : m3;
@@ -476,30 +555,69 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <typename T, int DP>
-cudaError_t launch(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned blocks, cudaStream_t s) {
-  auto kernel = paged_umma_kernel<T, DP>;
+// [pages][heads][page rows][d] of a cache in any order of strides, boxes of 64
+// elements by a page's rows (128 at most).
+template <typename T>
+int make_map(b2k_ctx *ctx, CUtensorMap *map, const Args &a, bool keys) {
+  auto encode = b2k::tensor_map_encoder();
+  if (!encode) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  const void *base = keys ? a.k : a.v;
+  const int64_t row = keys ? a.k_row : a.v_row, head = keys ? a.k_head : a.v_head, page = keys ? a.k_page : a.v_page;
+  cuuint64_t dims[4] = {(cuuint64_t)a.d, (cuuint64_t)a.page_size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+  cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)std::min(a.page_size, kKeys), 1, 1};
+  cuuint32_t elem[4] = {1, 1, 1, 1};
+  const CUresult res =
+      encode(map, Type<T>::kFormat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+             const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)res);
+  return B2K_OK;
+}
+
+// Whether pages are boxes: whole swizzle atoms (8 rows) that tile 128 keys, or
+// 128 keys a part of one; and strides and extents a tensor map can hold.
+bool boxes_fit(const Args &a) {
+  const int64_t most = (int64_t)1 << 38;  // 2^39 bytes
+  return a.page_size >= 8 && (kKeys % a.page_size == 0 || a.page_size % kKeys == 0) && a.pages <= INT32_MAX &&
+         a.k_row < most && a.k_head < most && a.k_page < most && a.v_row < most && a.v_head < most && a.v_page < most;
+}
+
+template <typename T, int DP, bool TMA>
+int launch(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned blocks, cudaStream_t s) {
+  auto kernel = paged_umma_kernel<T, DP, TMA>;
+  CUtensorMap map_k = {}, map_v = {};
+  int status;
+  if (TMA && (status = make_map<T>(ctx, &map_k, a, true)) != B2K_OK) return status;
+  if (TMA && (status = make_map<T>(ctx, &map_v, a, false)) != B2K_OK) return status;
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, smem_bytes<DP>());
-  if (err != cudaSuccess) return err;
-  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP>(), s, a, prefix,
-                            row_blocks);
+  if (err == cudaSuccess)
+    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP>(), s, map_k, map_v, a,
+                             prefix, row_blocks);
+  return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
+}
+
+template <typename T>
+int pick(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned blocks, cudaStream_t s) {
+  const bool tma = boxes_fit(a);
+  if (a.d <= 64)
+    return tma ? launch<T, 64, true>(ctx, a, prefix, row_blocks, blocks, s)
+               : launch<T, 64, false>(ctx, a, prefix, row_blocks, blocks, s);
+  return tma ? launch<T, 128, true>(ctx, a, prefix, row_blocks, blocks, s)
+             : launch<T, 128, false>(ctx, a, prefix, row_blocks, blocks, s);
 }
 
 }  // namespace
 
 namespace paged {
 
-cudaError_t umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s) {
+int umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s) {
   const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
   const int64_t row_blocks = (rows + kUmmaRows - 1) / kUmmaRows;
   const int64_t blocks = row_blocks * a.kv_heads * (prefix ? a.prefix_splits : (int64_t)a.own_splits * a.sequences);
-  if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
-  const unsigned n = (unsigned)blocks;
-  const int rb = (int)row_blocks;
-  if (dtype == B2K_F16)
-    return a.d <= 64 ? launch<__half, 64>(ctx, a, prefix, rb, n, s) : launch<__half, 128>(ctx, a, prefix, rb, n, s);
-  return a.d <= 64 ? launch<__nv_bfloat16, 64>(ctx, a, prefix, rb, n, s)
-                   : launch<__nv_bfloat16, 128>(ctx, a, prefix, rb, n, s);
+  if (blocks > INT32_MAX) return b2k::fail(ctx, B2K_EUNSUPPORTED, "paged_attention: %lld blocks", (long long)blocks);
+  return dtype == B2K_F16 ? pick<__half>(ctx, a, prefix, (int)row_blocks, (unsigned)blocks, s)
+                          : pick<__nv_bfloat16>(ctx, a, prefix, (int)row_blocks, (unsigned)blocks, s);
 }
 
 }  // namespace paged
