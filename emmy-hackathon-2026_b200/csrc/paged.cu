@@ -9,7 +9,8 @@
 // RW rows (query heads of one cache head, tokens side by side) and streams 32
 // keys at a time through shared memory as FP32.  Scores: lane = key, each
 // warp its own RW rows, so a key is read once for RW rows and the softmax of a
-// tile is one butterfly.  P V: lane = four dims, the probabilities shuffled
+// tile is one butterfly; the next tile is on its way meanwhile (asynchronous
+// copies where the cache is f32 in 16-byte pieces).  P V: lane = four dims, the probabilities shuffled
 // from their lanes; a probability of exactly zero skips its key, so what a
 // masked place of the cache holds (infinities and NaN too) has no effect.
 #include <math.h>
@@ -32,17 +33,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// 16-byte copy global to shared.
+__device__ __forceinline__ void copy16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
 // DV: float4s of a head that a lane holds (head dim up to 128 DV).
 // V: elements of one access to the cache (16 bytes, or 1).
 template <typename T, int RW, int DV, int V>
-__global__ void __launch_bounds__(kThreads) paged_rows_kernel(const __grid_constant__ Args a, bool prefix, int row_blocks) {
+__global__ void __launch_bounds__(kThreads)
+    paged_rows_kernel(const __grid_constant__ Args a, bool prefix, int row_blocks, bool beside) {
   constexpr int R = RW * kWarps;
+  constexpr bool kAsync = sizeof(T) == 4 && V == 4;  // the cache's bytes are the tile's
   extern __shared__ __align__(16) float smem[];
-  __shared__ int64_t k_at[kTile], v_at[kTile];
+  __shared__ int64_t k_at[3][kTile], v_at[3][kTile];
   const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4;
-  float *qs = smem, *ks = qs + R * dp, *vs = ks + kTile * ldk;
-  grid_dependency_wait();
-  grid_dependents_launch();
+  const int stage_floats = kTile * (ldk + dp);  // keys, then values; two stages behind the queries
+  float *qs = smem, *tiles = qs + R * dp;
+  paged::part_begin(beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.y, head = blockIdx.x / row_blocks, block = blockIdx.x % row_blocks, b = blockIdx.z;
@@ -51,13 +59,63 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const __grid_const
   if (prefix) s.n = paged::used_tokens(a);
   else s = paged::sequence(a, b);
   const int rows = s.n * a.group, row0 = block * R;
-  if (row0 >= rows) return;
+  if (row0 >= rows) return paged::part_end(beside);
   const int last_token = (min(row0 + R, rows) - 1) / a.group;
   const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
   const int key0 = split * chunk;
   const int key_end = min(prefix ? a.prefix_len : paged::own_limit(a, s, last_token), key0 + chunk);
   const bool direct = a.own_splits + a.prefix_splits == 1;
-  if (key0 >= key_end && !(direct && key0 == 0)) return;
+  if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(beside);
+  const int n_tiles = (key_end - key0 + kTile - 1) / kTile;
+
+  // Offsets of a tile's rows, two tiles ahead of their use; -1: no such key.
+  auto look_up = [&](int i) {
+    if (threadIdx.x >= kTile || i >= n_tiles) return;
+    const int at = key0 + i * kTile + threadIdx.x;
+    int64_t ko = -1, vo = -1;
+    if (at < key_end) {
+      int r;
+      const int64_t page = paged::key_page(a, prefix, b, at, r);
+      if (page >= 0) {
+        ko = page * a.k_page + r * a.k_row + head * a.k_head;
+        vo = page * a.v_page + r * a.v_row + head * a.v_head;
+      }
+    }
+    k_at[i % 3][threadIdx.x] = ko;
+    v_at[i % 3][threadIdx.x] = vo;
+  };
+  const int per_row = dp / V;
+  auto load = [&](int i) {
+    if (i >= n_tiles) return;
+    float *ks = tiles + (i & 1) * stage_floats, *vs = ks + kTile * ldk;
+    for (int p = threadIdx.x; p < kTile * per_row; p += kThreads) {
+      const int r = p / per_row, c = (p - r * per_row) * V;
+      const int64_t ko = k_at[i % 3][r], vo = v_at[i % 3][r];
+      const T *kx = static_cast<const T *>(a.k) + ko + c, *vx = static_cast<const T *>(a.v) + vo + c;
+      if (kAsync) {
+        if (ko >= 0) {
+          copy16(ks + r * ldk + c, kx);
+          copy16(vs + r * dp + c, vx);
+        } else {
+          *reinterpret_cast<float4 *>(ks + r * ldk + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          *reinterpret_cast<float4 *>(vs + r * dp + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      } else {
+        serve::Pack<T, V> kp = {}, vp = {};
+        if (ko >= 0 && c < a.d) {
+          kp = *reinterpret_cast<const serve::Pack<T, V> *>(kx);
+          vp = *reinterpret_cast<const serve::Pack<T, V> *>(vx);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          ks[r * ldk + c + e] = serve::to_f32(kp.v[e]);
+          vs[r * dp + c + e] = serve::to_f32(vp.v[e]);
+        }
+      }
+    }
+  };
+  look_up(0);
+  look_up(1);
 
   // this block's queries, FP32, times log2(e) / scale
   for (int i = threadIdx.x; i < R * dp; i += kThreads) {
@@ -80,38 +138,17 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const __grid_const
 #pragma unroll
     for (int c = 0; c < DV; ++c) o[i][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
+  __syncthreads();
+  load(0);
+  asm volatile("cp.async.commit_group;" ::: "memory");
 
-  for (int key = key0; key < key_end; key += kTile) {
-    __syncthreads();  // the last tile's readers are done (and qs is written)
-    if (threadIdx.x < kTile) {
-      const int at = key + threadIdx.x;
-      int64_t ko = -1, vo = -1;
-      if (at < key_end) {
-        int r;
-        const int64_t page = paged::key_page(a, prefix, b, at, r);
-        if (page >= 0) {
-          ko = page * a.k_page + r * a.k_row + head * a.k_head;
-          vo = page * a.v_page + r * a.v_row + head * a.v_head;
-        }
-      }
-      k_at[threadIdx.x] = ko;
-      v_at[threadIdx.x] = vo;
-    }
-    __syncthreads();
-    const int per_row = dp / V;
-    for (int i = threadIdx.x; i < kTile * per_row; i += kThreads) {
-      const int r = i / per_row, c = (i % per_row) * V;
-      serve::Pack<T, V> kx = {}, vx = {};
-      if (k_at[r] >= 0 && c < a.d) {
-        kx = *reinterpret_cast<const serve::Pack<T, V> *>(static_cast<const T *>(a.k) + k_at[r] + c);
-        vx = *reinterpret_cast<const serve::Pack<T, V> *>(static_cast<const T *>(a.v) + v_at[r] + c);
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        ks[r * ldk + c + e] = serve::to_f32(kx.v[e]);
-        vs[r * dp + c + e] = serve::to_f32(vx.v[e]);
-      }
-    }
+  for (int tile = 0; tile < n_tiles; ++tile) {
+    const int key = key0 + tile * kTile;
+    const float *ks = tiles + (tile & 1) * stage_floats, *vs = ks + kTile * ldk;
+    load(tile + 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    look_up(tile + 2);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
 
     float p[RW];
@@ -127,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const __grid_const
           acc[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, acc[i]))));
         }
       }
-      const bool there = k_at[lane] >= 0;
+      const bool there = k_at[tile % 3][lane] >= 0;
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
         const float sc = there && key + lane < limit[i] ? acc[i] : -INFINITY;
@@ -168,6 +205,7 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const __grid_const
         }
       }
     }
+    __syncthreads();  // the stage, and its offsets, may be written again
   }
 
 #pragma unroll
@@ -199,46 +237,113 @@ __global__ void __launch_bounds__(kThreads) paged_rows_kernel(const __grid_const
       }
     }
   }
+  paged::part_end(beside);
 }
 
-// Joins a row's parts: one warp a row (token, query head), lanes over the dims,
-// parts in order, so the result does not depend on which part ended first.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_constant__ Args a) {
+// Joins a row's parts, in an order that does not depend on which part ended
+// first.  A row (token, query head) is one warp's, or, SHARED, a block's, whose
+// warps take every fourth part: many parts mean few rows, and a warp alone
+// then waits for one part's load after the other (36 parts of 32 rows: 41 us
+// against 4).  Lanes over the dims, V at a time.
+template <typename T, int V, bool SHARED>
+__global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_constant__ Args a, bool vec_out) {
+  constexpr int kPieces = B2K_MAX_HEAD_DIM / 32 / V;  // of a lane
+  constexpr int kStep = SHARED ? kWarps : 1;          // parts from one of a warp's to the next
+  constexpr int kAhead = 4;
+  __shared__ float sums[SHARED ? kWarps : 1][SHARED ? B2K_MAX_HEAD_DIM : 1];
   grid_dependency_wait();
   grid_dependents_launch();
-  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_heads = a.kv_heads * a.group;
   const paged::Sequence s = paged::sequence(a, blockIdx.x);
   const int64_t stride = a.tokens * q_heads;
-  for (int64_t row = (int64_t)blockIdx.y * kWarps + (threadIdx.x >> 5); row < (int64_t)s.n * q_heads;
-       row += (int64_t)gridDim.y * kWarps) {
+  const int64_t step = (int64_t)gridDim.y * (SHARED ? 1 : kWarps);
+  for (int64_t row = (int64_t)blockIdx.y * (SHARED ? 1 : kWarps) + (SHARED ? 0 : warp); row < (int64_t)s.n * q_heads;
+       row += step) {
     const int j = (int)(row / q_heads), qh = (int)(row % q_heads);
     const int64_t at = (int64_t)(s.first + j) * q_heads + qh;
     const int own = (paged::own_limit(a, s, j) + a.own_chunk - 1) / a.own_chunk;
     const int parts = own + a.prefix_splits;
     auto slot = [&](int i) { return (int64_t)(i < own ? i : a.own_splits + i - own) * stride + at; };
-    float mx = -INFINITY;
+    float mx = -INFINITY, total = 0.0f;
     for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, a.part_ml[slot(i)].x);
     mx = warp_max(mx);
     const float base = mx == -INFINITY ? 0.0f : mx;
-    float total = 0.0f;
     for (int i = lane; i < parts; i += 32) {
       const float2 ml = a.part_ml[slot(i)];
       total += ml.y * exp2_fast(ml.x - base);
     }
     total = warp_sum(total);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    T *out = static_cast<T *>(a.o) + (int64_t)(s.first + j) * a.o_token + qh * a.o_head;
-    for (int c = lane; c < a.d; c += 32) {
-      float x = 0.0f;
-      for (int i = 0; i < parts; ++i) {
+    float x[kPieces][V];
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[c][e] = 0.0f;
+    for (int i0 = SHARED ? warp : 0; i0 < parts; i0 += kAhead * kStep) {
+      float w[kAhead];
+      serve::Pack<float, V> v[kAhead][kPieces];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kStep;
+        w[u] = 0.0f;
+        if (i >= parts) continue;
         const int64_t p = slot(i);
-        x = fmaf(a.part_o[p * a.d + c], exp2_fast(a.part_ml[p].x - base), x);
+        w[u] = exp2_fast(a.part_ml[p].x - base);
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c)
+          if ((c * 32 + lane) * V < a.d)
+            v[u][c] = *reinterpret_cast<const serve::Pack<float, V> *>(a.part_o + p * a.d + (c * 32 + lane) * V);
       }
-      out[c] = serve::from_f32<T>(x * inv);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i0 + u * kStep < parts)
+#pragma unroll
+          for (int c = 0; c < kPieces; ++c)
+            if ((c * 32 + lane) * V < a.d)
+#pragma unroll
+              for (int e = 0; e < V; ++e) x[c][e] = fmaf(v[u][c].v[e], w[u], x[c][e]);
+    }
+    if (SHARED) {
+      __syncthreads();  // the last row's readers are done
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sums[warp][(c * 32 + lane) * V + e] = x[c][e];
+      __syncthreads();
+      T *out = static_cast<T *>(a.o) + (int64_t)(s.first + j) * a.o_token + qh * a.o_head;
+      for (int c = threadIdx.x; c < a.d; c += kThreads)
+        out[c] = serve::from_f32<T>(((sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c])) * inv);
+    } else {
+      T *out = static_cast<T *>(a.o) + (int64_t)(s.first + j) * a.o_token + qh * a.o_head;
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const int col = (c * 32 + lane) * V;
+        if (col >= a.d) continue;
+        serve::Pack<T, V> y;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y.v[e] = serve::from_f32<T>(x[c][e] * inv);
+        if (vec_out) {
+          *reinterpret_cast<serve::Pack<T, V> *>(out + col) = y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) out[col + e] = y.v[e];
+        }
+      }
     }
   }
+}
+
+template <typename T>
+cudaError_t merge(const Args &a, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
+  const bool shared = a.own_splits + a.prefix_splits > 8;
+  const int64_t blocks = shared ? rows : (rows + kWarps - 1) / kWarps;
+  const dim3 grid(a.sequences, (unsigned)std::min<int64_t>(blocks, 65535));
+  const bool vec_out = serve::vec_ok(a.o, a.o_token, a.o_head, 0, sizeof(T), 4 * sizeof(T));
+  auto kernel = a.d % 4 == 0 ? (shared ? paged_merge_kernel<T, 4, true> : paged_merge_kernel<T, 4, false>)
+                             : (shared ? paged_merge_kernel<T, 1, true> : paged_merge_kernel<T, 1, false>);
+  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), 0, s, a, vec_out);
 }
 
 // The kernel of a part: paged_rows_kernel, warp MMAs (paged_mma.cu) or the
@@ -280,10 +385,10 @@ int block_rows(Path path, int d, int64_t rows) {
 
 // Splits of `keys` keys so that `units` independent row blocks become `want`
 // blocks, each at least `least` keys long.
-void split_keys(int64_t keys, int64_t units, int64_t want, int least, int &splits, int &chunk) {
+void split_keys(int64_t keys, int64_t units, int64_t want, int least, int tile, int &splits, int &chunk) {
   want = std::max<int64_t>(1, want / std::max<int64_t>(1, units));
   int64_t c = std::max<int64_t>(least, (keys + want - 1) / want);
-  c = (c + 127) / 128 * 128;  // whole tiles of every kernel
+  c = (c + tile - 1) / tile * tile;
   splits = (int)std::max<int64_t>(1, (keys + c - 1) / c);
   chunk = (int)c;
 }
@@ -299,17 +404,21 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   p.joined = b.prefix_len > 0 && own >= 128;
   // blocks that the GPU holds at once, and keys that make a block worth its start
   auto wave = [&](Path path) { return (int64_t)sms * (path == kPlain ? 6 : path == kUmma || c.d > 128 ? 1 : 2); };
-  auto least = [](Path path) { return path == kPlain ? 128 : path == kMma ? 256 : 512; };
+  auto least = [](Path path) { return path == kPlain ? 64 : path == kMma ? 256 : 128; };
+  auto tile = [](Path path) { return path == kUmma ? 128 : 64; };  // keys of a block's step
   // the tensor-memory kernel's tiles end with the prefix
   p.joined_keys = !p.joined ? 0 : p.own_path == kUmma ? (b.prefix_len + 127) / 128 * 128 : b.prefix_len;
+  // Sequences of different lengths leave a single wave's blocks unequal: several
+  // waves of shorter ones even that out.
+  const int64_t own_wave = wave(p.own_path) * (b.sequences > 1 && p.own_path != kUmma ? 4 : 1);
   split_keys((int64_t)b.max_len + p.joined_keys,
-             (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, wave(p.own_path), least(p.own_path),
-             p.own_splits, p.own_chunk);
+             (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, own_wave, least(p.own_path),
+             tile(p.own_path), p.own_splits, p.own_chunk);
   if (b.prefix_len > 0 && !p.joined) {
     p.prefix_path = pick_path(tensor, c.d, prefix);
     p.prefix_rows = block_rows(p.prefix_path, c.d, prefix);
     split_keys(b.prefix_len, (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads, wave(p.prefix_path),
-               least(p.prefix_path), p.prefix_splits, p.prefix_chunk);
+               least(p.prefix_path), tile(p.prefix_path), p.prefix_splits, p.prefix_chunk);
   }
   const size_t slots = (size_t)p.own_splits + p.prefix_splits;
   if (slots > 1) p.bytes = ml_bytes(slots, b.tokens, q_heads) + slots * (size_t)b.tokens * q_heads * c.d * sizeof(float);
@@ -317,20 +426,20 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
 }
 
 template <typename T, int RW, int DV>
-int launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, dim3 grid, int row_blocks, cudaStream_t s) {
+int launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, bool beside, dim3 grid, int row_blocks, cudaStream_t s) {
   const int dp = (a.d + 3) / 4 * 4;
-  const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + kTile * (dp + 4) + kTile * dp);
+  const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + 2 * kTile * (2 * dp + 4));
   constexpr int kFull = 16 / sizeof(T);
   auto kernel = vec ? paged_rows_kernel<T, RW, DV, kFull> : paged_rows_kernel<T, RW, DV, 1>;
-  constexpr int most = sizeof(float) * (RW * kWarps * 128 * DV + kTile * (128 * DV + 4) + kTile * 128 * DV);
+  constexpr int most = sizeof(float) * (RW * kWarps * 128 * DV + 2 * kTile * (2 * 128 * DV + 4));
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
   if (err == cudaSuccess)
-    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), smem, s, a, prefix, row_blocks);
+    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), smem, s, a, prefix, row_blocks, beside);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }
 
 template <typename T>
-int rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, cudaStream_t s) {
+int rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, bool beside, cudaStream_t s) {
   const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
   const int rw = block_rows / kWarps;
   const int row_blocks = (int)((rows + 4 * rw - 1) / (4 * rw));
@@ -339,13 +448,13 @@ int rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, cudaStre
   const bool vec = a.d % (16 / (int)size) == 0 && serve::vec_ok(a.k, a.k_page, a.k_row, a.k_head, size, 16) &&
                    serve::vec_ok(a.v, a.v_page, a.v_row, a.v_head, size, 16);
   if (a.d <= 128) {
-    if (rw == 1) return launch_rows<T, 1, 1>(ctx, a, prefix, vec, grid, row_blocks, s);
-    if (rw == 2) return launch_rows<T, 2, 1>(ctx, a, prefix, vec, grid, row_blocks, s);
-    return launch_rows<T, 8, 1>(ctx, a, prefix, vec, grid, row_blocks, s);
+    if (rw == 1) return launch_rows<T, 1, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+    if (rw == 2) return launch_rows<T, 2, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+    return launch_rows<T, 8, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
   }
-  if (rw == 1) return launch_rows<T, 1, 2>(ctx, a, prefix, vec, grid, row_blocks, s);
-  if (rw == 2) return launch_rows<T, 2, 2>(ctx, a, prefix, vec, grid, row_blocks, s);
-  return launch_rows<T, 8, 2>(ctx, a, prefix, vec, grid, row_blocks, s);
+  if (rw == 1) return launch_rows<T, 1, 2>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+  if (rw == 2) return launch_rows<T, 2, 2>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+  return launch_rows<T, 8, 2>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
 }
 
 template <typename T>
@@ -353,11 +462,12 @@ int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t 
   int launches = 1, status = B2K_OK;
   const bool prefix = a.prefix_splits > 0;
   if (p.own_path == kMma && (!prefix || (p.prefix_path == kMma && p.prefix_rows == p.own_rows))) {
-    status = paged::mma_parts(ctx, a, dtype, prefix, true, p.own_rows, s);
+    status = paged::mma_parts(ctx, a, dtype, prefix, true, p.own_rows, false, s);
   } else {
     auto part = [&](bool pre, Path path, int rows) {
-      return path == kPlain ? rows_part<T>(ctx, a, pre, rows, s)
-             : path == kMma ? paged::mma_parts(ctx, a, dtype, pre, !pre, rows, s)
+      const bool beside = !pre && prefix;
+      return path == kPlain ? rows_part<T>(ctx, a, pre, rows, beside, s)
+             : path == kMma ? paged::mma_parts(ctx, a, dtype, pre, !pre, rows, beside, s)
                             : paged::umma_part(ctx, a, dtype, pre, s);
     };
     if (prefix) {
@@ -368,9 +478,7 @@ int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t 
   }
   if (status != B2K_OK) return status;
   if (a.own_splits + a.prefix_splits > 1) {
-    const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
-    const dim3 grid(a.sequences, (unsigned)std::min<int64_t>((rows + kWarps - 1) / kWarps, 65535));
-    const cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), paged_merge_kernel<T>, grid, dim3(kThreads), 0, s, a);
+    const cudaError_t err = merge<T>(a, s);
     if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "paged_attention launch");
     ++launches;
   }

@@ -90,10 +90,25 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
   return -1;
 }
 
+// The own part runs beside the prefix part, the kernel before it in the stream,
+// whose results it does not read.  Every block of the prefix part lets the
+// next kernel start only behind its own wait for what precedes the call, so a
+// block of the own part that has started needs no wait to read queries and
+// cache.  It waits at its end instead, so that the merge, which waits for the
+// own part, has both.
+__device__ __forceinline__ void part_begin(bool beside) {
+  if (!beside) grid_dependency_wait();
+  grid_dependents_launch();
+}
+__device__ __forceinline__ void part_end(bool beside) {
+  if (beside) grid_dependency_wait();
+}
+
 // paged_mma.cu: rows of a block (16 or 32) for `rows` rows of one cache head, and
 // the launch of the prefix part, the sequences' own parts or both.
 int mma_rows(int d, int64_t rows);
-int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s);
+int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, bool beside,
+              cudaStream_t s);
 
 // paged_umma.cu: rows of a block, and the launch of one part.
 constexpr int kUmmaRows = 256;

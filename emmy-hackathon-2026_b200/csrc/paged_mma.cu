@@ -100,6 +100,7 @@ struct Type<__nv_bfloat16> {
 struct Grid {
   unsigned prefix_blocks;  // blocks of the prefix part in this launch (0: none)
   int prefix_row_blocks, own_row_blocks;
+  bool beside;  // the prefix part is the kernel before: run beside it (paged.cuh, part_begin)
 };
 
 template <typename T, int DP, int MT>
@@ -113,8 +114,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
   __shared__ float2 ml[kWarps][kRows];
   __shared__ uint32_t there_s[kWarps][kStages];
   static_assert(kWarps * kRows * kLdo * 4 <= smem_bytes<DP>(), "the sums fit where the keys were");
-  grid_dependency_wait();
-  grid_dependents_launch();
+  paged::part_begin(grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool prefix = blockIdx.x < grid.prefix_blocks;
@@ -131,13 +131,13 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
   if (prefix) s.n = paged::used_tokens(a);
   else s = paged::sequence(a, b);
   const int rows = s.n * a.group, row0 = block * kRows;
-  if (row0 >= rows) return;
+  if (row0 >= rows) return paged::part_end(grid.beside);
   const int last_token = (min(row0 + kRows, rows) - 1) / a.group;
   const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
   const int key0 = split * chunk;
   const int key_end = min(prefix ? a.prefix_len : paged::own_limit(a, s, last_token), key0 + chunk);
   const bool direct = a.own_splits + a.prefix_splits == 1;
-  if (key0 >= key_end && !(direct && key0 == 0)) return;
+  if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(grid.beside);
   const int q_heads = a.kv_heads * a.group;
 
   // Queries as A fragments, straight from global memory: thread (g, t) holds
@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
         *reinterpret_cast<float2 *>(a.part_o + part * a.d + col) = v;
     }
   }
+  paged::part_end(grid.beside);
 }
 
 template <typename T, int DP, int MT>
@@ -414,8 +415,10 @@ namespace paged {
 
 int mma_rows(int d, int64_t rows) { return d <= 128 && rows > 16 ? 32 : 16; }
 
-int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, cudaStream_t s) {
+int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, bool beside,
+              cudaStream_t s) {
   Grid g = {};
+  g.beside = beside;
   g.prefix_row_blocks = (int)((a.tokens * a.group + rows - 1) / rows);
   g.own_row_blocks = (int)(((int64_t)a.max_new * a.group + rows - 1) / rows);
   const int64_t prefix = with_prefix ? (int64_t)g.prefix_row_blocks * a.kv_heads * a.prefix_splits : 0;

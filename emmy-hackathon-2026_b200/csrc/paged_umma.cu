@@ -15,12 +15,15 @@
 //               of a page (or 128 rows of one); pages outside the cache are
 //               outside the tensor map and arrive as zeros
 //   warp 10     MMA issuer: S_j = Q K_j^T (128 x 128), then O += P_j V_j with P
-//               from tensor memory and V as it lies (N-major)
-//   warp 11     (pages that no box fits: sizes that neither divide 128 nor are a
-//               multiple of it, or below 8) passes on what has landed: there, warps 8
-//               and 9 copy row by row, 16 bytes a lane, and the tensor core sees
-//               such copies behind a proxy fence alone.  Those copies' issue
-//               bounds the kernel then: 7000 cycles a pair of tiles
+//               from tensor memory and V as it lies (N-major), in the order O_A,
+//               S_A, O_B, S_B: while one tile has the tensor core the other is in
+//               its softmax (an issuer for each tile lets the two fall into step,
+//               and each then waits for both: 3 to 5 % slower)
+//   (pages that no box fits -- sizes that neither divide 128 nor are a multiple of
+//               it, or below 8 -- are copied row by row by warps 8 and 9, 16 bytes a
+//               lane; warp 11 passes on what has landed, since the tensor core sees
+//               such copies behind a proxy fence alone.  Those copies' issue bounds the kernel then: 7000
+//               cycles a pair of tiles)
 //
 // Mathematics: O stays in tensor memory over all tiles.  The exponents' base is
 // the running maximum of the time when it was last moved: it moves only when a
@@ -73,6 +76,31 @@ constexpr uint32_t kColS = 0, kColO = 256;  // S (then P) of tile A, B: 128 each
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
   return r;
 }
 
@@ -168,12 +196,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::mbar_init(&empty[i], 1);
     }
     sm100::mbar_init(&q_full, kSoftmaxWarps);
+    sm100::mbar_init(&drain, 1);
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&s_full[i], 1);
       sm100::mbar_init(&p_full[i], 4);
       sm100::mbar_init(&o_full[i], 1);
     }
-    sm100::mbar_init(&drain, 1);
     sm100::fence_barrier_init();
   }
   if (warp == kSoftmaxWarps + kLoadWarps) sm100::tmem_alloc(&tmem_slot, 512);
@@ -372,10 +400,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_ts(d, p + kk * 8, desc_mn(v + kk * 2048, kHalf, 1024), id_o, j != 0 || kk != 0);
       if (last) sm100::mma_commit(&o_full[x]);
     };
+    auto tiles_of = [&](int x) { return x == 0 ? tiles_a : tiles_b; };
     if (ok && tiles > 0) {
       wait_item(0);
-      if (ok && tiles_a > 0) issue_s(0, 0);
-      if (ok && tiles_b > 0) issue_s(1, 0);
+      for (int x = 0; ok && x < 2; ++x)
+        if (tiles_of(x) > 0) issue_s(x, 0);
       if (ok) sm100::mma_commit(&empty[0]);
       for (int j = 0; ok && j < tiles; ++j) {
         wait_item(2 * j + 1);
@@ -390,12 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           sm100::fence_proxy_async_smem();
           __syncwarp();
         }
-        if (ok && j < tiles_a) issue_o(0, j, j + 1 == tiles_a);
-        if (ok && j + 1 < tiles) wait_item(2 * j + 2);
-        if (ok && j + 1 < tiles_a) issue_s(0, j + 1);
-        if (ok && j < tiles_b) issue_o(1, j, j + 1 == tiles_b);
-        if (ok) sm100::mma_commit(&empty[(2 * j + 1) % kStages]);
-        if (ok && j + 1 < tiles_b) issue_s(1, j + 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (ok && j < tiles_of(x)) issue_o(x, j, j + 1 == tiles_of(x));
+          if (ok && x == 1) sm100::mma_commit(&empty[(2 * j + 1) % kStages]);
+          if (ok && x == 0 && j + 1 < tiles) wait_item(2 * j + 2);
+          if (ok && j + 1 < tiles_of(x)) issue_s(x, j + 1);
+        }
         if (ok && j + 1 < tiles) sm100::mma_commit(&empty[(2 * j + 2) % kStages]);
       }
     }
@@ -459,9 +489,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kKeys; i += 4)
+      for (int i = 0; i < kKeys; i += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(sr[i + e]));
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + 2 * e]), __uint_as_float(sr[i + 2 * e + 1]));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c - Type<T>::kLift;
       if (__any_sync(0xffffffffu, top > base + Type<T>::kSlack || (base == -INFINITY && top > base))) {
         const float moved = fmaxf(base, top);
@@ -482,21 +512,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float from = base == -INFINITY ? 0.0f : base;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint64_t sum[2] = {0, 0};
+      const uint64_t c2 = pair(c, c), from2 = pair(-from, -from);
       uint32_t pk[32];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
-          const float p0 = exp2_fast(fmaf(__uint_as_float(sr[64 * h + i]), c, -from));
-          const float p1 = exp2_fast(fmaf(__uint_as_float(sr[64 * h + i + 1]), c, -from));
-          sum[i & 2] += p0;
-          sum[(i & 2) + 1] += p1;
+          float p0, p1;
+          unpair(fma2(pair(__uint_as_float(sr[64 * h + i]), __uint_as_float(sr[64 * h + i + 1])), c2, from2), p0, p1);
+          p0 = exp2_fast(p0);
+          p1 = exp2_fast(p1);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair(p0, p1));
           pk[i / 2] = Type<T>::pack(p0, p1);
         }
         sm100::tmem_st_32x32b_x32(s_at + 32 * h, pk);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float l0, l1;
+      unpair(add2(sum[0], sum[1]), l0, l1);
+      l += l0 + l1;
       sm100::tmem_st_wait();
       sm100::tc_fence_before();
       __syncwarp();

@@ -24,7 +24,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;       // heads a thread has in flight
+constexpr int kAhead = 3;       // heads a thread has in flight
 constexpr int kMaxTokens = 4;   // tokens of a block
 constexpr int kMaxPairs = B2K_ROPE_MAX_PAIRS;
 
@@ -57,7 +57,7 @@ struct RotaryArgs {
 };
 
 template <typename T, int V, bool PAGED>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   using P = serve::Pack<T, V>;
   __shared__ float cs[kMaxTokens][kMaxPairs], sn[kMaxTokens][kMaxPairs];
   grid_dependency_wait();
@@ -221,10 +221,14 @@ int run(b2k_ctx *ctx, RotaryArgs &a, int count, int32_t dtype, int64_t tokens_ea
   const size_t size = serve::type_size(dtype);
   const int v = pick_vector(a, count, size);
   a.items = a.interleaved ? (a.d + 2 * v - 1) / (2 * v) : a.rot / 2 / v + (a.d - a.rot + 2 * v - 1) / (2 * v);
-  // Four tokens share a block's set-up once there are blocks enough for the
-  // GPU without that; fewer tokens spread one to a block.
+  // As many tokens to a block as leave each thread one batch of kAhead heads
+  // (a second one would wait for memory again), once there are blocks enough
+  // for the GPU without that; fewer tokens spread one to a block.
   const int64_t all = PAGED ? tokens_each * sequences : tokens_each;
-  a.tokens_per_block = all >= (int64_t)ctx->sm_count * 16 ? std::min(kMaxTokens, kThreads / a.items) : 1;
+  a.tokens_per_block = 1;
+  if (all >= (int64_t)ctx->sm_count * 16)
+    while (a.tokens_per_block < kMaxTokens && kThreads / a.items / (2 * a.tokens_per_block) * kAhead >= a.heads)
+      a.tokens_per_block *= 2;
   if (PAGED && tokens_each < a.tokens_per_block) a.tokens_per_block = 1;
   const int64_t chunks = (tokens_each + a.tokens_per_block - 1) / a.tokens_per_block;
   const dim3 grid = PAGED ? dim3(sequences, (unsigned)std::min<int64_t>(chunks, 65535))

@@ -12,10 +12,12 @@
 // one launch: a cluster of eight CTAs takes a sequence, each an eighth of the
 // row, each warp a contiguous run of that.  The runs' sums meet through
 // distributed shared memory, every CTA finds the run that holds the
-// threshold, and the one warp that owns it reads it again (from L2) in order.
-// Few sequences then still use eight SMs each, and nothing is kept in global
-// memory between the two passes.
+// threshold, and the CTA that owns it reads it again (from L2) in order, all
+// its threads side by side.  Few sequences then still use eight SMs each, and
+// nothing is kept in global memory between the two passes.
 #include <cooperative_groups.h>
+
+#include <limits.h>
 
 #include <algorithm>
 
@@ -24,10 +26,8 @@
 namespace {
 
 constexpr int kCluster = 8;
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kAhead = 8;   // elements a lane has in flight in the first pass
-constexpr int kRun = 8;     // consecutive elements of a lane in the second
+constexpr int kRun = 4;     // consecutive elements of a thread in the second
 
 struct VerifyArgs {
   b2k_drafts d;
@@ -56,11 +56,14 @@ struct Rest {
   }
 };
 
+template <int kThreads>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
+  constexpr int kWarps = kThreads / 32;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ double run_sum[kWarps], slice_sum;
+  __shared__ double run_sum[kWarps], scan_sum[kWarps], slice_sum;
   __shared__ int taken_s;
+  __shared__ long long first_hit, last_held;
   grid_dependency_wait();
   grid_dependents_launch();
 
@@ -104,7 +107,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
   const int64_t run = (d.vocab + kCluster * kWarps - 1) / (kCluster * kWarps);
   const int64_t lo = min(d.vocab, (rank * kWarps + warp) * run), hi = min(d.vocab, lo + run);
 
-  int64_t token = -1;
+  int64_t token = -1;   // of the CTA that owns the draw
   bool owner = false;
   for (int pass = 0; pass < 2; ++pass) {  // the second only where the rest is zero everywhere
     double sum = 0.0;
@@ -168,49 +171,58 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
         }
         at += run_sum[w];
       }
-      if (run_at == warp) {
-        owner = true;
-        double base = run_start;
-        for (int64_t i0 = lo; i0 < hi; i0 += 32 * kRun) {
-          double v[kRun], mine = 0.0;
-          const int64_t i = i0 + lane * kRun;
-#pragma unroll
-          for (int u = 0; u < kRun; ++u) {
-            v[u] = i + u < hi ? rest.value(i + u) : 0.0;
-            mine += v[u];
-          }
-          double upto = mine;  // inclusive scan over the lanes
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double other = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += other;
-          }
-          double c = base + (upto - mine);
-          int64_t hit = -1, last = -1;
-#pragma unroll
-          for (int u = 0; u < kRun; ++u) {
-            c += v[u];
-            if (v[u] > 0.0) {
-              last = i + u;
-              if (hit < 0 && c > threshold) hit = i + u;
-            }
-          }
-          const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0);
-          if (hits) {
-            token = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
-            break;
-          }
-          const unsigned lasts = __ballot_sync(0xffffffffu, last >= 0);
-          if (lasts) token = __shfl_sync(0xffffffffu, last, 31 - __clz(lasts));
-          base += __shfl_sync(0xffffffffu, upto, 31);
-        }
+      // run_at is one for the whole CTA: its elements in order, kRun a thread,
+      // kRun * kThreads at a time
+      owner = true;
+      const int64_t run_lo = min(d.vocab, (rank * kWarps + run_at) * run), run_hi = min(d.vocab, run_lo + run);
+      if (threadIdx.x == 0) {
+        first_hit = LLONG_MAX;
+        last_held = -1;
       }
+      double base = run_start;
+      for (int64_t i0 = run_lo; i0 < run_hi; i0 += kRun * kThreads) {
+        double v[kRun], mine = 0.0;
+        const int64_t i = i0 + threadIdx.x * kRun;
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) {
+          v[u] = i + u < run_hi ? rest.value(i + u) : 0.0;
+          mine += v[u];
+        }
+        double upto = mine;  // inclusive scan over the lanes, then over the warps
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double other = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += other;
+        }
+        if (lane == 31) scan_sum[warp] = upto;
+        __syncthreads();
+        double c = base + (upto - mine), whole = base;
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) c += scan_sum[w];
+          whole += scan_sum[w];
+        }
+        int64_t hit = -1, last = -1;
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) {
+          c += v[u];
+          if (v[u] > 0.0) {
+            last = i + u;
+            if (hit < 0 && c > threshold) hit = i + u;
+          }
+        }
+        if (hit >= 0) atomicMin(&first_hit, (long long)hit);
+        if (last >= 0) atomicMax(&last_held, (long long)last);
+        base = whole;
+        __syncthreads();
+        if (first_hit != LLONG_MAX) break;
+      }
+      token = first_hit != LLONG_MAX ? first_hit : last_held;
     } else if (slice_at < 0) {
-      owner = rank == 0 && warp == 0;  // nothing above zero: token -1
+      owner = rank == 0;  // nothing above zero: token -1
     }
     break;
   }
-  if (owner && lane == 0) a.tokens[b * (d.drafts + 1) + taken] = (int32_t)token;
+  if (owner && threadIdx.x == 0) a.tokens[b * (d.drafts + 1) + taken] = (int32_t)token;
   if (rank == 0 && warp == 1) {
     if (lane == 0) a.accepted[b] = taken;
     for (int i = lane; i <= d.drafts; i += 32)
@@ -235,8 +247,12 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   cudaStream_t s = (cudaStream_t)stream;
   b2k::PhaseTimer timer(ctx, B2K_PHASE_VERIFY, s);
   const VerifyArgs a{*d, accepted, tokens};
-  cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), verify_kernel, dim3((unsigned)(d->batch * kCluster)),
-                                       dim3(kThreads), 0, s, a);
+  // A few sequences leave an SM to each CTA, which then wants many loads in
+  // flight; a batch wants all its CTAs resident at once (64 sequences of
+  // 131071: 33 us with 512 threads, 1.7 waves, against 256).
+  const bool few = d->batch * kCluster <= ctx->sm_count;
+  cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), few ? verify_kernel<1024> : verify_kernel<256>,
+                                       dim3((unsigned)(d->batch * kCluster)), dim3(few ? 1024 : 256), 0, s, a);
   if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "verify_drafts launch");
   return b2k::check_launch(ctx, "verify_drafts launch");
 }
