@@ -188,54 +188,71 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
   const T *kc = static_cast<const T *>(a.k) + (int64_t)head * a.k_head;
   const T *vc = static_cast<const T *>(a.v) + (int64_t)head * a.v_head;
   auto tile_key = [&](int i) { return key0 + (warp + kWarps * i) * kTile; };
+  constexpr int kRowsAtOnce = kChunks >= 32 ? 1 : 32 / kChunks;  // rows of one pass over the lanes
+  constexpr int kPieces = kChunks >= 32 ? kChunks / 32 : 1;
+  constexpr int kPasses = kTile / kRowsAtOnce;
+  const int lane_row = kChunks >= 32 ? 0 : lane / kChunks, lane_chunk = kChunks >= 32 ? lane : lane % kChunks;
+  const bool full_width = a.d == DP;
   auto issue = [&](int i) {
     if (i < mine) {
       const int key = tile_key(i), stage = i % kStages;
-      int64_t ko = 0, vo = 0;  // lane r < 16: offsets of key + r
-      bool on = false;
+      const uint32_t kd = ring + stage * 2 * tile_bytes<DP>(), vd = kd + tile_bytes<DP>();
+      int page = -1, row0 = 0;
       if (whole) {
         if (i % 32 == 0) {
           int row;
           const int k = tile_key(i + lane);
           pages32 = i + lane < mine ? (int)paged::key_page(a, prefix, b, k, row) : -1;
         }
-        const int page = __shfl_sync(0xffffffffu, pages32, i % 32);
+        page = __shfl_sync(0xffffffffu, pages32, i % 32);
         const int own = prefix || !a.joined || key < a.prefix_len ? key : key - a.prefix_len;
-        const int row = own % a.page_size + (lane & 15);
-        on = page >= 0 && key + (lane & 15) < key_end;
-        if (on) {
-          ko = page * a.k_page + row * a.k_row;
-          vo = page * a.v_page + row * a.v_row;
+        row0 = (int)((unsigned)own % (unsigned)a.page_size);
+      }
+      if (whole && page >= 0 && key + kTile <= key_end && full_width) {
+        // a whole tile of one page: the rows follow each other
+        if (lane == 0) there_s[warp][stage] = 0xffffu;
+        const T *kp = kc + (page * a.k_page + (row0 + lane_row) * a.k_row + lane_chunk * 8);
+        const T *vp = vc + (page * a.v_page + (row0 + lane_row) * a.v_row + lane_chunk * 8);
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          const int r = p * kRowsAtOnce + lane_row;
+#pragma unroll
+          for (int e = 0; e < kPieces; ++e) {
+            const uint32_t to = r * DP * 2 + (((lane_chunk + 32 * e) ^ (r & 7)) << 4);
+            copy16(kd + to, kp + 256 * e, true);
+            copy16(vd + to, vp + 256 * e, true);
+          }
+          kp += kRowsAtOnce * a.k_row;
+          vp += kRowsAtOnce * a.v_row;
         }
       } else {
+        int64_t ko = 0, vo = 0;  // lane r < 16: offsets of key + r
+        int row = row0 + (lane & 15);
         const int k = key + (lane & 15);
-        if (k < key_end) {
-          int row;
-          const int64_t page = paged::key_page(a, prefix, b, k, row);
+        bool on = k < key_end;
+        if (on) {
+          if (!whole) page = (int)paged::key_page(a, prefix, b, k, row);
           on = page >= 0;
           if (on) {
             ko = page * a.k_page + row * a.k_row;
             vo = page * a.v_page + row * a.v_row;
           }
         }
-      }
-      const uint32_t there = __ballot_sync(0xffffffffu, on) & 0xffffu;
-      if (lane == 0) there_s[warp][stage] = there;
-      const uint32_t kd = ring + stage * 2 * tile_bytes<DP>(), vd = kd + tile_bytes<DP>();
-      constexpr int kRowsAtOnce = kChunks >= 32 ? 1 : 32 / kChunks;  // rows of one pass over the lanes
-      constexpr int kPieces = kChunks >= 32 ? kChunks / 32 : 1;
+        const uint32_t there = __ballot_sync(0xffffffffu, on) & 0xffffu;
+        if (lane == 0) there_s[warp][stage] = there;
 #pragma unroll
-      for (int p = 0; p < kTile / kRowsAtOnce; ++p) {
-        const int r = p * kRowsAtOnce + (kChunks >= 32 ? 0 : lane / kChunks);
-        const int64_t rk = __shfl_sync(0xffffffffu, ko, r), rv = __shfl_sync(0xffffffffu, vo, r);
-        const bool row_on = (there >> r) & 1u;
+        for (int p = 0; p < kPasses; ++p) {
+          const int r = p * kRowsAtOnce + lane_row;
+          const int64_t rk = __shfl_sync(0xffffffffu, ko, r), rv = __shfl_sync(0xffffffffu, vo, r);
+          const bool row_on = (there >> r) & 1u;
 #pragma unroll
-        for (int e = 0; e < kPieces; ++e) {
-          const int c = (kChunks >= 32 ? lane : lane % kChunks) + 32 * e;
-          const uint32_t to = r * DP * 2 + ((c ^ (r & 7)) << 4);
-          const bool yes = row_on && c * 8 < a.d;
-          copy16(kd + to, kc + (yes ? rk + c * 8 : 0), yes);
-          copy16(vd + to, vc + (yes ? rv + c * 8 : 0), yes);
+          for (int e = 0; e < kPieces; ++e) {
+            const int c = lane_chunk + 32 * e;
+            const uint32_t to = r * DP * 2 + ((c ^ (r & 7)) << 4);
+            const bool yes = row_on && c * 8 < a.d;
+            copy16(kd + to, kc + (yes ? rk + c * 8 : 0), yes);
+            copy16(vd + to, vc + (yes ? rv + c * 8 : 0), yes);
+          }
         }
       }
     }

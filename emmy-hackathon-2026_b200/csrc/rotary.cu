@@ -10,22 +10,24 @@
 // most 2^-25 half turns), at any position: no table of cosines is read, kept
 // or outgrown, and no FP32 product position * f loses the far positions.
 //
-// Bound: HBM (each element read and written once).  A block takes 1 or 4
-// tokens; its cosines and sines are computed once into shared memory while
-// the first heads' loads are in flight, then every thread keeps one place of
-// the head (16 bytes of each half of its pairs) and walks the heads, four
-// loads of two vectors ahead.
+// Bound: HBM (each element read and written once).  A warp takes a token, or
+// some of its heads where tokens are few; nothing in a block waits for another
+// warp.  The lanes share out the token's cosines and sines through shared memory
+// while the first heads' loads are in flight; then every lane keeps one place
+// of the head (16 bytes of each half of its pairs, its cosines in registers)
+// and walks the heads, four loads of two vectors ahead.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "serve.cuh"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 3;       // heads a thread has in flight
-constexpr int kMaxTokens = 4;   // tokens of a block
+constexpr int kWarps = kThreads / 32;
+constexpr int kAhead = 4;       // heads a lane has in flight
 constexpr int kMaxPairs = B2K_ROPE_MAX_PAIRS;
 
 enum Target : int { kLinear = 0, kKeys = 1, kValues = 2 };
@@ -44,8 +46,8 @@ struct RotaryArgs {
   Segment seg[3];
   int heads, d, rot, interleaved;
   float magnitude, sine;  // sine: +magnitude, or -magnitude for the transpose
-  int items;              // places of a head: a thread keeps one
-  int tokens_per_block;
+  int items;              // places of a head: a lane keeps one
+  int warps_per_token;    // 1, 2, 4 or 8
   int64_t tokens;
   const int64_t *positions;  // unpaged
   // paged
@@ -56,94 +58,124 @@ struct RotaryArgs {
   uint64_t turn[kMaxPairs];
 };
 
+// V values from and to T, two at a time where the type has such an instruction.
+template <typename T, int V>
+__device__ __forceinline__ void widen(const serve::Pack<T, V> &p, float (&x)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = serve::to_f32(p.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void narrow(const float (&x)[V], serve::Pack<T, V> &p) {
+  if constexpr (V % 2 == 0 && sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2 *>(&p.v[i]) = __floats2half2_rn(x[i], x[i + 1]);
+      else
+        *reinterpret_cast<__nv_bfloat162 *>(&p.v[i]) = __floats2bfloat162_rn(x[i], x[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.v[i] = serve::from_f32<T>(x[i]);
+  }
+}
+
 template <typename T, int V, bool PAGED>
-__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, V * sizeof(T) == 16 ? 2 : 3) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   using P = serve::Pack<T, V>;
-  __shared__ float cs[kMaxTokens][kMaxPairs], sn[kMaxTokens][kMaxPairs];
+  __shared__ __align__(16) float cs[kWarps][kMaxPairs], sn[kWarps][kMaxPairs];
   grid_dependency_wait();
   grid_dependents_launch();
 
-  const int tpb = a.tokens_per_block;
-  const int slots = kThreads / a.items;  // (token, head) places of the block
-  const int head_step = slots / tpb;
-  const int j = threadIdx.x % a.items, slot = threadIdx.x / a.items;
-  const int t = slot % tpb, h_first = slot / tpb;
-  const bool mine = h_first < head_step;
-  // The two vectors of the head this thread moves: the two halves of V pairs
-  // (half layout, rotated part), or neighbours.
-  int e0, e1;
-  const int half_items = a.interleaved ? 0 : a.rot / 2 / V;
-  if (j < half_items) {
-    e0 = j * V;
-    e1 = e0 + a.rot / 2;
-  } else {
-    e0 = (a.interleaved ? 0 : a.rot) + (j - half_items) * 2 * V;
-    e1 = e0 + V < a.d ? e0 + V : -1;
-  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wpt = a.warps_per_token, tokens_per_block = kWarps / wpt;
   const int pairs = a.rot / 2;
-
-  // tokens of this block: global rows row0 .. row0 + count - 1
-  int64_t row_begin, row_end, first_row = 0, own0 = 0;
+  // rows of this block's sequence (paged) or of the call
+  int64_t row_begin = 0, row_end = a.tokens, own0 = 0;
   if (PAGED) {
     const int b = blockIdx.x;
-    first_row = a.first[b];
-    const int64_t n = (int64_t)a.first[b + 1] - first_row;
+    row_begin = a.first[b];
+    const int64_t n = (int64_t)a.first[b + 1] - row_begin;
     own0 = (int64_t)a.lengths[b] - n;
-    if (first_row < 0 || first_row + n > a.tokens || n > a.max_new) {
+    row_end = row_begin + n;
+    if (row_begin < 0 || row_end > a.tokens || n > a.max_new) {
       if (threadIdx.x == 0) atomicOr(a.err, serve::kErrIndex);
       return;
     }
-    row_begin = first_row;
-    row_end = first_row + n;
-  } else {
-    row_begin = 0;
-    row_end = a.tokens;
   }
+  // A head has at most 32 places for a whole warp to walk several heads at once;
+  // more (single elements) are walked 32 at a time, one head after the other.
+  const int per_warp = a.items <= 32 ? 32 / a.items : 1;
+  const int slot = a.items <= 32 ? lane / a.items : 0, j_first = a.items <= 32 ? lane - slot * a.items : lane;
+  const int head_step = per_warp * wpt, h_first = (warp % wpt) * per_warp + slot;
+  const int half_items = a.interleaved ? 0 : a.rot / 2 / V;
+
   const int64_t chunk0 = PAGED ? blockIdx.y : blockIdx.x, chunk_step = PAGED ? gridDim.y : gridDim.x;
-  for (int64_t row0 = row_begin + chunk0 * tpb; row0 < row_end; row0 += chunk_step * tpb) {
-    const int64_t row = row0 + t;
-    const bool on = mine && row < row_end;
-    P va[kAhead], vb[kAhead];
-    auto segment = [&](int h) { return (h >= a.seg[1].head0) + (h >= a.seg[2].head0); };
-    auto load = [&](int hb) {
+  for (int64_t row = row_begin + chunk0 * tokens_per_block + warp / wpt; row < row_end; row += chunk_step * tokens_per_block) {
+    int64_t page = -1;
+    int page_row = 0;
+    bool turned = false;  // cosines and sines are there
+    for (int j = j_first; j < a.items; j += 32) {
+      const bool on = slot < per_warp;
+      // The two vectors of the head this lane moves: the two halves of V pairs
+      // (half layout, rotated part), or neighbours.
+      int e0, e1;
+      if (j < half_items) {
+        e0 = j * V;
+        e1 = e0 + a.rot / 2;
+      } else {
+        e0 = (a.interleaved ? 0 : a.rot) + (j - half_items) * 2 * V;
+        e1 = e0 + V < a.d ? e0 + V : -1;
+      }
+      P va[kAhead], vb[kAhead];
+      auto segment = [&](int h) { return (h >= a.seg[1].head0) + (h >= a.seg[2].head0); };
+      auto load = [&](int hb) {
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int h = hb + u * head_step;
-        if (!on || h >= a.heads) continue;
-        const Segment &s = a.seg[segment(h)];
-        const T *x = reinterpret_cast<const T *>(s.x + row * s.xt + (h - s.head0) * s.xh);
-        va[u] = *reinterpret_cast<const P *>(x + e0);
-        if (e1 >= 0) vb[u] = *reinterpret_cast<const P *>(x + e1);
+        for (int u = 0; u < kAhead; ++u) {
+          const int h = hb + u * head_step;
+          if (!on || h >= a.heads) continue;
+          const Segment &s = a.seg[segment(h)];
+          const T *x = reinterpret_cast<const T *>(s.x + row * s.xt + (h - s.head0) * s.xh);
+          va[u] = *reinterpret_cast<const P *>(x + e0);
+          if (e1 >= 0) vb[u] = *reinterpret_cast<const P *>(x + e1);
+        }
+      };
+      load(h_first);
+      if (!turned) {
+        const int64_t own = own0 + (row - row_begin);
+        const int64_t pos = PAGED ? a.prefix_len + own : pairs ? a.positions[row] : 0;
+        if (PAGED) {
+          // where this token's keys and values go
+          page = serve::page_of(a.table + blockIdx.x * a.table_stride, a.table_width, a.pages, a.page_size, own);
+          page_row = (int)((uint32_t)own % (uint32_t)a.page_size);
+          if (page < 0) atomicOr(a.err, serve::kErrIndex);
+        }
+        __syncwarp();  // the last token's cosines have been read
+        for (int p = lane; p < pairs; p += 32) {
+          const uint64_t turns = a.turn[p] * (uint64_t)pos;
+          float s, c;
+          sincospif((float)(int32_t)(turns >> 32) * 4.656612873077392578125e-10f, &s, &c);  // 2^-31
+          cs[warp][p] = c * a.magnitude;
+          sn[warp][p] = s * a.sine;
+        }
+        __syncwarp();
+        turned = true;
       }
-    };
-    load(h_first);
-    // where this token's keys and values go
-    int64_t page = -1, page_row = 0;
-    if (PAGED && on) {
-      const int64_t own = own0 + (row - first_row);
-      page = serve::page_of(a.table + blockIdx.x * a.table_stride, a.table_width, a.pages, a.page_size, own);
-      page_row = (uint32_t)own % (uint32_t)a.page_size;
-      if (page < 0) atomicOr(a.err, serve::kErrIndex);
-    }
-    for (int i = threadIdx.x; i < tpb * pairs; i += kThreads) {
-      const int ti = i / pairs, p = i % pairs;
-      if (row0 + ti < row_end) {
-        const int64_t pos = PAGED ? a.prefix_len + own0 + (row0 + ti - first_row) : a.positions[row0 + ti];
-        const uint64_t turns = a.turn[p] * (uint64_t)pos;
-        float s, c;
-        sincospif((float)(int32_t)(turns >> 32) * 4.656612873077392578125e-10f, &s, &c);  // 2^-31
-        cs[ti][p] = c * a.magnitude;
-        sn[ti][p] = s * a.sine;
+      // this lane's V pairs
+      const bool turns = a.interleaved ? j * V < pairs : j < half_items;
+      float c[V], sv[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool in = turns && j * V + i < pairs;
+        c[i] = in ? cs[warp][j * V + i] : 0.0f;
+        sv[i] = in ? sn[warp][j * V + i] : 0.0f;
       }
-    }
-    __syncthreads();
-    if (on) {
       for (int hb = h_first; hb < a.heads; hb += kAhead * head_step) {
         if (hb != h_first) load(hb);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           const int h = hb + u * head_step;
-          if (h >= a.heads) break;
+          if (!on || h >= a.heads) continue;
           const Segment &s = a.seg[segment(h)];
           T *y;
           if (PAGED && s.target != kLinear) {
@@ -152,31 +184,43 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
           } else {
             y = reinterpret_cast<T *>(s.y + row * s.yt + (h - s.head0) * s.yh);
           }
-          if (s.rotate) {
+          if (s.rotate && turns) {
+            float xa[V], xb[V];
             if (a.interleaved) {
-              T r[2 * V];
-#pragma unroll
-              for (int i = 0; i < V; ++i) r[i] = va[u].v[i], r[V + i] = e1 >= 0 ? vb[u].v[i] : va[u].v[i];
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                const int p = j * V + i;
-                if (p < pairs) {
-                  const float c = cs[t][p], sv = sn[t][p];
-                  const float xa = serve::to_f32(r[2 * i]), xb = serve::to_f32(r[2 * i + 1]);
-                  r[2 * i] = serve::from_f32<T>(xa * c - xb * sv);
-                  r[2 * i + 1] = serve::from_f32<T>(xb * c + xa * sv);
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < V; ++i) va[u].v[i] = r[i], vb[u].v[i] = r[V + i];
-            } else if (j < half_items) {
+              // neighbours a, b, a, b ...: V pairs over the two vectors
+              float lo[V], hi[V];
+              widen<T, V>(va[u], lo);
+              widen<T, V>(vb[u], hi);
 #pragma unroll
               for (int i = 0; i < V; ++i) {
-                const float c = cs[t][j * V + i], sv = sn[t][j * V + i];
-                const float xa = serve::to_f32(va[u].v[i]), xb = serve::to_f32(vb[u].v[i]);
-                va[u].v[i] = serve::from_f32<T>(xa * c - xb * sv);
-                vb[u].v[i] = serve::from_f32<T>(xb * c + xa * sv);
+                xa[i] = 2 * i < V ? lo[2 * i % V] : hi[2 * i % V];
+                xb[i] = 2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V];
               }
+            } else {
+              widen<T, V>(va[u], xa);
+              widen<T, V>(vb[u], xb);
+            }
+            float ya[V], yb[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              ya[i] = xa[i] * c[i] - xb[i] * sv[i];
+              yb[i] = xb[i] * c[i] + xa[i] * sv[i];
+            }
+            if (a.interleaved) {
+              // pairs behind the rotated part stay as they were, bit for bit
+              float lo[V], hi[V];
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                const bool in = j * V + i < pairs;
+                const float oa = in ? ya[i] : xa[i], ob = in ? yb[i] : xb[i];
+                (2 * i < V ? lo[2 * i % V] : hi[2 * i % V]) = oa;
+                (2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V]) = ob;
+              }
+              narrow<T, V>(lo, va[u]);
+              narrow<T, V>(hi, vb[u]);
+            } else {
+              narrow<T, V>(ya, va[u]);
+              narrow<T, V>(yb, vb[u]);
             }
           }
           *reinterpret_cast<P *>(y + e0) = va[u];
@@ -184,7 +228,6 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
         }
       }
     }
-    __syncthreads();  // the next tokens' cosines overwrite these
   }
 }
 
@@ -221,16 +264,16 @@ int run(b2k_ctx *ctx, RotaryArgs &a, int count, int32_t dtype, int64_t tokens_ea
   const size_t size = serve::type_size(dtype);
   const int v = pick_vector(a, count, size);
   a.items = a.interleaved ? (a.d + 2 * v - 1) / (2 * v) : a.rot / 2 / v + (a.d - a.rot + 2 * v - 1) / (2 * v);
-  // As many tokens to a block as leave each thread one batch of kAhead heads
-  // (a second one would wait for memory again), once there are blocks enough
-  // for the GPU without that; fewer tokens spread one to a block.
+  // A warp to a token once that fills the GPU (eight blocks' worth of warps an
+  // SM); fewer tokens are shared out, down to four heads' loads a lane.
   const int64_t all = PAGED ? tokens_each * sequences : tokens_each;
-  a.tokens_per_block = 1;
-  if (all >= (int64_t)ctx->sm_count * 16)
-    while (a.tokens_per_block < kMaxTokens && kThreads / a.items / (2 * a.tokens_per_block) * kAhead >= a.heads)
-      a.tokens_per_block *= 2;
-  if (PAGED && tokens_each < a.tokens_per_block) a.tokens_per_block = 1;
-  const int64_t chunks = (tokens_each + a.tokens_per_block - 1) / a.tokens_per_block;
+  const int per_warp = a.items <= 32 ? 32 / a.items : 1;
+  a.warps_per_token = 1;
+  while (a.warps_per_token < kWarps && all * a.warps_per_token < (int64_t)ctx->sm_count * 8 * kWarps &&
+         per_warp * a.warps_per_token < a.heads)
+    a.warps_per_token *= 2;
+  const int tokens_per_block = kWarps / a.warps_per_token;
+  const int64_t chunks = (tokens_each + tokens_per_block - 1) / tokens_per_block;
   const dim3 grid = PAGED ? dim3(sequences, (unsigned)std::min<int64_t>(chunks, 65535))
                           : dim3((unsigned)std::min<int64_t>(chunks, INT32_MAX));
   b2k::PhaseTimer timer(ctx, phase, s);

@@ -40,6 +40,29 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
+// Inclusive sum over the lanes, in a fixed order.
+__device__ __forceinline__ double warp_scan(double v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += other;
+  }
+  return v;
+}
+
+// Of 32 lanes' sums in order: the first whose cumulative sum passes the
+// threshold, or the last that holds anything where rounding leaves none (-1:
+// none does), and the sum before it.
+__device__ __forceinline__ int pick(double v, double start, double threshold, double &before) {
+  const double upto = warp_scan(v);
+  const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && start + upto > threshold);
+  const unsigned held = __ballot_sync(0xffffffffu, v > 0.0);
+  const int at = over ? __ffs(over) - 1 : held ? 31 - __clz(held) : -1;
+  before = start + __shfl_sync(0xffffffffu, upto - v, at < 0 ? 0 : at);
+  return at;
+}
+
 // The rest that the token is drawn from: max(p - q, 0), p where q is not
 // there, and nothing of the rejected draft where that was certain.
 struct Rest {
@@ -126,18 +149,12 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
     sum = warp_sum(sum);
     if (lane == 0) run_sum[warp] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      double s = 0.0;
-      for (int w = 0; w < kWarps; ++w) s += run_sum[w];
-      slice_sum = s;
-    }
+    const double mine_of = lane < kWarps ? run_sum[lane] : 0.0;  // each warp scans the runs' sums for itself
+    const double slice_total = __shfl_sync(0xffffffffu, warp_scan(mine_of), 31);
+    if (threadIdx.x == 0) slice_sum = slice_total;
     cluster.sync();
-    double slice[kCluster], total = 0.0;
-#pragma unroll
-    for (int r = 0; r < kCluster; ++r) {
-      slice[r] = *cluster.map_shared_rank(&slice_sum, r);
-      total += slice[r];
-    }
+    const double slice = lane < kCluster ? *cluster.map_shared_rank(&slice_sum, lane < kCluster ? lane : 0) : 0.0;
+    const double total = __shfl_sync(0xffffffffu, warp_scan(slice), 31);
     cluster.sync();  // every CTA has read: the sums may be written again, or the CTA leave
     if (!(total > 0.0) && pass == 0 && taken < n) {
       rest.q = nullptr;
@@ -147,30 +164,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
     // the slice, then the run in it, whose cumulative sum first passes the
     // threshold; rounding may leave none, then the last one that holds anything
     const double threshold = (double)d.u_sample[b] * total;
-    double before = 0.0, start = 0.0;
-    int slice_at = -1;
-    bool over = false;
-#pragma unroll
-    for (int r = 0; r < kCluster; ++r) {
-      if (!over && slice[r] > 0.0) {
-        slice_at = r;
-        start = before;
-        over = before + slice[r] > threshold;
-      }
-      before += slice[r];
-    }
+    double start, run_start;
+    const int slice_at = pick(slice, 0.0, threshold, start);
     if (slice_at == rank) {
-      int run_at = -1;
-      double at = start, run_start = start;
-      bool found = false;
-      for (int w = 0; w < kWarps; ++w) {
-        if (!found && run_sum[w] > 0.0) {
-          run_at = w;
-          run_start = at;
-          found = at + run_sum[w] > threshold;
-        }
-        at += run_sum[w];
-      }
+      const int run_at = pick(mine_of, start, threshold, run_start);
       // run_at is one for the whole CTA: its elements in order, kRun a thread,
       // kRun * kThreads at a time
       owner = true;
@@ -188,19 +185,12 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
           v[u] = i + u < run_hi ? rest.value(i + u) : 0.0;
           mine += v[u];
         }
-        double upto = mine;  // inclusive scan over the lanes, then over the warps
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double other = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += other;
-        }
+        const double upto = warp_scan(mine);  // over the lanes, then over the warps
         if (lane == 31) scan_sum[warp] = upto;
         __syncthreads();
-        double c = base + (upto - mine), whole = base;
-        for (int w = 0; w < kWarps; ++w) {
-          if (w < warp) c += scan_sum[w];
-          whole += scan_sum[w];
-        }
+        const double warps = lane < kWarps ? scan_sum[lane] : 0.0, warps_upto = warp_scan(warps);
+        double c = base + __shfl_sync(0xffffffffu, warps_upto - warps, warp) + (upto - mine);
+        const double whole = base + __shfl_sync(0xffffffffu, warps_upto, 31);
         int64_t hit = -1, last = -1;
 #pragma unroll
         for (int u = 0; u < kRun; ++u) {
@@ -251,8 +241,8 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   // flight; a batch wants all its CTAs resident at once (64 sequences of
   // 131071: 33 us with 512 threads, 1.7 waves, against 256).
   const bool few = d->batch * kCluster <= ctx->sm_count;
-  cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), few ? verify_kernel<1024> : verify_kernel<256>,
-                                       dim3((unsigned)(d->batch * kCluster)), dim3(few ? 1024 : 256), 0, s, a);
+  cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), few ? verify_kernel<512> : verify_kernel<256>,
+                                       dim3((unsigned)(d->batch * kCluster)), dim3(few ? 512 : 256), 0, s, a);
   if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "verify_drafts launch");
   return b2k::check_launch(ctx, "verify_drafts launch");
 }
