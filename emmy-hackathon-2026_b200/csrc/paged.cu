@@ -242,9 +242,9 @@ __global__ void __launch_bounds__(kThreads)
 
 // Joins a row's parts, in an order that does not depend on which part ended
 // first.  A row (token, query head) is one warp's, or, SHARED, a block's, whose
-// warps take every fourth part: many parts mean few rows, and a warp alone
-// then waits for one part's load after the other (36 parts of 32 rows: 41 us
-// against 4).  Lanes over the dims, V at a time.
+// warps take every fourth part: with many parts and too few rows to fill the
+// GPU, a warp alone waits for one batch of loads after the other (36 parts of
+// 32 rows: 41 us against 4).  Lanes over the dims, V at a time.
 template <typename T, int V, bool SHARED>
 __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_constant__ Args a, bool vec_out) {
   constexpr int kPieces = B2K_MAX_HEAD_DIM / 32 / V;  // of a lane
@@ -335,9 +335,9 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
 }
 
 template <typename T>
-cudaError_t merge(const Args &a, cudaStream_t s) {
+cudaError_t merge(const Args &a, int sms, cudaStream_t s) {
   const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
-  const bool shared = a.own_splits + a.prefix_splits > 8;
+  const bool shared = a.own_splits + a.prefix_splits > 4 && rows * a.sequences < (int64_t)sms * 8;
   const int64_t blocks = shared ? rows : (rows + kWarps - 1) / kWarps;
   const dim3 grid(a.sequences, (unsigned)std::min<int64_t>(blocks, 65535));
   const bool vec_out = serve::vec_ok(a.o, a.o_token, a.o_head, 0, sizeof(T), 4 * sizeof(T));
@@ -404,13 +404,14 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   p.joined = b.prefix_len > 0 && own >= 128;
   // blocks that the GPU holds at once, and keys that make a block worth its start
   auto wave = [&](Path path) { return (int64_t)sms * (path == kPlain ? 6 : path == kUmma || c.d > 128 ? 1 : 2); };
-  auto least = [](Path path) { return path == kPlain ? 64 : path == kMma ? 256 : 128; };
+  auto least = [&](Path path) { return path == kPlain ? 64 : path == kMma ? (c.d <= 64 ? 512 : 256) : 128; };
   auto tile = [](Path path) { return path == kUmma ? 128 : 64; };  // keys of a block's step
   // the tensor-memory kernel's tiles end with the prefix
   p.joined_keys = !p.joined ? 0 : p.own_path == kUmma ? (b.prefix_len + 127) / 128 * 128 : b.prefix_len;
-  // Sequences of different lengths leave a single wave's blocks unequal: several
-  // waves of shorter ones even that out.
-  const int64_t own_wave = wave(p.own_path) * (b.sequences > 1 && p.own_path != kUmma ? 4 : 1);
+  // Sequences of different lengths leave a single wave's blocks unequal: two
+  // waves of shorter ones even that out (33 sequences of 625 to 2500 keys, 20
+  // rows of 64: 38 us with one, 33 with two, 33 to 39 with four).
+  const int64_t own_wave = wave(p.own_path) * (b.sequences > 1 && p.own_path != kUmma ? 2 : 1);
   split_keys((int64_t)b.max_len + p.joined_keys,
              (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, own_wave, least(p.own_path),
              tile(p.own_path), p.own_splits, p.own_chunk);
@@ -478,7 +479,7 @@ int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t 
   }
   if (status != B2K_OK) return status;
   if (a.own_splits + a.prefix_splits > 1) {
-    const cudaError_t err = merge<T>(a, s);
+    const cudaError_t err = merge<T>(a, ctx->sm_count, s);
     if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "paged_attention launch");
     ++launches;
   }

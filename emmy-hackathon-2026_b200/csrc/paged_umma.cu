@@ -204,6 +204,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     sm100::fence_barrier_init();
   }
+  if (TMA && threadIdx.x == 32 * kSoftmaxWarps) {
+    sm100::prefetch_tensormap(&map_k);
+    sm100::prefetch_tensormap(&map_v);
+  }
   if (warp == kSoftmaxWarps + kLoadWarps) sm100::tmem_alloc(&tmem_slot, 512);
   sm100::tc_fence_before();
   __syncthreads();
@@ -440,16 +444,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
       // both tiles' queries into shared memory, 16 bytes at a time
       constexpr int kPieces = DP / 8;
-      for (int i = threadIdx.x; i < 2 * kRows * kPieces; i += 32 * kSoftmaxWarps) {
-        const int qr = i / kPieces, c = i % kPieces, row = row0 + qr;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < rows && c * 8 < a.d) {
-          const int j = row / a.group;
-          v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (int64_t)(s.first + j) * a.q_token +
-                                               (int64_t)(head * a.group + row - j * a.group) * a.q_head + c * 8);
+      // eight loads in flight before the first is stored
+      constexpr int kStep = 32 * kSoftmaxWarps, kBatch = 8;
+      for (int i0 = threadIdx.x; i0 < 2 * kRows * kPieces; i0 += kBatch * kStep) {
+        uint4 v[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int i = i0 + u * kStep, qr = i / kPieces, c = i % kPieces, row = row0 + qr;
+          v[u] = make_uint4(0, 0, 0, 0);
+          if (row < rows && c * 8 < a.d) {
+            const int j = row / a.group;
+            v[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (int64_t)(s.first + j) * a.q_token +
+                                                    (int64_t)(head * a.group + row - j * a.group) * a.q_head + c * 8);
+          }
         }
-        const int tr = qr & 127;
-        *reinterpret_cast<uint4 *>(qs + (qr >> 7) * kTile + (c >> 3) * kHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = v;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int i = i0 + u * kStep, qr = i / kPieces, c = i % kPieces, tr = qr & 127;
+          *reinterpret_cast<uint4 *>(qs + (qr >> 7) * kTile + (c >> 3) * kHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = v[u];
+        }
       }
       sm100::fence_proxy_async_smem();
       __syncwarp();

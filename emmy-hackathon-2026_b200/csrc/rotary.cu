@@ -39,16 +39,15 @@ struct Segment {
   char *y;
   int64_t xt, xh;      // source strides in bytes: token, head
   int64_t yp, yt, yh;  // destination strides in bytes: page, token or row, head
-  int head0;           // first of its heads among the call's
-  int target, rotate;
+  int heads, target, rotate;
 };
 
 struct RotaryArgs {
   Segment seg[3];
-  int heads, d, rot, interleaved;
+  int count, heads, d, rot, interleaved;  // heads: of all segments
   float magnitude, sine;  // sine: +magnitude, or -magnitude for the transpose
   int items;              // places of a head: a lane keeps one
-  int warps_per_token;    // 1, 2, 4 or 8
+  int warps_log2;         // of the warps that share a token (1, 2, 4 or 8)
   int64_t tokens;
   const int64_t *positions;  // unpaged
   // paged
@@ -89,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
   grid_dependents_launch();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wpt = a.warps_per_token, tokens_per_block = kWarps / wpt;
+  const int tokens_per_block = kWarps >> a.warps_log2;
   const int pairs = a.rot / 2;
   // rows of this block's sequence (paged) or of the call
   int64_t row_begin = 0, row_end = a.tokens, own0 = 0;
@@ -108,11 +107,11 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
   // more (single elements) are walked 32 at a time, one head after the other.
   const int per_warp = a.items <= 32 ? 32 / a.items : 1;
   const int slot = a.items <= 32 ? lane / a.items : 0, j_first = a.items <= 32 ? lane - slot * a.items : lane;
-  const int head_step = per_warp * wpt, h_first = (warp % wpt) * per_warp + slot;
+  const int head_step = per_warp << a.warps_log2, h_first = (warp & ((1 << a.warps_log2) - 1)) * per_warp + slot;
   const int half_items = a.interleaved ? 0 : a.rot / 2 / V;
 
   const int64_t chunk0 = PAGED ? blockIdx.y : blockIdx.x, chunk_step = PAGED ? gridDim.y : gridDim.x;
-  for (int64_t row = row_begin + chunk0 * tokens_per_block + warp / wpt; row < row_end; row += chunk_step * tokens_per_block) {
+  for (int64_t row = row_begin + chunk0 * tokens_per_block + (warp >> a.warps_log2); row < row_end; row += chunk_step * tokens_per_block) {
     int64_t page = -1;
     int page_row = 0;
     bool turned = false;  // cosines and sines are there
@@ -134,19 +133,16 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
         if (e1 >= a.d) e1 = -1;
       }
       P va[kAhead], vb[kAhead];
-      auto segment = [&](int h) { return (h >= a.seg[1].head0) + (h >= a.seg[2].head0); };
-      auto load = [&](int hb) {
+      auto load = [&](const char *x, int64_t step, int h, int heads) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int h = hb + u * head_step;
-          if (!on || h >= a.heads) continue;
-          const Segment &s = a.seg[segment(h)];
-          const T *x = reinterpret_cast<const T *>(s.x + row * s.xt + (h - s.head0) * s.xh);
-          va[u] = *reinterpret_cast<const P *>(x + e0);
-          if (e1 >= 0) vb[u] = *reinterpret_cast<const P *>(x + e1);
+        for (int u = 0; u < kAhead; ++u, x += step, h += head_step) {
+          if (h >= heads) break;
+          va[u] = *reinterpret_cast<const P *>(x + e0 * (int)sizeof(T));
+          if (e1 >= 0) vb[u] = *reinterpret_cast<const P *>(x + e1 * (int)sizeof(T));
         }
       };
-      load(h_first);
+      auto source = [&](const Segment &s) { return s.x + row * s.xt + h_first * s.xh; };
+      if (on) load(source(a.seg[0]), head_step * a.seg[0].xh, h_first, a.seg[0].heads);
       if (!turned) {
         const int64_t own = own0 + (row - row_begin);
         const int64_t pos = PAGED ? a.prefix_len + own : pairs ? a.positions[row] : 0;
@@ -183,61 +179,66 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_consta
         c[i] = in ? cs[warp][p] : 0.0f;
         sv[i] = in ? sn[warp][p] : 0.0f;
       }
-      for (int hb = h_first; hb < a.heads; hb += kAhead * head_step) {
-        if (hb != h_first) load(hb);
+      if (!on) continue;
+      for (int g = 0; g < a.count; ++g) {
+        const Segment &s = a.seg[g];
+        const int64_t x_step = head_step * s.xh, y_step = head_step * s.yh;
+        const char *x = source(s);
+        char *y = s.y + h_first * s.yh;
+        if (PAGED && s.target != kLinear) {
+          if (page < 0) continue;
+          y += page * s.yp + page_row * s.yt;
+        } else {
+          y += row * s.yt;
+        }
+        const bool rotate = s.rotate && turns;
+        for (int hb = h_first; hb < s.heads; hb += kAhead * head_step, x += kAhead * x_step) {
+          if (g > 0 || hb != h_first) load(x, x_step, hb, s.heads);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int h = hb + u * head_step;
-          if (!on || h >= a.heads) continue;
-          const Segment &s = a.seg[segment(h)];
-          T *y;
-          if (PAGED && s.target != kLinear) {
-            if (page < 0) continue;
-            y = reinterpret_cast<T *>(s.y + page * s.yp + page_row * s.yt + (h - s.head0) * s.yh);
-          } else {
-            y = reinterpret_cast<T *>(s.y + row * s.yt + (h - s.head0) * s.yh);
-          }
-          if (s.rotate && turns) {
-            float xa[V], xb[V];
-            if (a.interleaved) {
-              // neighbours a, b, a, b ...: pair i is in the first vector for i < V / 2
-              float lo[V], hi[V];
-              widen<T, V>(va[u], lo);
-              widen<T, V>(vb[u], hi);
+          for (int u = 0; u < kAhead; ++u, y += y_step) {
+            if (hb + u * head_step >= s.heads) break;
+            if (rotate) {
+              float xa[V], xb[V];
+              if (a.interleaved) {
+                // neighbours a, b, a, b ...: pair i is in the first vector for i < V / 2
+                float lo[V], hi[V];
+                widen<T, V>(va[u], lo);
+                widen<T, V>(vb[u], hi);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                  xa[i] = 2 * i < V ? lo[2 * i % V] : hi[2 * i % V];
+                  xb[i] = 2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V];
+                }
+              } else {
+                widen<T, V>(va[u], xa);
+                widen<T, V>(vb[u], xb);
+              }
+              float ya[V], yb[V];
 #pragma unroll
               for (int i = 0; i < V; ++i) {
-                xa[i] = 2 * i < V ? lo[2 * i % V] : hi[2 * i % V];
-                xb[i] = 2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V];
+                ya[i] = xa[i] * c[i] - xb[i] * sv[i];
+                yb[i] = xb[i] * c[i] + xa[i] * sv[i];
               }
-            } else {
-              widen<T, V>(va[u], xa);
-              widen<T, V>(vb[u], xb);
-            }
-            float ya[V], yb[V];
+              if (a.interleaved) {
+                // pairs behind the rotated part stay as they were, bit for bit
+                float lo[V], hi[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              ya[i] = xa[i] * c[i] - xb[i] * sv[i];
-              yb[i] = xb[i] * c[i] + xa[i] * sv[i];
-            }
-            if (a.interleaved) {
-              // pairs behind the rotated part stay as they were, bit for bit
-              float lo[V], hi[V];
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                const bool in = pair_of(i) < pairs;
-                const float oa = in ? ya[i] : xa[i], ob = in ? yb[i] : xb[i];
-                (2 * i < V ? lo[2 * i % V] : hi[2 * i % V]) = oa;
-                (2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V]) = ob;
+                for (int i = 0; i < V; ++i) {
+                  const bool in = pair_of(i) < pairs;
+                  const float oa = in ? ya[i] : xa[i], ob = in ? yb[i] : xb[i];
+                  (2 * i < V ? lo[2 * i % V] : hi[2 * i % V]) = oa;
+                  (2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V]) = ob;
+                }
+                narrow<T, V>(lo, va[u]);
+                narrow<T, V>(hi, vb[u]);
+              } else {
+                narrow<T, V>(ya, va[u]);
+                narrow<T, V>(yb, vb[u]);
               }
-              narrow<T, V>(lo, va[u]);
-              narrow<T, V>(hi, vb[u]);
-            } else {
-              narrow<T, V>(ya, va[u]);
-              narrow<T, V>(yb, vb[u]);
             }
+            *reinterpret_cast<P *>(y + e0 * (int)sizeof(T)) = va[u];
+            if (e1 >= 0) *reinterpret_cast<P *>(y + e1 * (int)sizeof(T)) = vb[u];
           }
-          *reinterpret_cast<P *>(y + e0) = va[u];
-          if (e1 >= 0) *reinterpret_cast<P *>(y + e1) = vb[u];
         }
       }
     }
@@ -273,7 +274,7 @@ cudaError_t launch(const RotaryArgs &a, int v, dim3 grid, cudaStream_t s) {
 template <bool PAGED>
 int run(b2k_ctx *ctx, RotaryArgs &a, int count, int32_t dtype, int64_t tokens_each, unsigned sequences, int phase,
         cudaStream_t s, const char *what) {
-  for (int i = count; i < 3; ++i) a.seg[i].head0 = INT32_MAX;
+  a.count = count;
   const size_t size = serve::type_size(dtype);
   const int v = pick_vector(a, count, size);
   a.items = a.interleaved ? (a.d + 2 * v - 1) / (2 * v) : a.rot / 2 / v + (a.d - a.rot + 2 * v - 1) / (2 * v);
@@ -281,11 +282,13 @@ int run(b2k_ctx *ctx, RotaryArgs &a, int count, int32_t dtype, int64_t tokens_ea
   // SM); fewer tokens are shared out, down to one batch of loads a lane.
   const int64_t all = PAGED ? tokens_each * sequences : tokens_each;
   const int per_warp = a.items <= 32 ? 32 / a.items : 1;
-  a.warps_per_token = 1;
-  while (a.warps_per_token < kWarps && all * a.warps_per_token < (int64_t)ctx->sm_count * 8 * kWarps &&
-         per_warp * a.warps_per_token < a.heads)
-    a.warps_per_token *= 2;
-  const int tokens_per_block = kWarps / a.warps_per_token;
+  int wpt = 1;
+  a.warps_log2 = 0;
+  while (wpt < kWarps && all * wpt < (int64_t)ctx->sm_count * 8 * kWarps && per_warp * wpt < a.heads) {
+    wpt *= 2;
+    ++a.warps_log2;
+  }
+  const int tokens_per_block = kWarps / wpt;
   const int64_t chunks = (tokens_each + tokens_per_block - 1) / tokens_per_block;
   const dim3 grid = PAGED ? dim3(sequences, (unsigned)std::min<int64_t>(chunks, 65535))
                           : dim3((unsigned)std::min<int64_t>(chunks, INT32_MAX));
@@ -427,7 +430,7 @@ int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count,
     if (x[i].data == y[i].data && (x[i].stride_token != y[i].stride_token || x[i].stride_head != y[i].stride_head))
       return b2k::fail(ctx, B2K_EINVAL, "rotary: tensor %d is rotated in place with other strides", i);
     a.seg[i] = {static_cast<const char *>(x[i].data), static_cast<char *>(y[i].data), x[i].stride_token * size,
-                x[i].stride_head * size, 0, y[i].stride_token * size, y[i].stride_head * size, a.heads, kLinear, 1};
+                x[i].stride_head * size, 0, y[i].stride_token * size, y[i].stride_head * size, x[i].heads, kLinear, 1};
     a.heads += x[i].heads;
   }
   if (tokens == 0) return B2K_OK;
@@ -465,15 +468,15 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
         (q->data == q_out->data && (q->stride_token != q_out->stride_token || q->stride_head != q_out->stride_head)))
       return b2k::fail(ctx, B2K_EINVAL, "%s: q and q_out differ in heads, or in strides in place", what);
     a.seg[count++] = {static_cast<const char *>(q->data), static_cast<char *>(q_out->data), q->stride_token * size,
-                      q->stride_head * size, 0, q_out->stride_token * size, q_out->stride_head * size, 0, kLinear, 1};
+                      q->stride_head * size, 0, q_out->stride_token * size, q_out->stride_head * size, q->heads, kLinear, 1};
     a.heads += q->heads;
   }
   a.seg[count++] = {static_cast<const char *>(k->data), static_cast<char *>(cache->k), k->stride_token * size,
-                    k->stride_head * size, cache->k_page * size, cache->k_row * size, cache->k_head * size, a.heads,
+                    k->stride_head * size, cache->k_page * size, cache->k_row * size, cache->k_head * size, k->heads,
                     kKeys, rope != nullptr};
   a.heads += k->heads;
   a.seg[count++] = {static_cast<const char *>(v->data), static_cast<char *>(cache->v), v->stride_token * size,
-                    v->stride_head * size, cache->v_page * size, cache->v_row * size, cache->v_head * size, a.heads,
+                    v->stride_head * size, cache->v_page * size, cache->v_row * size, cache->v_head * size, v->heads,
                     kValues, 0};
   a.heads += v->heads;
   if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
