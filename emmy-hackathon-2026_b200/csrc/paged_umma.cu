@@ -6,22 +6,24 @@
 // are read once for 256 rows, and the tensor core works on one tile while the
 // softmax works on the other:
 //
-//   warps 0-3   softmax of tile A, one thread a row: S_j from tensor memory,
-//   warps 4-7   (tile B the same) running maximum, P_j back into S_j's columns
-//               in the operands' type, where the second product reads it;
-//               at the end the rows' output
-//   warp 8      loads: keys and values into 128-byte-swizzled tiles of 128 keys, in
+//   warps 0-7   softmax of tile A, two threads a row (64 keys, later half of the
+//   warps 8-15  output's columns, each; tile B the same): S_j from tensor memory,
+//               running maximum, P_j back into S_j's columns in the operands'
+//               type, where the second product reads it; at the end the rows'
+//               output.  One thread a row left a scheduler one warp of each
+//               tile, whose exponentials alone took 1500 cycles a tile
+//   warp 16     loads: keys and values into 128-byte-swizzled tiles of 128 keys, in
 //               the order K_0, V_0, K_1, V_1 ... through one ring, by TMA boxes
 //               of a page (or 128 rows of one); pages outside the cache are
 //               outside the tensor map and arrive as zeros
-//   warp 10     MMA issuer: S_j = Q K_j^T (128 x 128), then O += P_j V_j with P
+//   warp 18     MMA issuer: S_j = Q K_j^T (128 x 128), then O += P_j V_j with P
 //               from tensor memory and V as it lies (N-major), in the order O_A,
 //               S_A, O_B, S_B: while one tile has the tensor core the other is in
 //               its softmax (an issuer for each tile lets the two fall into step,
 //               and each then waits for both: 3 to 5 % slower)
 //   (pages that no box fits -- sizes that neither divide 128 nor are a multiple of
-//               it, or below 8 -- are copied row by row by warps 8 and 9, 16 bytes a
-//               lane; warp 11 passes on what has landed, since the tensor core sees
+//               it, or below 8 -- are copied row by row by warps 16 and 17, 16 bytes a
+//               lane; warp 19 passes on what has landed, since the tensor core sees
 //               such copies behind a proxy fence alone.  Those copies' issue bounds the kernel then: 7000
 //               cycles a pair of tiles)
 //
@@ -50,7 +52,7 @@ using paged::Args;
 
 constexpr int kRows = 128;    // rows of a tile
 constexpr int kKeys = 128;    // keys of a tile
-constexpr int kSoftmaxWarps = 8, kLoadWarps = 2;
+constexpr int kSoftmaxWarps = 16, kLoadWarps = 2;
 constexpr int kThreads = 32 * (kSoftmaxWarps + kLoadWarps + 2);
 constexpr int kHalf = kKeys * 128;  // bytes of a tile's 64 columns: 128 rows of 128 bytes
 constexpr int kMarks = 8;     // tiles whose key marks are kept
@@ -83,6 +85,19 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
+}
+// Barrier of 64 threads (two warps) that returns whether any of them said so.
+__device__ __forceinline__ bool barrier_or(int id, bool said) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %2, 0;\n\t"
+      "barrier.cta.red.or.pred p, %1, 64, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"((uint32_t)said)
+      : "memory");
+  return r != 0;
 }
 // Two FP32 operations in one instruction.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -182,6 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ uint32_t marks[kMarks][4];  // keys of a tile that are there
+  __shared__ float shared_row[2][2][kRows];  // between a row's two threads: maxima, at the end sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int *abort = &abort_word;
@@ -199,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm100::mbar_init(&drain, 1);
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&s_full[i], 1);
-      sm100::mbar_init(&p_full[i], 4);
+      sm100::mbar_init(&p_full[i], kSoftmaxWarps / 2);
       sm100::mbar_init(&o_full[i], 1);
     }
     sm100::fence_barrier_init();
@@ -437,15 +453,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     int never = 0;
     sm100::mbar_wait(&drain, 0, a.err, sm100::kSiteDrain, &never);
   } else if (work && warp < kSoftmaxWarps) {
-    // ---------------- softmax, one thread a row
-    const int x = warp >> 2;  // tile
-    const int r = (warp & 3) * 32 + lane;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    // ---------------- softmax, two threads a row
+    const int x = warp >> 3, side = (warp >> 2) & 1, quarter = warp & 3;  // tile, half of its columns, rows
+    const int r = quarter * 32 + lane;
+    const int meet = 1 + x * 4 + quarter;  // named barrier of the two warps that share these rows
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     {
       // both tiles' queries into shared memory, 16 bytes at a time
       constexpr int kPieces = DP / 8;
-      // eight loads in flight before the first is stored
-      constexpr int kStep = 32 * kSoftmaxWarps, kBatch = 8;
+      // all of a thread's loads in flight before the first is stored
+      constexpr int kStep = 32 * kSoftmaxWarps, kBatch = 2 * kRows * kPieces / kStep < 8 ? 2 * kRows * kPieces / kStep : 8;
       for (int i0 = threadIdx.x; i0 < 2 * kRows * kPieces; i0 += kBatch * kStep) {
         uint4 v[kBatch];
 #pragma unroll
@@ -477,44 +494,50 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int o = 16; o > 0; o >>= 1) free_end = min(free_end, __shfl_xor_sync(0xffffffffu, free_end, o));
     const int mine = x == 0 ? tiles_a : tiles_b;
     const float c = a.scale_log2;
-    const uint32_t s_at = tmem + lane_base + kColS + x * 128, o_at = tmem + lane_base + kColO + x * 128;
+    constexpr int kMine = kKeys / 2, kOut = DP / 2;  // keys, output columns of a thread
+    const uint32_t s_at = tmem + lane_base + kColS + x * 128, o_at = tmem + lane_base + kColO + x * 128 + side * kOut;
     float base = -INFINITY, l = 0.0f;
     bool ok = true;
+    // Both warps of a row pass every barrier of every tile, after a failed wait
+    // too: a failure skips the work between.
     for (int j = 0; j < mine; ++j) {
       ok = ok && sm100::mbar_wait_warp(&s_full[x], j & 1, a.err, sm100::kSiteAttention, abort);
-      if (!ok) break;
       sm100::tc_fence_after();
-      uint32_t sr[kKeys];
+      uint32_t sr[kMine];
+      float top = -INFINITY;
+      if (ok) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sm100::tmem_ld_32x32b_x32(s_at + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * i]));
-      sm100::tmem_ld_wait();
-      const int key = key0 + j * kKeys, part_end = tile0 + j < prefix_tiles ? a.prefix_len : INT32_MAX;
-      const uint32_t *mk = marks[j % kMarks];
-      const uint32_t m0 = mk[0], m1 = mk[1], m2 = mk[2], m3 = mk[3];
-      if (key + kKeys > min(free_end, part_end) || (m0 & m1 & m2 & m3) != 0xffffffffu) {
-        const int lim = min(limit, part_end) - key;
+        for (int i = 0; i < kMine / 32; ++i)
+          sm100::tmem_ld_32x32b_x32(s_at + side * kMine + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * i]));
+        sm100::tmem_ld_wait();
+        const int key = key0 + j * kKeys, part_end = tile0 + j < prefix_tiles ? a.prefix_len : INT32_MAX;
+        const uint32_t m0 = marks[j % kMarks][2 * side], m1 = marks[j % kMarks][2 * side + 1];
+        if (key + (side + 1) * kMine > min(free_end, part_end) || (m0 & m1) != 0xffffffffu) {
+          const int lim = min(limit, part_end) - key - side * kMine;
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) {
-          const uint32_t word = i < 32 ? m0 : i < 64 ? m1 : i < 96 ? m2 : m3;
-          if (i >= lim || !((word >> (i & 31)) & 1u)) sr[i] = __float_as_uint(-INFINITY);
+          for (int i = 0; i < kMine; ++i)
+            if (i >= lim || !(((i < 32 ? m0 : m1) >> (i & 31)) & 1u)) sr[i] = __float_as_uint(-INFINITY);
         }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kMine; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            mx[e] = max3(mx[e], __uint_as_float(sr[i + 2 * e]), __uint_as_float(sr[i + 2 * e + 1]));
+        top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c - Type<T>::kLift;
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < kKeys; i += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + 2 * e]), __uint_as_float(sr[i + 2 * e + 1]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c - Type<T>::kLift;
-      if (__any_sync(0xffffffffu, top > base + Type<T>::kSlack || (base == -INFINITY && top > base))) {
-        const float moved = fmaxf(base, top);
+      // (the barrier also lets P_j overwrite S_j: both halves of it have been read)
+      if (barrier_or(meet, top > base + Type<T>::kSlack || (base == -INFINITY && top > base))) {
+        shared_row[x][side][r] = top;
+        sm100::named_barrier(meet, 64);
+        const float moved = fmaxf(base, fmaxf(top, shared_row[x][side ^ 1][r]));
         const float alpha = moved == -INFINITY ? 1.0f : exp2_fast(base - moved);
         base = moved;
         l *= alpha;
-        if (j > 0) {
+        if (j > 0 && ok) {
           // S_j is complete, so is the product before it: O holds still
 #pragma unroll
-          for (int i = 0; i < DP; i += 16) {
+          for (int i = 0; i < kOut; i += 16) {
             uint32_t ov[16];
             sm100::tmem_ld_32x32b_x16(o_at + i, ov);
             sm100::tmem_ld_wait();
@@ -524,22 +547,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      if (!ok) continue;
       const float from = base == -INFINITY ? 0.0f : base;
       uint64_t sum[2] = {0, 0};
       const uint64_t c2 = pair(c, c), from2 = pair(-from, -from);
-      uint32_t pk[32];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kMine; h += 32) {
+        uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
+        for (int i = 0; i < 32; i += 2) {
           float p0, p1;
-          unpair(fma2(pair(__uint_as_float(sr[64 * h + i]), __uint_as_float(sr[64 * h + i + 1])), c2, from2), p0, p1);
+          unpair(fma2(pair(__uint_as_float(sr[h + i]), __uint_as_float(sr[h + i + 1])), c2, from2), p0, p1);
           p0 = exp2_fast(p0);
           p1 = exp2_fast(p1);
           sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair(p0, p1));
           pk[i / 2] = Type<T>::pack(p0, p1);
         }
-        sm100::tmem_st_32x32b_x32(s_at + 32 * h, pk);
+        sm100::tmem_st_32x32b_x16(s_at + (side * kMine + h) / 2, pk);
       }
       float l0, l1;
       unpair(add2(sum[0], sum[1]), l0, l1);
@@ -549,7 +573,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(&p_full[x]);
     }
-    // ---------------- the row's output
+    // ---------------- the row's output, half of its columns a thread
+    sm100::named_barrier(meet, 64);  // the last maxima have been read
+    shared_row[x][side][r] = l;
+    sm100::named_barrier(meet, 64);
+    l += shared_row[x][side ^ 1][r];
     if (mine > 0) ok = ok && sm100::mbar_wait_warp(&o_full[x], 0, a.err, sm100::kSiteEpilogueAccum, abort);
     if (ok && row0 + x * kRows < rows) {
       sm100::tc_fence_after();
@@ -557,14 +585,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t token = s.first + j_row;
       const int qh = head * a.group + row - j_row * a.group;
       const bool on = row < rows;
-      const bool some = l != 0.0f;  // (NaN too)
+      const bool some = l != 0.0f && mine > 0;  // (NaN too)
       const float inv = !direct ? 1.0f : some ? 1.0f / l : 0.0f;
       const int64_t part = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
       // rows of a split that see none of its keys are not read by the merge
-      if (!direct && on) a.part_ml[part] = make_float2(base, l);
+      if (!direct && on && side == 0) a.part_ml[part] = make_float2(base, l);
 #pragma unroll
-      for (int i = 0; i < DP; i += 32) {
-        if (i >= a.d) break;
+      for (int i = 0; i < kOut; i += 32) {
+        const int col = side * kOut + i;
+        if (col >= a.d) break;
         uint32_t ov[32];
         if (mine > 0) {
           sm100::tmem_ld_32x32b_x32(o_at + i, ov);
@@ -572,24 +601,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!on) continue;
         if (direct) {
-          T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + i;
+          T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + col;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint32_t w[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              w[u] = some && mine > 0 ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
-            if (i + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              w[u] = some ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
+            if (col + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          float *out = a.part_o + part * a.d + i;
+          float *out = a.part_o + part * a.d + col;
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            if (i + e < a.d)
+            if (col + e < a.d)
               *reinterpret_cast<float4 *>(out + e) =
-                  some && mine > 0 ? make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
-                                                 __uint_as_float(ov[e + 3]))
-                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                  some ? make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
+                                     __uint_as_float(ov[e + 3]))
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
       }
     }
