@@ -6,24 +6,25 @@
 // are read once for 256 rows, and the tensor core works on one tile while the
 // softmax works on the other:
 //
-//   warps 0-7   softmax of tile A, two threads a row (64 keys, later half of the
-//   warps 8-15  output's columns, each; tile B the same): S_j from tensor memory,
-//               running maximum, P_j back into S_j's columns in the operands'
-//               type, where the second product reads it; at the end the rows'
-//               output.  One thread a row left a scheduler one warp of each
-//               tile, whose exponentials alone took 1500 cycles a tile
-//   warp 16     loads: keys and values into 128-byte-swizzled tiles of 128 keys, in
+//   warps 0-3   softmax of tile A, one thread a row: S_j from tensor memory,
+//   warps 4-7   (tile B the same) running maximum, P_j back into S_j's columns
+//               in the operands' type, where the second product reads it;
+//               at the end the rows' output
+//   warp 8      loads: keys and values into 128-byte-swizzled tiles of 128 keys, in
 //               the order K_0, V_0, K_1, V_1 ... through one ring, by TMA boxes
 //               of a page (or 128 rows of one); pages outside the cache are
-//               outside the tensor map and arrive as zeros
-//   warp 18     MMA issuer: S_j = Q K_j^T (128 x 128), then O += P_j V_j with P
+//               outside the tensor map and arrive as zeros.  Queries the same way,
+//               as boxes of tokens by heads, where a cache head's query heads
+//               divide 128 (row by row by the softmax warps they take 8000
+//               cycles of a block's start)
+//   warp 10     MMA issuer: S_j = Q K_j^T (128 x 128), then O += P_j V_j with P
 //               from tensor memory and V as it lies (N-major), in the order O_A,
 //               S_A, O_B, S_B: while one tile has the tensor core the other is in
 //               its softmax (an issuer for each tile lets the two fall into step,
 //               and each then waits for both: 3 to 5 % slower)
 //   (pages that no box fits -- sizes that neither divide 128 nor are a multiple of
-//               it, or below 8 -- are copied row by row by warps 16 and 17, 16 bytes a
-//               lane; warp 19 passes on what has landed, since the tensor core sees
+//               it, or below 8 -- are copied row by row by warps 8 and 9, 16 bytes a
+//               lane; warp 11 passes on what has landed, since the tensor core sees
 //               such copies behind a proxy fence alone.  Those copies' issue bounds the kernel then: 7000
 //               cycles a pair of tiles)
 //
@@ -52,7 +53,7 @@ using paged::Args;
 
 constexpr int kRows = 128;    // rows of a tile
 constexpr int kKeys = 128;    // keys of a tile
-constexpr int kSoftmaxWarps = 16, kLoadWarps = 2;
+constexpr int kSoftmaxWarps = 8, kLoadWarps = 2;
 constexpr int kThreads = 32 * (kSoftmaxWarps + kLoadWarps + 2);
 constexpr int kHalf = kKeys * 128;  // bytes of a tile's 64 columns: 128 rows of 128 bytes
 constexpr int kMarks = 8;     // tiles whose key marks are kept
@@ -85,19 +86,6 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
-}
-// Barrier of 64 threads (two warps) that returns whether any of them said so.
-__device__ __forceinline__ bool barrier_or(int id, bool said) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %2, 0;\n\t"
-      "barrier.cta.red.or.pred p, %1, 64, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"((uint32_t)said)
-      : "memory");
-  return r != 0;
 }
 // Two FP32 operations in one instruction.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -189,15 +177,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 template <typename T, int DP, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                      const __grid_constant__ Args a, const bool prefix, const int row_blocks) {
+                      const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Args a, const bool prefix,
+                      const int row_blocks, const bool q_boxes) {
   constexpr int kStages = stages<DP>();
   constexpr int kTile = tile_bytes<DP>();
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(8) uint64_t landed[kStages], full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2], drain;
+  __shared__ __align__(8) uint64_t landed[kStages], full[kStages], empty[kStages], q_full, s_full[2], p_full[2][2], o_full[2], drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ uint32_t marks[kMarks][4];  // keys of a tile that are there
-  __shared__ float shared_row[2][2][kRows];  // between a row's two threads: maxima, at the end sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int *abort = &abort_word;
@@ -211,11 +199,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::mbar_init(&full[i], 1);  // TMA: the bytes; else warp 11
       sm100::mbar_init(&empty[i], 1);
     }
-    sm100::mbar_init(&q_full, kSoftmaxWarps);
+    sm100::mbar_init(&q_full, q_boxes ? 1 : kSoftmaxWarps);
     sm100::mbar_init(&drain, 1);
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&s_full[i], 1);
-      sm100::mbar_init(&p_full[i], kSoftmaxWarps / 2);
+      sm100::mbar_init(&p_full[i][0], 4);  // P's first 64 keys, the others
+      sm100::mbar_init(&p_full[i][1], 4);
       sm100::mbar_init(&o_full[i], 1);
     }
     sm100::fence_barrier_init();
@@ -278,6 +267,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       return lane < boxes && lane * box < valid(j) ? (pre ? a.prefix_table : own_table)[(unsigned)key / (unsigned)a.page_size] : -1;
     };
     bool ok = true;
+    if (q_boxes && lane == 0 && tiles > 0) {
+      // a tile's rows are whole tokens: 128 / group of them, group heads each
+      sm100::mbar_arrive_expect_tx(&q_full, 2 * kTile);
+      for (int x = 0; x < 2; ++x)
+        for (int half = 0; half < DP / 64; ++half)
+          sm100::tma_load_3d(qs + x * kTile + half * kHalf, &map_q, &q_full, 64 * half, head * a.group,
+                             s.first + (row0 + x * kRows) / a.group);
+    }
+    __syncwarp();
     int page = look_up(0);
     for (int j = 0; ok && j < tiles; ++j) {
       const bool pre = prefix || tile0 + j < prefix_tiles;
@@ -411,13 +409,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::mma_commit(&s_full[x]);
     };
     auto issue_o = [&](int x, int j, bool last) {
-      ok = ok && sm100::mbar_wait_warp(&p_full[x], j & 1, a.err, sm100::kSiteMmaFull, abort);
-      if (!ok) return;
-      sm100::tc_fence_after();
       const uint32_t v = item_addr(2 * j + 1), p = tmem + kColS + x * 128, d = tmem + kColO + x * 128;
 #pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk)
-        mma_ts(d, p + kk * 8, desc_mn(v + kk * 2048, kHalf, 1024), id_o, j != 0 || kk != 0);
+      for (int half = 0; half < 2; ++half) {
+        ok = ok && sm100::mbar_wait_warp(&p_full[x][half], j & 1, a.err, sm100::kSiteMmaFull, abort);
+        if (!ok) return;
+        sm100::tc_fence_after();
+#pragma unroll
+        for (int kk = half * kKeys / 32; kk < (half + 1) * kKeys / 32; ++kk)
+          mma_ts(d, p + kk * 8, desc_mn(v + kk * 2048, kHalf, 1024), id_o, j != 0 || kk != 0);
+      }
       if (last) sm100::mma_commit(&o_full[x]);
     };
     auto tiles_of = [&](int x) { return x == 0 ? tiles_a : tiles_b; };
@@ -453,16 +454,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     int never = 0;
     sm100::mbar_wait(&drain, 0, a.err, sm100::kSiteDrain, &never);
   } else if (work && warp < kSoftmaxWarps) {
-    // ---------------- softmax, two threads a row
-    const int x = warp >> 3, side = (warp >> 2) & 1, quarter = warp & 3;  // tile, half of its columns, rows
-    const int r = quarter * 32 + lane;
-    const int meet = 1 + x * 4 + quarter;  // named barrier of the two warps that share these rows
-    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    {
+    // ---------------- softmax, one thread a row
+    const int x = warp >> 2;  // tile
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    if (!q_boxes) {
       // both tiles' queries into shared memory, 16 bytes at a time
       constexpr int kPieces = DP / 8;
-      // all of a thread's loads in flight before the first is stored
-      constexpr int kStep = 32 * kSoftmaxWarps, kBatch = 2 * kRows * kPieces / kStep < 8 ? 2 * kRows * kPieces / kStep : 8;
+      // eight loads in flight before the first is stored
+      constexpr int kStep = 32 * kSoftmaxWarps, kBatch = 8;
       for (int i0 = threadIdx.x; i0 < 2 * kRows * kPieces; i0 += kBatch * kStep) {
         uint4 v[kBatch];
 #pragma unroll
@@ -494,50 +494,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int o = 16; o > 0; o >>= 1) free_end = min(free_end, __shfl_xor_sync(0xffffffffu, free_end, o));
     const int mine = x == 0 ? tiles_a : tiles_b;
     const float c = a.scale_log2;
-    constexpr int kMine = kKeys / 2, kOut = DP / 2;  // keys, output columns of a thread
-    const uint32_t s_at = tmem + lane_base + kColS + x * 128, o_at = tmem + lane_base + kColO + x * 128 + side * kOut;
+    const uint32_t s_at = tmem + lane_base + kColS + x * 128, o_at = tmem + lane_base + kColO + x * 128;
     float base = -INFINITY, l = 0.0f;
     bool ok = true;
-    // Both warps of a row pass every barrier of every tile, after a failed wait
-    // too: a failure skips the work between.
     for (int j = 0; j < mine; ++j) {
       ok = ok && sm100::mbar_wait_warp(&s_full[x], j & 1, a.err, sm100::kSiteAttention, abort);
+      if (!ok) break;
       sm100::tc_fence_after();
-      uint32_t sr[kMine];
-      float top = -INFINITY;
-      if (ok) {
+      uint32_t sr[kKeys];
 #pragma unroll
-        for (int i = 0; i < kMine / 32; ++i)
-          sm100::tmem_ld_32x32b_x32(s_at + side * kMine + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * i]));
-        sm100::tmem_ld_wait();
-        const int key = key0 + j * kKeys, part_end = tile0 + j < prefix_tiles ? a.prefix_len : INT32_MAX;
-        const uint32_t m0 = marks[j % kMarks][2 * side], m1 = marks[j % kMarks][2 * side + 1];
-        if (key + (side + 1) * kMine > min(free_end, part_end) || (m0 & m1) != 0xffffffffu) {
-          const int lim = min(limit, part_end) - key - side * kMine;
+      for (int i = 0; i < 4; ++i)
+        sm100::tmem_ld_32x32b_x32(s_at + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * i]));
+      sm100::tmem_ld_wait();
+      const int key = key0 + j * kKeys, part_end = tile0 + j < prefix_tiles ? a.prefix_len : INT32_MAX;
+      const uint32_t *mk = marks[j % kMarks];
+      const uint32_t m0 = mk[0], m1 = mk[1], m2 = mk[2], m3 = mk[3];
+      if (key + kKeys > min(free_end, part_end) || (m0 & m1 & m2 & m3) != 0xffffffffu) {
+        const int lim = min(limit, part_end) - key;
 #pragma unroll
-          for (int i = 0; i < kMine; ++i)
-            if (i >= lim || !(((i < 32 ? m0 : m1) >> (i & 31)) & 1u)) sr[i] = __float_as_uint(-INFINITY);
+        for (int i = 0; i < kKeys; ++i) {
+          const uint32_t word = i < 32 ? m0 : i < 64 ? m1 : i < 96 ? m2 : m3;
+          if (i >= lim || !((word >> (i & 31)) & 1u)) sr[i] = __float_as_uint(-INFINITY);
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kMine; i += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            mx[e] = max3(mx[e], __uint_as_float(sr[i + 2 * e]), __uint_as_float(sr[i + 2 * e + 1]));
-        top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c - Type<T>::kLift;
       }
-      // (the barrier also lets P_j overwrite S_j: both halves of it have been read)
-      if (barrier_or(meet, top > base + Type<T>::kSlack || (base == -INFINITY && top > base))) {
-        shared_row[x][side][r] = top;
-        sm100::named_barrier(meet, 64);
-        const float moved = fmaxf(base, fmaxf(top, shared_row[x][side ^ 1][r]));
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < kKeys; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[i + 2 * e]), __uint_as_float(sr[i + 2 * e + 1]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c - Type<T>::kLift;
+      if (__any_sync(0xffffffffu, top > base + Type<T>::kSlack || (base == -INFINITY && top > base))) {
+        const float moved = fmaxf(base, top);
         const float alpha = moved == -INFINITY ? 1.0f : exp2_fast(base - moved);
         base = moved;
         l *= alpha;
-        if (j > 0 && ok) {
+        if (j > 0) {
           // S_j is complete, so is the product before it: O holds still
 #pragma unroll
-          for (int i = 0; i < kOut; i += 16) {
+          for (int i = 0; i < DP; i += 16) {
             uint32_t ov[16];
             sm100::tmem_ld_32x32b_x16(o_at + i, ov);
             sm100::tmem_ld_wait();
@@ -547,37 +541,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (!ok) continue;
       const float from = base == -INFINITY ? 0.0f : base;
       uint64_t sum[2] = {0, 0};
       const uint64_t c2 = pair(c, c), from2 = pair(-from, -from);
+      // (A third of the exponentials as a polynomial on the FMA units lengthens
+      // the tile, 257 -> 282 us for prompt chunks: two warps a scheduler do not
+      // hide its chains.)
 #pragma unroll
-      for (int h = 0; h < kMine; h += 32) {
-        uint32_t pk[16];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
+        for (int i = 0; i < 64; i += 2) {
           float p0, p1;
-          unpair(fma2(pair(__uint_as_float(sr[h + i]), __uint_as_float(sr[h + i + 1])), c2, from2), p0, p1);
+          unpair(fma2(pair(__uint_as_float(sr[64 * h + i]), __uint_as_float(sr[64 * h + i + 1])), c2, from2), p0, p1);
           p0 = exp2_fast(p0);
           p1 = exp2_fast(p1);
           sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair(p0, p1));
           pk[i / 2] = Type<T>::pack(p0, p1);
         }
-        sm100::tmem_st_32x32b_x16(s_at + (side * kMine + h) / 2, pk);
+        sm100::tmem_st_32x32b_x32(s_at + 32 * h, pk);
+        sm100::tmem_st_wait();
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&p_full[x][h]);  // the product of these keys may begin
       }
       float l0, l1;
       unpair(add2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;
-      sm100::tmem_st_wait();
-      sm100::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&p_full[x]);
     }
-    // ---------------- the row's output, half of its columns a thread
-    sm100::named_barrier(meet, 64);  // the last maxima have been read
-    shared_row[x][side][r] = l;
-    sm100::named_barrier(meet, 64);
-    l += shared_row[x][side ^ 1][r];
+    // ---------------- the row's output
     if (mine > 0) ok = ok && sm100::mbar_wait_warp(&o_full[x], 0, a.err, sm100::kSiteEpilogueAccum, abort);
     if (ok && row0 + x * kRows < rows) {
       sm100::tc_fence_after();
@@ -585,15 +577,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t token = s.first + j_row;
       const int qh = head * a.group + row - j_row * a.group;
       const bool on = row < rows;
-      const bool some = l != 0.0f && mine > 0;  // (NaN too)
+      const bool some = l != 0.0f;  // (NaN too)
       const float inv = !direct ? 1.0f : some ? 1.0f / l : 0.0f;
       const int64_t part = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
       // rows of a split that see none of its keys are not read by the merge
-      if (!direct && on && side == 0) a.part_ml[part] = make_float2(base, l);
+      if (!direct && on) a.part_ml[part] = make_float2(base, l);
 #pragma unroll
-      for (int i = 0; i < kOut; i += 32) {
-        const int col = side * kOut + i;
-        if (col >= a.d) break;
+      for (int i = 0; i < DP; i += 32) {
+        if (i >= a.d) break;
         uint32_t ov[32];
         if (mine > 0) {
           sm100::tmem_ld_32x32b_x32(o_at + i, ov);
@@ -601,24 +592,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!on) continue;
         if (direct) {
-          T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + col;
+          T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + i;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint32_t w[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              w[u] = some ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
-            if (col + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              w[u] = some && mine > 0 ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
+            if (i + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          float *out = a.part_o + part * a.d + col;
+          float *out = a.part_o + part * a.d + i;
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            if (col + e < a.d)
+            if (i + e < a.d)
               *reinterpret_cast<float4 *>(out + e) =
-                  some ? make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
-                                     __uint_as_float(ov[e + 3]))
-                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                  some && mine > 0 ? make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
+                                                 __uint_as_float(ov[e + 3]))
+                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
       }
     }
@@ -659,17 +650,40 @@ bool boxes_fit(const Args &a) {
          a.k_row < most && a.k_head < most && a.k_page < most && a.v_row < most && a.v_head < most && a.v_page < most;
 }
 
+// Queries [tokens][heads][d], boxes of 64 elements by a cache head's query heads
+// by the tokens that make 128 rows.
+template <typename T>
+int make_q_map(b2k_ctx *ctx, CUtensorMap *map, const Args &a) {
+  auto encode = b2k::tensor_map_encoder();
+  if (!encode) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)a.d, (cuuint64_t)(a.kv_heads * a.group), (cuuint64_t)a.tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_token * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(kRows / a.group)};
+  cuuint32_t elem[3] = {1, 1, 1};
+  const CUresult res =
+      encode(map, Type<T>::kFormat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+             const_cast<void *>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)res);
+  return B2K_OK;
+}
+
 template <typename T, int DP, bool TMA>
 int launch(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned blocks, cudaStream_t s) {
   auto kernel = paged_umma_kernel<T, DP, TMA>;
-  CUtensorMap map_k = {}, map_v = {};
-  int status;
-  if (TMA && (status = make_map<T>(ctx, &map_k, a, true)) != B2K_OK) return status;
-  if (TMA && (status = make_map<T>(ctx, &map_v, a, false)) != B2K_OK) return status;
+  CUtensorMap map_k = {}, map_v = {}, map_q = {};
+  // A single head's stride is not used, but a tensor map wants one it can hold.
+  const int64_t most = (int64_t)1 << 38;
+  const bool q_boxes = TMA && kRows % a.group == 0 && a.q_head > 0 && a.q_token > 0 && a.q_head < most && a.q_token < most;
+  int status = B2K_OK;
+  if (TMA) status = make_map<T>(ctx, &map_k, a, true);
+  if (TMA && status == B2K_OK) status = make_map<T>(ctx, &map_v, a, false);
+  if (q_boxes && status == B2K_OK) status = make_q_map<T>(ctx, &map_q, a);
+  if (status != B2K_OK) return status;
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, smem_bytes<DP>());
   if (err == cudaSuccess)
-    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP>(), s, map_k, map_v, a,
-                             prefix, row_blocks);
+    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP>(), s, map_k, map_v,
+                             map_q, a, prefix, row_blocks, q_boxes);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }
 
