@@ -117,14 +117,21 @@ __global__ void __launch_bounds__(kThreads)
   look_up(0);
   look_up(1);
 
-  // this block's queries, FP32, times log2(e) / scale
-  for (int i = threadIdx.x; i < R * dp; i += kThreads) {
-    const int r = i / dp, c = i % dp, row = row0 + r;
-    float x = 0.0f;
-    if (row < rows && c < a.d)
-      x = serve::to_f32(static_cast<const T *>(a.q)[(int64_t)(s.first + row / a.group) * a.q_token +
-                                                     (head * a.group + row % a.group) * a.q_head + c]);
-    qs[i] = x * a.scale_log2;
+  // this block's queries, FP32, times log2(e) / scale; eight loads in flight
+  constexpr int kBatch = 8;
+  for (int i0 = threadIdx.x; i0 < R * dp; i0 += kBatch * kThreads) {
+    float x[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kThreads, r = i / dp, c = i - r * dp, row = row0 + r;
+      x[u] = 0.0f;
+      if (r < R && row < rows && c < a.d)
+        x[u] = serve::to_f32(static_cast<const T *>(a.q)[(int64_t)(s.first + row / a.group) * a.q_token +
+                                                          (head * a.group + row % a.group) * a.q_head + c]);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (i0 + u * kThreads < R * dp) qs[i0 + u * kThreads] = x[u] * a.scale_log2;
   }
   int limit[RW];
   float m[RW], l[RW];
@@ -249,7 +256,7 @@ template <typename T, int V, bool SHARED>
 __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_constant__ Args a, bool vec_out) {
   constexpr int kPieces = B2K_MAX_HEAD_DIM / 32 / V;  // of a lane
   constexpr int kStep = SHARED ? kWarps : 1;          // parts from one of a warp's to the next
-  constexpr int kAhead = 4;
+  constexpr int kAhead = SHARED ? 10 : 4;  // parts a warp has in flight: up to 40 of a row at once
   __shared__ float sums[SHARED ? kWarps : 1][SHARED ? B2K_MAX_HEAD_DIM : 1];
   grid_dependency_wait();
   grid_dependents_launch();
@@ -265,6 +272,21 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
     const int own = (paged::own_limit(a, s, j) + a.own_chunk - 1) / a.own_chunk;
     const int parts = own + a.prefix_splits;
     auto slot = [&](int i) { return (int64_t)(i < own ? i : a.own_splits + i - own) * stride + at; };
+    // the first parts' sums are on their way while the weights are found
+    serve::Pack<float, V> v[kAhead][kPieces];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kStep;
+        if (i >= parts) break;
+        const float *from = a.part_o + slot(i) * a.d;
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c)
+          if ((c * 32 + lane) * V < a.d) v[u][c] = *reinterpret_cast<const serve::Pack<float, V> *>(from + (c * 32 + lane) * V);
+      }
+    };
+    const int mine = SHARED ? warp : 0;
+    load(mine);
     float mx = -INFINITY, total = 0.0f;
     for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, a.part_ml[slot(i)].x);
     mx = warp_max(mx);
@@ -280,29 +302,19 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
     for (int c = 0; c < kPieces; ++c)
 #pragma unroll
       for (int e = 0; e < V; ++e) x[c][e] = 0.0f;
-    for (int i0 = SHARED ? warp : 0; i0 < parts; i0 += kAhead * kStep) {
-      float w[kAhead];
-      serve::Pack<float, V> v[kAhead][kPieces];
+    for (int i0 = mine; i0 < parts; i0 += kAhead * kStep) {
+      if (i0 != mine) load(i0);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int i = i0 + u * kStep;
-        w[u] = 0.0f;
-        if (i >= parts) continue;
-        const int64_t p = slot(i);
-        w[u] = exp2_fast(a.part_ml[p].x - base);
+        if (i >= parts) break;
+        const float w = exp2_fast(a.part_ml[slot(i)].x - base);
 #pragma unroll
         for (int c = 0; c < kPieces; ++c)
           if ((c * 32 + lane) * V < a.d)
-            v[u][c] = *reinterpret_cast<const serve::Pack<float, V> *>(a.part_o + p * a.d + (c * 32 + lane) * V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[c][e] = fmaf(v[u][c].v[e], w, x[c][e]);
       }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (i0 + u * kStep < parts)
-#pragma unroll
-          for (int c = 0; c < kPieces; ++c)
-            if ((c * 32 + lane) * V < a.d)
-#pragma unroll
-              for (int e = 0; e < V; ++e) x[c][e] = fmaf(v[u][c].v[e], w[u], x[c][e]);
     }
     if (SHARED) {
       __syncthreads();  // the last row's readers are done
@@ -372,12 +384,16 @@ bool cache_pieces(const b2k_paged_cache &c) {
 }
 bool rows_pieces(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_token, x.stride_head, 0, 2, 16); }
 
-// Kernel for a part with `rows` rows a cache head.  Up to 32 rows fit one block
-// of the warp kernel, which then reads the keys once as well, two blocks an
-// SM; above that the tensor-memory kernel's 256 rows save re-reading them.
-// Head dims above 128 do not fit its tensor memory twice.
-Path pick_path(bool tensor, int d, int64_t rows) {
-  return !tensor ? kPlain : rows > 32 && d <= 128 ? kUmma : kMma;
+// Kernel for a part with `rows` rows and `keys` keys a cache head, in `units`
+// such pairs.  Up to 32 rows fit one block of the warp kernel, which then reads
+// the keys once as well, two blocks an SM; above that the tensor-memory kernel's
+// 256 rows save re-reading them, and at 2.4 times the rate (2.4 against 1.0
+// million rows x keys a microsecond at head dim 128) it repays the 10 us that
+// its launch and its blocks' starts cost from about 16 million on.  Head dims
+// above 128 do not fit its tensor memory twice.
+Path pick_path(bool tensor, int d, int64_t rows, int64_t keys, int64_t units) {
+  if (!tensor) return kPlain;
+  return rows > 32 && d <= 128 && (double)rows * keys * units * d > 16e6 * 128 ? kUmma : kMma;
 }
 int block_rows(Path path, int d, int64_t rows) {
   return path == kPlain ? plain_rows(rows) : path == kMma ? paged::mma_rows(d, rows) : paged::kUmmaRows;
@@ -397,7 +413,7 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   Plan p = {};
   const int64_t group = q_heads / c.heads;
   const int64_t own = b.max_new * group, prefix = b.tokens * group;
-  p.own_path = pick_path(tensor, c.d, own);
+  p.own_path = pick_path(tensor, c.d, own, (int64_t)b.max_len + b.prefix_len, (int64_t)c.heads * b.sequences);
   p.own_rows = block_rows(p.own_path, c.d, own);
   // Sequences whose own rows fill a block read the prefix with their own keys:
   // stacking the rows of several sequences would save no reads of it.
@@ -416,7 +432,7 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
              (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, own_wave, least(p.own_path),
              tile(p.own_path), p.own_splits, p.own_chunk);
   if (b.prefix_len > 0 && !p.joined) {
-    p.prefix_path = pick_path(tensor, c.d, prefix);
+    p.prefix_path = pick_path(tensor, c.d, prefix, b.prefix_len, c.heads);
     p.prefix_rows = block_rows(p.prefix_path, c.d, prefix);
     split_keys(b.prefix_len, (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads, wave(p.prefix_path),
                least(p.prefix_path), tile(p.prefix_path), p.prefix_splits, p.prefix_chunk);

@@ -3,11 +3,13 @@
 // cache head, tokens side by side) and one split of the keys; its four warps
 // take 16 keys at a time in turn, each on its own.
 //
-// Bound: HBM, the cache read once.  Each warp keeps a ring of three tiles of
-// 16 keys and values in flight with 16-byte asynchronous copies that only it
-// waits for (no block barrier until the end), two blocks an SM: 96 to 128 KB on
-// the way at any time, where the copy bandwidth times the latency of HBM is about
-// 45 KB an SM.  The products are 16 x 8 x 16 warp MMAs with the probabilities
+// Bound: HBM, the cache read once, and with many rows the instructions about it.
+// Each warp keeps a ring of two to four tiles of 16 keys and values in flight
+// with 16-byte asynchronous copies that only it waits for (no block barrier
+// until the end), two or three blocks an SM: about 96 KB on the way at any
+// time, where the copy bandwidth times the latency of HBM is about 45 KB an SM.
+// The third block is worth its tighter registers (33 sequences of 20 rows of
+// 64: 30 us with two, 25 with three).  The products are 16 x 8 x 16 warp MMAs with the probabilities
 // taken from the score registers as they lie; rows that are not there cost
 // nothing that the loads would not hide, so the 16-row tile is not split
 // further.  The tensor-memory instructions need 64 rows and more to one tile:
@@ -30,12 +32,19 @@ constexpr int kThreads = 128;
 constexpr int kWarps = 4;
 constexpr int kTile = 16;  // keys of a warp's step
 
-template <int DP>
-constexpr int stages() { return DP == 64 ? 4 : 3; }
+// Tiles a warp has in its ring.  Two at head dim 128 with 16 rows leave room for
+// a third block on an SM (one sequence of 50001 keys: 42 us with three tiles
+// and two blocks, 40 with two and three).
+template <int DP, int MT>
+constexpr int stages() { return DP == 64 ? 4 : DP == 128 && MT == 1 ? 2 : 3; }
 template <int DP>
 constexpr int tile_bytes() { return kTile * DP * 2; }  // one of K, V
-template <int DP>
-constexpr int smem_bytes() { return kWarps * stages<DP>() * 2 * tile_bytes<DP>(); }
+template <int DP, int MT>
+constexpr int sums_bytes() { return kWarps * 16 * MT * (DP + 8) * 4; }  // at the end, where the keys were
+template <int DP, int MT>
+constexpr int smem_bytes() {
+  return std::max(kWarps * stages<DP, MT>() * 2 * tile_bytes<DP>(), sums_bytes<DP, MT>());
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -104,16 +113,15 @@ struct Grid {
 };
 
 template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : DP == 128 && MT == 2 ? 2 : 3)
     paged_mma_kernel(const __grid_constant__ Args a, const Grid grid) {
-  constexpr int kStages = stages<DP>();
+  constexpr int kStages = stages<DP, MT>();
   constexpr int kChunks = DP / 8;        // 16-byte pieces of a row
   constexpr int kRows = 16 * MT;
   constexpr int kLdo = DP + 8;           // row stride of the warps' sums in shared memory
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 ml[kWarps][kRows];
   __shared__ uint32_t there_s[kWarps][kStages];
-  static_assert(kWarps * kRows * kLdo * 4 <= smem_bytes<DP>(), "the sums fit where the keys were");
   paged::part_begin(grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,29 +148,6 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
   if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(grid.beside);
   const int q_heads = a.kv_heads * a.group;
 
-  // Queries as A fragments, straight from global memory: thread (g, t) holds
-  // rows g and g + 8 of each 16, columns 2t, 2t + 1 and 8 further.
-  const int g = lane >> 2, t = lane & 3;
-  uint32_t qf[MT][DP / 16][4];
-  int limit[MT][2];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = row0 + 16 * i + 8 * h + g;
-      const bool on = row < rows;
-      const int j = on ? row / a.group : 0;
-      limit[i][h] = !on ? 0 : prefix ? a.prefix_len : paged::own_limit(a, s, j);
-      const T *q = static_cast<const T *>(a.q) + (int64_t)(s.first + j) * a.q_token +
-                   (int64_t)(head * a.group + (on ? row - j * a.group : 0)) * a.q_head;
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        const int c = kk * 16 + 2 * t;
-        qf[i][kk][h] = on && c < a.d ? *reinterpret_cast<const uint32_t *>(q + c) : 0u;
-        qf[i][kk][2 + h] = on && c + 8 < a.d ? *reinterpret_cast<const uint32_t *>(q + c + 8) : 0u;
-      }
-    }
-  }
   // keys below this are seen by every row of the block
   const int free_end = prefix ? a.prefix_len : paged::own_limit(a, s, row0 / a.group);
 
@@ -260,6 +245,30 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+  // The first tiles are on their way.  Queries as A fragments, straight from global memory: thread (g, t) holds
+  // rows g and g + 8 of each 16, columns 2t, 2t + 1 and 8 further.
+  const int g = lane >> 2, t = lane & 3;
+  uint32_t qf[MT][DP / 16][4];
+  int limit[MT][2];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = row0 + 16 * i + 8 * h + g;
+      const bool on = row < rows;
+      const int j = on ? row / a.group : 0;
+      limit[i][h] = !on ? 0 : prefix ? a.prefix_len : paged::own_limit(a, s, j);
+      const T *q = static_cast<const T *>(a.q) + (int64_t)(s.first + j) * a.q_token +
+                   (int64_t)(head * a.group + (on ? row - j * a.group : 0)) * a.q_head;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const int c = kk * 16 + 2 * t;
+        qf[i][kk][h] = on && c < a.d ? *reinterpret_cast<const uint32_t *>(q + c) : 0u;
+        qf[i][kk][2 + h] = on && c + 8 < a.d ? *reinterpret_cast<const uint32_t *>(q + c + 8) : 0u;
+      }
+    }
+  }
 
   const float c = a.scale_log2;
   const int id = lane >> 3, ir = lane & 7;
@@ -414,9 +423,9 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
 template <typename T, int DP, int MT>
 cudaError_t launch(b2k_ctx *ctx, const Args &a, const Grid &g, unsigned blocks, cudaStream_t s) {
   auto kernel = paged_mma_kernel<T, DP, MT>;
-  cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, smem_bytes<DP>());
+  cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, smem_bytes<DP, MT>());
   if (err != cudaSuccess) return err;
-  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP>(), s, a, g);
+  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP, MT>(), s, a, g);
 }
 
 template <typename T>
