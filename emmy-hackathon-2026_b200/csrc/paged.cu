@@ -10,8 +10,10 @@
 // keys at a time through shared memory as FP32.  Scores: lane = key, each
 // warp its own RW rows, so a key is read once for RW rows and the softmax of a
 // tile is one butterfly; the next tile is on its way meanwhile (asynchronous
-// copies where the cache is f32 in 16-byte pieces).  P V: lane = four dims, the probabilities shuffled
-// from their lanes; a probability of exactly zero skips its key, so what a
+// copies where the cache is f32 in 16-byte pieces).  P V: lane = four
+// dims, the probabilities read back four keys at a time as one broadcast
+// (shuffled one by one they took two thirds of the kernel's instructions).  In a
+// tile with masked keys a probability of exactly zero skips its key, so what a
 // masked place of the cache holds (infinities and NaN too) has no effect.
 #include <math.h>
 
@@ -38,21 +40,25 @@ __device__ __forceinline__ void copy16(void *dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 
-// DV: float4s of a head that a lane holds (head dim up to 128 DV).
+// DV: float4s of a head that a lane holds (head dim up to 128 DV; 0: up to 64,
+// where the two halves of a warp take every other four keys and add up at the end).
 // V: elements of one access to the cache (16 bytes, or 1).
-template <typename T, int RW, int DV, int V>
+template <typename T, int RW, int DV0, int V>
 __global__ void __launch_bounds__(kThreads)
     paged_rows_kernel(const __grid_constant__ Args a, bool prefix, int row_blocks, bool beside) {
   constexpr int R = RW * kWarps;
+  constexpr int DV = DV0 == 0 ? 1 : DV0, kSides = DV0 == 0 ? 2 : 1;
   constexpr bool kAsync = sizeof(T) == 4 && V == 4;  // the cache's bytes are the tile's
   extern __shared__ __align__(16) float smem[];
   __shared__ int64_t k_at[3][kTile], v_at[3][kTile];
+  __shared__ __align__(16) float ps[kWarps][RW][kTile];  // a warp's probabilities
   const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4;
   const int stage_floats = kTile * (ldk + dp);  // keys, then values; two stages behind the queries
   float *qs = smem, *tiles = qs + R * dp;
   paged::part_begin(beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int side = kSides == 2 ? lane >> 4 : 0, col = 4 * (kSides == 2 ? lane & 15 : lane);  // of a lane's output
   const int split = blockIdx.y, head = blockIdx.x / row_blocks, block = blockIdx.x % row_blocks, b = blockIdx.z;
   const int q_heads = a.kv_heads * a.group;
   paged::Sequence s = {0, 0, 0};
@@ -158,7 +164,11 @@ __global__ void __launch_bounds__(kThreads)
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
 
-    float p[RW];
+    // every key of the tile is seen by every row of the warp
+    bool open = key + kTile <= key_end;
+#pragma unroll
+    for (int i = 0; i < RW; ++i) open = open && key + kTile <= limit[i];
+    open = __all_sync(0xffffffffu, open && k_at[tile % 3][lane] >= 0);
     {
       float acc[RW];
 #pragma unroll
@@ -178,8 +188,9 @@ __global__ void __launch_bounds__(kThreads)
         const float mx = fmaxf(m[i], warp_max(sc));
         const float base = mx == -INFINITY ? 0.0f : mx;
         const float alpha = exp2_fast(m[i] - base);
-        p[i] = exp2_fast(sc - base);
-        l[i] = l[i] * alpha + p[i];  // this lane's keys; the lanes are added at the end
+        const float p = exp2_fast(sc - base);
+        ps[warp][i][lane] = p;
+        l[i] = l[i] * alpha + p;  // this lane's keys; the lanes are added at the end
         m[i] = mx;
 #pragma unroll
         for (int c = 0; c < DV; ++c) {
@@ -190,24 +201,28 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    const int keys = min(kTile, key_end - key);
-    for (int t = 0; t < keys; ++t) {
-      float4 vv[DV];
+    __syncwarp();
+    for (int t0 = 4 * side; t0 < kTile; t0 += 4 * kSides) {
+      float4 vv[4][DV];
 #pragma unroll
-      for (int c = 0; c < DV; ++c) {
-        const int at = 4 * lane + 128 * c;
-        vv[c] = at < dp ? *reinterpret_cast<const float4 *>(vs + t * dp + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int c = 0; c < DV; ++c)
+          vv[u][c] = col + 128 * c < dp ? *reinterpret_cast<const float4 *>(vs + (t0 + u) * dp + col + 128 * c)
+                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
-        const float pt = __shfl_sync(0xffffffffu, p[i], t);
-        if (pt != 0.0f) {
+        const float4 p4 = *reinterpret_cast<const float4 *>(&ps[warp][i][t0]);
+        const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (!open && p[u] == 0.0f) continue;  // a masked value may be anything
 #pragma unroll
           for (int c = 0; c < DV; ++c) {
-            o[i][c].x = fmaf(pt, vv[c].x, o[i][c].x);
-            o[i][c].y = fmaf(pt, vv[c].y, o[i][c].y);
-            o[i][c].z = fmaf(pt, vv[c].z, o[i][c].z);
-            o[i][c].w = fmaf(pt, vv[c].w, o[i][c].w);
+            o[i][c].x = fmaf(p[u], vv[u][c].x, o[i][c].x);
+            o[i][c].y = fmaf(p[u], vv[u][c].y, o[i][c].y);
+            o[i][c].z = fmaf(p[u], vv[u][c].z, o[i][c].z);
+            o[i][c].w = fmaf(p[u], vv[u][c].w, o[i][c].w);
           }
         }
       }
@@ -219,7 +234,13 @@ __global__ void __launch_bounds__(kThreads)
   for (int i = 0; i < RW; ++i) {
     const int row = row0 + warp * RW + i;
     const float total = warp_sum(l[i]);
-    if (row >= rows) continue;
+    if (kSides == 2) {
+      o[i][0].x += __shfl_xor_sync(0xffffffffu, o[i][0].x, 16);
+      o[i][0].y += __shfl_xor_sync(0xffffffffu, o[i][0].y, 16);
+      o[i][0].z += __shfl_xor_sync(0xffffffffu, o[i][0].z, 16);
+      o[i][0].w += __shfl_xor_sync(0xffffffffu, o[i][0].w, 16);
+    }
+    if (row >= rows || side == 1) continue;
     const int64_t token = s.first + row / a.group;
     const int qh = head * a.group + row % a.group;
     if (direct) {
@@ -230,7 +251,7 @@ __global__ void __launch_bounds__(kThreads)
         const float x[4] = {o[i][c].x, o[i][c].y, o[i][c].z, o[i][c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (4 * lane + 128 * c + e < a.d) out[4 * lane + 128 * c + e] = serve::from_f32<T>(x[e] * inv);
+          if (col + 128 * c + e < a.d) out[col + 128 * c + e] = serve::from_f32<T>(x[e] * inv);
       }
     } else {
       const int64_t at = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
@@ -240,7 +261,7 @@ __global__ void __launch_bounds__(kThreads)
         const float x[4] = {o[i][c].x, o[i][c].y, o[i][c].z, o[i][c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (4 * lane + 128 * c + e < a.d) a.part_o[at * a.d + 4 * lane + 128 * c + e] = x[e];
+          if (col + 128 * c + e < a.d) a.part_o[at * a.d + col + 128 * c + e] = x[e];
       }
     }
   }
@@ -448,7 +469,8 @@ int launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, bool beside,
   const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + 2 * kTile * (2 * dp + 4));
   constexpr int kFull = 16 / sizeof(T);
   auto kernel = vec ? paged_rows_kernel<T, RW, DV, kFull> : paged_rows_kernel<T, RW, DV, 1>;
-  constexpr int most = sizeof(float) * (RW * kWarps * 128 * DV + 2 * kTile * (2 * 128 * DV + 4));
+  constexpr int kMost = DV == 0 ? 64 : 128 * DV;  // head dim
+  constexpr int most = sizeof(float) * (RW * kWarps * kMost + 2 * kTile * (2 * kMost + 4));
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
   if (err == cudaSuccess)
     err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), smem, s, a, prefix, row_blocks, beside);
@@ -464,6 +486,11 @@ int rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, bool bes
   const size_t size = sizeof(T);
   const bool vec = a.d % (16 / (int)size) == 0 && serve::vec_ok(a.k, a.k_page, a.k_row, a.k_head, size, 16) &&
                    serve::vec_ok(a.v, a.v_page, a.v_row, a.v_head, size, 16);
+  if (a.d <= 64) {
+    if (rw == 1) return launch_rows<T, 1, 0>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+    if (rw == 2) return launch_rows<T, 2, 0>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+    return launch_rows<T, 8, 0>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+  }
   if (a.d <= 128) {
     if (rw == 1) return launch_rows<T, 1, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
     if (rw == 2) return launch_rows<T, 2, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
