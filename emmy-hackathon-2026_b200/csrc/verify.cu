@@ -17,9 +17,8 @@
 // nothing is kept in global memory between the two passes.
 #include <cooperative_groups.h>
 
-#include <limits.h>
-
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -27,7 +26,7 @@ namespace {
 
 constexpr int kCluster = 8;
 constexpr int kAhead = 8;   // elements a lane has in flight in the first pass
-constexpr int kRun = 4;     // consecutive elements of a thread in the second
+constexpr int kRun = 8;     // consecutive elements of a thread in the second
 
 struct VerifyArgs {
   b2k_drafts d;
@@ -51,11 +50,10 @@ __device__ __forceinline__ double warp_scan(double v) {
   return v;
 }
 
-// Of 32 lanes' sums in order: the first whose cumulative sum passes the
-// threshold, or the last that holds anything where rounding leaves none (-1:
-// none does), and the sum before it.
-__device__ __forceinline__ int pick(double v, double start, double threshold, double &before) {
-  const double upto = warp_scan(v);
+// Of 32 lanes' sums v in order, `upto` their cumulative sums: the first whose
+// cumulative sum passes the threshold, or the last that holds anything where
+// rounding leaves none (-1: none does), and the sum before it.
+__device__ __forceinline__ int pick(double v, double upto, double start, double threshold, double &before) {
   const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && start + upto > threshold);
   const unsigned held = __ballot_sync(0xffffffffu, v > 0.0);
   const int at = over ? __ffs(over) - 1 : held ? 31 - __clz(held) : -1;
@@ -68,15 +66,6 @@ __device__ __forceinline__ int pick(double v, double start, double threshold, do
 struct Rest {
   const float *p, *q;
   int64_t without;
-  __device__ __forceinline__ float at(int64_t i) const {
-    const float pi = __ldg(p + i);
-    const float qi = q ? __ldg(q + i) : 0.0f;
-    return pi > qi && i != without ? pi : 0.0f;  // the difference is taken in FP64
-  }
-  __device__ __forceinline__ double value(int64_t i) const {
-    const float pi = at(i);
-    return pi > 0.0f ? (double)pi - (q ? (double)__ldg(q + i) : 0.0) : 0.0;
-  }
 };
 
 template <int kThreads>
@@ -84,9 +73,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
   constexpr int kWarps = kThreads / 32;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ double run_sum[kWarps], scan_sum[kWarps], slice_sum;
+  __shared__ double run_sum[kWarps], scan_sum[kWarps], slice_sum[2];
   __shared__ int taken_s;
-  __shared__ long long first_hit, last_held;
+  __shared__ int warp_hit[kWarps], warp_last[kWarps];
   grid_dependency_wait();
   grid_dependents_launch();
 
@@ -133,56 +122,83 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
   int64_t token = -1;   // of the CTA that owns the draw
   bool owner = false;
   for (int pass = 0; pass < 2; ++pass) {  // the second only where the rest is zero everywhere
-    double sum = 0.0;
-    for (int64_t i = lo + lane; i < hi; i += 32 * kAhead) {
-      float pv[kAhead], qv[kAhead];
+    // FP64 sums of the run's elements, four chains a lane.  HAS_Q and WITHOUT as
+    // the rest has them: fewer comparisons where it has not.
+    auto sum_run = [&](auto has_q, auto without) {
+      constexpr bool kQ = decltype(has_q)::value, kWithout = decltype(without)::value;
+      double s[4] = {0.0, 0.0, 0.0, 0.0};
+      const float *p = rest.p + lane, *q = rest.q + (kQ ? lane : 0);
+      const int skip = kWithout ? (int)(rest.without - lane) : 0;  // (vocab is below 2^31)
+      int i = (int)lo;
+      const int end = (int)hi;
+      for (; i + 32 * kAhead <= end; i += 32 * kAhead) {
+        float pv[kAhead], qv[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const bool in = i + 32 * u < hi;
-        pv[u] = in ? __ldg(rest.p + i + 32 * u) : 0.0f;
-        qv[u] = in && rest.q ? __ldg(rest.q + i + 32 * u) : 0.0f;
+        for (int u = 0; u < kAhead; ++u) {
+          pv[u] = __ldg(p + i + 32 * u);
+          qv[u] = kQ ? __ldg(q + i + 32 * u) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (pv[u] > qv[u] && !(kWithout && i + 32 * u == skip)) s[u & 3] += kQ ? (double)pv[u] - (double)qv[u] : (double)pv[u];
       }
+      if (i < end) {  // the rest of the run, all of it in flight too
+        float pv[kAhead], qv[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (pv[u] > qv[u] && i + 32 * u != rest.without) sum += (double)pv[u] - (double)qv[u];
-    }
+        for (int u = 0; u < kAhead; ++u) {
+          const bool in = i + 32 * u + lane < end;
+          pv[u] = in ? __ldg(p + i + 32 * u) : 0.0f;
+          qv[u] = in && kQ ? __ldg(q + i + 32 * u) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (pv[u] > qv[u] && !(kWithout && i + 32 * u == skip)) s[u & 3] += kQ ? (double)pv[u] - (double)qv[u] : (double)pv[u];
+      }
+      return (s[0] + s[1]) + (s[2] + s[3]);
+    };
+    double sum = rest.q ? sum_run(std::true_type{}, std::false_type{})
+                 : rest.without >= 0 ? sum_run(std::false_type{}, std::true_type{})
+                                     : sum_run(std::false_type{}, std::false_type{});
     sum = warp_sum(sum);
     if (lane == 0) run_sum[warp] = sum;
     __syncthreads();
     const double mine_of = lane < kWarps ? run_sum[lane] : 0.0;  // each warp scans the runs' sums for itself
-    const double slice_total = __shfl_sync(0xffffffffu, warp_scan(mine_of), 31);
-    if (threadIdx.x == 0) slice_sum = slice_total;
+    const double mine_upto = warp_scan(mine_of), slice_total = __shfl_sync(0xffffffffu, mine_upto, 31);
+    if (threadIdx.x == 0) slice_sum[pass] = slice_total;
     cluster.sync();
-    const double slice = lane < kCluster ? *cluster.map_shared_rank(&slice_sum, lane < kCluster ? lane : 0) : 0.0;
-    const double total = __shfl_sync(0xffffffffu, warp_scan(slice), 31);
-    cluster.sync();  // every CTA has read: the sums may be written again, or the CTA leave
+    const double slice = lane < kCluster ? *cluster.map_shared_rank(&slice_sum[pass], lane < kCluster ? lane : 0) : 0.0;
+    const double slices_upto = warp_scan(slice), total = __shfl_sync(0xffffffffu, slices_upto, 31);
     if (!(total > 0.0) && pass == 0 && taken < n) {
       rest.q = nullptr;
       rest.without = -1;
       continue;
     }
+    cluster.barrier_arrive();  // this thread has read; who leaves waits for all of them
     // the slice, then the run in it, whose cumulative sum first passes the
     // threshold; rounding may leave none, then the last one that holds anything
     const double threshold = (double)d.u_sample[b] * total;
     double start, run_start;
-    const int slice_at = pick(slice, 0.0, threshold, start);
+    const int slice_at = pick(slice, slices_upto, 0.0, threshold, start);
     if (slice_at == rank) {
-      const int run_at = pick(mine_of, start, threshold, run_start);
+      const int run_at = pick(mine_of, mine_upto, start, threshold, run_start);
       // run_at is one for the whole CTA: its elements in order, kRun a thread,
       // kRun * kThreads at a time
       owner = true;
       const int64_t run_lo = min(d.vocab, (rank * kWarps + run_at) * run), run_hi = min(d.vocab, run_lo + run);
-      if (threadIdx.x == 0) {
-        first_hit = LLONG_MAX;
-        last_held = -1;
-      }
       double base = run_start;
       for (int64_t i0 = run_lo; i0 < run_hi; i0 += kRun * kThreads) {
-        double v[kRun], mine = 0.0;
         const int64_t i = i0 + threadIdx.x * kRun;
+        float pv[kRun], qv[kRun];
 #pragma unroll
         for (int u = 0; u < kRun; ++u) {
-          v[u] = i + u < run_hi ? rest.value(i + u) : 0.0;
+          const bool in = i + u < run_hi;
+          pv[u] = in ? __ldg(rest.p + i + u) : 0.0f;
+          qv[u] = in && rest.q ? __ldg(rest.q + i + u) : 0.0f;
+        }
+        double v[kRun], mine = 0.0;
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) {
+          v[u] = pv[u] > qv[u] && i + u != rest.without ? (double)pv[u] - (double)qv[u] : 0.0;
           mine += v[u];
         }
         const double upto = warp_scan(mine);  // over the lanes, then over the warps
@@ -190,23 +206,33 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
         __syncthreads();
         const double warps = lane < kWarps ? scan_sum[lane] : 0.0, warps_upto = warp_scan(warps);
         double c = base + __shfl_sync(0xffffffffu, warps_upto - warps, warp) + (upto - mine);
-        const double whole = base + __shfl_sync(0xffffffffu, warps_upto, 31);
-        int64_t hit = -1, last = -1;
+        base += __shfl_sync(0xffffffffu, warps_upto, 31);
+        int hit = -1, last = -1;
 #pragma unroll
         for (int u = 0; u < kRun; ++u) {
           c += v[u];
           if (v[u] > 0.0) {
-            last = i + u;
-            if (hit < 0 && c > threshold) hit = i + u;
+            last = (int)(i + u);
+            if (hit < 0 && c > threshold) hit = (int)(i + u);
           }
         }
-        if (hit >= 0) atomicMin(&first_hit, (long long)hit);
-        if (last >= 0) atomicMax(&last_held, (long long)last);
-        base = whole;
+        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), held = __ballot_sync(0xffffffffu, last >= 0);
+        hit = hits ? __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1) : -1;
+        last = held ? __shfl_sync(0xffffffffu, last, 31 - __clz(held)) : -1;
+        if (lane == 0) {
+          warp_hit[warp] = hit;
+          warp_last[warp] = last;
+        }
         __syncthreads();
-        if (first_hit != LLONG_MAX) break;
+        hit = lane < kWarps ? warp_hit[lane] : -1;
+        last = lane < kWarps ? warp_last[lane] : -1;
+        const unsigned hit_warps = __ballot_sync(0xffffffffu, hit >= 0), held_warps = __ballot_sync(0xffffffffu, last >= 0);
+        if (hit_warps) {
+          token = __shfl_sync(0xffffffffu, hit, __ffs(hit_warps) - 1);
+          break;
+        }
+        if (held_warps) token = __shfl_sync(0xffffffffu, last, 31 - __clz(held_warps));
       }
-      token = first_hit != LLONG_MAX ? first_hit : last_held;
     } else if (slice_at < 0) {
       owner = rank == 0;  // nothing above zero: token -1
     }
@@ -218,6 +244,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
     for (int i = lane; i <= d.drafts; i += 32)
       if (i != taken) a.tokens[b * (d.drafts + 1) + i] = i < taken ? drafted[i] : -1;
   }
+  cluster.barrier_wait();
 }
 
 }  // namespace
