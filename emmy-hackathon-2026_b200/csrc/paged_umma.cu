@@ -154,22 +154,35 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t mn_stride, 
          static_cast<uint64_t>(2u) << 61;
 }
 
-// D (+)= A B, both operands in shared memory / A in tensor memory; warp-wide.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+// Four products D (+)= A B of 16 steps of K each, issued by one elected lane of a
+// converged warp: A in shared memory, K-major like B, 32 bytes (2 units of a
+// descriptor's address) a step; or A in tensor memory, eight columns a step,
+// and B N-major, 2048 bytes a step.  The first overwrites D unless `accumulate`.
+__device__ __forceinline__ void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred e, p;\n\t"
+      "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
+      "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred e, p;\n\t"
+      "{\n\t.reg .pred e, p, t;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.s64 b1, %2, 128;\n\tadd.u32 a2, %1, 16;\n\tadd.s64 b2, %2, 256;\n\t"
+      "add.u32 a3, %1, 24;\n\tadd.s64 b3, %2, 384;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
@@ -402,10 +415,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto issue_s = [&](int x, int j) {
       const uint32_t k = item_addr(2 * j), q = q_addr + x * kTile, d = tmem + kColS + x * 128;
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
-        mma_ss(d, sm100::desc_kmajor<128>(q + off), sm100::desc_kmajor<128>(k + off), id_s, kk != 0);
-      }
+      for (int half = 0; half < DP / 64; ++half)
+        mma4_ss(d, sm100::desc_kmajor<128>(q + half * kHalf), sm100::desc_kmajor<128>(k + half * kHalf), id_s, half != 0);
       sm100::mma_commit(&s_full[x]);
     };
     auto issue_o = [&](int x, int j, bool last) {
@@ -415,9 +426,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && sm100::mbar_wait_warp(&p_full[x][half], j & 1, a.err, sm100::kSiteMmaFull, abort);
         if (!ok) return;
         sm100::tc_fence_after();
-#pragma unroll
-        for (int kk = half * kKeys / 32; kk < (half + 1) * kKeys / 32; ++kk)
-          mma_ts(d, p + kk * 8, desc_mn(v + kk * 2048, kHalf, 1024), id_o, j != 0 || kk != 0);
+        mma4_ts(d, p + half * 32, desc_mn(v + half * 8192, kHalf, 1024), id_o, j != 0 || half != 0);
+        // the keys of the next score, looked for while the second half is computed
+        if (half == 0 && x == 0 && j + 1 < tiles) wait_item(2 * j + 2);
       }
       if (last) sm100::mma_commit(&o_full[x]);
     };
@@ -444,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < 2; ++x) {
           if (ok && j < tiles_of(x)) issue_o(x, j, j + 1 == tiles_of(x));
           if (ok && x == 1) sm100::mma_commit(&empty[(2 * j + 1) % kStages]);
-          if (ok && x == 0 && j + 1 < tiles) wait_item(2 * j + 2);
+          if (ok && x == 0 && j >= tiles_of(0) && j + 1 < tiles) wait_item(2 * j + 2);
           if (ok && j + 1 < tiles_of(x)) issue_s(x, j + 1);
         }
         if (ok && j + 1 < tiles) sm100::mma_commit(&empty[(2 * j + 2) % kStages]);
@@ -547,24 +558,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (A third of the exponentials as a polynomial on the FMA units lengthens
       // the tile, 257 -> 282 us for prompt chunks: two warps a scheduler do not
       // hide its chains.)
+      auto release = [&](int h) {  // the product of these keys may begin
+        sm100::tmem_st_wait();
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&p_full[x][h]);
+      };
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pk[32];
+      for (int h = 0; h < 4; ++h) {
+        uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
+        for (int i = 0; i < 32; i += 2) {
           float p0, p1;
-          unpair(fma2(pair(__uint_as_float(sr[64 * h + i]), __uint_as_float(sr[64 * h + i + 1])), c2, from2), p0, p1);
+          unpair(fma2(pair(__uint_as_float(sr[32 * h + i]), __uint_as_float(sr[32 * h + i + 1])), c2, from2), p0, p1);
           p0 = exp2_fast(p0);
           p1 = exp2_fast(p1);
           sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair(p0, p1));
           pk[i / 2] = Type<T>::pack(p0, p1);
         }
-        sm100::tmem_st_32x32b_x32(s_at + 32 * h, pk);
-        sm100::tmem_st_wait();
-        sm100::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&p_full[x][h]);  // the product of these keys may begin
+        if (h == 2) release(0);  // its stores have landed meanwhile
+        sm100::tmem_st_32x32b_x16(s_at + 16 * h, pk);
       }
+      release(1);
       float l0, l1;
       unpair(add2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;

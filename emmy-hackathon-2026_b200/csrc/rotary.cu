@@ -15,8 +15,7 @@
 // warp.  The lanes share out the token's cosines and sines through shared memory
 // while the first heads' loads are in flight; then every lane keeps one place
 // of the head (16 bytes of each half of its pairs, its cosines in registers)
-// and walks the heads, two loads of two vectors ahead (four halve the warps that
-// fit an SM: 61 us against 59 for 16384 tokens x 40 heads of 128, bf16).
+// and walks the heads, a few loads of two vectors ahead.
 #include <math.h>
 
 #include <algorithm>
@@ -28,7 +27,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kAhead = 2;       // heads a lane has in flight
 constexpr int kMaxPairs = B2K_ROPE_MAX_PAIRS;
 
 enum Target : int { kLinear = 0, kKeys = 1, kValues = 2 };
@@ -80,9 +78,19 @@ __device__ __forceinline__ void narrow(const float (&x)[V], serve::Pack<T, V> &p
   }
 }
 
+// Heads a lane has in flight, and blocks an SM.  Sixteen cosines and sines of
+// 16-byte vectors of a 16-bit type leave registers for two blocks without
+// spills, which then load four heads ahead (16384 tokens x 40 heads of 128,
+// bf16: 58 us; two heads and three blocks 60, and four blocks 68 with spills);
+// the others run four blocks two heads ahead (6001 tokens x 32 heads of 64,
+// f32: 21 us, with three blocks 24, with two 30).
+template <typename T, int V>
+constexpr bool kWide = V * sizeof(T) == 16 && sizeof(T) == 2;
+
 template <typename T, int V, bool PAGED>
-__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, kWide<T, V> ? 2 : 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   using P = serve::Pack<T, V>;
+  constexpr int kAhead = kWide<T, V> ? 4 : 2;
   __shared__ __align__(16) float cs[kWarps][kMaxPairs], sn[kWarps][kMaxPairs];
   grid_dependency_wait();
   grid_dependents_launch();
