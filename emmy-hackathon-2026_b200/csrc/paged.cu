@@ -455,8 +455,23 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   if (b.prefix_len > 0 && !p.joined) {
     p.prefix_path = pick_path(tensor, c.d, prefix, b.prefix_len, c.heads);
     p.prefix_rows = block_rows(p.prefix_path, c.d, prefix);
-    split_keys(b.prefix_len, (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads, wave(p.prefix_path),
-               least(p.prefix_path), tile(p.prefix_path), p.prefix_splits, p.prefix_chunk);
+    const int64_t units = (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads;
+    int64_t want = wave(p.prefix_path);
+    if (p.prefix_path == kUmma && p.own_path != kUmma) {
+      // The prefix part's blocks, one an SM, run beside the own part, which
+      // needs the other SMs' loads more than it needs the prefix part done:
+      // the fewest splits that do not make it the last to end, by what both
+      // take (a block 8 us and 2 us for each 128 keys; the own part the time of
+      // its bytes at 5.4 TB/s, for sequences that are 0.6 of the longest on
+      // average).  128 sequences of up to 1000 behind 8192 tokens, 32 units:
+      // 152 us with one split, 95 with two, 102 with three, 109 with four.
+      const double own_us = 0.6 * b.sequences * (double)b.max_len * c.heads * c.d * 4 / 5.4e6;
+      for (int64_t s = 1; s * units < want; ++s) {
+        const double block_us = 8.0 + 2.0 * ((b.prefix_len + s * 128 - 1) / (s * 128));
+        if (block_us <= (units * s * block_us) / sms + own_us) want = s * units;
+      }
+    }
+    split_keys(b.prefix_len, units, want, least(p.prefix_path), tile(p.prefix_path), p.prefix_splits, p.prefix_chunk);
   }
   const size_t slots = (size_t)p.own_splits + p.prefix_splits;
   if (slots > 1) p.bytes = ml_bytes(slots, b.tokens, q_heads) + slots * (size_t)b.tokens * q_heads * c.d * sizeof(float);

@@ -94,14 +94,17 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
 // whose results it does not read.  Every block of the prefix part lets the
 // next kernel start only behind its own wait for what precedes the call, so a
 // block of the own part that has started needs no wait to read queries and
-// cache.  It waits at its end instead, so that the merge, which waits for the
-// own part, has both.
+// cache.  Its last block waits at its end instead, so that the own part's end
+// means the prefix part's too and the merge, which waits for the own part, has
+// both.  (The last block alone: waiting blocks hold their place on an SM, and
+// with all of them waiting the two parts all but took turns.)
 __device__ __forceinline__ void part_begin(bool beside) {
   if (!beside) grid_dependency_wait();
   grid_dependents_launch();
 }
 __device__ __forceinline__ void part_end(bool beside) {
-  if (beside) grid_dependency_wait();
+  if (beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+    grid_dependency_wait();
 }
 
 // paged_mma.cu: rows of a block (16 or 32) for `rows` rows of one cache head, and
