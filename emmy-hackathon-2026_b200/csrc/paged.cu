@@ -412,8 +412,11 @@ bool rows_pieces(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_tok
 // million rows x keys a microsecond at head dim 128) it repays the 10 us that
 // its launch and its blocks' starts cost from about 16 million on.  Head dims
 // above 128 do not fit its tensor memory twice.
+int g_kernel = 0;  // b2k_paged_attention_set_kernel
+
 Path pick_path(bool tensor, int d, int64_t rows, int64_t keys, int64_t units) {
-  if (!tensor) return kPlain;
+  if (!tensor || g_kernel == 1) return kPlain;
+  if (g_kernel > 1) return g_kernel == 3 && d <= 128 ? kUmma : kMma;
   return rows > 32 && d <= 128 && (double)rows * keys * units * d > 16e6 * 128 ? kUmma : kMma;
 }
 int block_rows(Path path, int d, int64_t rows) {
@@ -560,6 +563,38 @@ int check_call(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch
 
 }  // namespace
 
+// Everything about a call's arguments but its workspace, and its plan.
+static int check_operands(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch, const b2k_heads *q,
+                          const b2k_heads *o, int sms, Plan &p) {
+  const char *what = "paged_attention";
+  if (!q) return b2k::fail(ctx, B2K_EINVAL, "%s: no q", what);
+  int status = check_call(ctx, cache, batch, q->heads);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "o", o, batch->tokens, cache->d);
+  if (status != B2K_OK) return status;
+  if (q->heads != o->heads) return b2k::fail(ctx, B2K_EINVAL, "%s: %d heads in, %d out", what, q->heads, o->heads);
+  if (q->data == o->data && batch->tokens > 0) return b2k::fail(ctx, B2K_EINVAL, "%s: o is q", what);
+  p = make_plan(*cache, *batch, q->heads, sms, cache_pieces(*cache) && rows_pieces(*q) && rows_pieces(*o));
+  return B2K_OK;
+}
+
+extern "C" int b2k_paged_attention_set_kernel(int mode) {
+  if (mode < 0 || mode > 3) return B2K_EINVAL;
+  g_kernel = mode;
+  return B2K_OK;
+}
+
+extern "C" int b2k_paged_attention_plan(int32_t sms, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
+                                        const b2k_heads *q, const b2k_heads *o, b2k_paged_attention_plan_info *out) {
+  if (sms < 1 || !out) return B2K_EINVAL;
+  Plan p;
+  const int status = check_operands(nullptr, cache, batch, q, o, sms, p);
+  if (status != B2K_OK) return status;
+  *out = {(int32_t)p.own_path, p.prefix_splits > 0 ? (int32_t)p.prefix_path : -1, p.own_splits, p.own_chunk,
+          p.prefix_splits, p.prefix_chunk, p.joined, 0, (int64_t)p.bytes};
+  return B2K_OK;
+}
+
 extern "C" int b2k_paged_attention_workspace(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
                                              int32_t q_heads, size_t *bytes) {
   if (!ctx) return B2K_EINVAL;
@@ -577,17 +612,11 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
                                    size_t workspace_bytes, void *stream) {
   B2K_CHECK_CTX(ctx);
   const char *what = "paged_attention";
-  if (!q) return b2k::fail(ctx, B2K_EINVAL, "%s: no q", what);
-  int status = check_call(ctx, cache, batch, q->heads);
-  if (status == B2K_OK) status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d);
-  if (status == B2K_OK) status = serve::check_heads(ctx, what, "o", o, batch->tokens, cache->d);
-  if (status != B2K_OK) return status;
-  if (q->heads != o->heads) return b2k::fail(ctx, B2K_EINVAL, "%s: %d heads in, %d out", what, q->heads, o->heads);
-  if (q->data == o->data && batch->tokens > 0) return b2k::fail(ctx, B2K_EINVAL, "%s: o is q", what);
   if (!(scale_div > 0.0f) || !isfinite(scale_div)) return b2k::fail(ctx, B2K_EINVAL, "%s: scale %g", what, scale_div);
+  Plan p;
+  const int status = check_operands(ctx, cache, batch, q, o, ctx->sm_count, p);
+  if (status != B2K_OK) return status;
   if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
-  const Plan p = make_plan(*cache, *batch, q->heads, ctx->sm_count,
-                           cache_pieces(*cache) && rows_pieces(*q) && rows_pieces(*o));
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return b2k::fail(ctx, B2K_EINVAL, "%s: a workspace of %zu bytes where %zu are needed", what,
                      workspace ? workspace_bytes : (size_t)0, p.bytes);

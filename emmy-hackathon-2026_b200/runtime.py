@@ -131,6 +131,13 @@ class PagedBatch(C.Structure):
                 ("max_len", C.c_int32), ("prefix_len", C.c_int32), ("prefix_table", C.c_void_p)]
 
 
+class PagedAttentionPlan(C.Structure):
+    """b2k_paged_attention_plan_info: what one b2k_paged_attention call launches."""
+    _fields_ = [("own_kernel", C.c_int32), ("prefix_kernel", C.c_int32), ("own_splits", C.c_int32),
+                ("own_chunk", C.c_int32), ("prefix_splits", C.c_int32), ("prefix_chunk", C.c_int32),
+                ("joined", C.c_int32), ("reserved", C.c_int32), ("workspace_bytes", C.c_int64)]
+
+
 class Drafts(C.Structure):
     """b2k_drafts: drafted tokens, both models' probabilities and the random numbers."""
     _fields_ = [("target", C.c_void_p), ("draft", C.c_void_p), ("ld_target", C.c_int64), ("ld_draft", C.c_int64),
@@ -195,6 +202,9 @@ SIGNATURES: dict[str, tuple] = {
                                       C.c_int),
     "b2k_paged_attention": ([_P, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(Heads), C.POINTER(Heads), _F,
                              _P, _SZ, _P], C.c_int),
+    "b2k_paged_attention_plan": ([_I32, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(Heads),
+                                  C.POINTER(Heads), C.POINTER(PagedAttentionPlan)], C.c_int),
+    "b2k_paged_attention_set_kernel": ([C.c_int], C.c_int),
     "b2k_verify_drafts": ([_P, C.POINTER(Drafts), _P, _P, _P], C.c_int),
     "b2k_mgpu_partition": ([_I64, _I32, _I32, _I64, C.POINTER(_I64), C.POINTER(_I64)], C.c_int),
     "b2k_mgpu_unique_id": ([_P], C.c_int),
@@ -309,6 +319,17 @@ def paged_slot(table_row, pages: int, page_size: int, position: int) -> int:
     """Cache row of a position under a table row (b2k_paged_slot; host arithmetic), -1 where there is none."""
     row = (C.c_int32 * max(1, len(table_row)))(*table_row)
     return library().b2k_paged_slot(row, len(table_row), pages, page_size, position)
+
+
+def paged_attention_plan(sms: int, cache: PagedCache, batch: PagedBatch, q: Heads, o: Heads) -> dict:
+    """What :meth:`Context.paged_attention` launches for these operands on a GPU of `sms` SMs
+    (b2k_paged_attention_plan): host arithmetic, no GPU; addresses are read only for their alignment."""
+    out = PagedAttentionPlan()
+    status = library().b2k_paged_attention_plan(sms, C.byref(cache), C.byref(batch), C.byref(q), C.byref(o),
+                                                C.byref(out))
+    if status != B2K_OK:
+        raise B2KError(status, "arguments b2k_paged_attention refuses", "b2k_paged_attention_plan")
+    return {name: getattr(out, name) for name, _ in PagedAttentionPlan._fields_ if name != "reserved"}
 
 
 class BoundCall:
@@ -530,6 +551,10 @@ class Context:
         return BoundCall(self, "b2k_paged_attention", self._paged_attention_args(cache, batch, q, o, workspace,
                                                                                  nbytes, **kw),
                          keep=(cache, batch, q, o))
+
+    def set_paged_attention_kernel(self, mode: int) -> None:
+        """0 = by operands and sizes (default); 1 = plain cores, 2 = warp MMAs, 3 = tensor memory, where they apply."""
+        self.check(self.lib.b2k_paged_attention_set_kernel(int(mode)), "b2k_paged_attention_set_kernel")
 
     def _verify_args(self, target, drafted, u_accept, u_sample, accepted, tokens, batch, drafts, vocab, draft=0,
                      counts=0, ld_target=None, ld_draft=None, stream=0) -> tuple:

@@ -432,7 +432,9 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
  *   o = sum_s softmax_s(q . k_s / scale_div) v_s.
  * Query head h reads cache head h / (q heads / cache heads).  A row that sees
  * no key is zero.  FP32 softmax and sums; f16 and bf16 operands run on the
- * tensor cores, with the probabilities rounded to the operands' type.
+ * tensor cores, with the probabilities rounded to the operands' type.  Rows of a
+ * page that hold no token may hold anything.  A later token's value that an
+ * earlier one may not see is multiplied by zero there, so it has to be finite.
  * `workspace` (device memory of the caller's, `workspace_bytes` at least what
  * b2k_paged_attention_workspace says, 16-byte aligned; may be NULL when that
  * is 0) holds what parts of one row's keys have summed; calls that may run at
@@ -441,6 +443,26 @@ int b2k_paged_attention_workspace(b2k_ctx *ctx, const b2k_paged_cache *cache, co
                                   int32_t q_heads, size_t *bytes);
 int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch, const b2k_heads *q,
                         const b2k_heads *o, float scale_div, void *workspace, size_t workspace_bytes, void *stream);
+/* What a call with these operands launches on a GPU of `sms` SMs, under the
+ * current setting below: host arithmetic only (no GPU; no pointer is
+ * dereferenced, addresses are read for their alignment).  B2K_EINVAL and
+ * B2K_EUNSUPPORTED where the call is refused. */
+typedef struct b2k_paged_attention_plan_info {
+  int32_t own_kernel, prefix_kernel; /* 0 plain cores, 1 warp MMAs, 2 tensor memory; prefix -1: no part of its own */
+  int32_t own_splits, own_chunk;     /* splits of the sequences' own keys, keys of each */
+  int32_t prefix_splits, prefix_chunk;
+  int32_t joined;                    /* 1: each sequence reads the prefix with its own keys */
+  int32_t reserved;
+  int64_t workspace_bytes;
+} b2k_paged_attention_plan_info;
+int b2k_paged_attention_plan(int32_t sms, const b2k_paged_cache *cache, const b2k_paged_batch *batch, const b2k_heads *q,
+                             const b2k_heads *o, b2k_paged_attention_plan_info *out);
+/* Process-wide choice of b2k_paged_attention's kernels, kept for comparisons
+ * and tests: 0 (default) by operands and sizes; 1 the plain cores always; 2
+ * warp MMAs, 3 tensor memory, wherever the operands (and for 3 the head dim, at
+ * most 128) allow, and 1 or 2 elsewhere.  Other values return B2K_EINVAL.  A
+ * workspace is asked for under the setting it is used with. */
+int b2k_paged_attention_set_kernel(int mode);
 
 /* --- verification of drafted tokens ------------------------------------------------
  * For each of `batch` sequences with `drafts` drafted tokens x_0 .. x_{n-1},

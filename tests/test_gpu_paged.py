@@ -15,6 +15,17 @@ rt = importlib.import_module(f"{PKG}.runtime")
 CODES = {torch.float32: rt.F32, torch.float16: rt.F16, torch.bfloat16: rt.BF16}
 
 
+KERNELS = {"rule": 0, "plain": 1, "warp": 2, "memory": 3}
+
+
+@pytest.fixture(params=list(KERNELS))
+def kernel(request, ctx):
+    """Each kernel in turn, wherever it applies, and the rule that chooses among them."""
+    ctx.set_paged_attention_kernel(KERNELS[request.param])
+    yield request.param
+    ctx.set_paged_attention_kernel(0)
+
+
 def heads(x):
     return rt.heads(x.data_ptr(), x.shape[1], x.stride(0), x.stride(1))
 
@@ -76,7 +87,9 @@ CASES = [
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("case", range(len(CASES)))
-def test_attention_matches(ctx, torch_cuda, dtype, case):
+def test_attention_matches(ctx, torch_cuda, kernel, dtype, case):
+    if dtype == "f32" and kernel != "rule":
+        pytest.skip("f32 has one kernel")
     new, lengths, prefix, page, hq, hkv, d, head_major = CASES[case]
     bt = refs.batch(new, lengths, prefix=prefix, page=page, heads=hkv, d=d, dtype=refs.DTYPES[dtype], head_major=head_major,
                     seed=case, extra_rows=2)
@@ -92,9 +105,20 @@ def test_attention_odd_head_dims(ctx, torch_cuda, dtype, d):
     check(ctx, bt, q, scale=0.7)
 
 
+@pytest.mark.parametrize("page", [1, 4, 8, 16, 20, 24, 64, 128, 256, 384])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (3, 1, 128), (14, 2, 80), (16, 1, 128), (32, 2, 40)])
+def test_attention_page_sizes_and_groups(ctx, torch_cuda, kernel, page, hq, hkv, d):
+    """Boxes of pages, of tokens by heads, and what neither fits; tiles that end in a prefix, a page and a length."""
+    dt = torch.bfloat16 if page % 16 else torch.float16
+    bt = refs.batch([33, 1, 0, 150], [260, 129, 7, 150], prefix=157, page=page, heads=hkv, d=d, dtype=dt, seed=page + d,
+                    head_major=bool(hq % 2), extra_rows=1)
+    q = torch.randn(bt.tokens, hq, d, device="cuda", generator=bt.generator).to(dt)
+    check(ctx, bt, q)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("shift", [0, 1])
-def test_attention_strided_operands(ctx, torch_cuda, dtype, shift):
+def test_attention_strided_operands(ctx, torch_cuda, kernel, dtype, shift):
     """Keys and values side by side in one buffer, queries out of a fused projection, outputs with gaps; shift moves every
     base off its 16 bytes."""
     dt, d, h = refs.DTYPES[dtype], 64, 2
@@ -117,7 +141,7 @@ def test_attention_strided_operands(ctx, torch_cuda, dtype, shift):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("new,lengths,prefix", [([1, 3], [200, 90], 64), ([70, 150], [170, 150], 100)])
-def test_attention_large_scores_and_one_hot_rows(ctx, torch_cuda, dtype, new, lengths, prefix):
+def test_attention_large_scores_and_one_hot_rows(ctx, torch_cuda, kernel, dtype, new, lengths, prefix):
     """Scores of hundreds: the running maximum moves far, and a row may be one key alone."""
     dt = refs.DTYPES[dtype]
     bt = refs.batch(new, lengths, prefix=prefix, heads=2, d=64, dtype=dt, seed=9)
@@ -126,7 +150,7 @@ def test_attention_large_scores_and_one_hot_rows(ctx, torch_cuda, dtype, new, le
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_attention_far_pages(ctx, torch_cuda, dtype):
+def test_attention_far_pages(ctx, torch_cuda, kernel, dtype):
     """Pages beyond 2^31 elements of the cache's start."""
     dt, page, h, d = refs.DTYPES[dtype], 64, 4, 128
     per = page * h * d
@@ -149,7 +173,7 @@ def test_attention_far_pages(ctx, torch_cuda, dtype):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("new", [[1, 1], [3, 90]])
-def test_attention_in_graphs_and_streams(ctx, torch_cuda, dtype, new):
+def test_attention_in_graphs_and_streams(ctx, torch_cuda, kernel, dtype, new):
     """Two captured calls with workspaces of their own, replayed at once with lengths changed since the capture."""
     dt, runs = refs.DTYPES[dtype], []
     for seed in (1, 2):
@@ -179,7 +203,7 @@ def test_attention_in_graphs_and_streams(ctx, torch_cuda, dtype, new):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_attention_same_bits_every_time(ctx, torch_cuda, dtype):
+def test_attention_same_bits_every_time(ctx, torch_cuda, kernel, dtype):
     bt = refs.batch([1, 4, 60], [900, 500, 300], prefix=800, heads=2, d=128, dtype=refs.DTYPES[dtype])
     q = torch.randn(bt.tokens, 8, 128, device="cuda").to(bt.dtype)
     one = run(ctx, bt, q)
@@ -190,7 +214,7 @@ def test_attention_same_bits_every_time(ctx, torch_cuda, dtype):
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("new", [[1, 1, 1], [2, 80, 1]])
 @pytest.mark.parametrize("what", ["page", "negative page", "prefix page", "long", "too many new"])
-def test_attention_index_out_of_bounds(ctx, torch_cuda, dtype, new, what):
+def test_attention_index_out_of_bounds(ctx, torch_cuda, kernel, dtype, new, what):
     """A bad page hides its keys, a bad length or count leaves its rows alone; the next sync reports it."""
     bt = refs.batch(new, [90, 90, 45], prefix=40, heads=2, d=64, dtype=refs.DTYPES[dtype])
     q = torch.randn(bt.tokens, 4, 64, device="cuda", generator=bt.generator).to(bt.dtype)
@@ -239,6 +263,56 @@ def bt_without(bt, b, page, keep):
     for cache, rows in ((c.k, rows_k), (c.v, rows_v)):
         refs.write_rows(c, cache, b, rows[keep.cuda()])
     return c
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_only_prefix(ctx, torch_cuda, kernel, dtype):
+    """No own keys at all, and no table for them: every row sees the prefix alone."""
+    bt = refs.batch([1, 2], [0, 0], prefix=333, heads=2, d=64, dtype=refs.DTYPES[dtype])
+    q = torch.randn(3, 4, 64, device="cuda", generator=bt.generator).to(bt.dtype)
+    cache, batch = call_parts(bt)
+    batch.table, batch.table_width, batch.table_stride = None, 0, 0
+    o = run(ctx, bt, q, parts=(cache, batch))
+    want, tol = refs.attention(bt, q)
+    refs.close(o, want, tol, q.dtype, "prefix alone")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_calls_side_by_side(ctx, torch_cuda, kernel, dtype):
+    """Calls on several streams at once, each with its own workspace, and back to back in one with one workspace."""
+    dt, jobs = refs.DTYPES[dtype], []
+    for seed in range(4):
+        bt = refs.batch([1 + seed, 40], [500, 200 + seed], prefix=200, heads=2, d=128, dtype=dt, seed=seed)
+        q = torch.randn(bt.tokens, 8, 128, device="cuda", generator=bt.generator).to(dt)
+        cache, batch = call_parts(bt)
+        nbytes = ctx.paged_attention_workspace(cache, batch, 8)
+        jobs.append((bt, q, torch.zeros_like(q), torch.empty(max(16, nbytes), dtype=torch.uint8, device="cuda"), nbytes,
+                     cache, batch, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for bt, q, o, ws, nbytes, cache, batch, s in jobs:
+            ctx.paged_attention(cache, batch, heads(q), heads(o), ws.data_ptr(), nbytes, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for bt, q, o, *_ in jobs:
+        want, tol = refs.attention(bt, q)
+        refs.close(o, want, tol, dt, "streams")
+        o.zero_()
+    shared = torch.empty(max(16, *(j[4] for j in jobs)), dtype=torch.uint8, device="cuda")
+    for bt, q, o, _, nbytes, cache, batch, _ in jobs:
+        ctx.paged_attention(cache, batch, heads(q), heads(o), shared.data_ptr(), nbytes)
+    ctx.sync()
+    for bt, q, o, *_ in jobs:
+        want, tol = refs.attention(bt, q)
+        refs.close(o, want, tol, dt, "one after the other")
+
+
+def test_attention_values_of_later_tokens(ctx, torch_cuda):
+    """The plain kernel keeps what a row may not see out of it altogether."""
+    bt = refs.batch([4], [20], heads=1, d=64, dtype=torch.float32)
+    refs.write_rows(bt, bt.v, 0, torch.cat([refs.read_rows(bt, bt.v, 0, 20)[:19], torch.full((1, 1, 64), float("nan"), device="cuda")]))
+    q = torch.randn(4, 2, 64, device="cuda")
+    o = run(ctx, bt, q)
+    assert torch.isfinite(o[:3]).all() and torch.isnan(o[3]).all()
 
 
 def test_attention_refusals(ctx, torch_cuda):

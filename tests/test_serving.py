@@ -77,3 +77,83 @@ def test_contexts_calls_need_a_context():
     assert lib.b2k_paged_append(None, None, None, None, None, None, None, None, None) == rt.B2K_EINVAL
     assert lib.b2k_paged_attention(None, None, None, None, None, 1.0, None, 0, None) == rt.B2K_EINVAL
     assert lib.b2k_verify_drafts(None, None, None, None, None) == rt.B2K_EINVAL
+
+
+# --- the plan of a paged attention call: host arithmetic on made-up addresses ------------------------------------
+
+
+def parts(sequences=4, new=1, length=1000, prefix=0, hq=32, hkv=8, d=128, dtype=rt.BF16, page=16, at=4096, **kw):
+    cache = rt.paged_cache(at, at + 64, dtype, 1000, page, hkv, d)
+    batch = rt.paged_batch(sequences, sequences * new, 256, 256, 256, -(-length // page), max_new=new, max_len=length,
+                           prefix_len=prefix, prefix_table=256)
+    x = rt.heads(kw.get("q", 4096), hq, hq * d, d)
+    return cache, batch, x, rt.heads(kw.get("o", 8192), hq, hq * d, d)
+
+
+def test_paged_plan_kernels():
+    plain, warp, memory = 0, 1, 2
+    plan = lambda **kw: rt.paged_attention_plan(148, *parts(**kw))  # noqa: E731
+    assert plan()["own_kernel"] == warp                                   # decode
+    assert plan(dtype=rt.F32)["own_kernel"] == plain
+    assert plan(d=100)["own_kernel"] == plain                             # no 16-byte pieces
+    assert plan(at=4098)["own_kernel"] == plain and plan(q=4098)["own_kernel"] == plain and plan(o=8194)["own_kernel"] == plain
+    assert plan(new=512, length=4096)["own_kernel"] == memory             # prompts
+    assert plan(new=512, length=4096, d=256)["own_kernel"] == warp        # too wide for tensor memory
+    assert plan(new=8, length=64)["own_kernel"] == warp                   # 32 rows fit the warp kernel
+    assert plan(new=9, length=40)["own_kernel"] == warp                   # more, but too little work to repay a block's start
+    decode = plan(sequences=128, prefix=8192, hq=64)
+    assert (decode["own_kernel"], decode["prefix_kernel"], decode["joined"]) == (warp, memory, 0)
+    assert plan(prefix=64)["prefix_kernel"] == warp and plan()["prefix_kernel"] == -1
+    chunk = plan(new=512, length=4096, prefix=1000)
+    assert (chunk["joined"], chunk["prefix_kernel"], chunk["prefix_splits"]) == (1, -1, 0)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(sequences=1, length=50001), dict(sequences=128, prefix=8192, hq=64),
+                                dict(new=512, length=4096, prefix=1000), dict(dtype=rt.F32, prefix=77), dict(d=256, new=33),
+                                dict(sequences=1, length=1), dict(length=2 ** 30, page=2 ** 20), dict(new=40, length=700, prefix=129)])
+def test_paged_plan_covers_the_keys(kw):
+    """Splits cover the keys without an empty one, whole tiles each, and the workspace holds every part."""
+    p, (cache, batch, q, _) = rt.paged_attention_plan(148, *parts(**kw)), parts(**kw)
+    step = 128 if p["own_kernel"] == 2 else 64
+    start = 0 if not p["joined"] else -(-batch.prefix_len // 128) * 128 if p["own_kernel"] == 2 else batch.prefix_len
+    assert p["own_chunk"] % step == 0
+    assert (p["own_splits"] - 1) * p["own_chunk"] < batch.max_len + start <= p["own_splits"] * p["own_chunk"]
+    if p["prefix_splits"]:
+        assert (p["prefix_splits"] - 1) * p["prefix_chunk"] < batch.prefix_len <= p["prefix_splits"] * p["prefix_chunk"]
+    slots = p["own_splits"] + p["prefix_splits"]
+    need = slots * batch.tokens * q.heads * (cache.d + 2) * 4
+    assert p["workspace_bytes"] == 0 if slots == 1 else need <= p["workspace_bytes"] < need + 16
+
+
+def changed(s, **kw):
+    c = type(s).from_buffer_copy(s)
+    for name, value in kw.items():
+        setattr(c, name, value)
+    return c
+
+
+@pytest.mark.parametrize("which,kw", [
+    (0, dict(k=None)), (0, dict(v=None)), (0, dict(dtype=3)), (0, dict(page_size=0)), (0, dict(pages=0)), (0, dict(heads=0)),
+    (0, dict(d=0)), (0, dict(d=257)), (0, dict(k_row=1)), (0, dict(v_head=1)), (0, dict(k_page=1)),
+    (1, dict(sequences=-1)), (1, dict(tokens=-1)), (1, dict(max_new=-1)), (1, dict(max_len=-1)), (1, dict(prefix_len=-1)),
+    (1, dict(first=None)), (1, dict(lengths=None)), (1, dict(table=None)), (1, dict(table_stride=1)), (1, dict(max_len=10 ** 6)),
+    (1, dict(prefix_len=5, prefix_table=None)), (1, dict(tokens=2 ** 31)),
+    (2, dict(heads=12)), (2, dict(heads=0)), (2, dict(data=None)), (2, dict(stride_head=3)), (2, dict(stride_token=-1)),
+    (3, dict(heads=8)), (3, dict(data=4096)), (3, dict(data=None))])
+def test_paged_plan_refuses(which, kw):
+    args = list(parts())
+    args[which] = changed(args[which], **kw)
+    with pytest.raises(rt.B2KError) as e:
+        rt.paged_attention_plan(148, *args)
+    assert e.value.status == rt.B2K_EINVAL
+
+
+@pytest.mark.parametrize("kw", [dict(sequences=65536), dict(tokens=2 ** 31 - 1), dict(max_new=2 ** 30)])
+def test_paged_plan_too_large(kw):
+    cache, batch, q, o = parts()
+    with pytest.raises(rt.B2KError) as e:
+        rt.paged_attention_plan(148, cache, changed(batch, **kw), q, o)
+    assert e.value.status == rt.B2K_EUNSUPPORTED
+    assert rt.library().b2k_paged_attention_set_kernel(4) == rt.B2K_EINVAL
+    assert rt.library().b2k_paged_attention_plan(0, C.byref(cache), C.byref(batch), C.byref(q), C.byref(o),
+                                                 C.byref(rt.PagedAttentionPlan())) == rt.B2K_EINVAL
