@@ -16,6 +16,8 @@ import numpy as np
 from . import runtime
 
 F32 = np.dtype(np.float32)
+#: Element types of the serving operators by NumPy type; uint16 holds bf16 bit patterns.
+ELEMENTS = {np.dtype(np.float32): runtime.F32, np.dtype(np.float16): runtime.F16, np.dtype(np.uint16): runtime.BF16}
 
 
 class DeviceArray:
@@ -34,6 +36,37 @@ class DeviceArray:
         if self.ptr:
             self.session.ctx.free(self.ptr)
             self.ptr = 0
+
+
+def _heads(x: DeviceArray) -> runtime.Heads:
+    if len(x.shape) != 3:
+        raise ValueError(f"expected [tokens, heads, d], got shape {x.shape}")
+    return runtime.heads(x.ptr, x.shape[1], x.shape[1] * x.shape[2], x.shape[2])
+
+
+class PagedKV:
+    """Keys and values in pages [pages, page_size, heads, d], and the workspace of the attention over them."""
+
+    def __init__(self, session: "Session", pages: int, page_size: int, heads: int, d: int, dtype=F32):
+        self.session, self.dtype = session, np.dtype(dtype)
+        shape = (pages, page_size, heads, d)
+        self.k, self.v = session.empty(shape, dtype), session.empty(shape, dtype)
+        self.cache = runtime.paged_cache(self.k.ptr, self.v.ptr, ELEMENTS[self.dtype], pages, page_size, heads, d)
+        self._workspace: DeviceArray | None = None
+
+    def workspace(self, nbytes: int) -> DeviceArray:
+        """At least `nbytes` of device memory, kept from call to call (a session's calls share one stream)."""
+        if self._workspace is None or self._workspace.nbytes < nbytes:
+            if self._workspace is not None:
+                self.session.sync()
+                self._workspace.free()
+            self._workspace = self.session.empty((max(16, nbytes),), np.uint8)
+        return self._workspace
+
+    def free(self) -> None:
+        for array in (self.k, self.v, self._workspace):
+            if array is not None:
+                array.free()
 
 
 class Session:
@@ -105,6 +138,69 @@ class Session:
 
     def pointwise(self, program, inputs: list[DeviceArray], out: DeviceArray) -> None:
         self.ctx.pointwise(program, [t.ptr for t in inputs], out.ptr, out.size, stream=self.stream)
+
+    # --- serving: rotary positions, paged cache, drafted tokens -------------------
+    # Arrays are [tokens, heads, d] of float32, float16 or uint16 (bf16 bits);
+    # first, lengths, table (int32) and positions (int64) are device arrays too.
+    def rotary(self, rope: runtime.Rope, pairs: list[tuple[DeviceArray, DeviceArray]], positions: DeviceArray, *,
+               transpose: bool = False) -> None:
+        """y = rotary(x) for each (x, y); ``transpose`` gives the inputs' gradients from the outputs'."""
+        tokens, _, d = pairs[0][0].shape
+        if positions.shape != (tokens,) or positions.dtype != np.int64:
+            raise ValueError("rotary: positions must be int64, one for each token")
+        for x, y in pairs:
+            if x.shape != y.shape or x.shape[0] != tokens or x.shape[2] != d or {x.dtype, y.dtype} != {pairs[0][0].dtype}:
+                raise ValueError(f"rotary: {x.shape} {x.dtype} to {y.shape} {y.dtype}")
+        self.ctx.rotary(rope, ELEMENTS[pairs[0][0].dtype], [(_heads(x), _heads(y)) for x, y in pairs], positions.ptr, tokens,
+                        d, transpose=transpose, stream=self.stream)
+
+    def paged_kv(self, pages: int, page_size: int, heads: int, d: int, dtype=F32) -> PagedKV:
+        return PagedKV(self, pages, page_size, heads, d, dtype)
+
+    @staticmethod
+    def paged_batch(first: DeviceArray, lengths: DeviceArray, table: DeviceArray, tokens: int, *, max_new: int,
+                    max_len: int, prefix_table: DeviceArray | None = None, prefix_len: int = 0) -> runtime.PagedBatch:
+        """The sequences of a call: first [n + 1], lengths [n], table [n, pages], all int32."""
+        n, width = table.shape
+        arrays = [first, lengths, table] + ([prefix_table] if prefix_table is not None else [])
+        if first.shape != (n + 1,) or lengths.shape != (n,) or any(x.dtype != np.int32 for x in arrays):
+            raise ValueError("paged_batch: first [n + 1], lengths [n] and table [n, pages] must be int32")
+        return runtime.paged_batch(n, tokens, first.ptr, lengths.ptr, table.ptr, width, max_new=max_new, max_len=max_len,
+                                   prefix_len=prefix_len, prefix_table=prefix_table.ptr if prefix_table is not None else 0)
+
+    def paged_append(self, kv: PagedKV, batch: runtime.PagedBatch, k: DeviceArray, v: DeviceArray, *,
+                     q: DeviceArray | None = None, q_out: DeviceArray | None = None,
+                     rope: runtime.Rope | None = None) -> None:
+        for x in (k, v, q, q_out):
+            if x is not None and (x.dtype != kv.dtype or x.shape[0] != batch.tokens or x.shape[2] != kv.cache.d):
+                raise ValueError(f"paged_append: {x.shape} {x.dtype} for {batch.tokens} tokens of a {kv.dtype} cache")
+        self.ctx.paged_append(kv.cache, batch, _heads(k), _heads(v), q=None if q is None else _heads(q),
+                              q_out=None if q_out is None else _heads(q_out), rope=rope, stream=self.stream)
+
+    def paged_attention(self, kv: PagedKV, batch: runtime.PagedBatch, q: DeviceArray, o: DeviceArray, *,
+                        scale: float | None = None) -> None:
+        for x in (q, o):
+            if x.dtype != kv.dtype or x.shape[0] != batch.tokens or x.shape[2] != kv.cache.d:
+                raise ValueError(f"paged_attention: {x.shape} {x.dtype} for {batch.tokens} tokens of a {kv.dtype} cache")
+        nbytes = self.ctx.paged_attention_workspace(kv.cache, batch, q.shape[1])
+        self.ctx.paged_attention(kv.cache, batch, _heads(q), _heads(o), kv.workspace(nbytes).ptr if nbytes else 0, nbytes,
+                                 scale=scale, stream=self.stream)
+
+    def verify_drafts(self, target: DeviceArray, drafted: DeviceArray, u_accept: DeviceArray, u_sample: DeviceArray,
+                      accepted: DeviceArray, tokens: DeviceArray, *, draft: DeviceArray | None = None,
+                      counts: DeviceArray | None = None) -> None:
+        """target [batch, drafts + 1, vocab], draft [batch, drafts, vocab] float32; drafted [batch, drafts], accepted
+        [batch], tokens [batch, drafts + 1] int32; u_accept [batch, drafts], u_sample [batch] float32."""
+        batch, rows, vocab = target.shape
+        want = [(target, F32, (batch, rows, vocab)), (drafted, np.int32, (batch, rows - 1)), (u_accept, F32, (batch, rows - 1)),
+                (u_sample, F32, (batch,)), (accepted, np.int32, (batch,)), (tokens, np.int32, (batch, rows)),
+                (draft, F32, (batch, rows - 1, vocab)), (counts, np.int32, (batch,))]
+        for x, dtype, shape in want:
+            if x is not None and (x.dtype != dtype or x.shape != shape):
+                raise ValueError(f"verify_drafts: {x.shape} {x.dtype} where {shape} {np.dtype(dtype)} is wanted")
+        self.ctx.verify_drafts(target.ptr, drafted.ptr, u_accept.ptr, u_sample.ptr, accepted.ptr, tokens.ptr, batch, rows - 1,
+                               vocab, draft=draft.ptr if draft is not None else 0,
+                               counts=counts.ptr if counts is not None else 0, stream=self.stream)
 
     # --- end to end from host arrays --------------------------------------------
     # One library call per operation: the inputs are copied in slab by slab on

@@ -189,3 +189,49 @@ def test_append_and_attention_in_one_graph(ctx, torch_cuda):
         torch.cuda.synchronize()
         ctx.sync()
         assert torch.equal(o, want) and torch.equal(server.k.nan_to_num(9.0), mirror.k.nan_to_num(9.0))
+
+
+def test_session_arrays(ctx, torch_cuda):
+    """The same step from NumPy arrays, without PyTorch on the package's side."""
+    api = importlib.import_module(f"{PKG}.api")
+    rng = np.random.default_rng(4)
+    with api.Session(0) as s:
+        n, hq, hkv, d, page = 3, 4, 2, 32, 16
+        kv = s.paged_kv(8, page, hkv, d)
+        qkv = [rng.standard_normal((n, h, d)).astype(np.float32) for h in (hq, hkv, hkv)]
+        q, k, v = (s.upload(x) for x in qkv)
+        first, lengths = s.upload(np.array([0, 2, 3], np.int32)), s.upload(np.array([2, 1], np.int32))
+        table = s.upload(np.array([[5, 1], [3, 0]], np.int32))
+        batch = s.paged_batch(first, lengths, table, n, max_new=2, max_len=2)
+        rope, turned, o = rt.rope_plan(d), s.empty((n, hq, d)), s.empty((n, hq, d))
+        s.paged_append(kv, batch, k, v, q=q, q_out=turned, rope=rope)
+        s.paged_attention(kv, batch, turned, o)
+        pos, back = s.upload(np.array([0, 1, 0], np.int64)), s.empty((n, hq, d))
+        s.rotary(rope, [(turned, back)], pos, transpose=True)
+        s.sync()
+        got, same, cache = s.download(o), s.download(back), s.download(kv.k)
+        s.sync()
+        # a rotation's transpose is its inverse: two passes of FP32 roundings
+        assert np.abs(same - qkv[0]).max() <= 4e-6
+        keys = torch.from_numpy(np.stack([cache[5, 0], cache[5, 1], cache[3, 0]]))
+        want, tol = refs.rotary(torch.from_numpy(qkv[1]), torch.tensor([0, 1, 0]), refs.frequencies(d), False)
+        refs.close(keys, want, tol, torch.float32, "keys")
+        assert np.abs(got[0] - np.repeat(qkv[2][0], 2, 0)).max() <= 1e-6  # a first token sees itself alone
+        assert np.abs(got[2] - np.repeat(qkv[2][2], 2, 0)).max() <= 1e-6
+        target = rng.random((2, 3, 50)).astype(np.float32)
+        drafted = rng.integers(0, 50, (2, 2)).astype(np.int32)
+        u, us = rng.random((2, 2)).astype(np.float32), rng.random(2).astype(np.float32)
+        accepted, tokens = s.empty((2,), np.int32), s.empty((2, 3), np.int32)
+        s.verify_drafts(s.upload(target), s.upload(drafted), s.upload(u), s.upload(us), accepted, tokens)
+        s.sync()
+        a, out = s.download(accepted), s.download(tokens)
+        s.sync()
+        want = refs.verify(*(torch.from_numpy(target), None, torch.from_numpy(drafted), None, torch.from_numpy(u), torch.from_numpy(us)))
+        assert np.array_equal(a, want[0].numpy()) and np.array_equal(out, want[1].numpy())
+        with pytest.raises(ValueError):
+            s.rotary(rope, [(turned, back)], lengths)
+        with pytest.raises(ValueError):
+            s.paged_attention(kv, batch, s.empty((n, hq, d), np.float16), o)
+        with pytest.raises(ValueError):
+            s.paged_batch(first, first, table, n, max_new=2, max_len=2)
+        kv.free()
