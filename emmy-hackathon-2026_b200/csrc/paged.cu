@@ -45,7 +45,7 @@ __device__ __forceinline__ void copy16(void *dst, const void *src) {
 // V: elements of one access to the cache (16 bytes, or 1).
 template <typename T, int RW, int DV0, int V>
 __global__ void __launch_bounds__(kThreads)
-    paged_rows_kernel(const __grid_constant__ Args a, bool prefix, int row_blocks, bool beside) {
+    paged_rows_kernel(const __grid_constant__ Args a, const paged::Grid grid) {
   constexpr int R = RW * kWarps;
   constexpr int DV = DV0 == 0 ? 1 : DV0, kSides = DV0 == 0 ? 2 : 1;
   constexpr bool kAsync = sizeof(T) == 4 && V == 4;  // the cache's bytes are the tile's
@@ -55,23 +55,25 @@ __global__ void __launch_bounds__(kThreads)
   const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4;
   const int stage_floats = kTile * (ldk + dp);  // keys, then values; two stages behind the queries
   float *qs = smem, *tiles = qs + R * dp;
-  paged::part_begin(beside);
+  paged::part_begin(grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int side = kSides == 2 ? lane >> 4 : 0, col = 4 * (kSides == 2 ? lane & 15 : lane);  // of a lane's output
-  const int split = blockIdx.y, head = blockIdx.x / row_blocks, block = blockIdx.x % row_blocks, b = blockIdx.z;
+  const paged::Block at = paged::this_block(a, grid);
+  const bool prefix = at.prefix;
+  const int split = at.split, head = at.head, block = at.row_block, b = at.sequence;
   const int q_heads = a.kv_heads * a.group;
   paged::Sequence s = {0, 0, 0};
   if (prefix) s.n = paged::used_tokens(a);
   else s = paged::sequence(a, b);
   const int rows = s.n * a.group, row0 = block * R;
-  if (row0 >= rows) return paged::part_end(beside);
+  if (row0 >= rows) return paged::part_end(grid.beside);
   const int last_token = (min(row0 + R, rows) - 1) / a.group;
   const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
   const int key0 = split * chunk;
   const int key_end = min(prefix ? a.prefix_len : paged::own_limit(a, s, last_token), key0 + chunk);
   const bool direct = a.own_splits + a.prefix_splits == 1;
-  if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(beside);
+  if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(grid.beside);
   const int n_tiles = (key_end - key0 + kTile - 1) / kTile;
 
   // Offsets of a tile's rows, two tiles ahead of their use; -1: no such key.
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   }
-  paged::part_end(beside);
+  paged::part_end(grid.beside);
 }
 
 // Joins a row's parts, in an order that does not depend on which part ended
@@ -458,6 +460,9 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   if (b.prefix_len > 0 && !p.joined) {
     p.prefix_path = pick_path(tensor, c.d, prefix, b.prefix_len, c.heads);
     p.prefix_rows = block_rows(p.prefix_path, c.d, prefix);
+    // a few row blocks of the own part's height save a launch, at the price of
+    // as many readings of the prefix
+    if (p.prefix_path == p.own_path && p.own_path != kUmma && prefix <= 4 * p.own_rows) p.prefix_rows = p.own_rows;
     const int64_t units = (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads;
     int64_t want = wave(p.prefix_path);
     if (p.prefix_path == kUmma && p.own_path != kUmma) {
@@ -482,7 +487,7 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
 }
 
 template <typename T, int RW, int DV>
-int launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, bool beside, dim3 grid, int row_blocks, cudaStream_t s) {
+int launch_rows(b2k_ctx *ctx, const Args &a, bool vec, const paged::Grid &g, unsigned blocks, cudaStream_t s) {
   const int dp = (a.d + 3) / 4 * 4;
   const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + 2 * kTile * (2 * dp + 4));
   constexpr int kFull = 16 / sizeof(T);
@@ -490,53 +495,48 @@ int launch_rows(b2k_ctx *ctx, const Args &a, bool prefix, bool vec, bool beside,
   constexpr int kMost = DV == 0 ? 64 : 128 * DV;  // head dim
   constexpr int most = sizeof(float) * (RW * kWarps * kMost + 2 * kTile * (2 * kMost + 4));
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
-  if (err == cudaSuccess)
-    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), smem, s, a, prefix, row_blocks, beside);
+  if (err == cudaSuccess) err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem, s, a, g);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }
 
+template <typename T, int RW>
+int rows_by_dim(b2k_ctx *ctx, const Args &a, bool vec, const paged::Grid &g, unsigned blocks, cudaStream_t s) {
+  return a.d <= 64    ? launch_rows<T, RW, 0>(ctx, a, vec, g, blocks, s)
+         : a.d <= 128 ? launch_rows<T, RW, 1>(ctx, a, vec, g, blocks, s)
+                      : launch_rows<T, RW, 2>(ctx, a, vec, g, blocks, s);
+}
+
 template <typename T>
-int rows_part(b2k_ctx *ctx, const Args &a, bool prefix, int block_rows, bool beside, cudaStream_t s) {
-  const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
-  const int rw = block_rows / kWarps;
-  const int row_blocks = (int)((rows + 4 * rw - 1) / (4 * rw));
-  const dim3 grid((unsigned)(row_blocks * a.kv_heads), prefix ? a.prefix_splits : a.own_splits, prefix ? 1 : a.sequences);
+int rows_parts(b2k_ctx *ctx, const Args &a, bool with_prefix, bool with_own, int rows, bool beside, cudaStream_t s) {
+  paged::Grid g = {};
+  const int64_t n = paged::make_grid(ctx, a, with_prefix, with_own, rows, beside, g);
+  if (n < 0) return B2K_EUNSUPPORTED;
   const size_t size = sizeof(T);
   const bool vec = a.d % (16 / (int)size) == 0 && serve::vec_ok(a.k, a.k_page, a.k_row, a.k_head, size, 16) &&
                    serve::vec_ok(a.v, a.v_page, a.v_row, a.v_head, size, 16);
-  if (a.d <= 64) {
-    if (rw == 1) return launch_rows<T, 1, 0>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-    if (rw == 2) return launch_rows<T, 2, 0>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-    return launch_rows<T, 8, 0>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-  }
-  if (a.d <= 128) {
-    if (rw == 1) return launch_rows<T, 1, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-    if (rw == 2) return launch_rows<T, 2, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-    return launch_rows<T, 8, 1>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-  }
-  if (rw == 1) return launch_rows<T, 1, 2>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-  if (rw == 2) return launch_rows<T, 2, 2>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
-  return launch_rows<T, 8, 2>(ctx, a, prefix, vec, beside, grid, row_blocks, s);
+  const unsigned blocks = (unsigned)n;
+  return rows == 4   ? rows_by_dim<T, 1>(ctx, a, vec, g, blocks, s)
+         : rows == 8 ? rows_by_dim<T, 2>(ctx, a, vec, g, blocks, s)
+                     : rows_by_dim<T, 8>(ctx, a, vec, g, blocks, s);
 }
 
 template <typename T>
 int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
   int launches = 1, status = B2K_OK;
   const bool prefix = a.prefix_splits > 0;
-  if (p.own_path == kMma && (!prefix || (p.prefix_path == kMma && p.prefix_rows == p.own_rows))) {
-    status = paged::mma_parts(ctx, a, dtype, prefix, true, p.own_rows, false, s);
+  auto parts = [&](Path path, bool pre, bool own, int rows, bool beside) {
+    return path == kPlain ? rows_parts<T>(ctx, a, pre, own, rows, beside, s)
+           : path == kMma ? paged::mma_parts(ctx, a, dtype, pre, own, rows, beside, s)
+                          : paged::umma_part(ctx, a, dtype, pre, s);
+  };
+  if (!prefix) {
+    status = parts(p.own_path, false, true, p.own_rows, false);
+  } else if (p.own_path == p.prefix_path && p.own_path != kUmma && p.own_rows == p.prefix_rows) {
+    status = parts(p.own_path, true, true, p.own_rows, false);
   } else {
-    auto part = [&](bool pre, Path path, int rows) {
-      const bool beside = !pre && prefix;
-      return path == kPlain ? rows_part<T>(ctx, a, pre, rows, beside, s)
-             : path == kMma ? paged::mma_parts(ctx, a, dtype, pre, !pre, rows, beside, s)
-                            : paged::umma_part(ctx, a, dtype, pre, s);
-    };
-    if (prefix) {
-      status = part(true, p.prefix_path, p.prefix_rows);
-      ++launches;
-    }
-    if (status == B2K_OK) status = part(false, p.own_path, p.own_rows);
+    status = parts(p.prefix_path, true, false, p.prefix_rows, false);
+    if (status == B2K_OK) status = parts(p.own_path, false, true, p.own_rows, true);
+    ++launches;
   }
   if (status != B2K_OK) return status;
   if (a.own_splits + a.prefix_splits > 1) {

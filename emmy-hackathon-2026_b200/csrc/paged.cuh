@@ -103,8 +103,46 @@ __device__ __forceinline__ void part_begin(bool beside) {
   grid_dependents_launch();
 }
 __device__ __forceinline__ void part_end(bool beside) {
-  if (beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
-    grid_dependency_wait();
+  if (beside && blockIdx.x == gridDim.x - 1) grid_dependency_wait();
+}
+
+// The blocks of a launch of one or both parts, in one dimension: the prefix
+// part's first, then the sequences'; row blocks within heads within splits
+// (within sequences).
+struct Grid {
+  unsigned prefix_blocks;  // 0: no prefix part in this launch
+  int prefix_row_blocks, own_row_blocks;
+  bool beside;  // the prefix part is the kernel before: run beside it (part_begin)
+};
+struct Block {
+  bool prefix;
+  int row_block, head, split, sequence;
+};
+__device__ __forceinline__ Block this_block(const Args &a, const Grid &g) {
+  Block b;
+  b.prefix = blockIdx.x < g.prefix_blocks;
+  unsigned at = b.prefix ? blockIdx.x : blockIdx.x - g.prefix_blocks;
+  const unsigned row_blocks = b.prefix ? g.prefix_row_blocks : g.own_row_blocks;
+  b.row_block = at % row_blocks;
+  at /= row_blocks;
+  b.head = at % (unsigned)a.kv_heads;
+  at /= (unsigned)a.kv_heads;
+  const unsigned splits = b.prefix ? a.prefix_splits : a.own_splits;
+  b.split = at % splits;
+  b.sequence = at / splits;
+  return b;
+}
+// Fills `g` for blocks of `rows` rows; the number of blocks, or -1 (error recorded).
+inline int64_t make_grid(b2k_ctx *ctx, const Args &a, bool with_prefix, bool with_own, int rows, bool beside, Grid &g) {
+  g.prefix_row_blocks = (int)((a.tokens * a.group + rows - 1) / rows);
+  g.own_row_blocks = (int)(((int64_t)a.max_new * a.group + rows - 1) / rows);
+  g.beside = beside;
+  const int64_t prefix = with_prefix ? (int64_t)g.prefix_row_blocks * a.kv_heads * a.prefix_splits : 0;
+  const int64_t own = with_own ? (int64_t)g.own_row_blocks * a.kv_heads * a.own_splits * a.sequences : 0;
+  g.prefix_blocks = (unsigned)prefix;
+  if (prefix + own <= INT32_MAX) return prefix + own;
+  b2k::fail(ctx, B2K_EUNSUPPORTED, "paged_attention: %lld blocks", (long long)(prefix + own));
+  return -1;
 }
 
 // paged_mma.cu: rows of a block (16 or 32) for `rows` rows of one cache head, and

@@ -106,16 +106,9 @@ struct Type<__nv_bfloat16> {
   }
 };
 
-// Blocks of the prefix part come first, then the sequences'.
-struct Grid {
-  unsigned prefix_blocks;  // blocks of the prefix part in this launch (0: none)
-  int prefix_row_blocks, own_row_blocks;
-  bool beside;  // the prefix part is the kernel before: run beside it (paged.cuh, part_begin)
-};
-
 template <typename T, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : DP == 128 && MT == 2 ? 2 : 3)
-    paged_mma_kernel(const __grid_constant__ Args a, const Grid grid) {
+    paged_mma_kernel(const __grid_constant__ Args a, const paged::Grid grid) {
   constexpr int kStages = stages<DP, MT>();
   constexpr int kChunks = DP / 8;        // 16-byte pieces of a row
   constexpr int kRows = 16 * MT;
@@ -126,15 +119,10 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : DP == 128 && MT == 2
   paged::part_begin(grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool prefix = blockIdx.x < grid.prefix_blocks;
-  unsigned at = prefix ? blockIdx.x : blockIdx.x - grid.prefix_blocks;
+  const paged::Block at = paged::this_block(a, grid);
+  const bool prefix = at.prefix;
   const int row_blocks = prefix ? grid.prefix_row_blocks : grid.own_row_blocks;
-  const int block = at % row_blocks;
-  at /= row_blocks;
-  const int head = at % a.kv_heads;
-  at /= a.kv_heads;
-  const int splits = prefix ? a.prefix_splits : a.own_splits;
-  const int split = at % splits, b = at / splits;
+  const int block = at.row_block, head = at.head, split = at.split, b = at.sequence;
 
   paged::Sequence s = {0, 0, 0};
   if (prefix) s.n = paged::used_tokens(a);
@@ -428,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : DP == 128 && MT == 2
 }
 
 template <typename T, int DP, int MT>
-cudaError_t launch(b2k_ctx *ctx, const Args &a, const Grid &g, unsigned blocks, cudaStream_t s) {
+cudaError_t launch(b2k_ctx *ctx, const Args &a, const paged::Grid &g, unsigned blocks, cudaStream_t s) {
   auto kernel = paged_mma_kernel<T, DP, MT>;
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, smem_bytes<DP, MT>());
   if (err != cudaSuccess) return err;
@@ -436,7 +424,7 @@ cudaError_t launch(b2k_ctx *ctx, const Args &a, const Grid &g, unsigned blocks, 
 }
 
 template <typename T>
-cudaError_t pick(b2k_ctx *ctx, const Args &a, const Grid &g, unsigned blocks, int mt, cudaStream_t s) {
+cudaError_t pick(b2k_ctx *ctx, const Args &a, const paged::Grid &g, unsigned blocks, int mt, cudaStream_t s) {
   if (a.d <= 64) return mt == 1 ? launch<T, 64, 1>(ctx, a, g, blocks, s) : launch<T, 64, 2>(ctx, a, g, blocks, s);
   if (a.d <= 128) return mt == 1 ? launch<T, 128, 1>(ctx, a, g, blocks, s) : launch<T, 128, 2>(ctx, a, g, blocks, s);
   return launch<T, 256, 1>(ctx, a, g, blocks, s);
@@ -451,15 +439,9 @@ int mma_rows(int d, int64_t rows) { return d <= 128 && rows > 16 ? 32 : 16; }
 int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, bool beside,
               cudaStream_t s) {
   Grid g = {};
-  g.beside = beside;
-  g.prefix_row_blocks = (int)((a.tokens * a.group + rows - 1) / rows);
-  g.own_row_blocks = (int)(((int64_t)a.max_new * a.group + rows - 1) / rows);
-  const int64_t prefix = with_prefix ? (int64_t)g.prefix_row_blocks * a.kv_heads * a.prefix_splits : 0;
-  const int64_t own = with_own ? (int64_t)g.own_row_blocks * a.kv_heads * a.own_splits * a.sequences : 0;
-  if (prefix + own > INT32_MAX)
-    return b2k::fail(ctx, B2K_EUNSUPPORTED, "paged_attention: %lld blocks", (long long)(prefix + own));
-  g.prefix_blocks = (unsigned)prefix;
-  const unsigned blocks = (unsigned)(prefix + own);
+  const int64_t n = make_grid(ctx, a, with_prefix, with_own, rows, beside, g);
+  if (n < 0) return B2K_EUNSUPPORTED;
+  const unsigned blocks = (unsigned)n;
   const int mt = rows / 16;
   const cudaError_t err =
       dtype == B2K_F16 ? pick<__half>(ctx, a, g, blocks, mt, s) : pick<__nv_bfloat16>(ctx, a, g, blocks, mt, s);
