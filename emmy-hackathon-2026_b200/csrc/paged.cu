@@ -43,6 +43,10 @@ __device__ __forceinline__ void copy16(void *dst, const void *src) {
 // DV: float4s of a head that a lane holds (head dim up to 128 DV; 0: up to 64,
 // where the two halves of a warp take every other four keys and add up at the end).
 // V: elements of one access to the cache (16 bytes, or 1).
+// Tiles a block holds: one in use, the others on their way.
+template <int DV0>
+constexpr int rows_stages() { return DV0 == 0 ? 3 : 2; }
+
 template <typename T, int RW, int DV0, int V>
 __global__ void __launch_bounds__(kThreads)
     paged_rows_kernel(const __grid_constant__ Args a, const paged::Grid grid) {
@@ -50,10 +54,12 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int DV = DV0 == 0 ? 1 : DV0, kSides = DV0 == 0 ? 2 : 1;
   constexpr bool kAsync = sizeof(T) == 4 && V == 4;  // the cache's bytes are the tile's
   extern __shared__ __align__(16) float smem[];
-  __shared__ int64_t k_at[3][kTile], v_at[3][kTile];
+  constexpr int kStages = rows_stages<DV0>(), kSlots = kStages + 1;
+  static_assert(kStages * kTile <= kThreads, "a thread looks up one key of the first tiles");
+  __shared__ int64_t k_at[kSlots][kTile], v_at[kSlots][kTile];  // offsets of a tile's rows; -1: no such key
   __shared__ __align__(16) float ps[kWarps][RW][kTile];  // a warp's probabilities
   const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4;
-  const int stage_floats = kTile * (ldk + dp);  // keys, then values; two stages behind the queries
+  const int stage_floats = kTile * (ldk + dp);  // keys, then values; the stages behind the queries
   float *qs = smem, *tiles = qs + R * dp;
   paged::part_begin(grid.beside);
 
@@ -76,29 +82,39 @@ __global__ void __launch_bounds__(kThreads)
   if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(grid.beside);
   const int n_tiles = (key_end - key0 + kTile - 1) / kTile;
 
-  // Offsets of a tile's rows, two tiles ahead of their use; -1: no such key.
-  auto look_up = [&](int i) {
-    if (threadIdx.x >= kTile || i >= n_tiles) return;
-    const int at = key0 + i * kTile + threadIdx.x;
-    int64_t ko = -1, vo = -1;
-    if (at < key_end) {
-      int r;
-      const int64_t page = paged::key_page(a, prefix, b, at, r);
-      if (page >= 0) {
-        ko = page * a.k_page + r * a.k_row + head * a.k_head;
-        vo = page * a.v_page + r * a.v_row + head * a.v_head;
-      }
-    }
-    k_at[i % 3][threadIdx.x] = ko;
-    v_at[i % 3][threadIdx.x] = vo;
+  // A key's page is asked for one tile before its load is issued; the answer
+  // is used at the end of the tile in between.
+  int asked = 0, asked_row = 0;
+  bool wanted = false;
+  auto ask = [&](int tile, int i) {
+    const int at = key0 + tile * kTile + i;
+    wanted = at < key_end;
+    if (wanted) asked = paged::key_entry(a, prefix, b, at, asked_row);
   };
-  const int per_row = dp / V;
+  auto answer = [&](int tile, int i) {
+    int64_t ko = -1, vo = -1;
+    if (wanted && asked >= 0 && asked < a.pages) {
+      ko = asked * a.k_page + asked_row * a.k_row + head * a.k_head;
+      vo = asked * a.v_page + asked_row * a.v_row + head * a.v_head;
+    } else if (wanted) {
+      atomicOr(a.err, serve::kErrIndex);
+    }
+    k_at[tile % kSlots][i] = ko;
+    v_at[tile % kSlots][i] = vo;
+  };
+  // a thread's first piece of a tile, and the step to its next one
+  const int per_row = dp / V, r_first = threadIdx.x / per_row, c_first = threadIdx.x - r_first * per_row;
+  const int r_step = kThreads / per_row, c_step = kThreads - r_step * per_row;
   auto load = [&](int i) {
     if (i >= n_tiles) return;
-    float *ks = tiles + (i & 1) * stage_floats, *vs = ks + kTile * ldk;
-    for (int p = threadIdx.x; p < kTile * per_row; p += kThreads) {
-      const int r = p / per_row, c = (p - r * per_row) * V;
-      const int64_t ko = k_at[i % 3][r], vo = v_at[i % 3][r];
+    float *ks = tiles + i % kStages * stage_floats, *vs = ks + kTile * ldk;
+    for (int r = r_first, piece = c_first; r < kTile; r += r_step, piece += c_step) {
+      if (piece >= per_row) {
+        piece -= per_row;
+        if (++r >= kTile) break;
+      }
+      const int c = piece * V;
+      const int64_t ko = k_at[i % kSlots][r], vo = v_at[i % kSlots][r];
       const T *kx = static_cast<const T *>(a.k) + ko + c, *vx = static_cast<const T *>(a.v) + vo + c;
       if (kAsync) {
         if (ko >= 0) {
@@ -122,8 +138,10 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   };
-  look_up(0);
-  look_up(1);
+  if (threadIdx.x < kStages * kTile) {
+    ask(threadIdx.x / kTile, threadIdx.x % kTile);
+    answer(threadIdx.x / kTile, threadIdx.x % kTile);
+  }
 
   // this block's queries, FP32, times log2(e) / scale; eight loads in flight
   constexpr int kBatch = 8;
@@ -154,39 +172,46 @@ __global__ void __launch_bounds__(kThreads)
     for (int c = 0; c < DV; ++c) o[i][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   __syncthreads();
-  load(0);
-  asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    load(i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
 
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int key = key0 + tile * kTile;
-    const float *ks = tiles + (tile & 1) * stage_floats, *vs = ks + kTile * ldk;
-    load(tile + 1);
+    const float *ks = tiles + tile % kStages * stage_floats, *vs = ks + kTile * ldk;
+    if (threadIdx.x < kTile) ask(tile + kStages, threadIdx.x);
+    load(tile + kStages - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    look_up(tile + 2);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncthreads();
 
     // every key of the tile is seen by every row of the warp
     bool open = key + kTile <= key_end;
 #pragma unroll
     for (int i = 0; i < RW; ++i) open = open && key + kTile <= limit[i];
-    open = __all_sync(0xffffffffu, open && k_at[tile % 3][lane] >= 0);
+    open = __all_sync(0xffffffffu, open && k_at[tile % kSlots][lane] >= 0);
     {
-      float acc[RW];
+      float4 sum[RW];  // four chains a row: one would be as long as the head
 #pragma unroll
-      for (int i = 0; i < RW; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < RW; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
       for (int c = 0; c < dp; c += 4) {
         const float4 kv = *reinterpret_cast<const float4 *>(ks + lane * ldk + c);
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
           const float4 qv = *reinterpret_cast<const float4 *>(qs + (warp * RW + i) * dp + c);
-          acc[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, acc[i]))));
+          sum[i].x = fmaf(qv.x, kv.x, sum[i].x);
+          sum[i].y = fmaf(qv.y, kv.y, sum[i].y);
+          sum[i].z = fmaf(qv.z, kv.z, sum[i].z);
+          sum[i].w = fmaf(qv.w, kv.w, sum[i].w);
         }
       }
-      const bool there = k_at[tile % 3][lane] >= 0;
+      const bool there = k_at[tile % kSlots][lane] >= 0;
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
-        const float sc = there && key + lane < limit[i] ? acc[i] : -INFINITY;
+        const float sc = there && key + lane < limit[i] ? (sum[i].x + sum[i].y) + (sum[i].z + sum[i].w) : -INFINITY;
         const float mx = fmaxf(m[i], warp_max(sc));
         const float base = mx == -INFINITY ? 0.0f : mx;
         const float alpha = exp2_fast(m[i] - base);
@@ -229,7 +254,9 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    __syncthreads();  // the stage, and its offsets, may be written again
+    // (this tile's slot is not the one written: kSlots is one more than the stages)
+    if (threadIdx.x < kTile) answer(tile + kStages, threadIdx.x);
+    __syncthreads();  // the stage may be written again
   }
 
 #pragma unroll
@@ -489,11 +516,11 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
 template <typename T, int RW, int DV>
 int launch_rows(b2k_ctx *ctx, const Args &a, bool vec, const paged::Grid &g, unsigned blocks, cudaStream_t s) {
   const int dp = (a.d + 3) / 4 * 4;
-  const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + 2 * kTile * (2 * dp + 4));
+  const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + rows_stages<DV>() * kTile * (2 * dp + 4));
   constexpr int kFull = 16 / sizeof(T);
   auto kernel = vec ? paged_rows_kernel<T, RW, DV, kFull> : paged_rows_kernel<T, RW, DV, 1>;
   constexpr int kMost = DV == 0 ? 64 : 128 * DV;  // head dim
-  constexpr int most = sizeof(float) * (RW * kWarps * kMost + 2 * kTile * (2 * kMost + 4));
+  constexpr int most = sizeof(float) * (RW * kWarps * kMost + rows_stages<DV>() * kTile * (2 * kMost + 4));
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
   if (err == cudaSuccess) err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem, s, a, g);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");

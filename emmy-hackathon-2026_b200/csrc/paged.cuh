@@ -70,21 +70,22 @@ __device__ __forceinline__ int own_limit(const Args &a, const Sequence &s, int j
   return !a.joined ? own : own > 0 ? a.joined_keys + own : a.prefix_len;
 }
 
-// Offsets (elements) of a key's rows in the cache, for cache head 0; -1 for a page
-// outside the cache.  `at` counts from the start of the part: the prefix's
-// keys, or the own keys behind the prefix's where the part is joined
-// (joined_keys = prefix_len).
-__device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, int at, int &row) {
+// The page table's entry for a key, unchecked, and the key's row in that page.
+// `at` counts from the start of the part: the prefix's keys, or the own keys
+// behind the prefix's where the part is joined (joined_keys = prefix_len).
+__device__ __forceinline__ int key_entry(const Args &a, bool prefix, int b, int at, int &row) {
   const int32_t *table = a.prefix_table;
-  if (!prefix) {
-    if (!a.joined || at >= a.prefix_len) {
-      table = a.table + (int64_t)b * a.table_stride;
-      at -= a.joined ? a.prefix_len : 0;
-    }
+  if (!prefix && (!a.joined || at >= a.prefix_len)) {
+    table = a.table + (int64_t)b * a.table_stride;
+    at -= a.joined ? a.prefix_len : 0;
   }
   const int i = (int)((unsigned)at / (unsigned)a.page_size);
   row = at - i * a.page_size;
-  const int64_t page = table[i];
+  return table[i];
+}
+// The key's page; -1 (and the error word set) for one outside the cache.
+__device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, int at, int &row) {
+  const int64_t page = key_entry(a, prefix, b, at, row);
   if (page >= 0 && page < a.pages) return page;
   atomicOr(a.err, serve::kErrIndex);
   return -1;
