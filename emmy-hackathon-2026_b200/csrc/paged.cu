@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(kThreads)
   static_assert(kStages * kTile <= kThreads, "a thread looks up one key of the first tiles");
   __shared__ int64_t k_at[kSlots][kTile], v_at[kSlots][kTile];  // offsets of a tile's rows; -1: no such key
   __shared__ __align__(16) float ps[kWarps][RW][kTile];  // a warp's probabilities
+  __shared__ int64_t q_at[R];
   const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4;
   const int stage_floats = kTile * (ldk + dp);  // keys, then values; the stages behind the queries
   float *qs = smem, *tiles = qs + R * dp;
@@ -144,16 +145,20 @@ __global__ void __launch_bounds__(kThreads)
   }
 
   // this block's queries, FP32, times log2(e) / scale; eight loads in flight
+  if (threadIdx.x < R) {
+    const int row = row0 + threadIdx.x, j = row / a.group;
+    q_at[threadIdx.x] =
+        row < rows ? (int64_t)(s.first + j) * a.q_token + (int64_t)(head * a.group + row - j * a.group) * a.q_head : -1;
+  }
+  __syncthreads();
   constexpr int kBatch = 8;
   for (int i0 = threadIdx.x; i0 < R * dp; i0 += kBatch * kThreads) {
     float x[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kThreads, r = i / dp, c = i - r * dp, row = row0 + r;
-      x[u] = 0.0f;
-      if (r < R && row < rows && c < a.d)
-        x[u] = serve::to_f32(static_cast<const T *>(a.q)[(int64_t)(s.first + row / a.group) * a.q_token +
-                                                          (head * a.group + row % a.group) * a.q_head + c]);
+      const int i = i0 + u * kThreads, r = (unsigned)i / (unsigned)dp, c = i - r * dp;
+      const int64_t from = r < R ? q_at[r] : -1;
+      x[u] = from >= 0 && c < a.d ? serve::to_f32(static_cast<const T *>(a.q)[from + c]) : 0.0f;
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
@@ -408,9 +413,11 @@ cudaError_t merge(const Args &a, int sms, cudaStream_t s) {
   return b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), 0, s, a, vec_out);
 }
 
-// The kernel of a part: paged_rows_kernel, warp MMAs (paged_mma.cu) or the
-// tensor-memory kernel (paged_umma.cu).
-enum Path { kPlain, kMma, kUmma };
+// The kernel of a part: paged_rows_kernel, warp MMAs (paged_mma.cu), the
+// tensor-memory kernel (paged_umma.cu) or the f32 decode kernel (paged_f32.cu).
+enum Path { kPlain, kMma, kUmma, kF32 };
+// What a cache's type and alignment allow.
+enum Reach { kNoPieces, kHalfPieces, kFloatPieces };
 
 // What a call launches, from its host values alone.
 struct Plan {
@@ -427,10 +434,13 @@ size_t ml_bytes(size_t slots, int64_t tokens, int q_heads) {
 
 int plain_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 32; }
 
-// Whether the tensor-core kernels can read the cache: 16-byte pieces throughout.
-bool cache_pieces(const b2k_paged_cache &c) {
-  return c.dtype != B2K_F32 && c.d % 8 == 0 && serve::vec_ok(c.k, c.k_page, c.k_row, c.k_head, 2, 16) &&
-         serve::vec_ok(c.v, c.v_page, c.v_row, c.v_head, 2, 16);
+// Whether the cache can be read in 16-byte pieces throughout, and of what.
+Reach cache_pieces(const b2k_paged_cache &c) {
+  const int size = c.dtype == B2K_F32 ? 4 : 2;
+  if (c.d % (16 / size) || !serve::vec_ok(c.k, c.k_page, c.k_row, c.k_head, size, 16) ||
+      !serve::vec_ok(c.v, c.v_page, c.v_row, c.v_head, size, 16))
+    return kNoPieces;
+  return size == 4 ? kFloatPieces : kHalfPieces;
 }
 bool rows_pieces(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_token, x.stride_head, 0, 2, 16); }
 
@@ -443,13 +453,18 @@ bool rows_pieces(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_tok
 // above 128 do not fit its tensor memory twice.
 int g_kernel = 0;  // b2k_paged_attention_set_kernel
 
-Path pick_path(bool tensor, int d, int64_t rows, int64_t keys, int64_t units) {
-  if (!tensor || g_kernel == 1) return kPlain;
+// f32: up to 64 rows in the kernel that streams, eight to a block (42 rows of a
+// prefix of 333: 15 us a call in it, 20 in the other), more in the one whose
+// blocks hold 32 (160 rows of 1000: 64 us against 72; prompts of 430: 161
+// against 353).
+Path pick_path(Reach reach, int d, int64_t rows, int64_t keys, int64_t units) {
+  if (reach == kNoPieces || g_kernel == 1) return kPlain;
+  if (reach == kFloatPieces) return rows <= 64 ? kF32 : kPlain;
   if (g_kernel > 1) return g_kernel == 3 && d <= 128 ? kUmma : kMma;
   return rows > 32 && d <= 128 && (double)rows * keys * units * d > 16e6 * 128 ? kUmma : kMma;
 }
 int block_rows(Path path, int d, int64_t rows) {
-  return path == kPlain ? plain_rows(rows) : path == kMma ? paged::mma_rows(d, rows) : paged::kUmmaRows;
+  return path == kF32 ? (rows <= 4 ? 4 : 8) : path == kPlain ? plain_rows(rows) : path == kMma ? paged::mma_rows(d, rows) : paged::kUmmaRows;
 }
 
 // Splits of `keys` keys so that `units` independent row blocks become `want`
@@ -462,18 +477,18 @@ void split_keys(int64_t keys, int64_t units, int64_t want, int least, int tile, 
   chunk = (int)c;
 }
 
-Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, int sms, bool tensor) {
+Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, int sms, Reach reach) {
   Plan p = {};
   const int64_t group = q_heads / c.heads;
   const int64_t own = b.max_new * group, prefix = b.tokens * group;
-  p.own_path = pick_path(tensor, c.d, own, (int64_t)b.max_len + b.prefix_len, (int64_t)c.heads * b.sequences);
+  p.own_path = pick_path(reach, c.d, own, (int64_t)b.max_len + b.prefix_len, (int64_t)c.heads * b.sequences);
   p.own_rows = block_rows(p.own_path, c.d, own);
   // Sequences whose own rows fill a block read the prefix with their own keys:
   // stacking the rows of several sequences would save no reads of it.
   p.joined = b.prefix_len > 0 && own >= 128;
   // blocks that the GPU holds at once, and keys that make a block worth its start
-  auto wave = [&](Path path) { return (int64_t)sms * (path == kPlain ? 6 : path == kUmma || c.d > 128 ? 1 : 2); };
-  auto least = [&](Path path) { return path == kPlain ? 64 : path == kMma ? (c.d <= 64 ? 512 : 256) : 128; };
+  auto wave = [&](Path path) { return (int64_t)sms * (path == kPlain ? 6 : path == kUmma || (path == kMma && c.d > 128) ? 1 : 2); };
+  auto least = [&](Path path) { return path == kPlain ? 64 : path == kUmma ? 128 : path == kF32 ? 128 : c.d <= 64 ? 512 : 256; };
   auto tile = [](Path path) { return path == kUmma ? 128 : 64; };  // keys of a block's step
   // the tensor-memory kernel's tiles end with the prefix
   p.joined_keys = !p.joined ? 0 : p.own_path == kUmma ? (b.prefix_len + 127) / 128 * 128 : b.prefix_len;
@@ -485,11 +500,11 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
              (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, own_wave, least(p.own_path),
              tile(p.own_path), p.own_splits, p.own_chunk);
   if (b.prefix_len > 0 && !p.joined) {
-    p.prefix_path = pick_path(tensor, c.d, prefix, b.prefix_len, c.heads);
+    p.prefix_path = pick_path(reach, c.d, prefix, b.prefix_len, c.heads);
     p.prefix_rows = block_rows(p.prefix_path, c.d, prefix);
     // a few row blocks of the own part's height save a launch, at the price of
     // as many readings of the prefix
-    if (p.prefix_path == p.own_path && p.own_path != kUmma && prefix <= 4 * p.own_rows) p.prefix_rows = p.own_rows;
+    if (p.prefix_path == p.own_path && p.own_path != kUmma && prefix <= 8 * p.own_rows) p.prefix_rows = p.own_rows;
     const int64_t units = (prefix + p.prefix_rows - 1) / p.prefix_rows * c.heads;
     int64_t want = wave(p.prefix_path);
     if (p.prefix_path == kUmma && p.own_path != kUmma) {
@@ -554,6 +569,7 @@ int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t 
   auto parts = [&](Path path, bool pre, bool own, int rows, bool beside) {
     return path == kPlain ? rows_parts<T>(ctx, a, pre, own, rows, beside, s)
            : path == kMma ? paged::mma_parts(ctx, a, dtype, pre, own, rows, beside, s)
+           : path == kF32 ? paged::f32_parts(ctx, a, pre, own, rows, beside, s)
                           : paged::umma_part(ctx, a, dtype, pre, s);
   };
   if (!prefix) {
@@ -590,6 +606,14 @@ int check_call(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch
 
 }  // namespace
 
+// Workspace of a call with these host values, whatever its q and o are: those
+// off 16 bytes take the plain kernel, which splits otherwise.
+static size_t workspace_bytes_of(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, int sms) {
+  const Reach reach = cache_pieces(c);
+  const size_t plain = make_plan(c, b, q_heads, sms, kNoPieces).bytes;
+  return reach == kNoPieces ? plain : std::max(plain, make_plan(c, b, q_heads, sms, reach).bytes);
+}
+
 // Everything about a call's arguments but its workspace, and its plan.
 static int check_operands(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch *batch, const b2k_heads *q,
                           const b2k_heads *o, int sms, Plan &p) {
@@ -601,7 +625,9 @@ static int check_operands(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_
   if (status != B2K_OK) return status;
   if (q->heads != o->heads) return b2k::fail(ctx, B2K_EINVAL, "%s: %d heads in, %d out", what, q->heads, o->heads);
   if (q->data == o->data && batch->tokens > 0) return b2k::fail(ctx, B2K_EINVAL, "%s: o is q", what);
-  p = make_plan(*cache, *batch, q->heads, sms, cache_pieces(*cache) && rows_pieces(*q) && rows_pieces(*o));
+  Reach reach = cache_pieces(*cache);
+  if (reach == kHalfPieces && !(rows_pieces(*q) && rows_pieces(*o))) reach = kNoPieces;
+  p = make_plan(*cache, *batch, q->heads, sms, reach);
   return B2K_OK;
 }
 
@@ -617,8 +643,10 @@ extern "C" int b2k_paged_attention_plan(int32_t sms, const b2k_paged_cache *cach
   Plan p;
   const int status = check_operands(nullptr, cache, batch, q, o, sms, p);
   if (status != B2K_OK) return status;
-  *out = {(int32_t)p.own_path, p.prefix_splits > 0 ? (int32_t)p.prefix_path : -1, p.own_splits, p.own_chunk,
-          p.prefix_splits, p.prefix_chunk, p.joined, 0, (int64_t)p.bytes};
+  auto shown = [](Path path) { return path == kF32 ? 0 : (int32_t)path; };
+  *out = {shown(p.own_path), p.prefix_splits > 0 ? shown(p.prefix_path) : -1, p.own_splits, p.own_chunk,
+          p.prefix_splits, p.prefix_chunk, p.joined, 0,
+          (int64_t)workspace_bytes_of(*cache, *batch, q->heads, sms)};
   return B2K_OK;
 }
 
@@ -628,9 +656,7 @@ extern "C" int b2k_paged_attention_workspace(b2k_ctx *ctx, const b2k_paged_cache
   if (!bytes) return b2k::fail(ctx, B2K_EINVAL, "paged_attention_workspace: null result");
   int status = check_call(ctx, cache, batch, q_heads);
   if (status != B2K_OK) return status;
-  // queries or outputs off 16 bytes take the plain kernel, which splits otherwise
-  *bytes = make_plan(*cache, *batch, q_heads, ctx->sm_count, false).bytes;
-  if (cache_pieces(*cache)) *bytes = std::max(*bytes, make_plan(*cache, *batch, q_heads, ctx->sm_count, true).bytes);
+  *bytes = workspace_bytes_of(*cache, *batch, q_heads, ctx->sm_count);
   return B2K_OK;
 }
 
@@ -644,10 +670,11 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   const int status = check_operands(ctx, cache, batch, q, o, ctx->sm_count, p);
   if (status != B2K_OK) return status;
   if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+  const size_t needed = workspace_bytes_of(*cache, *batch, q->heads, ctx->sm_count);
+  if (needed > 0 && (!workspace || workspace_bytes < needed))
     return b2k::fail(ctx, B2K_EINVAL, "%s: a workspace of %zu bytes where %zu are needed", what,
-                     workspace ? workspace_bytes : (size_t)0, p.bytes);
-  if (p.bytes > 0 && !b2k::aligned16(workspace))
+                     workspace ? workspace_bytes : (size_t)0, needed);
+  if (needed > 0 && !b2k::aligned16(workspace))
     return b2k::fail(ctx, B2K_EINVAL, "%s: the workspace is not 16-byte aligned", what);
   Args a = {};
   a.q = q->data;

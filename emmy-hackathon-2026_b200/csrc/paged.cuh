@@ -152,6 +152,9 @@ int mma_rows(int d, int64_t rows);
 int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool with_own, int rows, bool beside,
               cudaStream_t s);
 
+// paged_f32.cu: the same for f32 in 16-byte pieces, blocks of 4 or 8 rows.
+int f32_parts(b2k_ctx *ctx, const Args &a, bool with_prefix, bool with_own, int rows, bool beside, cudaStream_t s);
+
 // paged_umma.cu: rows of a block, and the launch of one part.
 constexpr int kUmmaRows = 256;
 int umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s);
