@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -234,31 +235,36 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
     __syncwarp();
-    for (int t0 = 4 * side; t0 < kTile; t0 += 4 * kSides) {
-      float4 vv[4][DV];
+    // the test of a masked key costs as much as its products: only where there is one
+    auto values = [&](auto guarded) {
+      for (int t0 = 4 * side; t0 < kTile; t0 += 4 * kSides) {
+        float4 vv[4][DV];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int c = 0; c < DV; ++c)
-          vv[u][c] = col + 128 * c < dp ? *reinterpret_cast<const float4 *>(vs + (t0 + u) * dp + col + 128 * c)
-                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int c = 0; c < DV; ++c)
+            vv[u][c] = col + 128 * c < dp ? *reinterpret_cast<const float4 *>(vs + (t0 + u) * dp + col + 128 * c)
+                                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < RW; ++i) {
-        const float4 p4 = *reinterpret_cast<const float4 *>(&ps[warp][i][t0]);
-        const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+        for (int i = 0; i < RW; ++i) {
+          const float4 p4 = *reinterpret_cast<const float4 *>(&ps[warp][i][t0]);
+          const float p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (!open && p[u] == 0.0f) continue;  // a masked value may be anything
+          for (int u = 0; u < 4; ++u) {
+            if (decltype(guarded)::value && p[u] == 0.0f) continue;  // a masked value may be anything
 #pragma unroll
-          for (int c = 0; c < DV; ++c) {
-            o[i][c].x = fmaf(p[u], vv[u][c].x, o[i][c].x);
-            o[i][c].y = fmaf(p[u], vv[u][c].y, o[i][c].y);
-            o[i][c].z = fmaf(p[u], vv[u][c].z, o[i][c].z);
-            o[i][c].w = fmaf(p[u], vv[u][c].w, o[i][c].w);
+            for (int c = 0; c < DV; ++c) {
+              o[i][c].x = fmaf(p[u], vv[u][c].x, o[i][c].x);
+              o[i][c].y = fmaf(p[u], vv[u][c].y, o[i][c].y);
+              o[i][c].z = fmaf(p[u], vv[u][c].z, o[i][c].z);
+              o[i][c].w = fmaf(p[u], vv[u][c].w, o[i][c].w);
+            }
           }
         }
       }
-    }
+    };
+    if (open) values(std::false_type{});
+    else values(std::true_type{});
     // (this tile's slot is not the one written: kSlots is one more than the stages)
     if (threadIdx.x < kTile) answer(tile + kStages, threadIdx.x);
     __syncthreads();  // the stage may be written again
@@ -313,11 +319,12 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
   constexpr int kStep = SHARED ? kWarps : 1;          // parts from one of a warp's to the next
   constexpr int kAhead = SHARED ? 10 : 4;  // parts a warp has in flight: up to 40 of a row at once
   __shared__ float sums[SHARED ? kWarps : 1][SHARED ? B2K_MAX_HEAD_DIM : 1];
-  grid_dependency_wait();
-  grid_dependents_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_heads = a.kv_heads * a.group;
+  // (the sequence's numbers were there before the parts began: part_begin)
   const paged::Sequence s = paged::sequence(a, blockIdx.x);
+  grid_dependency_wait();
+  grid_dependents_launch();
   const int64_t stride = a.tokens * q_heads;
   const int64_t step = (int64_t)gridDim.y * (SHARED ? 1 : kWarps);
   for (int64_t row = (int64_t)blockIdx.y * (SHARED ? 1 : kWarps) + (SHARED ? 0 : warp); row < (int64_t)s.n * q_heads;

@@ -18,6 +18,8 @@
 // quarter warp meet eight different pieces in both products.
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace {
@@ -257,31 +259,36 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 2 : 3) paged_f32_kernel(
       }
     }
     __syncwarp();
+    // the test of a masked key costs as much as its products: only where there is one
+    auto values = [&](auto guarded) {
 #pragma unroll
-    for (int t0 = 0; t0 < kTile / kSides; t0 += 4) {
-      const int t = t0 * kSides + 4 * side;
-      float4 v[4][kDims];
+      for (int t0 = 0; t0 < kTile / kSides; t0 += 4) {
+        const int t = t0 * kSides + 4 * side;
+        float4 v[4][kDims];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int c = 0; c < kDims; ++c) v[u][c] = *reinterpret_cast<const float4 *>(vs + place(t + u, dim + 32 * c));
+          for (int c = 0; c < kDims; ++c) v[u][c] = *reinterpret_cast<const float4 *>(vs + place(t + u, dim + 32 * c));
 #pragma unroll
-      for (int x = 0; x < R; ++x) {
-        const float4 p4 = *reinterpret_cast<const float4 *>(&ps[warp][x][t]);
-        const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+        for (int x = 0; x < R; ++x) {
+          const float4 p4 = *reinterpret_cast<const float4 *>(&ps[warp][x][t]);
+          const float p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (!open && p[u] == 0.0f) continue;  // a masked value may be anything
+          for (int u = 0; u < 4; ++u) {
+            if (decltype(guarded)::value && p[u] == 0.0f) continue;  // a masked value may be anything
 #pragma unroll
-          for (int c = 0; c < kDims; ++c) {
-            o[x][c].x = fmaf(p[u], v[u][c].x, o[x][c].x);
-            o[x][c].y = fmaf(p[u], v[u][c].y, o[x][c].y);
-            o[x][c].z = fmaf(p[u], v[u][c].z, o[x][c].z);
-            o[x][c].w = fmaf(p[u], v[u][c].w, o[x][c].w);
+            for (int c = 0; c < kDims; ++c) {
+              o[x][c].x = fmaf(p[u], v[u][c].x, o[x][c].x);
+              o[x][c].y = fmaf(p[u], v[u][c].y, o[x][c].y);
+              o[x][c].z = fmaf(p[u], v[u][c].z, o[x][c].z);
+              o[x][c].w = fmaf(p[u], v[u][c].w, o[x][c].w);
+            }
           }
         }
       }
-    }
+    };
+    if (open) values(std::false_type{});
+    else values(std::true_type{});
     __syncwarp();  // the stage, and the probabilities, may be written again
   }
 
