@@ -155,8 +155,12 @@ int mma_parts(b2k_ctx *ctx, const Args &a, int32_t dtype, bool with_prefix, bool
 // paged_f32.cu: the same for f32 in 16-byte pieces, blocks of 4 or 8 rows.
 int f32_parts(b2k_ctx *ctx, const Args &a, bool with_prefix, bool with_own, int rows, bool beside, cudaStream_t s);
 
-// paged_umma.cu: rows of a block, and the launch of one part.
-constexpr int kUmmaRows = 256;
+// paged_umma.cu (and paged_umma_wide.cu for head dims above 128): rows of a block,
+// whether a cache's pages can be loaded as boxes, which the wide kernel needs,
+// and the launch of one part.
+inline int umma_rows(int d) { return d <= 128 ? 256 : 128; }
+bool umma_boxes(const b2k_paged_cache &c);
+int umma_wide_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, int row_blocks, unsigned blocks, cudaStream_t s);
 int umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s);
 
 }  // namespace paged

@@ -39,24 +39,14 @@
 // Bound: tensor core and exponentials alike: a pair of 128 x 128 tiles takes
 // 2 x 1024 tensor cycles at head dim 128 and 2 x 1024 of the special-function unit.
 // All mbarrier waits are bounded (sm100.cuh).
-#include <math.h>
-
-#include <algorithm>
-
-#include "paged.cuh"
-#include "sm100.cuh"
-#include "tmap.cuh"
+#include "paged_umma.cuh"
 
 namespace {
 
-using paged::Args;
+using namespace umma;
 
-constexpr int kRows = 128;    // rows of a tile
-constexpr int kKeys = 128;    // keys of a tile
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 2;
 constexpr int kThreads = 32 * (kSoftmaxWarps + kLoadWarps + 2);
-constexpr int kHalf = kKeys * 128;  // bytes of a tile's 64 columns: 128 rows of 128 bytes
-constexpr int kMarks = 8;     // tiles whose key marks are kept
 
 template <int DP>
 constexpr int tile_bytes() { return kHalf * (DP / 64); }
@@ -65,47 +55,8 @@ constexpr int stages() { return DP == 64 ? 8 : 5; }
 template <int DP>
 constexpr int smem_bytes() { return 2 * tile_bytes<DP>() + stages<DP>() * tile_bytes<DP>(); }
 
-// 4-D tile load: (element, row of the page, head, page).
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
-
 // Tensor-memory columns.
 constexpr uint32_t kColS = 0, kColO = 256;  // S (then P) of tile A, B: 128 each; O of A, B: 128 each
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
-// Two FP32 operations in one instruction.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float &lo, float &hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  return r;
-}
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {
   const int bytes = on ? 16 : 0;
@@ -116,76 +67,6 @@ __device__ __forceinline__ void copy_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sm100::smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
-template <typename T>
-struct Type;
-template <>
-struct Type<__half> {
-  static constexpr uint32_t kFormat = 0;
-  static constexpr float kLift = 6.0f, kSlack = 8.0f;  // 2^14 at most: within f16
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-};
-template <>
-struct Type<__nv_bfloat16> {
-  static constexpr uint32_t kFormat = 1;
-  static constexpr float kLift = 0.0f, kSlack = 8.0f;
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-};
-
-// Instruction descriptor, kind::f16, FP32 accumulate (fields as idesc_tf32).
-template <typename T>
-__device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
-  return (1u << 4) | (Type<T>::kFormat << 7) | (Type<T>::kFormat << 10) | (b_mn_major ? (1u << 16) : 0u) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
-}
-
-// MN-major 16-bit operand with the 128-byte swizzle: atoms of 64 MN-consecutive
-// elements (128 bytes) by 8 K rows (1024 bytes); bits 16-29 the stride between
-// atoms along MN, bits 32-45 along K.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t mn_stride, uint32_t k_stride) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>((mn_stride >> 4) & 0x3FFFu) << 16 |
-         static_cast<uint64_t>((k_stride >> 4) & 0x3FFFu) << 32 | static_cast<uint64_t>(1u) << 46 |
-         static_cast<uint64_t>(2u) << 61;
-}
-
-// Four products D (+)= A B of 16 steps of K each, issued by one elected lane of a
-// converged warp: A in shared memory, K-major like B, 32 bytes (2 units of a
-// descriptor's address) a step; or A in tensor memory, eight columns a step,
-// and B N-major, 2048 bytes a step.  The first overwrites D unless `accumulate`.
-__device__ __forceinline__ void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
-      "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
-      "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred e, p, t;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
-      "add.u32 a1, %1, 8;\n\tadd.s64 b1, %2, 128;\n\tadd.u32 a2, %1, 16;\n\tadd.s64 b2, %2, 256;\n\t"
-      "add.u32 a3, %1, 24;\n\tadd.s64 b3, %2, 384;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(accumulate)
-      : "memory");
-}
 
 template <typename T, int DP, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -605,8 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sm100::tmem_ld_32x32b_x32(o_at + i, ov);
           sm100::tmem_ld_wait();
         }
-        if (!on) continue;
-        if (direct) {
+        if (on && direct) {
           T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + i;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
@@ -616,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               w[u] = some && mine > 0 ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
             if (i + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-        } else {
+        } else if (on) {
           float *out = a.part_o + part * a.d + i;
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
@@ -626,6 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                  __uint_as_float(ov[e + 3]))
                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
+        __syncwarp();  // the next load is the whole warp's
       }
     }
   }
@@ -637,59 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// [pages][heads][page rows][d] of a cache in any order of strides, boxes of 64
-// elements by a page's rows (128 at most).
-template <typename T>
-int make_map(b2k_ctx *ctx, CUtensorMap *map, const Args &a, bool keys) {
-  auto encode = b2k::tensor_map_encoder();
-  if (!encode) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled is unavailable");
-  const void *base = keys ? a.k : a.v;
-  const int64_t row = keys ? a.k_row : a.v_row, head = keys ? a.k_head : a.v_head, page = keys ? a.k_page : a.v_page;
-  cuuint64_t dims[4] = {(cuuint64_t)a.d, (cuuint64_t)a.page_size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
-  cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)std::min(a.page_size, kKeys), 1, 1};
-  cuuint32_t elem[4] = {1, 1, 1, 1};
-  const CUresult res =
-      encode(map, Type<T>::kFormat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-             const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (res != CUDA_SUCCESS) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)res);
-  return B2K_OK;
-}
-
-// Whether pages are boxes: whole swizzle atoms (8 rows) that tile 128 keys, or
-// 128 keys a part of one; and strides and extents a tensor map can hold.
-bool boxes_fit(const Args &a) {
-  const int64_t most = (int64_t)1 << 38;  // 2^39 bytes
-  return a.page_size >= 8 && (kKeys % a.page_size == 0 || a.page_size % kKeys == 0) && a.pages <= INT32_MAX &&
-         a.k_row < most && a.k_head < most && a.k_page < most && a.v_row < most && a.v_head < most && a.v_page < most;
-}
-
-// Queries [tokens][heads][d], boxes of 64 elements by a cache head's query heads
-// by the tokens that make 128 rows.
-template <typename T>
-int make_q_map(b2k_ctx *ctx, CUtensorMap *map, const Args &a) {
-  auto encode = b2k::tensor_map_encoder();
-  if (!encode) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[3] = {(cuuint64_t)a.d, (cuuint64_t)(a.kv_heads * a.group), (cuuint64_t)a.tokens};
-  cuuint64_t strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_token * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(kRows / a.group)};
-  cuuint32_t elem[3] = {1, 1, 1};
-  const CUresult res =
-      encode(map, Type<T>::kFormat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-             const_cast<void *>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (res != CUDA_SUCCESS) return b2k::fail(ctx, B2K_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)res);
-  return B2K_OK;
-}
-
 template <typename T, int DP, bool TMA>
 int launch(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned blocks, cudaStream_t s) {
   auto kernel = paged_umma_kernel<T, DP, TMA>;
   CUtensorMap map_k = {}, map_v = {}, map_q = {};
-  // A single head's stride is not used, but a tensor map wants one it can hold.
-  const int64_t most = (int64_t)1 << 38;
-  const bool q_boxes = TMA && kRows % a.group == 0 && a.q_head > 0 && a.q_token > 0 && a.q_head < most && a.q_token < most;
+  const bool q_boxes = TMA && query_boxes_fit(a);
   int status = B2K_OK;
   if (TMA) status = make_map<T>(ctx, &map_k, a, true);
   if (TMA && status == B2K_OK) status = make_map<T>(ctx, &map_v, a, false);
@@ -716,11 +549,26 @@ int pick(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned bloc
 
 namespace paged {
 
+bool umma_boxes(const b2k_paged_cache &c) {
+  Args a = {};
+  a.page_size = c.page_size;
+  a.pages = c.pages;
+  a.k_row = c.k_row;
+  a.k_head = c.k_head;
+  a.k_page = c.k_page;
+  a.v_row = c.v_row;
+  a.v_head = c.v_head;
+  a.v_page = c.v_page;
+  return boxes_fit(a);
+}
+
 int umma_part(b2k_ctx *ctx, const Args &a, int32_t dtype, bool prefix, cudaStream_t s) {
   const int64_t rows = (prefix ? a.tokens : (int64_t)a.max_new) * a.group;
-  const int64_t row_blocks = (rows + kUmmaRows - 1) / kUmmaRows;
+  const int block_rows = umma_rows(a.d);
+  const int64_t row_blocks = (rows + block_rows - 1) / block_rows;
   const int64_t blocks = row_blocks * a.kv_heads * (prefix ? a.prefix_splits : (int64_t)a.own_splits * a.sequences);
   if (blocks > INT32_MAX) return b2k::fail(ctx, B2K_EUNSUPPORTED, "paged_attention: %lld blocks", (long long)blocks);
+  if (a.d > 128) return umma_wide_part(ctx, a, dtype, prefix, (int)row_blocks, (unsigned)blocks, s);
   return dtype == B2K_F16 ? pick<__half>(ctx, a, prefix, (int)row_blocks, (unsigned)blocks, s)
                           : pick<__nv_bfloat16>(ctx, a, prefix, (int)row_blocks, (unsigned)blocks, s);
 }

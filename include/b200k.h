@@ -459,8 +459,9 @@ int b2k_paged_attention_plan(int32_t sms, const b2k_paged_cache *cache, const b2
                              const b2k_heads *o, b2k_paged_attention_plan_info *out);
 /* Process-wide choice of b2k_paged_attention's kernels, kept for comparisons
  * and tests: 0 (default) by operands and sizes; 1 the plain cores always; 2
- * warp MMAs, 3 tensor memory, wherever the operands (and for 3 the head dim, at
- * most 128) allow, and 1 or 2 elsewhere.  Other values return B2K_EINVAL.  A
+ * warp MMAs, 3 tensor memory, wherever the operands (and for 3 with head dims
+ * above 128 the page size: 8 to 128 that divides 128, or a multiple of it)
+ * allow, and 1 or 2 elsewhere.  Other values return B2K_EINVAL.  A
  * workspace is asked for under the setting it is used with. */
 int b2k_paged_attention_set_kernel(int mode);
 

@@ -106,7 +106,7 @@ def test_attention_odd_head_dims(ctx, torch_cuda, dtype, d):
 
 
 @pytest.mark.parametrize("page", [1, 4, 8, 16, 20, 24, 64, 128, 256, 384])
-@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (3, 1, 128), (14, 2, 80), (16, 1, 128), (32, 2, 40)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (3, 1, 128), (14, 2, 80), (16, 1, 128), (32, 2, 40), (12, 4, 256), (8, 4, 192)])
 def test_attention_page_sizes_and_groups(ctx, torch_cuda, kernel, page, hq, hkv, d):
     """Boxes of pages, of tokens by heads, and what neither fits; tiles that end in a prefix, a page and a length."""
     dt = torch.bfloat16 if page % 16 else torch.float16

@@ -98,7 +98,8 @@ def test_paged_plan_kernels():
     assert plan(d=100)["own_kernel"] == plain                             # no 16-byte pieces
     assert plan(at=4098)["own_kernel"] == plain and plan(q=4098)["own_kernel"] == plain and plan(o=8194)["own_kernel"] == plain
     assert plan(new=512, length=4096)["own_kernel"] == memory             # prompts
-    assert plan(new=512, length=4096, d=256)["own_kernel"] == warp        # too wide for tensor memory
+    assert plan(new=512, length=4096, d=256)["own_kernel"] == memory
+    assert plan(new=512, length=4096, d=256, page=20)["own_kernel"] == warp   # no boxes, which wide heads need there
     assert plan(new=8, length=64)["own_kernel"] == warp                   # 32 rows fit the warp kernel
     assert plan(new=9, length=40)["own_kernel"] == warp                   # more, but too little work to repay a block's start
     decode = plan(sequences=128, prefix=8192, hq=64)
