@@ -453,23 +453,27 @@ bool rows_pieces(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_tok
 
 // Kernel for a part with `rows` rows and `keys` keys a cache head, in `units`
 // such pairs.  Up to 32 rows fit one block of the warp kernel, which then reads
-// the keys once as well, two blocks an SM; above that the tensor-memory kernel's
-// 256 rows save re-reading them, and at 2.4 times the rate (2.4 against 1.0
-// million rows x keys a microsecond at head dim 128) it repays the 10 us that
-// its launch and its blocks' starts cost from about 16 million on.  Head dims
-// above 128 need pages that are boxes there.
-int g_kernel = 0;  // b2k_paged_attention_set_kernel
-
+// the keys once as well, two or three blocks an SM; above that the tensor-memory
+// kernel's 256 rows save re-reading them, and its products cost less, but its
+// launch and its blocks' starts cost about 10 us.  By rows x keys x units: own
+// parts are even near 3 million (16 / 4 heads; 2.3 million at head dim 128: 19 us
+// with warps, 26 with tensor memory; 4.4 million: 31 and 20; 4.4 million at 64:
+// 21 and 17, at 256: 56 and 27), a prefix, whose blocks run beside the own
+// part's, near 1.5 million (2 million behind 32 single tokens: 25 and 22; 6.4
+// million behind 100: 44 and 31; 0.5 million: even).  Head dims above 128 need
+// pages that are boxes there.
 // f32: up to 64 rows in the kernel that streams, eight to a block (42 rows of a
 // prefix of 333: 15 us a call in it, 20 in the other), more in the one whose
 // blocks hold 32 (160 rows of 1000: 64 us against 72; prompts of 430: 161
 // against 353).
-Path pick_path(Reach reach, const b2k_paged_cache &c, int64_t rows, int64_t keys, int64_t units) {
+int g_kernel = 0;  // b2k_paged_attention_set_kernel
+
+Path pick_path(Reach reach, const b2k_paged_cache &c, int64_t rows, int64_t keys, int64_t units, double repaid) {
   if (reach == kNoPieces || g_kernel == 1) return kPlain;
   if (reach == kFloatPieces) return rows <= 64 ? kF32 : kPlain;
   const bool umma = c.d <= 128 || paged::umma_boxes(c);
   if (g_kernel > 1) return g_kernel == 3 && umma ? kUmma : kMma;
-  return umma && rows > 32 && (double)rows * keys * units * c.d > 16e6 * 128 ? kUmma : kMma;
+  return umma && rows > 32 && (double)rows * keys * units > repaid ? kUmma : kMma;
 }
 int block_rows(Path path, int d, int64_t rows) {
   return path == kF32 ? (rows <= 4 ? 4 : 8) : path == kPlain ? plain_rows(rows) : path == kMma ? paged::mma_rows(d, rows) : paged::umma_rows(d);
@@ -489,7 +493,7 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   Plan p = {};
   const int64_t group = q_heads / c.heads;
   const int64_t own = b.max_new * group, prefix = b.tokens * group;
-  p.own_path = pick_path(reach, c, own, (int64_t)b.max_len + b.prefix_len, (int64_t)c.heads * b.sequences);
+  p.own_path = pick_path(reach, c, own, (int64_t)b.max_len + b.prefix_len, (int64_t)c.heads * b.sequences, 3e6);
   p.own_rows = block_rows(p.own_path, c.d, own);
   // Sequences whose own rows fill a block read the prefix with their own keys:
   // stacking the rows of several sequences would save no reads of it.
@@ -508,7 +512,7 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
              (own + p.own_rows - 1) / p.own_rows * c.heads * b.sequences, own_wave, least(p.own_path),
              tile(p.own_path), p.own_splits, p.own_chunk);
   if (b.prefix_len > 0 && !p.joined) {
-    p.prefix_path = pick_path(reach, c, prefix, b.prefix_len, c.heads);
+    p.prefix_path = pick_path(reach, c, prefix, b.prefix_len, c.heads, 1.5e6);
     p.prefix_rows = block_rows(p.prefix_path, c.d, prefix);
     // a few row blocks of the own part's height save a launch, at the price of
     // as many readings of the prefix
