@@ -609,8 +609,9 @@ int check_call(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_paged_batch
   if (q_heads < 1 || q_heads > 65535 || q_heads % cache->heads)
     return b2k::fail(ctx, B2K_EINVAL, "paged_attention: %d query heads for %d cache heads", q_heads, cache->heads);
   // the limits of a launch's grid, and of a row's 32-bit number
-  if (batch->sequences > 65535 || batch->tokens * q_heads > INT32_MAX || (int64_t)batch->max_new * q_heads > INT32_MAX ||
-      (int64_t)batch->max_len + batch->prefix_len > INT32_MAX - 65536)
+  constexpr int64_t kMost = INT32_MAX - 65536;  // sums of a row's or key's number and a block's stay within 32 bits
+  if (batch->sequences > 65535 || batch->tokens * q_heads > kMost || (int64_t)batch->max_new * q_heads > kMost ||
+      (int64_t)batch->max_len + batch->prefix_len > kMost)
     return b2k::fail(ctx, B2K_EUNSUPPORTED, "paged_attention: a batch of %d sequences, %lld rows is too large",
                      batch->sequences, (long long)(batch->tokens * q_heads));
   return B2K_OK;
@@ -632,8 +633,8 @@ static int check_operands(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_
   const char *what = "paged_attention";
   if (!q) return b2k::fail(ctx, B2K_EINVAL, "%s: no q", what);
   int status = check_call(ctx, cache, batch, q->heads);
-  if (status == B2K_OK) status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d);
-  if (status == B2K_OK) status = serve::check_heads(ctx, what, "o", o, batch->tokens, cache->d);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d, cache->dtype);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "o", o, batch->tokens, cache->d, cache->dtype);
   if (status != B2K_OK) return status;
   if (q->heads != o->heads) return b2k::fail(ctx, B2K_EINVAL, "%s: %d heads in, %d out", what, q->heads, o->heads);
   if (q->data == o->data && batch->tokens > 0) return b2k::fail(ctx, B2K_EINVAL, "%s: o is q", what);

@@ -347,10 +347,13 @@ int use_rope(b2k_ctx *ctx, const char *what, const b2k_rope *rope, int32_t d, in
 
 namespace serve {
 
-int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d) {
+int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d,
+                int32_t dtype) {
   if (!x) return b2k::fail(ctx, B2K_EINVAL, "%s: no %s", what, name);
   if (x->heads < 1 || x->heads > 65535) return b2k::fail(ctx, B2K_EINVAL, "%s: %s has %d heads", what, name, x->heads);
   if (tokens > 0 && !x->data) return b2k::fail(ctx, B2K_EINVAL, "%s: null %s", what, name);
+  if (!on_boundary(x->data, type_size(dtype)))
+    return b2k::fail(ctx, B2K_EINVAL, "%s: %s is off its elements' boundary", what, name);
   if (x->stride_token < 0 || x->stride_head < 0 || (x->heads > 1 && x->stride_head < d))
     return b2k::fail(ctx, B2K_EINVAL, "%s: %s has strides %lld, %lld", what, name, (long long)x->stride_token,
                      (long long)x->stride_head);
@@ -365,6 +368,8 @@ int check_cache(b2k_ctx *ctx, const char *what, const b2k_paged_cache *c) {
                      c->page_size, c->heads);
   if (c->d < 1 || c->d > B2K_MAX_HEAD_DIM) return b2k::fail(ctx, B2K_EINVAL, "%s: head dim %d", what, c->d);
   if (!c->k || !c->v) return b2k::fail(ctx, B2K_EINVAL, "%s: null cache", what);
+  if (!on_boundary(c->k, type_size(c->dtype)) || !on_boundary(c->v, type_size(c->dtype)))
+    return b2k::fail(ctx, B2K_EINVAL, "%s: the cache is off its elements' boundary", what);
   if (c->k_page < c->d || c->k_row < c->d || c->k_head < c->d || c->v_page < c->d || c->v_row < c->d ||
       c->v_head < c->d)
     return b2k::fail(ctx, B2K_EINVAL, "%s: a cache stride is below the head dim", what);
@@ -383,6 +388,9 @@ int check_batch(b2k_ctx *ctx, const char *what, const b2k_paged_cache *c, const 
   if (b->max_len > (int64_t)b->table_width * c->page_size)
     return b2k::fail(ctx, B2K_EINVAL, "%s: max_len %d is beyond the table's %d pages of %d", what, b->max_len,
                      b->table_width, c->page_size);
+  if (!on_boundary(b->first, 4) || !on_boundary(b->lengths, 4) || !on_boundary(b->table, 4) ||
+      !on_boundary(b->prefix_table, 4))
+    return b2k::fail(ctx, B2K_EINVAL, "%s: first, lengths or a table is off 4 bytes", what);
   if (b->prefix_len > 0 && !b->prefix_table) return b2k::fail(ctx, B2K_EINVAL, "%s: no prefix table", what);
   return B2K_OK;
 }
@@ -455,8 +463,8 @@ int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count,
   if (status != B2K_OK) return status;
   const int64_t size = (int64_t)serve::type_size(dtype);
   for (int i = 0; i < count; ++i) {
-    if ((status = serve::check_heads(ctx, "rotary", "input", &x[i], tokens, d)) != B2K_OK) return status;
-    if ((status = serve::check_heads(ctx, "rotary", "output", &y[i], tokens, d)) != B2K_OK) return status;
+    if ((status = serve::check_heads(ctx, "rotary", "input", &x[i], tokens, d, dtype)) != B2K_OK) return status;
+    if ((status = serve::check_heads(ctx, "rotary", "output", &y[i], tokens, d, dtype)) != B2K_OK) return status;
     if (x[i].heads != y[i].heads)
       return b2k::fail(ctx, B2K_EINVAL, "rotary: tensor %d has %d heads in and %d out", i, x[i].heads, y[i].heads);
     if (x[i].data == y[i].data && (x[i].stride_token != y[i].stride_token || x[i].stride_head != y[i].stride_head))
@@ -466,7 +474,8 @@ int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count,
     a.heads += x[i].heads;
   }
   if (tokens == 0) return B2K_OK;
-  if (!positions) return b2k::fail(ctx, B2K_EINVAL, "rotary: null positions");
+  if (!positions || !serve::on_boundary(positions, 8))
+    return b2k::fail(ctx, B2K_EINVAL, "rotary: positions are null or off 8 bytes");
   a.d = d;
   a.tokens = tokens;
   a.positions = positions;
@@ -480,8 +489,8 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
   const char *what = "paged_append";
   int status = serve::check_cache(ctx, what, cache);
   if (status == B2K_OK) status = serve::check_batch(ctx, what, cache, batch);
-  if (status == B2K_OK) status = serve::check_heads(ctx, what, "k", k, batch->tokens, cache->d);
-  if (status == B2K_OK) status = serve::check_heads(ctx, what, "v", v, batch->tokens, cache->d);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "k", k, batch->tokens, cache->d, cache->dtype);
+  if (status == B2K_OK) status = serve::check_heads(ctx, what, "v", v, batch->tokens, cache->d, cache->dtype);
   if (status != B2K_OK) return status;
   if (k->heads != cache->heads || v->heads != cache->heads)
     return b2k::fail(ctx, B2K_EINVAL, "%s: %d key and %d value heads for a cache of %d", what, k->heads, v->heads,
@@ -494,8 +503,8 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
   const int64_t size = (int64_t)serve::type_size(cache->dtype);
   int count = 0;
   if (q) {
-    if ((status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d)) != B2K_OK) return status;
-    if ((status = serve::check_heads(ctx, what, "q_out", q_out, batch->tokens, cache->d)) != B2K_OK) return status;
+    if ((status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d, cache->dtype)) != B2K_OK) return status;
+    if ((status = serve::check_heads(ctx, what, "q_out", q_out, batch->tokens, cache->d, cache->dtype)) != B2K_OK) return status;
     if (q->heads != q_out->heads ||
         (q->data == q_out->data && (q->stride_token != q_out->stride_token || q->stride_head != q_out->stride_head)))
       return b2k::fail(ctx, B2K_EINVAL, "%s: q and q_out differ in heads, or in strides in place", what);

@@ -47,7 +47,11 @@ __host__ __device__ __forceinline__ int64_t page_of(const int32_t *table_row, in
 // b2k_paged_cache / b2k_paged_batch / b2k_heads argument checks (rotary.cu).
 int check_cache(b2k_ctx *ctx, const char *what, const b2k_paged_cache *cache);
 int check_batch(b2k_ctx *ctx, const char *what, const b2k_paged_cache *cache, const b2k_paged_batch *batch);
-int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d);
+int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d,
+                int32_t dtype);
+
+// Whether an array lies on its elements' boundary (a load off it faults).
+inline bool on_boundary(const void *p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 
 // Whether a tensor's base and strides allow accesses of `bytes` bytes.
 inline bool vec_ok(const void *p, int64_t s0, int64_t s1, int64_t s2, size_t size, size_t bytes) {

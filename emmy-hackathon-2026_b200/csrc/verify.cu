@@ -20,7 +20,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.cuh"
+#include "serve.cuh"
 
 namespace {
 
@@ -128,7 +128,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
       constexpr bool kQ = decltype(has_q)::value, kWithout = decltype(without)::value;
       double s[4] = {0.0, 0.0, 0.0, 0.0};
       const float *p = rest.p + lane, *q = rest.q + (kQ ? lane : 0);
-      const int skip = kWithout ? (int)(rest.without - lane) : 0;  // (vocab is below 2^31)
+      const int skip = kWithout ? (int)(rest.without - lane) : 0;  // (vocab is below 2^31 - 2^16)
       int i = (int)lo;
       const int end = (int)hi;
       for (; i + 32 * kAhead <= end; i += 32 * kAhead) {
@@ -252,7 +252,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
 extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *accepted, int32_t *tokens, void *stream) {
   B2K_CHECK_CTX(ctx);
   if (!d) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: null drafts");
-  if (d->batch < 0 || d->drafts < 0 || d->vocab < 1 || d->vocab > INT32_MAX)
+  if (d->batch < 0 || d->drafts < 0 || d->vocab < 1 || d->vocab > INT32_MAX - 65536)
     return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: batch %lld, %d drafts, vocab %lld", (long long)d->batch, d->drafts,
                      (long long)d->vocab);
   if (d->batch > INT32_MAX / kCluster) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: too many sequences");
@@ -261,6 +261,9 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   if (d->batch == 0) return B2K_OK;
   if (!d->target || !d->u_sample || !accepted || !tokens || (d->drafts > 0 && (!d->drafted || !d->u_accept)))
     return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: null buffer");
+  const void *arrays[] = {d->target, d->draft, d->drafted, d->counts, d->u_accept, d->u_sample, accepted, tokens};
+  for (const void *p : arrays)
+    if (!serve::on_boundary(p, 4)) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: a buffer is off 4 bytes");
   cudaStream_t s = (cudaStream_t)stream;
   b2k::PhaseTimer timer(ctx, B2K_PHASE_VERIFY, s);
   const VerifyArgs a{*d, accepted, tokens};

@@ -130,7 +130,10 @@ def test_rotary_refusals(ctx, torch_cuda):
                  (rope, rt.F32, [(heads(x), rt.heads(x.data_ptr(), 1, 64, 32))], pos.data_ptr(), 4, 32),
                  (rope, rt.F32, [(heads(x), rt.heads(0, 2, 64, 32))], pos.data_ptr(), 4, 32),
                  (rope, rt.F32, [(heads(x), rt.heads(x.data_ptr(), 2, 128, 32))], pos.data_ptr(), 4, 32),
-                 (rope, rt.F32, [(narrow, narrow)], pos.data_ptr(), 4, 32)]:
+                 (rope, rt.F32, [(narrow, narrow)], pos.data_ptr(), 4, 32),
+                 # off an element's boundary
+                 (rope, rt.F32, pair, pos.data_ptr() + 4, 2, 32),
+                 (rope, rt.F32, [(heads(x), rt.heads(x.data_ptr() + 2, 2, 64, 32))], pos.data_ptr(), 2, 32)]:
         with pytest.raises(rt.B2KError) as e:
             ctx.rotary(*args)
         assert e.value.status == rt.B2K_EINVAL

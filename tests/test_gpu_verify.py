@@ -114,7 +114,8 @@ def test_verify_refusals(ctx, torch_cuda):
                 accepted=i.data_ptr(), tokens=i.data_ptr(), batch=1, drafts=1, vocab=4)
     for kw in (dict(target=0), dict(drafted=0), dict(u_accept=0), dict(u_sample=0), dict(accepted=0), dict(tokens=0),
                dict(batch=-1), dict(drafts=-1), dict(vocab=0), dict(ld_target=3), dict(draft=x.data_ptr(), ld_draft=3),
-               dict(batch=2 ** 31)):
+               dict(batch=2 ** 31), dict(vocab=2 ** 31 - 1, ld_target=2 ** 31), dict(target=x.data_ptr() + 2), dict(tokens=i.data_ptr() + 1),
+               dict(counts=i.data_ptr() + 2)):
         with pytest.raises(rt.B2KError) as e:
             ctx.verify_drafts(**{**good, **kw})
         assert e.value.status == rt.B2K_EINVAL
