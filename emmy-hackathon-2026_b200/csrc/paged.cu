@@ -634,7 +634,7 @@ static int check_operands(b2k_ctx *ctx, const b2k_paged_cache *cache, const b2k_
   if (!q) return b2k::fail(ctx, B2K_EINVAL, "%s: no q", what);
   int status = check_call(ctx, cache, batch, q->heads);
   if (status == B2K_OK) status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d, cache->dtype);
-  if (status == B2K_OK) status = serve::check_heads(ctx, what, "o", o, batch->tokens, cache->d, cache->dtype);
+  if (status == B2K_OK) status = serve::check_output(ctx, what, "o", o, batch->tokens, cache->d, cache->dtype);
   if (status != B2K_OK) return status;
   if (q->heads != o->heads) return b2k::fail(ctx, B2K_EINVAL, "%s: %d heads in, %d out", what, q->heads, o->heads);
   if (q->data == o->data && batch->tokens > 0) return b2k::fail(ctx, B2K_EINVAL, "%s: o is q", what);

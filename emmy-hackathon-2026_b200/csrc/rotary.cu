@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, kWide<T, V> ? 2 : 4) rotary_kernel(c
     const int64_t n = (int64_t)a.first[b + 1] - row_begin;
     own0 = (int64_t)a.lengths[b] - n;
     row_end = row_begin + n;
-    if (row_begin < 0 || row_end > a.tokens || n > a.max_new) {
+    if (row_begin < 0 || n < 0 || row_end > a.tokens || n > a.max_new) {
       if (threadIdx.x == 0) atomicOr(a.err, serve::kErrIndex);
       return;
     }
@@ -360,6 +360,14 @@ int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_head
   return B2K_OK;
 }
 
+// check_heads, and no two tokens in one place (an input may repeat one).
+int check_output(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d,
+                 int32_t dtype) {
+  const int status = check_heads(ctx, what, name, x, tokens, d, dtype);
+  if (status != B2K_OK || tokens <= 1 || x->stride_token >= d) return status;
+  return b2k::fail(ctx, B2K_EINVAL, "%s: tokens of %s overlap, %lld elements apart", what, name, (long long)x->stride_token);
+}
+
 int check_cache(b2k_ctx *ctx, const char *what, const b2k_paged_cache *c) {
   if (!c) return b2k::fail(ctx, B2K_EINVAL, "%s: no cache", what);
   if (!type_ok(c->dtype)) return b2k::fail(ctx, B2K_EINVAL, "%s: unknown element type %d", what, c->dtype);
@@ -464,7 +472,7 @@ int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count,
   const int64_t size = (int64_t)serve::type_size(dtype);
   for (int i = 0; i < count; ++i) {
     if ((status = serve::check_heads(ctx, "rotary", "input", &x[i], tokens, d, dtype)) != B2K_OK) return status;
-    if ((status = serve::check_heads(ctx, "rotary", "output", &y[i], tokens, d, dtype)) != B2K_OK) return status;
+    if ((status = serve::check_output(ctx, "rotary", "output", &y[i], tokens, d, dtype)) != B2K_OK) return status;
     if (x[i].heads != y[i].heads)
       return b2k::fail(ctx, B2K_EINVAL, "rotary: tensor %d has %d heads in and %d out", i, x[i].heads, y[i].heads);
     if (x[i].data == y[i].data && (x[i].stride_token != y[i].stride_token || x[i].stride_head != y[i].stride_head))
@@ -504,7 +512,7 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
   int count = 0;
   if (q) {
     if ((status = serve::check_heads(ctx, what, "q", q, batch->tokens, cache->d, cache->dtype)) != B2K_OK) return status;
-    if ((status = serve::check_heads(ctx, what, "q_out", q_out, batch->tokens, cache->d, cache->dtype)) != B2K_OK) return status;
+    if ((status = serve::check_output(ctx, what, "q_out", q_out, batch->tokens, cache->d, cache->dtype)) != B2K_OK) return status;
     if (q->heads != q_out->heads ||
         (q->data == q_out->data && (q->stride_token != q_out->stride_token || q->stride_head != q_out->stride_head)))
       return b2k::fail(ctx, B2K_EINVAL, "%s: q and q_out differ in heads, or in strides in place", what);

@@ -49,6 +49,8 @@ int check_cache(b2k_ctx *ctx, const char *what, const b2k_paged_cache *cache);
 int check_batch(b2k_ctx *ctx, const char *what, const b2k_paged_cache *cache, const b2k_paged_batch *batch);
 int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d,
                 int32_t dtype);
+int check_output(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d,
+                 int32_t dtype);
 
 // Whether an array lies on its elements' boundary (a load off it faults).
 inline bool on_boundary(const void *p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }

@@ -261,6 +261,8 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   if (d->batch == 0) return B2K_OK;
   if (!d->target || !d->u_sample || !accepted || !tokens || (d->drafts > 0 && (!d->drafted || !d->u_accept)))
     return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: null buffer");
+  if (tokens == d->drafted || tokens == accepted)
+    return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: tokens is another argument's array");
   const void *arrays[] = {d->target, d->draft, d->drafted, d->counts, d->u_accept, d->u_sample, accepted, tokens};
   for (const void *p : arrays)
     if (!serve::on_boundary(p, 4)) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: a buffer is off 4 bytes");

@@ -353,7 +353,9 @@ typedef struct b2k_rope {
  * B2K_EINVAL for parameters outside the ranges above. */
 int b2k_rope_plan(const b2k_rope_params *params, b2k_rope *out);
 
-/* A tensor [tokens][heads][d] whose d elements are contiguous: strides in elements. */
+/* A tensor [tokens][heads][d] whose d elements are contiguous: strides in
+ * elements.  An input may repeat one token (stride_token < d); an output's
+ * tokens and heads may not overlap. */
 typedef struct b2k_heads {
   void *data;
   int64_t stride_token, stride_head;
@@ -388,7 +390,7 @@ int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count,
  *
  * Indexes from device memory are checked on the device: a page outside [0,
  * pages), a position outside the table, a sequence with more new tokens than
- * max_new or a length above max_len touches no memory (the token is not
+ * max_new (or fewer than none) or a length above max_len touches no memory (the token is not
  * written, the key is left out, the row not computed) and the next
  * b2k_stream_sync of the context returns B2K_EINDEX.  No counterpart in the
  * reference. */
@@ -477,9 +479,10 @@ int b2k_paged_attention_set_kernel(int mode);
  * last t with r_t > 0 should rounding leave none).  draft == NULL: the drafts
  * were certain (q_i(x_i) = 1, 0 elsewhere).  counts (may be NULL) holds each
  * sequence's own number of drafts, 0 .. drafts.  accepted [batch]; tokens
- * [batch][drafts + 1]: the taken drafts, the drawn token, then -1.  A drafted
- * token outside [0, vocab) is never taken.  Every draw follows its target
- * distribution exactly.  No counterpart in the reference. */
+ * [batch][drafts + 1]: the taken drafts, the drawn token, then -1; they overlap
+ * no other array.  A drafted token outside [0, vocab) is never taken.  Every
+ * draw follows its target distribution exactly.  No counterpart in the
+ * reference. */
 typedef struct b2k_drafts {
   const float *target, *draft;
   int64_t ld_target, ld_draft;

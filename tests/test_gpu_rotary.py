@@ -131,6 +131,8 @@ def test_rotary_refusals(ctx, torch_cuda):
                  (rope, rt.F32, [(heads(x), rt.heads(0, 2, 64, 32))], pos.data_ptr(), 4, 32),
                  (rope, rt.F32, [(heads(x), rt.heads(x.data_ptr(), 2, 128, 32))], pos.data_ptr(), 4, 32),
                  (rope, rt.F32, [(narrow, narrow)], pos.data_ptr(), 4, 32),
+                 # tokens of an output in one place
+                 (rope, rt.F32, [(heads(x), rt.heads(x.data_ptr() + 4096, 2, 0, 32))], pos.data_ptr(), 2, 32),
                  # off an element's boundary
                  (rope, rt.F32, pair, pos.data_ptr() + 4, 2, 32),
                  (rope, rt.F32, [(heads(x), rt.heads(x.data_ptr() + 2, 2, 64, 32))], pos.data_ptr(), 2, 32)]:
@@ -202,7 +204,7 @@ def test_append_without_rope_copies(ctx, torch_cuda):
     assert torch.equal(refs.read_rows(bt, bt.k, 0, 9)[7:], k[:2]) and torch.equal(refs.read_rows(bt, bt.v, 1, 3), v[2:])
 
 
-@pytest.mark.parametrize("what", ["page", "negative page", "past the table", "too many new", "before the start"])
+@pytest.mark.parametrize("what", ["page", "negative page", "past the table", "too many new", "first falls", "before the start"])
 def test_append_index_out_of_bounds(ctx, torch_cuda, what):
     """A bad index writes nothing for its token, leaves the others right and is reported at the next sync."""
     bt = refs.batch([2, 1], [20, 5], heads=1, d=16, dtype=torch.float32, poison=False)
@@ -217,6 +219,8 @@ def test_append_index_out_of_bounds(ctx, torch_cuda, what):
         bt.lens[0] = 40
     elif what == "too many new":
         batch.max_new = 1
+    elif what == "first falls":
+        bt.first[0], bt.first[1] = 3, 2  # -1 new tokens
     else:
         bt.lens[0] = 1  # two new tokens, one cached: the first has position -1
     ctx.paged_append(cache, batch, heads(k), heads(v))
@@ -224,7 +228,7 @@ def test_append_index_out_of_bounds(ctx, torch_cuda, what):
         ctx.sync()
     assert e.value.status == rt.B2K_EINDEX
     assert torch.equal(refs.read_rows(bt, bt.k, 1, 5)[4:], k[2:])
-    if what in ("page", "negative page", "past the table", "too many new"):
+    if what in ("page", "negative page", "past the table", "too many new", "first falls"):
         refs.write_rows(bt, bt.k, 1, refs.read_rows(bt, was, 1, 5))
         assert torch.equal(bt.k, was)
     ctx.sync()  # the context is usable, the report is given once

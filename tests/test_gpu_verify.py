@@ -111,10 +111,11 @@ def test_verify_refusals(ctx, torch_cuda):
     x = torch.zeros(64, device="cuda")
     i = torch.zeros(64, dtype=torch.int32, device="cuda")
     good = dict(target=x.data_ptr(), drafted=i.data_ptr(), u_accept=x.data_ptr(), u_sample=x.data_ptr(),
-                accepted=i.data_ptr(), tokens=i.data_ptr(), batch=1, drafts=1, vocab=4)
+                accepted=i.data_ptr() + 64, tokens=i.data_ptr() + 128, batch=1, drafts=1, vocab=4)
     for kw in (dict(target=0), dict(drafted=0), dict(u_accept=0), dict(u_sample=0), dict(accepted=0), dict(tokens=0),
                dict(batch=-1), dict(drafts=-1), dict(vocab=0), dict(ld_target=3), dict(draft=x.data_ptr(), ld_draft=3),
                dict(batch=2 ** 31), dict(vocab=2 ** 31 - 1, ld_target=2 ** 31), dict(target=x.data_ptr() + 2), dict(tokens=i.data_ptr() + 1),
+               dict(tokens=i.data_ptr()), dict(tokens=i.data_ptr() + 64),
                dict(counts=i.data_ptr() + 2)):
         with pytest.raises(rt.B2KError) as e:
             ctx.verify_drafts(**{**good, **kw})

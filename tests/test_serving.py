@@ -140,7 +140,7 @@ def changed(s, **kw):
     (1, dict(first=None)), (1, dict(lengths=None)), (1, dict(table=None)), (1, dict(table_stride=1)), (1, dict(max_len=10 ** 6)),
     (1, dict(prefix_len=5, prefix_table=None)), (1, dict(tokens=2 ** 31)),
     (2, dict(heads=12)), (2, dict(heads=0)), (2, dict(data=None)), (2, dict(stride_head=3)), (2, dict(stride_token=-1)),
-    (3, dict(heads=8)), (3, dict(data=4096)), (3, dict(data=None)),
+    (3, dict(heads=8)), (3, dict(data=4096)), (3, dict(data=None)), (3, dict(stride_token=0)), (3, dict(stride_token=1)),
     # off an element's boundary: loads there would fault
     (0, dict(k=4097)), (0, dict(v=4099)), (1, dict(first=258)), (1, dict(lengths=257)), (1, dict(table=258)),
     (1, dict(prefix_table=258)), (2, dict(data=4097)), (3, dict(data=8193))])
