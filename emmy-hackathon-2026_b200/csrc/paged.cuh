@@ -44,17 +44,35 @@ struct Args {
 struct Sequence {
   int first, n, own0;  // own0: own position of its first new token
 };
-__device__ __forceinline__ Sequence sequence(const Args &a, int b) {
+__device__ __forceinline__ Sequence sequence_of(const Args &a, int first, int next, int len) {
   Sequence s;
-  s.first = a.first[b];
-  s.n = a.first[b + 1] - s.first;
-  const int len = a.lengths[b];
+  s.first = first;
+  s.n = next - first;
   s.own0 = len - s.n;
   if (s.first < 0 || s.n < 0 || (int64_t)s.first + s.n > a.tokens || s.n > a.max_new || len > a.max_len || len < 0) {
     atomicOr(a.err, serve::kErrIndex);
     s.n = 0;
   }
   return s;
+}
+__device__ __forceinline__ Sequence sequence(const Args &a, int b) {
+  return sequence_of(a, a.first[b], a.first[b + 1], a.lengths[b]);
+}
+// The b-th longest of up to 32 sequences (in their own order above that; `b`
+// becomes its number).  For whole warps; one round of loads, as for one sequence.
+__device__ __forceinline__ Sequence sequence_by_length(const Args &a, int &b) {
+  if (a.sequences > 32) return sequence(a, b);
+  const int lane = threadIdx.x & 31;
+  const bool in = lane < a.sequences;
+  const int first = in ? a.first[lane] : 0, next = in ? a.first[lane + 1] : 0, len = in ? a.lengths[lane] : 0;
+  int longer = 0;
+  for (int i = 0; i < a.sequences; ++i) {
+    const int other = __shfl_sync(0xffffffffu, len, i);
+    longer += other > len || (other == len && i < lane);
+  }
+  b = __ffs(__ballot_sync(0xffffffffu, in && longer == b)) - 1;
+  return sequence_of(a, __shfl_sync(0xffffffffu, first, b), __shfl_sync(0xffffffffu, next, b),
+                     __shfl_sync(0xffffffffu, len, b));
 }
 // Packed rows in use.
 __device__ __forceinline__ int used_tokens(const Args &a) {

@@ -122,10 +122,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int head = at % a.kv_heads;
   at /= a.kv_heads;
   const int splits = prefix ? a.prefix_splits : a.own_splits;
-  const int split = at % splits, b = at / splits;
+  const int split = at % splits;
+  int b = at / splits;
   paged::Sequence s = {0, 0, 0};
   if (prefix) s.n = paged::used_tokens(a);
-  else s = paged::sequence(a, b);
+  else s = paged::sequence_by_length(a, b);  // the longest first: the last to start are short
   const int rows = s.n * a.group, row0 = block * 2 * kRows;
   const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
   const int key0 = split * chunk;
