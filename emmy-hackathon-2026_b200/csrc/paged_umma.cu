@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (TMA && threadIdx.x == 32 * kSoftmaxWarps) {
     sm100::prefetch_tensormap(&map_k);
     sm100::prefetch_tensormap(&map_v);
+    if (q_boxes) sm100::prefetch_tensormap(&map_q);
   }
   if (warp == kSoftmaxWarps + kLoadWarps) sm100::tmem_alloc(&tmem_slot, 512);
   sm100::tc_fence_before();
@@ -467,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       l += l0 + l1;
     }
     // ---------------- the row's output
+    if (tiles > 0 || !q_boxes) ok = ok && sm100::mbar_wait_warp(&q_full, 0, a.err, sm100::kSiteEpilogueAccum, abort);
     if (mine > 0) ok = ok && sm100::mbar_wait_warp(&o_full[x], 0, a.err, sm100::kSiteEpilogueAccum, abort);
     if (ok && row0 + x * kRows < rows) {
       sm100::tc_fence_after();
@@ -479,36 +481,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t part = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
       // rows of a split that see none of its keys are not read by the merge
       if (!direct && on) a.part_ml[part] = make_float2(base, l);
-#pragma unroll
-      for (int i = 0; i < DP; i += 32) {
-        if (i >= a.d) break;
-        uint32_t ov[32];
-        if (mine > 0) {
-          sm100::tmem_ld_32x32b_x32(o_at + i, ov);
-          sm100::tmem_ld_wait();
-        }
-        if (on && direct) {
-          T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + i;
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              w[u] = some && mine > 0 ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
-            if (i + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else if (on) {
-          float *out = a.part_o + part * a.d + i;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (i + e < a.d)
-              *reinterpret_cast<float4 *>(out + e) =
-                  some && mine > 0 ? make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
-                                                 __uint_as_float(ov[e + 3]))
-                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        __syncwarp();  // the next load is the whole warp's
-      }
+      // (the queries' place in shared memory is free: the products with them are
+      // complete, and all of them have arrived)
+      uint8_t *const stage = qs + x * kTile + (warp & 3) * 4096;
+      if (direct)
+        store_output<T>(stage, static_cast<T *>(a.o), on ? token * a.o_token + (int64_t)qh * a.o_head : -1, a.d, o_at, mine > 0, some, inv);
+      else
+        store_sums(stage, a.part_o, on ? part * a.d : -1, a.d, o_at, mine > 0, some);
     }
   }
   sm100::tc_fence_before();

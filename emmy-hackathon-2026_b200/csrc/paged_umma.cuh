@@ -182,4 +182,63 @@ inline bool query_boxes_fit(const Args &a) {
   return kRows % a.group == 0 && a.q_head > 0 && a.q_token > 0 && a.q_head < most && a.q_token < most;
 }
 
+// A warp's 32 rows to memory, one a lane, 128 bytes of each at a time through 4 KB
+// of shared memory, so that a store instruction writes whole lines of four rows
+// (16 bytes of 32 rows each instead take about 4000 cycles more at a block's end).  `own`: the row's
+// place in `out`, elements, -1 for none; load(c, w): its 128 bytes from element c.
+template <typename E, typename Load>
+__device__ __forceinline__ void store_rows(uint8_t *stage, E *out, int64_t own, int d, Load load) {
+  constexpr int kPiece = 16 / sizeof(E);
+  const int lane = threadIdx.x & 31, piece = lane & 7;
+  int64_t to[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) to[i] = __shfl_sync(0xffffffffu, own, 4 * i + (lane >> 3));
+  for (int c = 0; c < d; c += 8 * kPiece) {
+    uint32_t w[32];
+    __syncwarp();  // the last step's pieces have been read; the load is the whole warp's
+    load(c, w);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      *reinterpret_cast<uint4 *>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+          make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 4 * i + (lane >> 3);
+      const uint4 v = *reinterpret_cast<const uint4 *>(stage + row * 128 + ((piece ^ (row & 7)) << 4));
+      if (to[i] >= 0 && c + piece * kPiece < d) *reinterpret_cast<uint4 *>(out + to[i] + c + piece * kPiece) = v;
+    }
+  }
+}
+
+// The same from the accumulator at o_at: rounded to T and times inv, or in FP32;
+// zeros where `some` is false (a row without keys).  `filled`: the accumulator
+// holds anything (the warp's).
+template <typename T>
+__device__ __forceinline__ void store_output(uint8_t *stage, T *out, int64_t own, int d, uint32_t o_at, bool filled, bool some, float inv) {
+  store_rows(stage, out, own, d, [&](int c, uint32_t (&w)[32]) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t ov[32];
+      if (filled) {
+        sm100::tmem_ld_32x32b_x32(o_at + c + 32 * half, ov);
+        sm100::tmem_ld_wait();
+      }
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        w[16 * half + u] = filled && some ? Type<T>::pack(__uint_as_float(ov[2 * u]) * inv, __uint_as_float(ov[2 * u + 1]) * inv) : 0u;
+    }
+  });
+}
+__device__ __forceinline__ void store_sums(uint8_t *stage, float *out, int64_t own, int d, uint32_t o_at, bool filled, bool some) {
+  store_rows(stage, out, own, d, [&](int c, uint32_t (&w)[32]) {
+    if (filled) {
+      sm100::tmem_ld_32x32b_x32(o_at + c, w);
+      sm100::tmem_ld_wait();
+    }
+#pragma unroll
+    for (int u = 0; u < 32; ++u) w[u] = filled && some ? w[u] : 0u;
+  });
+}
+
 }  // namespace umma

@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- the row's output
     // the last two products, one after the other: with neither done, the
     // barrier's parity is that of the phase before both
+    if (tiles > 0 || !q_boxes) ok = ok && sm100::mbar_wait_warp(&q_full, 0, a.err, sm100::kSiteEpilogueAccum, abort);
     for (int j = max(0, tiles - 2); j < tiles; ++j)
       ok = ok && sm100::mbar_wait_warp(&pv_done, j & 1, a.err, sm100::kSiteEpilogueAccum, abort);
     if (ok) {
@@ -359,34 +360,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t part = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
       // rows of a split that see none of its keys are not read by the merge
       if (!direct && on) a.part_ml[part] = make_float2(base, l);
-      for (int i = 0; i < a.d; i += 32) {
-        uint32_t ov[32];
-        if (tiles > 0) {
-          sm100::tmem_ld_32x32b_x32(o_at + i, ov);
-          sm100::tmem_ld_wait();
-        }
-        if (on && direct) {
-          T *out = static_cast<T *>(a.o) + token * a.o_token + (int64_t)qh * a.o_head + i;
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              w[u] = some ? Type<T>::pack(__uint_as_float(ov[e + 2 * u]) * inv, __uint_as_float(ov[e + 2 * u + 1]) * inv) : 0u;
-            if (i + e < a.d) *reinterpret_cast<uint4 *>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else if (on) {
-          float *out = a.part_o + part * a.d + i;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (i + e < a.d)
-              *reinterpret_cast<float4 *>(out + e) =
-                  some ? make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
-                                     __uint_as_float(ov[e + 3]))
-                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        __syncwarp();  // the next load is the whole warp's
-      }
+      // (the queries' place in shared memory is free: the products with them are
+      // complete, and all of them have arrived)
+      uint8_t *const stage = qs + warp * 4096;
+      if (direct)
+        store_output<T>(stage, static_cast<T *>(a.o), on ? token * a.o_token + (int64_t)qh * a.o_head : -1, a.d, o_at, tiles > 0, some, inv);
+      else
+        store_sums(stage, a.part_o, on ? part * a.d : -1, a.d, o_at, tiles > 0, some);
     }
   }
   sm100::tc_fence_before();
