@@ -15,7 +15,7 @@
 // warp.  The lanes share out the token's cosines and sines through shared memory
 // while the first heads' loads are in flight; then every lane keeps one place
 // of the head (16 bytes of each half of its pairs, its cosines in registers)
-// and walks the heads, a few loads of two vectors ahead.
+// and walks the heads, whose loads are all on their way by then.
 #include <math.h>
 
 #include <algorithm>
@@ -78,29 +78,42 @@ __device__ __forceinline__ void narrow(const float (&x)[V], serve::Pack<T, V> &p
   }
 }
 
-// Heads a lane has in flight, and blocks an SM.  Sixteen cosines and sines of
-// 16-byte vectors of a 16-bit type leave registers for two blocks without
-// spills, which then load four heads ahead (16384 tokens x 40 heads of 128,
-// bf16: 58 us; two heads and three blocks 60, and four blocks 68 with spills);
-// the others run four blocks two heads ahead (6001 tokens x 32 heads of 64,
-// f32: 21 us, with three blocks 24, with two 30).
-template <typename T, int V>
-constexpr bool kWide = V * sizeof(T) == 16 && sizeof(T) == 2;
+// 16 bytes global to shared memory, for this thread alone.
+__device__ __forceinline__ void copy16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
 
-// FLAT: the heads of all segments in one walk, so that the few heads a lane has
-// of each load together (61 tokens into a cache: 5.5 -> 4.5 us); without it
-// segment after segment, whose addresses are then simple steps (16384 tokens:
-// 60 -> 58 us).
+// Many tokens of 16-byte vectors: a lane's loads wait in shared memory, kSlots
+// steps of two vectors of all the token's segments at once, and cost no
+// registers: six blocks of four warps an SM have 190 KB on the way, where four
+// heads ahead in registers were 64 (16384 tokens x 40 heads of 128, bf16: 58 ->
+// 56 us; 6001 x 32 of 64, f32: 20.6 -> 19.1; prompts into a cache: 48 -> 45.6).
+// Small blocks, a token a warp, keep the last wave short: blocks of eight warps
+// 57.5 us, with two tokens a warp 60, with four 71.
+constexpr int kSlots = 8, kStagedWarps = 4;
+template <typename T, int V, bool FLAT>
+constexpr bool kStaged = !FLAT && V * sizeof(T) == 16;
+template <typename T, int V, bool FLAT>
+constexpr int block_warps() { return kStaged<T, V, FLAT> ? kStagedWarps : kWarps; }
+template <typename T, int V, bool FLAT>
+constexpr int staged_bytes() { return kStaged<T, V, FLAT> ? kStagedWarps * kSlots * 2 * 32 * 16 : 0; }
+
+// FLAT, for few tokens with several warps to each: the heads of all segments in
+// one walk through registers, so that the few heads a lane has of each load
+// together (61 tokens into a cache: 5.5 -> 4.5 us); without it segment after
+// segment, whose addresses are simple steps (16384 tokens: 60 -> 58 us).
 template <typename T, int V, bool PAGED, bool FLAT>
-__global__ void __launch_bounds__(kThreads, kWide<T, V> ? 2 : 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(32 * block_warps<T, V, FLAT>(), kStaged<T, V, FLAT> ? 24 / kStagedWarps : V * sizeof(T) == 16 && sizeof(T) == 2 ? 2 : 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   using P = serve::Pack<T, V>;
-  constexpr int kAhead = kWide<T, V> ? 4 : 2;
-  __shared__ __align__(16) float cs[kWarps][kMaxPairs], sn[kWarps][kMaxPairs];
+  constexpr int kAhead = V * sizeof(T) == 16 && sizeof(T) == 2 ? 4 : 2;  // heads a lane has in registers
+  extern __shared__ uint4 slots[];  // staged: [warp][step][two vectors][lane]
+  constexpr int kBlockWarps = block_warps<T, V, FLAT>();
+  __shared__ __align__(16) float cs[kBlockWarps][kMaxPairs], sn[kBlockWarps][kMaxPairs];
   grid_dependency_wait();
   grid_dependents_launch();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tokens_per_block = kWarps >> a.warps_log2;
+  const int tokens_per_block = kBlockWarps >> a.warps_log2;
   const int pairs = a.rot / 2;
   // rows of this block's sequence (paged) or of the call
   int64_t row_begin = 0, row_end = a.tokens, own0 = 0;
@@ -166,7 +179,25 @@ __global__ void __launch_bounds__(kThreads, kWide<T, V> ? 2 : 4) rotary_kernel(c
           if (e1 >= 0) vb[u] = *reinterpret_cast<const P *>(x + e1 * (int)sizeof(T));
         }
       };
-      if (on) load(0, h_first);
+      uint4 *const slot_at = slots + threadIdx.x / 32 * (kSlots * 2 * 32) + lane;
+      // walks the steps from (g, hb) on, at most kSlots: f(segment, head, step)
+      auto walk = [&](int &g, int &hb, auto f) {
+        for (int n = 0; g < a.count && n < kSlots; ++n) {
+          const Segment &s = a.seg[g];
+          if (on && hb + h_first < s.heads) f(s, hb + h_first, n);
+          hb += head_step;
+          if (hb >= s.heads) ++g, hb = 0;
+        }
+      };
+      auto issue = [&](int g, int hb) {
+        walk(g, hb, [&](const Segment &s, int h, int n) {
+          const char *x = s.x + row * s.xt + h * s.xh;
+          copy16(slot_at + 64 * n, x + e0 * (int)sizeof(T));
+          if (e1 >= 0) copy16(slot_at + 64 * n + 32, x + e1 * (int)sizeof(T));
+        });
+      };
+      if constexpr (kStaged<T, V, FLAT>) issue(0, 0);
+      else if (on) load(0, h_first);
       if (!turned) {
         const int64_t own = own0 + (row - row_begin);
         const int64_t pos = PAGED ? a.prefix_len + own : pairs ? a.positions[row] : 0;
@@ -207,6 +238,62 @@ __global__ void __launch_bounds__(kThreads, kWide<T, V> ? 2 : 4) rotary_kernel(c
       auto target = [&](const Segment &s) {
         return s.y + (PAGED && s.target != kLinear ? page * s.yp + page_row * s.yt : row * s.yt);
       };
+      auto finish = [&](P &pa, P &pb, char *y, bool rotate) {
+        if (turns && rotate) {
+          float xa[V], xb[V];
+          if (a.interleaved) {
+            // neighbours a, b, a, b ...: pair i is in the first vector for i < V / 2
+            float lo[V], hi[V];
+            widen<T, V>(pa, lo);
+            widen<T, V>(pb, hi);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              xa[i] = 2 * i < V ? lo[2 * i % V] : hi[2 * i % V];
+              xb[i] = 2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V];
+            }
+          } else {
+            widen<T, V>(pa, xa);
+            widen<T, V>(pb, xb);
+          }
+          float ya[V], yb[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            ya[i] = xa[i] * c[i] - xb[i] * sv[i];
+            yb[i] = xb[i] * c[i] + xa[i] * sv[i];
+          }
+          if (a.interleaved) {
+            // pairs behind the rotated part stay as they were, bit for bit
+            float lo[V], hi[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const bool in = pair_of(i) < pairs;
+              const float oa = in ? ya[i] : xa[i], ob = in ? yb[i] : xb[i];
+              (2 * i < V ? lo[2 * i % V] : hi[2 * i % V]) = oa;
+              (2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V]) = ob;
+            }
+            narrow<T, V>(lo, pa);
+            narrow<T, V>(hi, pb);
+          } else {
+            narrow<T, V>(ya, pa);
+            narrow<T, V>(yb, pb);
+          }
+        }
+        *reinterpret_cast<P *>(y + e0 * (int)sizeof(T)) = pa;
+        if (e1 >= 0) *reinterpret_cast<P *>(y + e1 * (int)sizeof(T)) = pb;
+      };
+      if constexpr (kStaged<T, V, FLAT>) {
+        for (int g = 0, hb = 0; g < a.count;) {
+          if (g > 0 || hb > 0) issue(g, hb);
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          walk(g, hb, [&](const Segment &s, int h, int n) {
+            if (PAGED && page < 0 && s.target != kLinear) return;
+            P pa = *reinterpret_cast<const P *>(slot_at + 64 * n), pb = {};
+            if (e1 >= 0) pb = *reinterpret_cast<const P *>(slot_at + 64 * n + 32);
+            finish(pa, pb, target(s) + h * s.yh, s.rotate);
+          });
+        }
+        continue;
+      }
       char *y0 = nullptr, *y1 = nullptr, *y2 = nullptr;
       if (FLAT) y0 = target(a.seg[0]), y1 = target(a.seg[1]), y2 = target(a.seg[2]);
       for (int g = 0; g < (FLAT ? 1 : a.count); ++g) {
@@ -223,47 +310,7 @@ __global__ void __launch_bounds__(kThreads, kWide<T, V> ? 2 : 4) rotary_kernel(c
             if (FLAT && PAGED && page < 0 && pick(h, 0, a.seg[0].target, a.seg[1].target, a.seg[2].target) != kLinear) continue;
             char *y = pick(h, base, y0, y1, y2) +
                       (h - pick(h, 0, 0, h1, h2)) * pick(h, s.yh, a.seg[0].yh, a.seg[1].yh, a.seg[2].yh);
-            if (turns && pick(h, s.rotate, a.seg[0].rotate, a.seg[1].rotate, a.seg[2].rotate)) {
-              float xa[V], xb[V];
-              if (a.interleaved) {
-                // neighbours a, b, a, b ...: pair i is in the first vector for i < V / 2
-                float lo[V], hi[V];
-                widen<T, V>(va[u], lo);
-                widen<T, V>(vb[u], hi);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                  xa[i] = 2 * i < V ? lo[2 * i % V] : hi[2 * i % V];
-                  xb[i] = 2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V];
-                }
-              } else {
-                widen<T, V>(va[u], xa);
-                widen<T, V>(vb[u], xb);
-              }
-              float ya[V], yb[V];
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                ya[i] = xa[i] * c[i] - xb[i] * sv[i];
-                yb[i] = xb[i] * c[i] + xa[i] * sv[i];
-              }
-              if (a.interleaved) {
-                // pairs behind the rotated part stay as they were, bit for bit
-                float lo[V], hi[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                  const bool in = pair_of(i) < pairs;
-                  const float oa = in ? ya[i] : xa[i], ob = in ? yb[i] : xb[i];
-                  (2 * i < V ? lo[2 * i % V] : hi[2 * i % V]) = oa;
-                  (2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V]) = ob;
-                }
-                narrow<T, V>(lo, va[u]);
-                narrow<T, V>(hi, vb[u]);
-              } else {
-                narrow<T, V>(ya, va[u]);
-                narrow<T, V>(yb, vb[u]);
-              }
-            }
-            *reinterpret_cast<P *>(y + e0 * (int)sizeof(T)) = va[u];
-            if (e1 >= 0) *reinterpret_cast<P *>(y + e1 * (int)sizeof(T)) = vb[u];
+            finish(va[u], vb[u], y, pick(h, s.rotate, a.seg[0].rotate, a.seg[1].rotate, a.seg[2].rotate));
           }
         }
       }
@@ -287,18 +334,23 @@ int pick_vector(const RotaryArgs &a, int count, size_t size) {
 }
 
 template <typename T, int V, bool PAGED>
-cudaError_t launch(const RotaryArgs &a, dim3 grid, cudaStream_t s) {
+cudaError_t launch(b2k_ctx *ctx, const RotaryArgs &a, dim3 grid, cudaStream_t s) {
   // few tokens, several warps to each: few heads a lane
   auto kernel = a.warps_log2 > 1 ? rotary_kernel<T, V, PAGED, true> : rotary_kernel<T, V, PAGED, false>;
-  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), 0, s, a);
+  const int bytes = a.warps_log2 > 1 ? 0 : staged_bytes<T, V, false>();
+  if (bytes > 0) {
+    const cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, bytes);
+    if (err != cudaSuccess) return err;
+  }
+  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(32 * (bytes > 0 ? kStagedWarps : kWarps)), bytes, s, a);
 }
 
 template <typename T, bool PAGED>
-cudaError_t launch(const RotaryArgs &a, int v, dim3 grid, cudaStream_t s) {
+cudaError_t launch(b2k_ctx *ctx, const RotaryArgs &a, int v, dim3 grid, cudaStream_t s) {
   constexpr int kFull = 16 / sizeof(T);
-  if (v == kFull) return launch<T, kFull, PAGED>(a, grid, s);
-  if (v == kFull / 2) return launch<T, kFull / 2, PAGED>(a, grid, s);
-  return launch<T, 1, PAGED>(a, grid, s);
+  if (v == kFull) return launch<T, kFull, PAGED>(ctx, a, grid, s);
+  if (v == kFull / 2) return launch<T, kFull / 2, PAGED>(ctx, a, grid, s);
+  return launch<T, 1, PAGED>(ctx, a, grid, s);
 }
 
 // Fill in the vector width and the block shape, and launch.  `tokens_each`:
@@ -310,8 +362,8 @@ int run(b2k_ctx *ctx, RotaryArgs &a, int count, int32_t dtype, int64_t tokens_ea
   const size_t size = serve::type_size(dtype);
   const int v = pick_vector(a, count, size);
   a.items = a.interleaved ? (a.d + 2 * v - 1) / (2 * v) : a.rot / 2 / v + (a.d - a.rot + 2 * v - 1) / (2 * v);
-  // A warp to a token once that fills the GPU (eight blocks' worth of warps an
-  // SM); fewer tokens are shared out, down to one batch of loads a lane.
+  // A warp to a token once that fills the GPU (64 warps an SM); fewer tokens are
+  // shared out, down to one batch of loads a lane.
   const int64_t all = PAGED ? tokens_each * sequences : tokens_each;
   const int per_warp = a.items <= 32 ? 32 / a.items : 1;
   int wpt = 1;
@@ -320,14 +372,14 @@ int run(b2k_ctx *ctx, RotaryArgs &a, int count, int32_t dtype, int64_t tokens_ea
     wpt *= 2;
     ++a.warps_log2;
   }
-  const int tokens_per_block = kWarps / wpt;
+  const int tokens_per_block = (a.warps_log2 <= 1 && v * size == 16 ? kStagedWarps : kWarps) / wpt;
   const int64_t chunks = (tokens_each + tokens_per_block - 1) / tokens_per_block;
   const dim3 grid = PAGED ? dim3(sequences, (unsigned)std::min<int64_t>(chunks, 65535))
                           : dim3((unsigned)std::min<int64_t>(chunks, INT32_MAX));
   b2k::PhaseTimer timer(ctx, phase, s);
-  cudaError_t err = dtype == B2K_F32   ? launch<float, PAGED>(a, v, grid, s)
-                    : dtype == B2K_F16 ? launch<__half, PAGED>(a, v, grid, s)
-                                       : launch<__nv_bfloat16, PAGED>(a, v, grid, s);
+  cudaError_t err = dtype == B2K_F32   ? launch<float, PAGED>(ctx, a, v, grid, s)
+                    : dtype == B2K_F16 ? launch<__half, PAGED>(ctx, a, v, grid, s)
+                                       : launch<__nv_bfloat16, PAGED>(ctx, a, v, grid, s);
   if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, what);
   return b2k::check_launch(ctx, what);
 }
