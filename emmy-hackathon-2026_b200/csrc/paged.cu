@@ -7,9 +7,11 @@
 // for any layout that the tensor-core kernels do not read (element strides
 // and bases off 16 bytes, head dims off 8).  A block of four warps holds R = 4
 // RW rows (query heads of one cache head, tokens side by side) and streams 32
-// keys at a time through shared memory as FP32.  Scores: lane = key, each
-// warp its own RW rows, so a key is read once for RW rows and the softmax of a
-// tile is one butterfly; the next tile is on its way meanwhile (asynchronous
+// keys at a time through shared memory as FP32.  Scores: each warp its own RW
+// rows, lane = key, or with 32 rows lane = two rows by four keys and two dims an
+// instruction (prompts of 430 over 1430 keys, 12 / 4 heads, f32: 228 -> 211 us at
+// 64 dims, 728 -> 519 at 256; FMA pipe and shared memory both near half there,
+// with 8 to 12 warps an SM).  The next tile is on its way meanwhile (asynchronous
 // copies where the cache is f32 in 16-byte pieces).  P V: lane = four
 // dims, the probabilities read back four keys at a time as one broadcast
 // (shuffled one by one they took two thirds of the kernel's instructions).  In a
@@ -36,6 +38,26 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// Two FP32 products and sums in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+// o += p v, p twice in pp
+__device__ __forceinline__ void fma4(float4 &o, uint64_t pp, const float4 &v) {
+  unpair(fma2(pp, pair(v.x, v.y), pair(o.x, o.y)), o.x, o.y);
+  unpair(fma2(pp, pair(v.z, v.w), pair(o.z, o.w)), o.z, o.w);
+}
+
 // 16-byte copy global to shared.
 __device__ __forceinline__ void copy16(void *dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
@@ -58,11 +80,14 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int kStages = rows_stages<DV0>(), kSlots = kStages + 1;
   static_assert(kStages * kTile <= kThreads, "a thread looks up one key of the first tiles");
   __shared__ int64_t k_at[kSlots][kTile], v_at[kSlots][kTile];  // offsets of a tile's rows; -1: no such key
-  __shared__ __align__(16) float ps[kWarps][RW][kTile];  // a warp's probabilities
+  constexpr bool kSquare = RW == 8;  // scores: lane = two rows by four keys, else RW rows by one
+  constexpr int kPs = kSquare ? kTile + 4 : kTile;
+  __shared__ __align__(16) float ps[kWarps][RW][kPs];  // a warp's probabilities
+  __shared__ __align__(16) float alphas[kWarps][RW];   // (kSquare) and what its rows' sums are scaled by
   __shared__ int64_t q_at[R];
-  const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4;
+  const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4, ldq = dp + 4;
   const int stage_floats = kTile * (ldk + dp);  // keys, then values; the stages behind the queries
-  float *qs = smem, *tiles = qs + R * dp;
+  float *qs = smem, *tiles = qs + R * ldq;
   paged::part_begin(grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -163,19 +188,34 @@ __global__ void __launch_bounds__(kThreads)
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
-      if (i0 + u * kThreads < R * dp) qs[i0 + u * kThreads] = x[u] * a.scale_log2;
+      if (i0 + u * kThreads < R * dp) {
+        const int i = i0 + u * kThreads, r = (unsigned)i / (unsigned)dp;
+        qs[r * ldq + i - r * dp] = x[u] * a.scale_log2;
+      }
   }
   int limit[RW];
-  float m[RW], l[RW];
+  // the lane's rows of the scores, and their running maximum and sum of its keys
+  constexpr int kOwn = kSquare ? 2 : RW;
+  const int ty = lane >> 3, tx = lane & 7;
+  int row_limit[2];
+  float m[kOwn], l[kOwn];
   float4 o[RW][DV];
 #pragma unroll
   for (int i = 0; i < RW; ++i) {
     const int row = row0 + warp * RW + i;
     limit[i] = row >= rows ? 0 : prefix ? a.prefix_len : paged::own_limit(a, s, row / a.group);
-    m[i] = -INFINITY;
-    l[i] = 0.0f;
 #pragma unroll
     for (int c = 0; c < DV; ++c) o[i][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = row0 + warp * RW + 2 * ty + i;
+    row_limit[i] = !kSquare || row >= rows ? 0 : prefix ? a.prefix_len : paged::own_limit(a, s, row / a.group);
   }
   __syncthreads();
 #pragma unroll
@@ -198,7 +238,75 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < RW; ++i) open = open && key + kTile <= limit[i];
     open = __all_sync(0xffffffffu, open && k_at[tile % kSlots][lane] >= 0);
-    {
+    if constexpr (kSquare) {
+      // lane = rows 2 ty, 2 ty + 1 by keys tx, tx + 8, ..: six cycles of shared memory for
+      // 32 products, where a key a lane takes twelve; and a row's butterfly is
+      // over 8 lanes
+      uint64_t sum[2][4];  // of even and of odd dims
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] = 0;
+      const float *qr = qs + (warp * RW + 2 * ty) * ldq, *kr = ks + tx * ldk;
+#pragma unroll 4
+      for (int c = 0; c < dp; c += 4) {
+        float4 qv[2], kv[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qv[i] = *reinterpret_cast<const float4 *>(qr + i * ldq + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4 *>(kr + 8 * j * ldk + c);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sum[i][j] = fma2(pair(qv[i].x, qv[i].y), pair(kv[j].x, kv[j].y), sum[i][j]);
+            sum[i][j] = fma2(pair(qv[i].z, qv[i].w), pair(kv[j].z, kv[j].w), sum[i][j]);
+          }
+      }
+      bool there[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) there[j] = k_at[tile % kSlots][tx + 8 * j] >= 0;
+      bool moved = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mx = m[i], score[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float even, odd;
+          unpair(sum[i][j], even, odd);
+          score[j] = there[j] && key + tx + 8 * j < row_limit[i] ? even + odd : -INFINITY;
+          mx = fmaxf(mx, score[j]);
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        const float alpha = exp2_fast(m[i] - base);
+        l[i] *= alpha;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = exp2_fast(score[j] - base);
+          ps[warp][2 * ty + i][tx + 8 * j] = p;
+          l[i] += p;
+        }
+        m[i] = mx;
+        moved = moved || alpha != 1.0f;
+        if (tx == 0) alphas[warp][2 * ty + i] = alpha;
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+          const float alpha = alphas[warp][i];
+#pragma unroll
+          for (int c = 0; c < DV; ++c) {
+            o[i][c].x *= alpha;
+            o[i][c].y *= alpha;
+            o[i][c].z *= alpha;
+            o[i][c].w *= alpha;
+          }
+        }
+      }
+    } else {
       float4 sum[RW];  // four chains a row: one would be as long as the head
 #pragma unroll
       for (int i = 0; i < RW; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -207,7 +315,7 @@ __global__ void __launch_bounds__(kThreads)
         const float4 kv = *reinterpret_cast<const float4 *>(ks + lane * ldk + c);
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
-          const float4 qv = *reinterpret_cast<const float4 *>(qs + (warp * RW + i) * dp + c);
+          const float4 qv = *reinterpret_cast<const float4 *>(qs + (warp * RW + i) * ldq + c);
           sum[i].x = fmaf(qv.x, kv.x, sum[i].x);
           sum[i].y = fmaf(qv.y, kv.y, sum[i].y);
           sum[i].z = fmaf(qv.z, kv.z, sum[i].z);
@@ -254,10 +362,7 @@ __global__ void __launch_bounds__(kThreads)
             if (decltype(guarded)::value && p[u] == 0.0f) continue;  // a masked value may be anything
 #pragma unroll
             for (int c = 0; c < DV; ++c) {
-              o[i][c].x = fmaf(p[u], vv[u][c].x, o[i][c].x);
-              o[i][c].y = fmaf(p[u], vv[u][c].y, o[i][c].y);
-              o[i][c].z = fmaf(p[u], vv[u][c].z, o[i][c].z);
-              o[i][c].w = fmaf(p[u], vv[u][c].w, o[i][c].w);
+              fma4(o[i][c], pair(p[u], p[u]), vv[u][c]);
             }
           }
         }
@@ -270,10 +375,23 @@ __global__ void __launch_bounds__(kThreads)
     __syncthreads();  // the stage may be written again
   }
 
+  if (kSquare) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+  }
 #pragma unroll
   for (int i = 0; i < RW; ++i) {
     const int row = row0 + warp * RW + i;
-    const float total = warp_sum(l[i]);
+    float total, top;
+    if constexpr (kSquare) {
+      total = __shfl_sync(0xffffffffu, l[i & 1], i / 2 * 8);
+      top = __shfl_sync(0xffffffffu, m[i & 1], i / 2 * 8);
+    } else {
+      total = warp_sum(l[i]);
+      top = m[i];
+    }
     if (kSides == 2) {
       o[i][0].x += __shfl_xor_sync(0xffffffffu, o[i][0].x, 16);
       o[i][0].y += __shfl_xor_sync(0xffffffffu, o[i][0].y, 16);
@@ -295,7 +413,7 @@ __global__ void __launch_bounds__(kThreads)
       }
     } else {
       const int64_t at = (int64_t)(prefix ? a.own_splits + split : split) * a.tokens * q_heads + token * q_heads + qh;
-      if (lane == 0) a.part_ml[at] = make_float2(m[i], total);
+      if (lane == 0) a.part_ml[at] = make_float2(top, total);
 #pragma unroll
       for (int c = 0; c < DV; ++c) {
         const float x[4] = {o[i][c].x, o[i][c].y, o[i][c].z, o[i][c].w};
@@ -543,11 +661,11 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
 template <typename T, int RW, int DV>
 int launch_rows(b2k_ctx *ctx, const Args &a, bool vec, const paged::Grid &g, unsigned blocks, cudaStream_t s) {
   const int dp = (a.d + 3) / 4 * 4;
-  const size_t smem = sizeof(float) * (size_t)(RW * kWarps * dp + rows_stages<DV>() * kTile * (2 * dp + 4));
+  const size_t smem = sizeof(float) * (size_t)(RW * kWarps * (dp + 4) + rows_stages<DV>() * kTile * (2 * dp + 4));
   constexpr int kFull = 16 / sizeof(T);
   auto kernel = vec ? paged_rows_kernel<T, RW, DV, kFull> : paged_rows_kernel<T, RW, DV, 1>;
   constexpr int kMost = DV == 0 ? 64 : 128 * DV;  // head dim
-  constexpr int most = sizeof(float) * (RW * kWarps * kMost + rows_stages<DV>() * kTile * (2 * kMost + 4));
+  constexpr int most = sizeof(float) * (RW * kWarps * (kMost + 4) + rows_stages<DV>() * kTile * (2 * kMost + 4));
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
   if (err == cudaSuccess) err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem, s, a, g);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");

@@ -48,6 +48,24 @@ def test_rotary_matches(ctx, torch_cuda, dtype, interleaved, tokens, hq, hkv, d,
             refs.close(b, want, tol, dt, f"rotary {transpose=}")
 
 
+@pytest.mark.parametrize("dtype,tokens,hq,hkv,d,rot,interleaved", [
+    ("f32", 9601, 9, 10, 256, 256, False), ("bf16", 9500, 37, 5, 128, 64, True), ("f16", 5000, 24, 12, 64, 64, False),
+    ("f32", 20000, 1, 1, 24, 8, True)])
+def test_rotary_many_tokens(ctx, torch_cuda, dtype, tokens, hq, hkv, d, rot, interleaved):
+    """A warp or two to a token, more heads than one batch of loads, odd token counts."""
+    dt, g = refs.DTYPES[dtype], torch.Generator(device="cuda").manual_seed(tokens)
+    q, k = (torch.randn(tokens, h, d, device="cuda", generator=g).to(dt) for h in (hq, hkv))
+    pos = torch.randint(0, 100000, (tokens,), device="cuda", generator=g)
+    yq, yk = (torch.full((tokens + 1,) + x.shape[1:], 7.0, device="cuda", dtype=dt) for x in (q, k))
+    ctx.rotary(rt.rope_plan(rot, interleaved=interleaved), CODES[dtype],
+               [(heads(q), heads(yq)), (heads(k), heads(yk))], pos.data_ptr(), tokens, d)
+    ctx.sync()
+    for x, y in ((q, yq), (k, yk)):
+        want, tol = refs.rotary(x, pos, refs.frequencies(rot), interleaved)
+        refs.close(y[:-1], want, tol, dt, "many tokens")
+        assert (y[-1] == 7.0).all()
+
+
 def test_rotary_far_and_negative_positions(ctx, torch_cuda):
     """Angles stay exact where a 32-bit product of position and frequency holds no digit of them."""
     d, pos = 64, torch.tensor([0, 1, -1, -12345, 2 ** 24 + 1, 2 ** 31 + 7, 2 ** 40 + 3, -(2 ** 33)], device="cuda")
