@@ -38,6 +38,11 @@
 //
 // Bound: tensor core and exponentials alike: a pair of 128 x 128 tiles takes
 // 2 x 1024 tensor cycles at head dim 128 and 2 x 1024 of the special-function unit.
+// It takes 3430, each tile's own chain of steps: scores seen 850 cycles after
+// their products are issued, maximum 620 later, 128 exponentials a row 1800 (the
+// other tile's beside them), the last products 350 after that.  5 prompt chunks
+// of up to 1024 tokens over 1211 to 3500 keys and 1111 shared ones, 32 / 8 heads:
+// 233 us, 766 TFLOP/s.
 // All mbarrier waits are bounded (sm100.cuh).
 #include "paged_umma.cuh"
 
