@@ -269,10 +269,11 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   cudaStream_t s = (cudaStream_t)stream;
   b2k::PhaseTimer timer(ctx, B2K_PHASE_VERIFY, s);
   const VerifyArgs a{*d, accepted, tokens};
-  // A few sequences leave an SM to each CTA, which then wants many loads in
-  // flight; a batch wants all its CTAs resident at once (64 sequences of
-  // 131071: 33 us with 512 threads, 1.7 waves, against 256).
-  const bool few = d->batch * kCluster <= ctx->sm_count;
+  // A few sequences leave an SM to each CTA, which wants many loads in flight for
+  // a long row (131071: 7.2 us with 512 threads, 8.2 with 256) and fewer warps to
+  // wait for for a short one (32000: 5.7 and 5.4); a batch wants all its CTAs
+  // resident at once (64 sequences of 131071: 24 us with 512, 17 with 256).
+  const bool few = d->batch * kCluster <= ctx->sm_count && d->vocab > 65536;
   cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), few ? verify_kernel<512> : verify_kernel<256>,
                                        dim3((unsigned)(d->batch * kCluster)), dim3(few ? 512 : 256), 0, s, a);
   if (err != cudaSuccess) return b2k::cuda_fail(ctx, err, "verify_drafts launch");

@@ -56,6 +56,13 @@ def test_verify_matches(ctx, torch_cuda, certain, batch, drafts, vocab):
         same(ctx, *inputs(batch, drafts, vocab, certain, seed))
 
 
+@pytest.mark.parametrize("batch,vocab", [(1, 65536), (1, 65537), (2, 70001), (18, 131071), (19, 100003)])
+def test_verify_long_rows(ctx, torch_cuda, batch, vocab):
+    """Around the row length and the number of sequences at which the blocks grow."""
+    for certain in (False, True):
+        same(ctx, *inputs(batch, 3, vocab, certain, seed=vocab))
+
+
 def test_verify_counts_and_row_strides(ctx, torch_cuda):
     counts = torch.tensor([0, 1, 2, 3, 4, 9, -5], dtype=torch.int32, device="cuda")
     args = inputs(7, 4, 700, seed=3, pad=13)
