@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kThreads)
   const int last_token = (min(row0 + R, rows) - 1) / a.group;
   const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
   const int key0 = split * chunk;
-  const int key_end = min(prefix ? a.prefix_len : paged::own_limit(a, s, last_token), key0 + chunk);
+  const int key_end = paged::split_end(key0, chunk, prefix ? a.prefix_len : paged::own_limit(a, s, last_token));
   const bool direct = a.own_splits + a.prefix_splits == 1;
   if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(grid.beside);
   const int n_tiles = (key_end - key0 + kTile - 1) / kTile;
@@ -449,7 +449,8 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
        row += step) {
     const int j = (int)(row / q_heads), qh = (int)(row % q_heads);
     const int64_t at = (int64_t)(s.first + j) * q_heads + qh;
-    const int own = (paged::own_limit(a, s, j) + a.own_chunk - 1) / a.own_chunk;
+    // (rounded up without a sum: a split may be as long as the largest length)
+    const int limit = paged::own_limit(a, s, j), own = limit > 0 ? (limit - 1) / a.own_chunk + 1 : 0;
     const int parts = own + a.prefix_splits;
     auto slot = [&](int i) { return (int64_t)(i < own ? i : a.own_splits + i - own) * stride + at; };
     // the first parts' sums are on their way while the weights are found

@@ -88,6 +88,10 @@ __device__ __forceinline__ int own_limit(const Args &a, const Sequence &s, int j
   return !a.joined ? own : own > 0 ? a.joined_keys + own : a.prefix_len;
 }
 
+// A block's keys end: its split's, or where its last row sees no more.  (A split's
+// end is not computed by itself: near the largest lengths it passes 32 bits.)
+__device__ __forceinline__ int split_end(int key0, int chunk, int limit) { return key0 + min(chunk, limit - key0); }
+
 // The page table's entry for a key, unchecked, and the key's row in that page.
 // `at` counts from the start of the part: the prefix's keys, or the own keys
 // behind the prefix's where the part is joined (joined_keys = prefix_len).

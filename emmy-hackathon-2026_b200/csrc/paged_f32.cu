@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 2 : 3) paged_f32_kernel(
   const int last_token = (min(row0 + R, rows) - 1) / a.group;
   const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
   const int key0 = split * chunk;
-  const int key_end = min(prefix ? a.prefix_len : paged::own_limit(a, s, last_token), key0 + chunk);
+  const int key_end = paged::split_end(key0, chunk, prefix ? a.prefix_len : paged::own_limit(a, s, last_token));
   const bool direct = a.own_splits + a.prefix_splits == 1;
   if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(grid.beside);
   const int q_heads = a.kv_heads * a.group;

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : DP == 128 && MT == 2
   const int last_token = (min(row0 + kRows, rows) - 1) / a.group;
   const int chunk = prefix ? a.prefix_chunk : a.own_chunk;
   const int key0 = split * chunk;
-  const int key_end = min(prefix ? a.prefix_len : paged::own_limit(a, s, last_token), key0 + chunk);
+  const int key_end = paged::split_end(key0, chunk, prefix ? a.prefix_len : paged::own_limit(a, s, last_token));
   const bool direct = a.own_splits + a.prefix_splits == 1;
   if (key0 >= key_end && !(direct && key0 == 0)) return paged::part_end(grid.beside);
   const int q_heads = a.kv_heads * a.group;

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto keys_of = [&](int first) {
     if (first >= rows) return 0;
     const int last = (min(first + kRows, rows) - 1) / a.group;
-    return max(0, min(prefix ? a.prefix_len : paged::own_limit(a, s, last), key0 + chunk) - key0);
+    return max(0, paged::split_end(key0, chunk, prefix ? a.prefix_len : paged::own_limit(a, s, last)) - key0);
   };
   const int keys_a = keys_of(row0), keys_b = keys_of(row0 + kRows);
   const int tiles_a = (keys_a + kKeys - 1) / kKeys, tiles_b = (keys_b + kKeys - 1) / kKeys;

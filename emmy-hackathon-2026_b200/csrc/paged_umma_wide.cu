@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int key_end = key0;
   if (row0 < rows) {
     const int last = (min(row0 + kRows, rows) - 1) / a.group;
-    key_end = max(key0, min(prefix ? a.prefix_len : paged::own_limit(a, s, last), key0 + chunk));
+    key_end = max(key0, paged::split_end(key0, chunk, prefix ? a.prefix_len : paged::own_limit(a, s, last)));
   }
   const int tiles = (key_end - key0 + kKeys - 1) / kKeys;
   const bool direct = a.own_splits + a.prefix_splits == 1;
