@@ -51,7 +51,7 @@ struct RotaryArgs {
   // paged
   const int32_t *first, *lengths, *table;
   int64_t table_stride, pages;
-  int table_width, page_size, prefix_len, max_new;
+  int table_width, page_size, prefix_len, max_new, max_len;
   unsigned *err;
   uint64_t turn[kMaxPairs];
 };
@@ -121,9 +121,10 @@ __global__ void __launch_bounds__(32 * block_warps<T, V, FLAT>(), kStaged<T, V, 
     const int b = blockIdx.x;
     row_begin = a.first[b];
     const int64_t n = (int64_t)a.first[b + 1] - row_begin;
-    own0 = (int64_t)a.lengths[b] - n;
+    const int len = a.lengths[b];
+    own0 = len - n;
     row_end = row_begin + n;
-    if (row_begin < 0 || n < 0 || row_end > a.tokens || n > a.max_new) {
+    if (row_begin < 0 || n < 0 || row_end > a.tokens || n > a.max_new || len < 0 || len > a.max_len) {
       if (threadIdx.x == 0) atomicOr(a.err, serve::kErrIndex);
       return;
     }
@@ -591,6 +592,7 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
   a.page_size = cache->page_size;
   a.prefix_len = batch->prefix_len;
   a.max_new = batch->max_new;
+  a.max_len = batch->max_len;
   a.err = ctx->error_flag;
   return run<true>(ctx, a, count, cache->dtype, batch->max_new, (unsigned)batch->sequences, B2K_PHASE_APPEND,
                    (cudaStream_t)stream, "paged_append launch");

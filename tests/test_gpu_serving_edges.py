@@ -54,3 +54,48 @@ def test_max_len_near_its_limit(ctx, torch_cuda, dtype, new):
         batch = rt.paged_batch(n, n * new, first.data_ptr(), lens.data_ptr(), bt.table.data_ptr(), width, max_new=new,
                                max_len=max_len, prefix_len=64, prefix_table=bt.prefix_table.data_ptr())
         refs.close(attend(ctx, cache, batch, q), want, tol, dt, f"{max_len=}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("length", [41, 48, -1])
+def test_append_refuses_lengths_outside_max_len(ctx, torch_cuda, dtype, tokens, length):
+    """Above max_len, and within the table all the same: nothing of the sequence is written, its neighbours are."""
+    dt = refs.DTYPES[dtype]
+    bt = refs.batch([tokens, 2], [40, 9], page=16, heads=2, d=16, dtype=dt, poison=False)
+    bt.table[0] = torch.tensor([3, 4, 5])
+    bt.table[1] = torch.tensor([1, 2, 0])
+    k, v, q = (torch.randn(tokens + 2, 2, 16, device="cuda", generator=bt.generator).to(dt) for _ in range(3))
+    q_out = torch.full_like(q, 7.0)
+    cache = rt.paged_cache(bt.k.data_ptr(), bt.v.data_ptr(), CODES[dt], bt.pages, 16, 2, 16)
+    batch = rt.paged_batch(2, tokens + 2, bt.first.data_ptr(), bt.lens.data_ptr(), bt.table.data_ptr(), bt.width,
+                           max_new=tokens, max_len=40)
+    batch.max_new = max(2, tokens)
+    bt.lens[0] = length
+    was = bt.v.clone()
+    ctx.paged_append(cache, batch, heads(k), heads(v), q=heads(q), q_out=heads(q_out), rope=rt.rope_plan(16))
+    with pytest.raises(rt.B2KError) as e:
+        ctx.sync()
+    assert e.value.status == rt.B2K_EINDEX
+    assert torch.equal(refs.read_rows(bt, bt.v, 1, 9)[7:], v[tokens:]) and (q_out[:tokens] == 7.0).all()
+    refs.write_rows(bt, bt.v, 1, refs.read_rows(bt, was, 1, 9))
+    assert torch.equal(bt.v, was)
+    ctx.sync()
+
+
+def test_append_without_a_table(ctx, torch_cuda):
+    """max_len = 0 needs no table, and then no length from the device makes the kernel read one."""
+    lens, first = torch.tensor([5, 0], dtype=torch.int32, device="cuda"), torch.tensor([0, 2, 2], dtype=torch.int32, device="cuda")
+    k = torch.zeros(1, 16, 1, 16, device="cuda")
+    x = torch.ones(2, 1, 16, device="cuda")
+    cache = rt.paged_cache(k.data_ptr(), k.data_ptr(), rt.F32, 1, 16, 1, 16)
+    batch = rt.paged_batch(2, 2, first.data_ptr(), lens.data_ptr(), 0, 4, max_new=2, max_len=0)
+    ctx.paged_append(cache, batch, heads(x), heads(x))
+    with pytest.raises(rt.B2KError) as e:
+        ctx.sync()
+    assert e.value.status == rt.B2K_EINDEX and not k.any()
+    lens.zero_()
+    ctx.paged_append(cache, batch, heads(x), heads(x))  # two new tokens of none: positions -2 and -1
+    with pytest.raises(rt.B2KError):
+        ctx.sync()
+    assert not k.any()
