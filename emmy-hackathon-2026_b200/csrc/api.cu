@@ -154,8 +154,10 @@ int b2k_init(int device_ordinal, b2k_ctx **out) {
     delete ctx;
     return B2K_EUNSUPPORTED;
   }
-  err = cudaMalloc(&ctx->error_flag, sizeof(unsigned int) * 4);
-  if (err == cudaSuccess) err = cudaMemset(ctx->error_flag, 0, sizeof(unsigned int) * 4);
+  constexpr size_t words = 4 + b2k_ctx::kOrderWords;  // the error word's 16 bytes, the order words
+  err = cudaMalloc(&ctx->error_flag, sizeof(unsigned int) * words);
+  if (err == cudaSuccess) err = cudaMemset(ctx->error_flag, 0, sizeof(unsigned int) * words);
+  ctx->order_words = ctx->error_flag + 4;
   if (err != cudaSuccess) {
     delete ctx;
     return B2K_ECUDA;

@@ -30,6 +30,12 @@ struct b2k_ctx {
   bool fixed_scratch = false;
   // Device-side error word written by kernels whose bounded waits expire.
   unsigned int *error_flag = nullptr;
+  // Words by which a kernel tells the next one in its stream that what precedes
+  // both is complete (paged.cuh), one for each of the latest calls that have two
+  // such kernels, and the number of those calls.
+  static constexpr uint32_t kOrderWords = 64;
+  unsigned int *order_words = nullptr;
+  uint32_t order_calls = 0;
   // Kernels enqueued through this context (b2k_kernel_launches).
   int64_t kernel_launches = 0;
   // Pipelined host-array calls (host.cu): copy streams, dependency events
@@ -109,7 +115,8 @@ inline cudaError_t set_max_smem(b2k_ctx *ctx, const void *kernel, int bytes) {
 // prefetch) while the previous kernel in the stream drains.  Every kernel
 // launched this way executes grid_dependency_wait() before it touches global
 // memory, which orders it after the previous kernel's completion and makes
-// that kernel's writes visible.
+// that kernel's writes visible (or acquires a word that a kernel behind that wait
+// has released: paged.cuh, part_begin).
 bool pdl_enabled();
 
 template <typename... KArgs, typename... Args>

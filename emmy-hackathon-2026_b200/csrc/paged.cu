@@ -20,6 +20,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <vector>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(kThreads)
   const int dp = (a.d + 3) / 4 * 4, ldk = dp + 4, ldq = dp + 4;
   const int stage_floats = kTile * (ldk + dp);  // keys, then values; the stages behind the queries
   float *qs = smem, *tiles = qs + R * ldq;
-  paged::part_begin(grid.beside);
+  paged::part_begin(a, grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int side = kSides == 2 ? lane >> 4 : 0, col = 4 * (kSides == 2 ? lane & 15 : lane);  // of a lane's output
@@ -439,10 +440,9 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
   __shared__ float sums[SHARED ? kWarps : 1][SHARED ? B2K_MAX_HEAD_DIM : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_heads = a.kv_heads * a.group;
-  // (the sequence's numbers were there before the parts began: part_begin)
-  const paged::Sequence s = paged::sequence(a, blockIdx.x);
   grid_dependency_wait();
   grid_dependents_launch();
+  const paged::Sequence s = paged::sequence(a, blockIdx.x);
   const int64_t stride = a.tokens * q_heads;
   const int64_t step = (int64_t)gridDim.y * (SHARED ? 1 : kWarps);
   for (int64_t row = (int64_t)blockIdx.y * (SHARED ? 1 : kWarps) + (SHARED ? 0 : warp); row < (int64_t)s.n * q_heads;
@@ -536,7 +536,7 @@ cudaError_t merge(const Args &a, int sms, cudaStream_t s) {
   const bool vec_out = serve::vec_ok(a.o, a.o_token, a.o_head, 0, sizeof(T), 4 * sizeof(T));
   auto kernel = a.d % 4 == 0 ? (shared ? paged_merge_kernel<T, 4, true> : paged_merge_kernel<T, 4, false>)
                              : (shared ? paged_merge_kernel<T, 1, true> : paged_merge_kernel<T, 1, false>);
-  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, grid, dim3(kThreads), 0, s, a, vec_out);
+  return b2k::launch_kernel(a.pdl, kernel, grid, dim3(kThreads), 0, s, a, vec_out);
 }
 
 // The kernel of a part: paged_rows_kernel, warp MMAs (paged_mma.cu), the
@@ -670,7 +670,7 @@ int launch_rows(b2k_ctx *ctx, const Args &a, bool vec, const paged::Grid &g, uns
   constexpr int kMost = DV == 0 ? 64 : 128 * DV;  // head dim
   constexpr int most = sizeof(float) * (RW * kWarps * (kMost + 4) + rows_stages<DV>() * kTile * (2 * kMost + 4));
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, most);
-  if (err == cudaSuccess) err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem, s, a, g);
+  if (err == cudaSuccess) err = b2k::launch_kernel(a.pdl, kernel, dim3(blocks), dim3(kThreads), smem, s, a, g);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }
 
@@ -695,8 +695,46 @@ int rows_parts(b2k_ctx *ctx, const Args &a, bool with_prefix, bool with_own, int
                      : rows_by_dim<T, 8>(ctx, a, vec, g, blocks, s);
 }
 
+// Two launches of a call being captured, as parallel branches of its graph: what
+// the second depends on is set back to what the first did, and what follows
+// depends on both.  Not active outside a capture.
+class CapturedBranches {
+ public:
+  explicit CapturedBranches(cudaStream_t s) : s_(s) { active_ = dependencies(before_); }
+  bool active() const { return active_; }
+  cudaError_t second() { return dependencies(first_) ? set(before_, cudaStreamSetCaptureDependencies) : cudaErrorUnknown; }
+  cudaError_t join() { return set(first_, cudaStreamAddCaptureDependencies); }
+
+ private:
+  struct Set {
+    std::vector<cudaGraphNode_t> nodes;
+    std::vector<cudaGraphEdgeData> edges;
+  };
+  bool dependencies(Set &out) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    const cudaGraphNode_t *nodes = nullptr;
+    const cudaGraphEdgeData *edges = nullptr;
+    size_t n = 0;
+    if (cudaStreamGetCaptureInfo_v3(s_, &status, nullptr, nullptr, &nodes, &edges, &n) != cudaSuccess) {
+      cudaGetLastError();  // the legacy stream beside a capture in another: the launch itself says so
+      return false;
+    }
+    if (status != cudaStreamCaptureStatusActive) return false;
+    out.nodes.assign(nodes, nodes + n);
+    out.edges.assign(n, cudaGraphEdgeData{});
+    if (edges) out.edges.assign(edges, edges + n);
+    return true;
+  }
+  cudaError_t set(Set &deps, unsigned flags) {
+    return cudaStreamUpdateCaptureDependencies_v2(s_, deps.nodes.data(), deps.edges.data(), deps.nodes.size(), flags);
+  }
+  cudaStream_t s_;
+  bool active_ = false;
+  Set before_, first_;
+};
+
 template <typename T>
-int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
+int run(b2k_ctx *ctx, Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
   int launches = 1, status = B2K_OK;
   const bool prefix = a.prefix_splits > 0;
   auto parts = [&](Path path, bool pre, bool own, int rows, bool beside) {
@@ -709,9 +747,22 @@ int run(b2k_ctx *ctx, const Args &a, const Plan &p, int32_t dtype, cudaStream_t 
     status = parts(p.own_path, false, true, p.own_rows, false);
   } else if (p.own_path == p.prefix_path && p.own_path != kUmma && p.own_rows == p.prefix_rows) {
     status = parts(p.own_path, true, true, p.own_rows, false);
-  } else {
+  } else if (CapturedBranches branches(s); p.own_path != kUmma && branches.active()) {
     status = parts(p.prefix_path, true, false, p.prefix_rows, false);
-    if (status == B2K_OK) status = parts(p.own_path, false, true, p.own_rows, true);
+    cudaError_t err = status == B2K_OK ? branches.second() : cudaSuccess;
+    a.pdl = false;  // the own part's and the merge's dependences are whole
+    if (status == B2K_OK && err == cudaSuccess) status = parts(p.own_path, false, true, p.own_rows, false);
+    if (status == B2K_OK && err == cudaSuccess) err = branches.join();
+    if (err != cudaSuccess) status = b2k::cuda_fail(ctx, err, "paged_attention capture");
+    ++launches;
+  } else {
+    const bool beside = p.own_path != kUmma;  // (the tensor-memory kernel waits)
+    if (beside) {
+      a.call = ++ctx->order_calls;
+      a.ready = ctx->order_words + a.call % b2k_ctx::kOrderWords;
+    }
+    status = parts(p.prefix_path, true, false, p.prefix_rows, false);
+    if (status == B2K_OK) status = parts(p.own_path, false, true, p.own_rows, beside);
     ++launches;
   }
   if (status != B2K_OK) return status;
@@ -843,6 +894,7 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   a.max_len = batch->max_len;
   a.scale_log2 = (float)(1.4426950408889634074 / scale_div);
   a.err = ctx->error_flag;
+  a.pdl = b2k::pdl_enabled();
   a.own_splits = p.own_splits;
   a.own_chunk = p.own_chunk;
   a.prefix_splits = p.prefix_splits;

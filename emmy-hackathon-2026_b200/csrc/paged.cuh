@@ -35,6 +35,9 @@ struct Args {
   int own_splits, own_chunk, prefix_splits, prefix_chunk;
   int joined;
   int joined_keys;   // where a joined part's own keys begin in its numbering: prefix_len, or that rounded up to whole tiles
+  unsigned *ready;   // prefix and own part in two kernels side by side: the word that orders them (part_begin),
+  unsigned call;     // and this call's value of it; ready is null otherwise
+  bool pdl;          // launched with programmatic dependence on the kernel before
   float *part_o;   // [own_splits + prefix_splits][tokens * q heads][d]
   float2 *part_ml; // [own_splits + prefix_splits][tokens * q heads]: m, l
 };
@@ -114,15 +117,32 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
 }
 
 // The own part runs beside the prefix part, the kernel before it in the stream,
-// whose results it does not read.  Every block of the prefix part lets the
-// next kernel start only behind its own wait for what precedes the call, so a
-// block of the own part that has started needs no wait to read queries and
-// cache.  Its last block waits at its end instead, so that the own part's end
-// means the prefix part's too and the merge, which waits for the own part, has
-// both.  (The last block alone: waiting blocks hold their place on an SM, and
+// whose results it does not read: its blocks do not wait for that kernel, but
+// what precedes the call (queries, cache, lengths, the workspace's last readers)
+// has to be complete and visible to them.  The prefix part's first block waits
+// for that and then releases the call's number to a word of the context; a
+// thread of the own part that acquires this number is ordered behind that wait.
+// One that does not find it yet waits for the prefix part itself: nothing spins.
+// (Blocks of the prefix part let the next kernel start only behind their wait, so
+// nearly all find it.)  No number is used twice: a captured call, whose number would
+// repeat at every replay, has the two parts as parallel branches of its graph
+// instead (paged.cu).  (128 single tokens behind 8192 shared ones: 102 us a call in
+// a stream, 92 in a graph; with no ordering of the own part's reads 102 and 90,
+// with the parts one after the other 142.)
+// The own part's last block waits for the prefix part at its end, so that the own
+// part's end means the prefix part's too and the merge, which waits for the own
+// part, has both.  (The last block alone: waiting blocks hold their place on an SM, and
 // with all of them waiting the two parts all but took turns.)
-__device__ __forceinline__ void part_begin(bool beside) {
-  if (!beside) grid_dependency_wait();
+__device__ __forceinline__ void part_begin(const Args &a, bool beside) {
+  if (beside) {
+    unsigned seen;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(a.ready) : "memory");
+    if (seen != a.call) grid_dependency_wait();
+  } else {
+    grid_dependency_wait();
+    if (a.ready && blockIdx.x == 0 && threadIdx.x == 0)
+      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.ready), "r"(a.call) : "memory");
+  }
   grid_dependents_launch();
 }
 __device__ __forceinline__ void part_end(bool beside) {

@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 2 : 3) paged_f32_kernel(
   __shared__ float2 ml[kWarps][R];
   __shared__ int64_t q_at[R];
   __shared__ uint32_t there_s[kWarps][kStages];
-  paged::part_begin(grid.beside);
+  paged::part_begin(a, grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const paged::Block at = paged::this_block(a, grid);
@@ -346,7 +346,7 @@ int launch(b2k_ctx *ctx, const Args &a, const paged::Grid &g, unsigned blocks, c
   auto kernel = paged_f32_kernel<R, DP>;
   constexpr int bytes = ring_floats<R, DP>() * sizeof(float);
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, bytes);
-  if (err == cudaSuccess) err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), bytes, s, a, g);
+  if (err == cudaSuccess) err = b2k::launch_kernel(a.pdl, kernel, dim3(blocks), dim3(kThreads), bytes, s, a, g);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }
 

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : DP == 128 && MT == 2
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 ml[kWarps][kRows];
   __shared__ uint32_t there_s[kWarps][kStages];
-  paged::part_begin(grid.beside);
+  paged::part_begin(a, grid.beside);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const paged::Block at = paged::this_block(a, grid);
@@ -420,7 +420,7 @@ cudaError_t launch(b2k_ctx *ctx, const Args &a, const paged::Grid &g, unsigned b
   auto kernel = paged_mma_kernel<T, DP, MT>;
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, smem_bytes<DP, MT>());
   if (err != cudaSuccess) return err;
-  return b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP, MT>(), s, a, g);
+  return b2k::launch_kernel(a.pdl, kernel, dim3(blocks), dim3(kThreads), smem_bytes<DP, MT>(), s, a, g);
 }
 
 template <typename T>

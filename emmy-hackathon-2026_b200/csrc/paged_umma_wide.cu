@@ -73,8 +73,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  grid_dependency_wait();
-  grid_dependents_launch();
+  paged::part_begin(a, false);
 
   // --- this block's rows and keys ------------------------------------------------
   unsigned at = blockIdx.x;
@@ -388,7 +387,7 @@ int launch(b2k_ctx *ctx, const Args &a, bool prefix, int row_blocks, unsigned bl
   if (status != B2K_OK) return status;
   cudaError_t err = b2k::set_max_smem(ctx, (const void *)kernel, kSmem);
   if (err == cudaSuccess)
-    err = b2k::launch_kernel(b2k::pdl_enabled(), kernel, dim3(blocks), dim3(kThreads), kSmem, s, map_k, map_v, map_q, a, prefix,
+    err = b2k::launch_kernel(a.pdl, kernel, dim3(blocks), dim3(kThreads), kSmem, s, map_k, map_v, map_q, a, prefix,
                              row_blocks, q_boxes);
   return err == cudaSuccess ? B2K_OK : b2k::cuda_fail(ctx, err, "paged_attention launch");
 }

@@ -99,3 +99,145 @@ def test_append_without_a_table(ctx, torch_cuda):
     with pytest.raises(rt.B2KError):
         ctx.sync()
     assert not k.any()
+
+
+# --- steps without a synchronisation -----------------------------------------------------------------------
+
+
+# prefix part and own part in two kernels side by side: (dtype, prefix, kernels the plan names)
+TWO_KERNELS = [("bf16", 6000, (1, 2)), ("bf16", 4000, (1, 1)), ("f16", 300, (1, 1)), ("f32", 300, (0, 0))]
+
+
+class Steps:
+    """A decode loop of 40 sequences behind a prefix; everything that a step reads is overwritten by the next."""
+
+    def __init__(self, ctx, dtype, prefix, seed=0, steps=24):
+        self.ctx, self.dt, self.n, self.hq, self.hkv, self.d = ctx, refs.DTYPES[dtype], 40, 8, 2, 64
+        lengths = [1 + 17 * i % 500 for i in range(self.n)]
+        self.bt = refs.batch([1] * self.n, [x + steps for x in lengths], prefix=prefix, heads=self.hkv, d=self.d, dtype=self.dt,
+                             seed=seed, poison=False)
+        g = torch.Generator(device="cuda").manual_seed(seed + 100)
+        self.inputs = torch.randn(steps, self.n, self.hq + 2 * self.hkv, self.d, device="cuda", generator=g).to(self.dt)
+        self.start, self.k0, self.v0 = torch.tensor(lengths, dtype=torch.int32, device="cuda"), self.bt.k.clone(), self.bt.v.clone()
+        self.lens, self.qkv = self.start.clone(), torch.zeros_like(self.inputs[0])
+        self.turned, self.o = (torch.zeros(self.n, self.hq, self.d, device="cuda", dtype=self.dt) for _ in range(2))
+        bt = self.bt
+        self.cache = rt.paged_cache(bt.k.data_ptr(), bt.v.data_ptr(), CODES[self.dt], bt.pages, bt.page, self.hkv, self.d)
+        self.batch = rt.paged_batch(self.n, self.n, bt.first.data_ptr(), self.lens.data_ptr(), bt.table.data_ptr(), bt.width,
+                                    max_new=1, max_len=max(bt.lengths), prefix_len=prefix, prefix_table=bt.prefix_table.data_ptr())
+        self.nbytes = ctx.paged_attention_workspace(self.cache, self.batch, self.hq)
+        self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device="cuda")
+        self.rope = rt.rope_plan(self.d)
+        self.outs = torch.zeros(steps, *self.o.shape, device="cuda", dtype=self.dt)
+
+    def rewind(self):
+        self.lens.copy_(self.start)
+        self.bt.k.copy_(self.k0)
+        self.bt.v.copy_(self.v0)
+        self.outs.zero_()
+        self.ws.fill_(255)
+        torch.cuda.synchronize()
+
+    def calls(self, after=lambda: None):
+        stream = torch.cuda.current_stream().cuda_stream
+        q, k, v = self.qkv[:, :self.hq], self.qkv[:, self.hq:self.hq + self.hkv], self.qkv[:, self.hq + self.hkv:]
+        self.lens.add_(1)
+        after()
+        self.ctx.paged_append(self.cache, self.batch, heads(k), heads(v), q=heads(q), q_out=heads(self.turned), rope=self.rope,
+                              stream=stream)
+        after()
+        self.ctx.paged_attention(self.cache, self.batch, heads(self.turned), heads(self.o), self.ws.data_ptr(), self.nbytes,
+                                 stream=stream)
+        after()
+
+    def run(self, one, after=lambda: None):
+        for i, x in enumerate(self.inputs):
+            self.qkv.copy_(x)
+            one()
+            self.outs[i].copy_(self.o)
+            after()
+
+    def state(self):
+        torch.cuda.synchronize()
+        self.ctx.sync()
+        return [x.clone() for x in (self.outs, self.bt.k, self.bt.v)]
+
+
+@pytest.mark.parametrize("dtype,prefix,kernels", TWO_KERNELS)
+def test_steps_back_to_back(ctx, torch_cuda, dtype, prefix, kernels):
+    """Append, attention in two kernels, append ... on the same buffers, eager and captured: the bits of steps that are
+    waited for one by one."""
+    s = Steps(ctx, dtype, prefix)
+    plan = rt.paged_attention_plan(torch.cuda.get_device_properties(0).multi_processor_count, s.cache, s.batch, heads(s.turned),
+                                   heads(s.o))
+    assert (plan["own_kernel"], plan["prefix_kernel"], plan["joined"]) == (*kernels, 0)
+    s.run(lambda: s.calls(after=torch.cuda.synchronize), torch.cuda.synchronize)
+    want = s.state()
+    s.bt.lengths = s.lens.tolist()
+    exact, tol = refs.attention(s.bt, s.turned)
+    refs.close(want[0][-1], exact, tol, s.dt, "last step")
+    for _ in range(3):
+        s.rewind()
+        s.run(s.calls)
+        assert all(torch.equal(a, b) for a, b in zip(want, s.state()))
+    graph = torch.cuda.CUDAGraph()
+    s.rewind()
+    with torch.cuda.graph(graph):
+        s.calls()
+    for _ in range(3):
+        s.rewind()
+        s.run(graph.replay)
+        assert all(torch.equal(a, b) for a, b in zip(want, s.state()))
+
+
+@pytest.mark.parametrize("dtype,prefix,kernels", TWO_KERNELS)
+def test_steps_on_two_streams(ctx, torch_cuda, dtype, prefix, kernels):
+    """Two loops at once, of one context: eager in both, then captured in one and eager in the other."""
+    loops, want = [Steps(ctx, dtype, prefix, seed) for seed in (1, 2)], []
+    for s in loops:
+        s.run(s.calls)
+        want.append(s.state())
+        s.rewind()
+    streams = [torch.cuda.Stream() for _ in loops]
+
+    def both(*ones):
+        for s in loops:
+            s.rewind()
+        for i in range(len(loops[0].inputs)):
+            for s, stream, one in zip(loops, streams, ones):
+                with torch.cuda.stream(stream):
+                    s.qkv.copy_(s.inputs[i])
+                    one()
+                    s.outs[i].copy_(s.o)
+        for s, w in zip(loops, want):
+            assert all(torch.equal(a, b) for a, b in zip(w, s.state()))
+
+    both(loops[0].calls, loops[1].calls)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        loops[0].calls()
+    both(graph.replay, loops[1].calls)
+
+
+def test_capture_that_begins_with_attention(ctx, torch_cuda):
+    """Nothing before the two kernels in the graph, and an eager call between its captures."""
+    s = Steps(ctx, "bf16", 6000, steps=1)
+    s.lens.add_(1)
+    q = torch.randn(s.turned.shape, device="cuda").to(s.dt)
+    s.bt.lengths = s.lens.tolist()
+    want, tol = refs.attention(s.bt, q)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            ctx.paged_attention(s.cache, s.batch, heads(q), heads(s.o), s.ws.data_ptr(), s.nbytes,
+                                stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(graph)
+        refs.close(attend(ctx, s.cache, s.batch, q), want, tol, s.dt, "eager")
+    for graph in graphs:
+        s.o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        ctx.sync()
+        refs.close(s.o, want, tol, s.dt, "replayed")
