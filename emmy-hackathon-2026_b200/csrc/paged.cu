@@ -852,7 +852,8 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   const char *what = "paged_attention";
   if (!(scale_div > 0.0f) || !isfinite(scale_div)) return b2k::fail(ctx, B2K_EINVAL, "%s: scale %g", what, scale_div);
   Plan p;
-  const int status = check_operands(ctx, cache, batch, q, o, ctx->sm_count, p);
+  int status = check_operands(ctx, cache, batch, q, o, ctx->sm_count, p);
+  if (status == B2K_OK) status = serve::check_apart(ctx, what, "o", *o, *q, false, batch->tokens, cache->d, cache->dtype);
   if (status != B2K_OK) return status;
   if (batch->sequences == 0 || batch->tokens == 0 || batch->max_new == 0) return B2K_OK;
   const size_t needed = workspace_bytes_of(*cache, *batch, q->heads, ctx->sm_count);

@@ -413,12 +413,86 @@ int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_head
   return B2K_OK;
 }
 
-// check_heads, and no two tokens in one place (an input may repeat one).
+namespace {
+using Wide = __int128;  // products of strides and counts
+Wide floor_div(Wide a, Wide b) { return a / b - (a % b != 0 && (a < 0) != (b < 0)); }
+}  // namespace
+
+// Rows of d elements begin at t * st + h * sh, t < tokens, h < heads.
+bool overlaps_itself(const b2k_heads &x, int64_t tokens, int32_t d) {
+  const Wide st = x.stride_token, sh = x.stride_head;
+  if ((tokens > 1 && st < d) || (x.heads > 1 && sh < d)) return true;
+  if (tokens <= 1 || x.heads <= 1) return false;
+  if (st >= (x.heads - 1) * sh + d || sh >= (tokens - 1) * st + d) return false;  // one axis within the other's step
+  // h heads on and t tokens back, less than a row apart
+  for (Wide h = 1; h < x.heads; ++h) {
+    const Wide t = floor_div(h * sh, st);
+    if ((t >= 1 && t < tokens && h * sh - t * st < d) || (t + 1 < tokens && (t + 1) * st - h * sh < d)) return true;
+  }
+  return false;
+}
+
+// The same of rows of two tensors, y's from y - x bytes on.  Exact where the
+// tokens follow each other in both by the same step with a token's heads within
+// it, or where both strides are the same; other tensors, whose extents cross, count
+// as overlapping.
+bool overlap(const b2k_heads &x, const b2k_heads &y, int64_t tokens, int32_t d, size_t size) {
+  if (tokens == 0) return false;
+  const Wide row = (Wide)d * size, n = size;
+  const Wide from = (Wide)reinterpret_cast<uintptr_t>(y.data) - (Wide)reinterpret_cast<uintptr_t>(x.data);
+  const Wide tx = x.stride_token == 0 ? 1 : tokens, ty = y.stride_token == 0 ? 1 : tokens;  // tokens apart
+  Wide xt = x.stride_token * n, yt = y.stride_token * n, xh = x.stride_head * n, yh = y.stride_head * n;
+  if (tx == 1) xt = yt;
+  if (ty == 1) yt = xt;
+  if (x.heads == 1) xh = yh;
+  if (y.heads == 1) yh = xh;
+  const Wide x_row = (x.heads - 1) * xh + row, y_row = (y.heads - 1) * yh + row;  // bytes of a token with its heads
+  if (from >= (tx - 1) * xt + x_row || -from >= (ty - 1) * yt + y_row) return false;
+  if (tx == 1 && ty == 1) xt = yt = std::max(x_row, y_row);
+  if (xt != yt) return true;
+  if (xt >= x_row && xt >= y_row) {
+    // y's token t steps on from x's: the two walks over the heads, side by side
+    for (Wide t = std::max(1 - tx, floor_div(-from - y_row, xt)); t < ty && from + t * xt < x_row; ++t) {
+      const Wide off = from + t * xt;
+      if (-off >= y_row) continue;
+      for (int64_t i = 0, j = 0; i < x.heads && j < y.heads;) {
+        const Wide apart = off + j * yh - i * xh;
+        if (apart < row && -apart < row) return true;
+        if (apart > 0) ++i;
+        else ++j;
+      }
+    }
+    return false;
+  }
+  if (xh != yh) return true;
+  for (Wide h = 1 - x.heads; h < y.heads; ++h) {
+    // the tokens t apart whose heads h apart are nearest, below and above
+    const Wide off = from + h * xh, t = floor_div(-off, xt);
+    for (Wide u : {t, t + 1}) {
+      const Wide apart = off + std::min(std::max(u, 1 - tx), ty - 1) * xt;
+      if (apart < row && -apart < row) return true;
+    }
+  }
+  return false;
+}
+
+// check_heads, and no two rows of it in one place (an input may repeat a token).
 int check_output(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d,
                  int32_t dtype) {
   const int status = check_heads(ctx, what, name, x, tokens, d, dtype);
-  if (status != B2K_OK || tokens <= 1 || x->stride_token >= d) return status;
-  return b2k::fail(ctx, B2K_EINVAL, "%s: tokens of %s overlap, %lld elements apart", what, name, (long long)x->stride_token);
+  if (status != B2K_OK || !overlaps_itself(*x, tokens, d)) return status;
+  return b2k::fail(ctx, B2K_EINVAL, "%s: tokens or heads of %s overlap, strides %lld, %lld", what, name,
+                   (long long)x->stride_token, (long long)x->stride_head);
+}
+
+// An output in an input's (or another output's) place: refused, but for the whole
+// of `same`, the input it may replace.
+int check_apart(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads &out, const b2k_heads &other, bool same,
+                int64_t tokens, int32_t d, int32_t dtype) {
+  if (same && out.data == other.data && out.stride_token == other.stride_token && out.stride_head == other.stride_head)
+    return B2K_OK;
+  if (!overlap(other, out, tokens, d, type_size(dtype))) return B2K_OK;
+  return b2k::fail(ctx, B2K_EINVAL, "%s: %s overlaps another operand", what, name);
 }
 
 int check_cache(b2k_ctx *ctx, const char *what, const b2k_paged_cache *c) {
@@ -503,6 +577,14 @@ int b2k_rope_plan(const b2k_rope_params *p, b2k_rope *out) {
   return B2K_OK;
 }
 
+int b2k_heads_overlap(const b2k_heads *x, const b2k_heads *y, int64_t tokens, int32_t d, int32_t dtype) {
+  if (!x || tokens < 0 || d < 1 || !serve::type_ok(dtype)) return -1;
+  for (const b2k_heads *t : {x, y})
+    if (t && (t->heads < 1 || t->stride_token < 0 || t->stride_head < 0)) return -1;
+  const bool met = y ? serve::overlap(*x, *y, tokens, d, serve::type_size(dtype)) : serve::overlaps_itself(*x, tokens, d);
+  return met ? 1 : 0;
+}
+
 int64_t b2k_paged_slot(const int32_t *table_row, int32_t table_width, int64_t pages, int32_t page_size,
                        int64_t position) {
   if (!table_row || table_width < 0 || page_size < 1) return -1;
@@ -534,6 +616,12 @@ int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count,
                 x[i].stride_head * size, 0, y[i].stride_token * size, y[i].stride_head * size, x[i].heads, kLinear, 1};
     a.heads += x[i].heads;
   }
+  for (int i = 0; i < count; ++i)
+    for (int j = 0; j < count; ++j) {
+      status = serve::check_apart(ctx, "rotary", "an output", y[i], x[j], i == j, tokens, d, dtype);
+      if (status == B2K_OK && j < i) status = serve::check_apart(ctx, "rotary", "an output", y[i], y[j], false, tokens, d, dtype);
+      if (status != B2K_OK) return status;
+    }
   if (tokens == 0) return B2K_OK;
   if (!positions || !serve::on_boundary(positions, 8))
     return b2k::fail(ctx, B2K_EINVAL, "rotary: positions are null or off 8 bytes");
@@ -569,6 +657,9 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
     if (q->heads != q_out->heads ||
         (q->data == q_out->data && (q->stride_token != q_out->stride_token || q->stride_head != q_out->stride_head)))
       return b2k::fail(ctx, B2K_EINVAL, "%s: q and q_out differ in heads, or in strides in place", what);
+    for (const b2k_heads *in : {q, k, v})
+      if ((status = serve::check_apart(ctx, what, "q_out", *q_out, *in, in == q, batch->tokens, cache->d, cache->dtype)) != B2K_OK)
+        return status;
     a.seg[count++] = {static_cast<const char *>(q->data), static_cast<char *>(q_out->data), q->stride_token * size,
                       q->stride_head * size, 0, q_out->stride_token * size, q_out->stride_head * size, q->heads, kLinear, 1};
     a.heads += q->heads;

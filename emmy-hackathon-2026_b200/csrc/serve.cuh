@@ -51,6 +51,8 @@ int check_heads(b2k_ctx *ctx, const char *what, const char *name, const b2k_head
                 int32_t dtype);
 int check_output(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads *x, int64_t tokens, int32_t d,
                  int32_t dtype);
+int check_apart(b2k_ctx *ctx, const char *what, const char *name, const b2k_heads &out, const b2k_heads &other, bool same,
+                int64_t tokens, int32_t d, int32_t dtype);
 
 // Whether an array lies on its elements' boundary (a load off it faults).
 inline bool on_boundary(const void *p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }

@@ -195,6 +195,7 @@ SIGNATURES: dict[str, tuple] = {
     "b2k_rope_plan": ([C.POINTER(RopeParams), C.POINTER(Rope)], C.c_int),
     "b2k_rotary": ([_P, C.POINTER(Rope), _I32, _I32, C.POINTER(Heads), C.POINTER(Heads), _P, _I64, _I32, _I32, _P],
                    C.c_int),
+    "b2k_heads_overlap": ([C.POINTER(Heads), C.POINTER(Heads), _I64, _I32, _I32], C.c_int),
     "b2k_paged_slot": ([C.POINTER(_I32), _I32, _I64, _I32, _I64], _I64),
     "b2k_paged_append": ([_P, C.POINTER(Rope), C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(Heads),
                           C.POINTER(Heads), C.POINTER(Heads), C.POINTER(Heads), _P], C.c_int),
@@ -294,6 +295,14 @@ def rope_plan(rot: int, *, theta: float = 10000.0, interleaved: bool = False, sc
 def heads(data: int, count: int, stride_token: int, stride_head: int) -> Heads:
     """A [tokens][count][d] tensor at device address `data`, strides in elements."""
     return Heads(data or None, stride_token, stride_head, count)
+
+
+def heads_overlap(x: Heads, y: Heads | None, tokens: int, d: int, dtype: int) -> bool:
+    """Whether rows of x and y, or two rows of x (y None), share an element (b2k_heads_overlap; host arithmetic)."""
+    status = library().b2k_heads_overlap(C.byref(x), None if y is None else C.byref(y), tokens, d, dtype)
+    if status not in (0, 1):
+        raise B2KError(B2K_EINVAL, "extents or element type outside their ranges", "b2k_heads_overlap")
+    return bool(status)
 
 
 def paged_cache(k: int, v: int, dtype: int, pages: int, page_size: int, heads: int, d: int, *,

@@ -355,17 +355,26 @@ int b2k_rope_plan(const b2k_rope_params *params, b2k_rope *out);
 
 /* A tensor [tokens][heads][d] whose d elements are contiguous: strides in
  * elements.  An input may repeat one token (stride_token < d); an output's
- * tokens and heads may not overlap. */
+ * tokens and heads may not overlap, nor may an output and another operand
+ * (B2K_EINVAL; b2k_heads_overlap is the test), but for those that an entry point
+ * names. */
 typedef struct b2k_heads {
   void *data;
   int64_t stride_token, stride_head;
   int32_t heads;
 } b2k_heads;
+/* 1 where rows of x and y ([tokens][heads][d] of `dtype` both), or two rows of
+ * x (y == NULL), share an element, 0 where none do.  Exact where tokens lie the
+ * same stride apart in x and y with a token's heads within it, or where x and y
+ * have the same strides; of other tensors whose extents cross, 1.  Host
+ * arithmetic on the addresses; -1 for extents below zero or an unknown type. */
+int b2k_heads_overlap(const b2k_heads *x, const b2k_heads *y, int64_t tokens, int32_t d, int32_t dtype);
 /* y[i] = rotary(x[i]) for i < count (1 .. 3) tensors of the same tokens, one
  * launch (queries and keys, say); positions [tokens], any sign.  transpose
  * = 1 applies the transposed rotation, with the same g: given the gradient
  * of the outputs it returns the gradient of the inputs.  y[i] may be x[i]
- * (the same data and strides), but may not overlap it otherwise.  Products
+ * (the same data and strides), but may not overlap it or another tensor of the
+ * call otherwise.  Products
  * and sums are FP32, rounded once to `dtype`.  tokens may be 0. */
 int b2k_rotary(b2k_ctx *ctx, const b2k_rope *rope, int32_t dtype, int32_t count, const b2k_heads *x,
                const b2k_heads *y, const int64_t *positions, int64_t tokens, int32_t d, int32_t transpose,

@@ -241,3 +241,68 @@ def test_capture_that_begins_with_attention(ctx, torch_cuda):
         torch.cuda.synchronize()
         ctx.sync()
         refs.close(s.o, want, tol, s.dt, "replayed")
+
+
+# --- operands that meet ------------------------------------------------------------------------------------
+
+
+def test_outputs_that_meet_are_refused(ctx, torch_cuda):
+    """Two rows of an output, an output and another operand: refused before anything is launched; places side by side
+    are not."""
+    n, h, d = 6, 4, 32
+    buf = torch.randn(4 * n, 2 * h, d, device="cuda").bfloat16()
+    at = lambda row, head=0, heads_=h, st=2 * h * d, sh=d: rt.heads(buf[row, head].data_ptr(), heads_, st, sh)  # noqa: E731
+    pos, rope = torch.arange(n, device="cuda"), rt.rope_plan(d)
+    keep = buf.clone()
+
+    def refused(call, *args, **kw):
+        with pytest.raises(rt.B2KError) as e:
+            call(*args, **kw)
+        assert e.value.status == rt.B2K_EINVAL
+
+    rotate = lambda pairs: ctx.rotary(rope, rt.BF16, pairs, pos.data_ptr(), n, d)  # noqa: E731
+    for pairs in ([(at(0), at(n, st=d))], [(at(0), at(n, st=d, sh=2 * d))],     # the output's tokens in its heads' places
+                  [(at(0), at(1))], [(at(0), at(0, 1))],                          # a row, a head further
+                  [(at(0), at(n)), (at(n), at(2 * n))],                           # an output over the other tensor's input
+                  [(at(0), at(2 * n)), (at(n), at(2 * n, 3))]):                   # two outputs in one place
+        refused(rotate, pairs)
+    bt = refs.batch([1] * n, [20] * n, heads=h, d=d, poison=False)
+    cache = rt.paged_cache(bt.k.data_ptr(), bt.v.data_ptr(), rt.BF16, bt.pages, bt.page, h, d)
+    batch = rt.paged_batch(n, n, bt.first.data_ptr(), bt.lens.data_ptr(), bt.table.data_ptr(), bt.width, max_new=1, max_len=20)
+    append = lambda q_out, **kw: ctx.paged_append(cache, batch, at(0), at(0, h), q=at(n), q_out=q_out, rope=rope)  # noqa: E731
+    for q_out in (at(0), at(0, 1), at(n, 1), at(n + 1), at(2 * n, st=d)):
+        refused(append, q_out)
+    nbytes = ctx.paged_attention_workspace(cache, batch, h)
+    ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device="cuda")
+    for o in (at(0), at(0, 1), at(1), at(n, st=d)):
+        refused(ctx.paged_attention, cache, batch, at(0), o, ws.data_ptr(), nbytes)
+    ctx.sync()
+    assert torch.equal(buf, keep)
+    # side by side in one buffer
+    rotate([(at(0), at(0, h)), (at(n), at(n, h)), (at(2 * n), at(2 * n))])
+    append(at(n, h))
+    ctx.paged_attention(cache, batch, at(0), at(0, h), ws.data_ptr(), nbytes)
+    rotate([(at(0, heads_=1, sh=0), rt.heads(buf[3 * n].data_ptr(), 1, d, 0))])
+    ctx.sync()
+
+
+@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("d,new", [(64, [1, 3]), (128, [40, 90]), (256, [70, 1])])
+def test_attention_of_head_major_queries(ctx, torch_cuda, kernel, d, new):
+    """q and o as [heads][tokens][d]."""
+    bt = refs.batch(new, [130, 200], prefix=70, heads=2, d=d, dtype=torch.bfloat16)
+    q = torch.randn(8, bt.tokens, d, device="cuda").bfloat16().transpose(0, 1)
+    o = torch.zeros(8, bt.tokens, d, device="cuda").bfloat16().transpose(0, 1)
+    ctx.set_paged_attention_kernel(kernel)
+    try:
+        cache = rt.paged_cache(bt.k.data_ptr(), bt.v.data_ptr(), rt.BF16, bt.pages, bt.page, 2, d)
+        batch = rt.paged_batch(2, bt.tokens, bt.first.data_ptr(), bt.lens.data_ptr(), bt.table.data_ptr(), bt.width,
+                               max_new=max(new), max_len=200, prefix_len=70, prefix_table=bt.prefix_table.data_ptr())
+        nbytes = ctx.paged_attention_workspace(cache, batch, 8)
+        ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device="cuda")
+        ctx.paged_attention(cache, batch, heads(q), heads(o), ws.data_ptr(), nbytes)
+        ctx.sync()
+    finally:
+        ctx.set_paged_attention_kernel(0)
+    want, tol = refs.attention(bt, q)
+    refs.close(o, want, tol, torch.bfloat16, "head-major")

@@ -1,0 +1,92 @@
+"""Host side of the serving operators' edges: which operands meet (no GPU)."""
+from __future__ import annotations
+
+import ctypes as C
+import importlib
+import random
+
+import pytest
+
+from conftest import PKG
+
+rt = importlib.import_module(f"{PKG}.runtime")
+
+
+def rows(x, tokens, d, size):
+    return [x.data + (t * x.stride_token + h * x.stride_head) * size for t in range(tokens) for h in range(x.heads)]
+
+
+def met(x, y, tokens, d, size):
+    """By looking at every pair of rows; None where a tensor meets itself only in name (one row)."""
+    a = rows(x, tokens, d, size)
+    if y is None:
+        a = sorted(a)
+        return any(q - p < d * size for p, q in zip(a, a[1:]))
+    return any(abs(p - q) < d * size for p in a for q in rows(y, tokens, d, size))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_heads_that_meet_themselves(seed):
+    rng, seen = random.Random(seed), set()
+    for _ in range(1500):
+        d, tokens = rng.randint(1, 5), rng.randint(1, 6)
+        x = rt.heads(4096, rng.randint(1, 6), rng.randint(0, 40), rng.randint(0, 40))
+        want = met(x, None, tokens, d, 2)
+        assert rt.heads_overlap(x, None, tokens, d, rt.BF16) == want, (x.heads, x.stride_token, x.stride_head, tokens, d)
+        seen.add(want)
+    assert seen == {False, True}
+    # interleaved on purpose, and neither axis within the other's step
+    assert not rt.heads_overlap(rt.heads(4096, 3, 5, 7), None, 3, 2, rt.F32) and rt.heads_overlap(rt.heads(4096, 3, 5, 7), None, 3, 3, rt.F32)
+    assert rt.heads_overlap(rt.heads(4096, 32, 128, 128), None, 4, 128, rt.BF16)      # token 1 in head 1's place
+    assert rt.heads_overlap(rt.heads(4096, 8, 128, 256), None, 3, 128, rt.BF16)
+    assert not rt.heads_overlap(rt.heads(4096, 8, 128, 3 * 128), None, 3, 128, rt.BF16)  # head-major
+    assert not rt.heads_overlap(rt.heads(4096, 2 ** 15, 2 ** 61, 2 ** 45), None, 2 ** 31, 128, rt.F32)
+
+
+@pytest.mark.parametrize("kind", ["same steps", "same token step", "any"])
+@pytest.mark.parametrize("seed", range(4))
+def test_heads_that_meet_each_other(kind, seed):
+    """Exact for tensors with the same strides or the same token step; never a missed meeting for the others."""
+    rng, seen = random.Random(seed), set()
+    for _ in range(1500):
+        d, tokens, size = rng.randint(1, 4), rng.randint(1, 5), rng.choice([2, 4])
+        dtype = rt.F32 if size == 4 else rt.F16
+        x = rt.heads(2 ** 20, rng.randint(1, 5), rng.randint(0, 40), rng.randint(d, 30))
+        y = rt.heads(2 ** 20 + size * rng.randint(-90, 90), rng.randint(1, 5), rng.randint(0, 40), rng.randint(d, 30))
+        if kind == "same steps":
+            y.stride_token, y.stride_head = x.stride_token, x.stride_head
+        elif kind == "same token step":
+            wide = max((t.heads - 1) * t.stride_head + d for t in (x, y))
+            x.stride_token = y.stride_token = wide + rng.randint(0, 20)
+        want, got = met(x, y, tokens, d, size), rt.heads_overlap(x, y, tokens, d, dtype)
+        if kind == "any":
+            assert got or not want
+        else:
+            assert got == want, [(t.data, t.heads, t.stride_token, t.stride_head) for t in (x, y)] + [tokens, d, size]
+        seen.add(want)
+    assert seen == {False, True}
+
+
+def test_heads_of_a_fused_projection_lie_apart():
+    n, hq, hkv, d = 16384, 32, 8, 128
+    wide = (hq + 2 * hkv) * d
+    q, k = rt.heads(4096, hq, wide, d), rt.heads(4096 + 2 * hq * d, hkv, wide, d)
+    assert not rt.heads_overlap(q, k, n, d, rt.BF16) and not rt.heads_overlap(k, q, n, d, rt.BF16)
+    k.data -= 2  # one element into the last query head
+    assert rt.heads_overlap(q, k, n, d, rt.BF16) and rt.heads_overlap(k, q, n, d, rt.BF16)
+    o = rt.heads(4096 + 256, hq, wide, d)
+    assert rt.heads_overlap(q, o, n, d, rt.BF16) and not rt.heads_overlap(q, o, 0, d, rt.BF16)
+    for bad in [(rt.heads(4096, 0, 8, 8), 1, 8, rt.F32), (q, -1, 8, rt.F32), (q, 1, 0, rt.F32), (q, 1, 8, 3), (rt.heads(1, 1, -1, 8), 1, 8, 0)]:
+        with pytest.raises(rt.B2KError) as e:
+            rt.heads_overlap(bad[0], None, *bad[1:])
+        assert e.value.status == rt.B2K_EINVAL
+
+
+def test_paged_plan_refuses_outputs_that_meet_themselves():
+    cache = rt.paged_cache(4096, 8192, rt.BF16, 100, 16, 8, 128)
+    batch = rt.paged_batch(4, 4, 256, 256, 256, 8, max_new=1, max_len=100)
+    q = rt.heads(2 ** 20, 32, 32 * 128, 128)
+    for strides, fine in (((32 * 128, 128), True), ((128, 4 * 128), True), ((128, 128), False), ((128, 2 * 128), False), ((16 * 128, 128), False)):
+        o, out = rt.heads(2 ** 21, 32, *strides), rt.PagedAttentionPlan()
+        status = rt.library().b2k_paged_attention_plan(148, C.byref(cache), C.byref(batch), C.byref(q), C.byref(o), C.byref(out))
+        assert status == (rt.B2K_OK if fine else rt.B2K_EINVAL)
