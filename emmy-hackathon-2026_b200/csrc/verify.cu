@@ -261,11 +261,25 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   if (d->batch == 0) return B2K_OK;
   if (!d->target || !d->u_sample || !accepted || !tokens || (d->drafts > 0 && (!d->drafted || !d->u_accept)))
     return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: null buffer");
-  if (tokens == d->drafted || tokens == accepted)
-    return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: tokens is another argument's array");
-  const void *arrays[] = {d->target, d->draft, d->drafted, d->counts, d->u_accept, d->u_sample, accepted, tokens};
-  for (const void *p : arrays)
-    if (!serve::on_boundary(p, 4)) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: a buffer is off 4 bytes");
+  // every array's extent (elements of 4 bytes, rows of probabilities with what lies
+  // between them), the outputs first
+  const double rows = (double)d->batch * (d->drafts + 1.0), drafted = (double)d->batch * d->drafts;
+  const struct {
+    const void *p;
+    double n;
+  } arrays[] = {{accepted, (double)d->batch}, {tokens, rows}, {d->target, (rows - 1) * d->ld_target + d->vocab},
+                {d->draft, drafted > 0 ? (drafted - 1) * d->ld_draft + d->vocab : 0.0}, {d->drafted, drafted},
+                {d->counts, (double)d->batch}, {d->u_accept, drafted}, {d->u_sample, (double)d->batch}};
+  for (const auto &x : arrays)
+    if (!serve::on_boundary(x.p, 4)) return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: a buffer is off 4 bytes");
+  for (int i = 0; i < 2; ++i)
+    for (const auto &x : arrays) {
+      const auto &out = arrays[i];
+      if (&x == &out || !x.p) continue;
+      const double apart = (double)(reinterpret_cast<uintptr_t>(x.p) / 4) - (double)(reinterpret_cast<uintptr_t>(out.p) / 4);
+      if (apart < out.n && -apart < x.n)
+        return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: %s overlaps another array", i ? "tokens" : "accepted");
+    }
   cudaStream_t s = (cudaStream_t)stream;
   b2k::PhaseTimer timer(ctx, B2K_PHASE_VERIFY, s);
   const VerifyArgs a{*d, accepted, tokens};

@@ -488,8 +488,8 @@ int b2k_paged_attention_set_kernel(int mode);
  * last t with r_t > 0 should rounding leave none).  draft == NULL: the drafts
  * were certain (q_i(x_i) = 1, 0 elsewhere).  counts (may be NULL) holds each
  * sequence's own number of drafts, 0 .. drafts.  accepted [batch]; tokens
- * [batch][drafts + 1]: the taken drafts, the drawn token, then -1; they overlap
- * no other array.  A drafted token outside [0, vocab) is never taken.  Every
+ * [batch][drafts + 1]: the taken drafts, the drawn token, then -1; neither may
+ * overlap another array (from its first element to its last: B2K_EINVAL).  A drafted token outside [0, vocab) is never taken.  Every
  * draw follows its target distribution exactly.  No counterpart in the
  * reference. */
 typedef struct b2k_drafts {

@@ -306,3 +306,26 @@ def test_attention_of_head_major_queries(ctx, torch_cuda, kernel, d, new):
         ctx.set_paged_attention_kernel(0)
     want, tol = refs.attention(bt, q)
     refs.close(o, want, tol, torch.bfloat16, "head-major")
+
+
+def test_verification_refuses_outputs_in_other_arrays(ctx, torch_cuda):
+    batch, drafts, vocab = 3, 2, 8
+    ints, floats = torch.zeros(256, dtype=torch.int32, device="cuda"), torch.full((256,), 0.125, device="cuda")
+    i, f = (lambda n: ints.data_ptr() + 4 * n), (lambda n: floats.data_ptr() + 4 * n)  # noqa: E731
+    # drafted 0..5, counts 6..8, accepted 16..18, tokens 32..40; target 0..71, u_accept 72..77, u_sample 78..80, draft 96..143
+    good = dict(target=f(0), drafted=i(0), u_accept=f(72), u_sample=f(78), accepted=i(16), tokens=i(32), batch=batch,
+                drafts=drafts, vocab=vocab, counts=i(6), draft=f(96))
+    bad = [dict(tokens=i(5)), dict(tokens=i(8)), dict(tokens=i(8), accepted=i(40)), dict(tokens=i(18)), dict(accepted=i(5)),
+           dict(accepted=i(31)), dict(accepted=i(40)), dict(accepted=i(8)), dict(tokens=f(71)), dict(tokens=f(77)), dict(accepted=f(80)),
+           dict(tokens=f(143)), dict(accepted=f(95)), dict(drafted=i(27)), dict(target=i(0), tokens=i(32)),
+           dict(ld_draft=16, accepted=f(96 + 5 * 16 + 7))]
+    for kw in bad:
+        with pytest.raises(rt.B2KError) as e:
+            ctx.verify_drafts(**{**good, **kw})
+        assert e.value.status == rt.B2K_EINVAL, kw
+    ctx.sync()
+    assert not ints.any()
+    for kw in (dict(), dict(tokens=i(9), accepted=i(60)), dict(tokens=i(19)), dict(accepted=i(9)), dict(accepted=i(13)), dict(accepted=i(41)),
+               dict(accepted=f(144)), dict(tokens=f(81))):
+        ctx.verify_drafts(**{**good, **kw})
+    ctx.sync()
