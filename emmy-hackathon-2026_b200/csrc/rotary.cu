@@ -263,17 +263,23 @@ __global__ void __launch_bounds__(32 * block_warps<T, V, FLAT>(), kStaged<T, V, 
             yb[i] = xb[i] * c[i] + xa[i] * sv[i];
           }
           if (a.interleaved) {
-            // pairs behind the rotated part stay as they were, bit for bit
             float lo[V], hi[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const bool in = pair_of(i) < pairs;
-              const float oa = in ? ya[i] : xa[i], ob = in ? yb[i] : xb[i];
-              (2 * i < V ? lo[2 * i % V] : hi[2 * i % V]) = oa;
-              (2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V]) = ob;
+              (2 * i < V ? lo[2 * i % V] : hi[2 * i % V]) = ya[i];
+              (2 * i + 1 < V ? lo[(2 * i + 1) % V] : hi[(2 * i + 1) % V]) = yb[i];
             }
-            narrow<T, V>(lo, pa);
-            narrow<T, V>(hi, pb);
+            P ta, tb;
+            narrow<T, V>(lo, ta);
+            narrow<T, V>(hi, tb);
+            // pairs behind the rotated part stay as they were, bit for bit: a NaN
+            // would lose its sign and payload on the way through FP32
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (pair_of(i) < pairs) {
+                (2 * i < V ? pa : pb).v[2 * i % V] = (2 * i < V ? ta : tb).v[2 * i % V];
+                (2 * i + 1 < V ? pa : pb).v[(2 * i + 1) % V] = (2 * i + 1 < V ? ta : tb).v[(2 * i + 1) % V];
+              }
           } else {
             narrow<T, V>(ya, pa);
             narrow<T, V>(yb, pb);

@@ -329,3 +329,26 @@ def test_verification_refuses_outputs_in_other_arrays(ctx, torch_cuda):
                dict(accepted=f(144)), dict(tokens=f(81))):
         ctx.verify_drafts(**{**good, **kw})
     ctx.sync()
+
+
+# --- what is copied ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens", [1, 3000])
+@pytest.mark.parametrize("d,rot", [(40, 34), (48, 16), (37, 6)])
+def test_elements_outside_pairs_keep_their_bits(ctx, torch_cuda, dtype, interleaved, tokens, d, rot):
+    """NaNs with signs and payloads behind the rotated part, in vectors that are rotated in part."""
+    dt = refs.DTYPES[dtype]
+    bits = torch.int32 if dt == torch.float32 else torch.int16
+    odd = {"f32": 0x7f800001, "f16": 0x7c01, "bf16": 0x7f81}[dtype]
+    x = torch.randn(tokens, 3, d, device="cuda").to(dt)
+    tail = torch.tensor([-1, -2, odd, -5] * d, device="cuda")[:d - rot]
+    x.view(bits)[:, :, rot:] = tail.to(bits)
+    y, pos = torch.zeros_like(x), torch.arange(tokens, device="cuda")
+    ctx.rotary(rt.rope_plan(rot, interleaved=interleaved), CODES[dt], [(heads(x), heads(y))], pos.data_ptr(), tokens, d)
+    ctx.sync()
+    assert torch.equal(x.view(bits)[:, :, rot:], y.view(bits)[:, :, rot:])
+    want, tol = refs.rotary(x[..., :rot], pos, refs.frequencies(rot), interleaved)
+    refs.close(y[..., :rot], want, tol, dt, "rotated part")
