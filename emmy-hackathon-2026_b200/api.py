@@ -45,28 +45,32 @@ def _heads(x: DeviceArray) -> runtime.Heads:
 
 
 class PagedKV:
-    """Keys and values in pages [pages, page_size, heads, d], and the workspace of the attention over them."""
+    """Keys and values in pages [pages, page_size, heads, d], and the workspace of the attention over them.
+
+    All calls on one PagedKV share its workspace, so they go one after the other: the session's stream sees to
+    that, and captured ones are replayed on one stream at a time.  Calls that overlap need
+    ``runtime.Context.paged_attention`` with a workspace each."""
 
     def __init__(self, session: "Session", pages: int, page_size: int, heads: int, d: int, dtype=F32):
         self.session, self.dtype = session, np.dtype(dtype)
         shape = (pages, page_size, heads, d)
         self.k, self.v = session.empty(shape, dtype), session.empty(shape, dtype)
         self.cache = runtime.paged_cache(self.k.ptr, self.v.ptr, ELEMENTS[self.dtype], pages, page_size, heads, d)
-        self._workspace: DeviceArray | None = None
+        self._workspaces: list[DeviceArray] = []
 
     def workspace(self, nbytes: int) -> DeviceArray:
-        """At least `nbytes` of device memory, kept from call to call (a session's calls share one stream)."""
-        if self._workspace is None or self._workspace.nbytes < nbytes:
-            if self._workspace is not None:
-                self.session.sync()
-                self._workspace.free()
-            self._workspace = self.session.empty((max(16, nbytes),), np.uint8)
-        return self._workspace
+        """At least `nbytes` of device memory, kept from call to call.  A larger one does not replace those before
+        it until :meth:`free`: calls captured into a graph go on using theirs.  (Each is twice the last at least, so
+        all of them are no more than twice the largest.)"""
+        if not self._workspaces or self._workspaces[-1].nbytes < nbytes:
+            last = self._workspaces[-1].nbytes if self._workspaces else 8
+            self._workspaces.append(self.session.empty((max(2 * last, nbytes),), np.uint8))
+        return self._workspaces[-1]
 
     def free(self) -> None:
-        for array in (self.k, self.v, self._workspace):
-            if array is not None:
-                array.free()
+        """Free keys, values and workspaces; graphs with calls on them must not be replayed any more."""
+        for array in (self.k, self.v, *self._workspaces):
+            array.free()
 
 
 class Session:

@@ -90,3 +90,47 @@ def test_paged_plan_refuses_outputs_that_meet_themselves():
         o, out = rt.heads(2 ** 21, 32, *strides), rt.PagedAttentionPlan()
         status = rt.library().b2k_paged_attention_plan(148, C.byref(cache), C.byref(batch), C.byref(q), C.byref(o), C.byref(out))
         assert status == (rt.B2K_OK if fine else rt.B2K_EINVAL)
+
+
+# --- api.Session's side, with a session that has no device --------------------------------------------------
+
+
+class FakeSession:
+    """Hands out addresses and keeps count of them."""
+
+    def __init__(self):
+        self.live, self.next, self.calls, self.stream = set(), 4096, [], 0
+        self.ctx = self
+
+    def empty(self, shape, dtype="f4"):
+        return importlib.import_module(f"{PKG}.api").DeviceArray(self, tuple(shape), dtype)
+
+    def malloc(self, nbytes):
+        at, self.next = self.next, self.next + (nbytes + 4095) // 4096 * 4096
+        self.live.add(at)
+        return at
+
+    def free(self, ptr):
+        self.live.remove(ptr)
+
+    def sync(self, stream=0):
+        pass
+
+    def __getattr__(self, name):  # the context's calls
+        return lambda *args, **kw: self.calls.append(name) or 64
+
+
+def test_workspace_outlives_larger_calls():
+    """A captured call goes on using the workspace of its time: a larger one takes a new one beside it."""
+    api = importlib.import_module(f"{PKG}.api")
+    s = FakeSession()
+    kv = api.PagedKV(s, 4, 16, 2, 64)
+    small, large = kv.workspace(100), kv.workspace(5000)
+    assert {small.ptr, large.ptr} <= s.live and small.ptr != large.ptr
+    assert kv.workspace(200).nbytes >= 200 and kv.workspace(5000).ptr == large.ptr
+    sizes = [kv.workspace(n).nbytes for n in range(5000, 300000, 1000)]
+    held = s.next - 4096
+    assert sizes == sorted(sizes) and held <= 4 * max(sizes)  # a growing call does not pile up one for each size
+    kv.free()
+    assert not s.live
+    kv.free()
