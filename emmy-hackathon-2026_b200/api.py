@@ -38,6 +38,13 @@ class DeviceArray:
             self.ptr = 0
 
 
+def _element(dtype) -> int:
+    code = ELEMENTS.get(np.dtype(dtype))
+    if code is None:
+        raise ValueError(f"expected float32, float16 or uint16 (bf16 bits), got {np.dtype(dtype)}")
+    return code
+
+
 def _heads(x: DeviceArray) -> runtime.Heads:
     if len(x.shape) != 3:
         raise ValueError(f"expected [tokens, heads, d], got shape {x.shape}")
@@ -53,9 +60,9 @@ class PagedKV:
 
     def __init__(self, session: "Session", pages: int, page_size: int, heads: int, d: int, dtype=F32):
         self.session, self.dtype = session, np.dtype(dtype)
-        shape = (pages, page_size, heads, d)
+        shape, code = (pages, page_size, heads, d), _element(dtype)
         self.k, self.v = session.empty(shape, dtype), session.empty(shape, dtype)
-        self.cache = runtime.paged_cache(self.k.ptr, self.v.ptr, ELEMENTS[self.dtype], pages, page_size, heads, d)
+        self.cache = runtime.paged_cache(self.k.ptr, self.v.ptr, code, pages, page_size, heads, d)
         self._workspaces: list[DeviceArray] = []
 
     def workspace(self, nbytes: int) -> DeviceArray:
@@ -149,13 +156,15 @@ class Session:
     def rotary(self, rope: runtime.Rope, pairs: list[tuple[DeviceArray, DeviceArray]], positions: DeviceArray, *,
                transpose: bool = False) -> None:
         """y = rotary(x) for each (x, y); ``transpose`` gives the inputs' gradients from the outputs'."""
+        if not pairs:
+            raise ValueError("rotary: no tensors")
         tokens, _, d = pairs[0][0].shape
         if positions.shape != (tokens,) or positions.dtype != np.int64:
             raise ValueError("rotary: positions must be int64, one for each token")
         for x, y in pairs:
             if x.shape != y.shape or x.shape[0] != tokens or x.shape[2] != d or {x.dtype, y.dtype} != {pairs[0][0].dtype}:
                 raise ValueError(f"rotary: {x.shape} {x.dtype} to {y.shape} {y.dtype}")
-        self.ctx.rotary(rope, ELEMENTS[pairs[0][0].dtype], [(_heads(x), _heads(y)) for x, y in pairs], positions.ptr, tokens,
+        self.ctx.rotary(rope, _element(pairs[0][0].dtype), [(_heads(x), _heads(y)) for x, y in pairs], positions.ptr, tokens,
                         d, transpose=transpose, stream=self.stream)
 
     def paged_kv(self, pages: int, page_size: int, heads: int, d: int, dtype=F32) -> PagedKV:
@@ -169,14 +178,16 @@ class Session:
         arrays = [first, lengths, table] + ([prefix_table] if prefix_table is not None else [])
         if first.shape != (n + 1,) or lengths.shape != (n,) or any(x.dtype != np.int32 for x in arrays):
             raise ValueError("paged_batch: first [n + 1], lengths [n] and table [n, pages] must be int32")
-        return runtime.paged_batch(n, tokens, first.ptr, lengths.ptr, table.ptr, width, max_new=max_new, max_len=max_len,
-                                   prefix_len=prefix_len, prefix_table=prefix_table.ptr if prefix_table is not None else 0)
+        batch = runtime.paged_batch(n, tokens, first.ptr, lengths.ptr, table.ptr, width, max_new=max_new, max_len=max_len,
+                                    prefix_len=prefix_len, prefix_table=prefix_table.ptr if prefix_table is not None else 0)
+        batch.prefix_pages = prefix_table.size if prefix_table is not None else 0
+        return batch
 
     def paged_append(self, kv: PagedKV, batch: runtime.PagedBatch, k: DeviceArray, v: DeviceArray, *,
                      q: DeviceArray | None = None, q_out: DeviceArray | None = None,
                      rope: runtime.Rope | None = None) -> None:
         for x in (k, v, q, q_out):
-            if x is not None and (x.dtype != kv.dtype or x.shape[0] != batch.tokens or x.shape[2] != kv.cache.d):
+            if x is not None and (x.dtype != kv.dtype or len(x.shape) != 3 or (x.shape[0], x.shape[2]) != (batch.tokens, kv.cache.d)):
                 raise ValueError(f"paged_append: {x.shape} {x.dtype} for {batch.tokens} tokens of a {kv.dtype} cache")
         self.ctx.paged_append(kv.cache, batch, _heads(k), _heads(v), q=None if q is None else _heads(q),
                               q_out=None if q_out is None else _heads(q_out), rope=rope, stream=self.stream)
@@ -184,8 +195,12 @@ class Session:
     def paged_attention(self, kv: PagedKV, batch: runtime.PagedBatch, q: DeviceArray, o: DeviceArray, *,
                         scale: float | None = None) -> None:
         for x in (q, o):
-            if x.dtype != kv.dtype or x.shape[0] != batch.tokens or x.shape[2] != kv.cache.d:
+            if x.dtype != kv.dtype or len(x.shape) != 3 or (x.shape[0], x.shape[2]) != (batch.tokens, kv.cache.d):
                 raise ValueError(f"paged_attention: {x.shape} {x.dtype} for {batch.tokens} tokens of a {kv.dtype} cache")
+        # the kernels read the prefix's table up to its last token (a batch made by runtime.paged_batch says nothing of it)
+        pages = getattr(batch, "prefix_pages", None)
+        if pages is not None and batch.prefix_len > pages * kv.cache.page_size:
+            raise ValueError(f"paged_attention: a prefix of {batch.prefix_len} tokens in {pages} pages of {kv.cache.page_size}")
         nbytes = self.ctx.paged_attention_workspace(kv.cache, batch, q.shape[1])
         self.ctx.paged_attention(kv.cache, batch, _heads(q), _heads(o), kv.workspace(nbytes).ptr if nbytes else 0, nbytes,
                                  scale=scale, stream=self.stream)

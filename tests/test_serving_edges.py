@@ -134,3 +134,36 @@ def test_workspace_outlives_larger_calls():
     kv.free()
     assert not s.live
     kv.free()
+
+
+def session(fake):
+    api = importlib.import_module(f"{PKG}.api")
+    s = api.Session.__new__(api.Session)
+    s.ctx, s.stream, s._pinned = fake, 0, []
+    return s
+
+
+def test_session_checks_its_arrays():
+    import numpy as np
+    api = importlib.import_module(f"{PKG}.api")
+    fake = FakeSession()
+    s = session(fake)
+    kv = s.paged_kv(8, 16, 2, 32)
+    ints = lambda *shape: s.empty(shape, np.int32)  # noqa: E731
+    batch = s.paged_batch(ints(3), ints(2), ints(2, 4), 5, max_new=3, max_len=60, prefix_table=ints(2), prefix_len=33)
+    q, o, flat, k = s.empty((5, 4, 32)), s.empty((5, 4, 32)), s.empty((5, 32)), s.empty((5, 2, 32))
+    with pytest.raises(ValueError):
+        s.paged_attention(kv, batch, q, o)  # 33 tokens in two pages of 16: the third page would be read behind the table
+    batch.prefix_len = 32
+    s.paged_attention(kv, batch, q, o)
+    for call in (lambda: s.paged_attention(kv, batch, flat, o), lambda: s.paged_append(kv, batch, flat, k),
+                 lambda: s.paged_append(kv, batch, k, k, q=flat, q_out=q, rope=rt.rope_plan(32)),
+                 lambda: s.rotary(rt.rope_plan(32), [], s.empty((5,), np.int64)),
+                 lambda: s.rotary(rt.rope_plan(32), [(s.empty((5, 4, 32), np.float64),) * 2], s.empty((5,), np.int64)),
+                 lambda: s.rotary(rt.rope_plan(32), [(flat, flat)], s.empty((5,), np.int64)),
+                 lambda: s.paged_kv(8, 16, 2, 32, np.float64),
+                 lambda: s.paged_batch(ints(3), ints(2), ints(8), 5, max_new=3, max_len=60)):
+        with pytest.raises(ValueError):
+            call()
+    assert fake.calls.count("paged_attention") == 1 and "rotary" not in fake.calls and "paged_append" not in fake.calls
+    assert api.ELEMENTS[np.dtype(np.uint16)] == rt.BF16
