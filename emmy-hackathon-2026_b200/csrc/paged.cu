@@ -644,11 +644,13 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
       // The prefix part's blocks, one an SM, run beside the own part, which
       // needs the other SMs' loads more than it needs the prefix part done:
       // the fewest splits that do not make it the last to end, by what both
-      // take (a block 8 us and 2 us for each 128 keys; the own part the time of
-      // its bytes at 5.4 TB/s, for sequences that are 0.6 of the longest on
-      // average).  128 sequences of up to 1000 behind 8192 tokens, 32 units:
-      // 152 us with one split, 95 with two, 102 with three, 109 with four.
-      const double own_us = 0.6 * b.sequences * (double)b.max_len * c.heads * c.d * 4 / 5.4e6;
+      // take: a block 8 us and 2 us for each 128 keys; the own part the time of
+      // its bytes at 5.4 TB/s.  The host knows of the lengths only that none is
+      // above max_len: half of that stands for them, as for lengths spread evenly
+      // below it (a max_len far above the lengths in use makes the splits too few).
+      // 128 sequences of up to 1000 behind 8192 tokens, 32 units: 152 us with one
+      // split, 95 with two, 102 with three, 109 with four.
+      const double own_us = 0.5 * b.sequences * (double)b.max_len * c.heads * c.d * 4 / 5.4e6;
       for (int64_t s = 1; s * units < want; ++s) {
         const double block_us = 8.0 + 2.0 * ((b.prefix_len + s * 128 - 1) / (s * 128));
         if (block_us <= (units * s * block_us) / sms + own_us) want = s * units;

@@ -167,3 +167,14 @@ def test_session_checks_its_arrays():
             call()
     assert fake.calls.count("paged_attention") == 1 and "rotary" not in fake.calls and "paged_append" not in fake.calls
     assert api.ELEMENTS[np.dtype(np.uint16)] == rt.BF16
+
+
+def test_prefix_splits_by_lengths_spread_below_their_bound():
+    """128 sequences behind 8192 tokens: two splits while the own keys, half of the bound each, end before one would."""
+    def splits(max_len):
+        cache = rt.paged_cache(4096, 8192, rt.BF16, 10 ** 6, 16, 8, 128)
+        batch = rt.paged_batch(128, 128, 256, 256, 256, 10 ** 4, max_new=1, max_len=max_len, prefix_len=8192, prefix_table=256)
+        plan = rt.paged_attention_plan(148, cache, batch, rt.heads(2 ** 20, 64, 64 * 128, 128), rt.heads(2 ** 30, 64, 64 * 128, 128))
+        assert plan["own_kernel"] == 1 and plan["prefix_kernel"] == 2
+        return plan["prefix_splits"]
+    assert [splits(n) for n in (1000, 2000, 2500)] == [2, 2, 1]
