@@ -832,7 +832,8 @@ extern "C" int b2k_paged_attention_plan(int32_t sms, const b2k_paged_cache *cach
   if (status != B2K_OK) return status;
   auto shown = [](Path path) { return path == kF32 ? 0 : (int32_t)path; };
   *out = {shown(p.own_path), p.prefix_splits > 0 ? shown(p.prefix_path) : -1, p.own_splits, p.own_chunk,
-          p.prefix_splits, p.prefix_chunk, p.joined, 0,
+          p.prefix_splits, p.prefix_chunk, p.joined,
+          (p.own_path == kF32 ? 1 : 0) + (p.prefix_splits > 0 && p.prefix_path == kF32 ? 2 : 0),
           (int64_t)workspace_bytes_of(*cache, *batch, q->heads, sms)};
   return B2K_OK;
 }

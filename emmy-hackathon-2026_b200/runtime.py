@@ -135,7 +135,7 @@ class PagedAttentionPlan(C.Structure):
     """b2k_paged_attention_plan_info: what one b2k_paged_attention call launches."""
     _fields_ = [("own_kernel", C.c_int32), ("prefix_kernel", C.c_int32), ("own_splits", C.c_int32),
                 ("own_chunk", C.c_int32), ("prefix_splits", C.c_int32), ("prefix_chunk", C.c_int32),
-                ("joined", C.c_int32), ("reserved", C.c_int32), ("workspace_bytes", C.c_int64)]
+                ("joined", C.c_int32), ("streaming", C.c_int32), ("workspace_bytes", C.c_int64)]
 
 
 class Drafts(C.Structure):
@@ -338,7 +338,7 @@ def paged_attention_plan(sms: int, cache: PagedCache, batch: PagedBatch, q: Head
                                                 C.byref(out))
     if status != B2K_OK:
         raise B2KError(status, "arguments b2k_paged_attention refuses", "b2k_paged_attention_plan")
-    return {name: getattr(out, name) for name, _ in PagedAttentionPlan._fields_ if name != "reserved"}
+    return {name: getattr(out, name) for name, _ in PagedAttentionPlan._fields_}
 
 
 class BoundCall:

@@ -463,7 +463,7 @@ typedef struct b2k_paged_attention_plan_info {
   int32_t own_splits, own_chunk;     /* splits of the sequences' own keys, keys of each */
   int32_t prefix_splits, prefix_chunk;
   int32_t joined;                    /* 1: each sequence reads the prefix with its own keys */
-  int32_t reserved;
+  int32_t streaming;                 /* plain cores: 1 the own part, 2 the prefix by the kernel that streams f32 (3: both) */
   int64_t workspace_bytes;           /* as b2k_paged_attention_workspace says */
 } b2k_paged_attention_plan_info;
 int b2k_paged_attention_plan(int32_t sms, const b2k_paged_cache *cache, const b2k_paged_batch *batch, const b2k_heads *q,

@@ -11,6 +11,7 @@ from conftest import PKG
 
 torch = pytest.importorskip("torch")
 import serving_refs as refs  # noqa: E402
+from test_gpu_paged import CASES, call_parts, check  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 rt = importlib.import_module(f"{PKG}.runtime")
@@ -352,3 +353,52 @@ def test_elements_outside_pairs_keep_their_bits(ctx, torch_cuda, dtype, interlea
     assert torch.equal(x.view(bits)[:, :, rot:], y.view(bits)[:, :, rot:])
     want, tol = refs.rotary(x[..., :rot], pos, refs.frequencies(rot), interleaved)
     refs.close(y[..., :rot], want, tol, dt, "rotated part")
+
+
+# --- f32: the kernel that streams, and the blocks of 4, 8 and 32 rows ---------------------------------------
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_f32_blocks_of_rows(ctx, torch_cuda, case):
+    """The plain kernel where the rule takes the streaming one."""
+    new, lengths, prefix, page, hq, hkv, d, head_major = CASES[case]
+    bt = refs.batch(new, lengths, prefix=prefix, page=page, heads=hkv, d=d, dtype=torch.float32, head_major=head_major,
+                    seed=case, extra_rows=2)
+    q = 1.5 * torch.randn(bt.tokens, hq, d, device="cuda", generator=bt.generator)
+    ctx.set_paged_attention_kernel(1)
+    try:
+        check(ctx, bt, q)
+    finally:
+        ctx.set_paged_attention_kernel(0)
+
+
+@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("page", [1, 4, 16, 20, 128, 384])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (6, 2, 80), (12, 2, 128), (4, 4, 256)])
+def test_f32_page_sizes_and_groups(ctx, torch_cuda, kernel, page, hq, hkv, d):
+    """Pages that end in, at and behind a tile; one to eight rows of a decode, and many."""
+    for new, lengths in (([1, 1, 0, 2], [260, 129, 7, 2]), ([33, 1, 0, 150], [260, 129, 7, 150])):
+        bt = refs.batch(new, lengths, prefix=157, page=page, heads=hkv, d=d, dtype=torch.float32, seed=page + d,
+                        head_major=bool(page % 3), extra_rows=1)
+        q = torch.randn(bt.tokens, hq, d, device="cuda", generator=bt.generator)
+        ctx.set_paged_attention_kernel(kernel)
+        try:
+            check(ctx, bt, q)
+        finally:
+            ctx.set_paged_attention_kernel(0)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [4, 5, 8, 9, 32, 33, 63, 64, 65])
+def test_f32_rows_around_the_rules(ctx, torch_cuda, rows, d):
+    bt = refs.batch([rows, 1], [300, 77], prefix=50, heads=2, d=d, dtype=torch.float32, seed=rows)
+    q = torch.randn(bt.tokens, 2, d, device="cuda", generator=bt.generator)
+    cache, batch = call_parts(bt)
+    plan = rt.paged_attention_plan(torch.cuda.get_device_properties(0).multi_processor_count, cache, batch, heads(q), heads(torch.empty_like(q)))
+    assert plan["streaming"] & 1 == (rows <= 64)
+    for kernel in (0, 1):
+        ctx.set_paged_attention_kernel(kernel)
+        try:
+            check(ctx, bt, q)
+        finally:
+            ctx.set_paged_attention_kernel(0)

@@ -178,3 +178,20 @@ def test_prefix_splits_by_lengths_spread_below_their_bound():
         assert plan["own_kernel"] == 1 and plan["prefix_kernel"] == 2
         return plan["prefix_splits"]
     assert [splits(n) for n in (1000, 2000, 2500)] == [2, 2, 1]
+
+
+def test_plan_tells_the_f32_kernels_apart():
+    """Up to 64 rows a cache head in 16-byte pieces stream; more, odd head dims and bases off 16 bytes do not."""
+    def plan(new=1, prefix=0, sequences=2, d=64, at=4096, dtype=rt.F32, kernel=0):
+        cache = rt.paged_cache(at, at, dtype, 1000, 16, 2, d)
+        batch = rt.paged_batch(sequences, sequences * new, 256, 256, 256, 100, max_new=new, max_len=1000, prefix_len=prefix,
+                               prefix_table=256)
+        assert rt.library().b2k_paged_attention_set_kernel(kernel) == rt.B2K_OK
+        try:
+            return rt.paged_attention_plan(148, cache, batch, rt.heads(2 ** 20, 4, 4 * d, d), rt.heads(2 ** 30, 4, 4 * d, d))["streaming"]
+        finally:
+            rt.library().b2k_paged_attention_set_kernel(0)
+    assert [plan(new=n) for n in (1, 32, 33)] == [1, 1, 0]
+    assert plan(prefix=100) == 3 and plan(prefix=100, sequences=32) == 3 and plan(prefix=100, sequences=33) == 1
+    assert plan(new=32, prefix=100, sequences=1) == 3 and plan(new=33, prefix=100, sequences=1) == 0
+    assert plan(d=66) == 0 and plan(at=4100) == 0 and plan(kernel=1) == 0 and plan(dtype=rt.BF16, prefix=100) == 0
