@@ -440,9 +440,11 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
   __shared__ float sums[SHARED ? kWarps : 1][SHARED ? B2K_MAX_HEAD_DIM : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_heads = a.kv_heads * a.group;
-  grid_dependency_wait();
-  grid_dependents_launch();
+  const bool ready = paged::call_ready(a);
+  if (!ready) grid_dependency_wait();
   const paged::Sequence s = paged::sequence(a, blockIdx.x);
+  if (ready) grid_dependency_wait();
+  grid_dependents_launch();
   const int64_t stride = a.tokens * q_heads;
   const int64_t step = (int64_t)gridDim.y * (SHARED ? 1 : kWarps);
   for (int64_t row = (int64_t)blockIdx.y * (SHARED ? 1 : kWarps) + (SHARED ? 0 : warp); row < (int64_t)s.n * q_heads;
@@ -702,7 +704,7 @@ int rows_parts(b2k_ctx *ctx, const Args &a, bool with_prefix, bool with_own, int
 // depends on both.  Not active outside a capture.
 class CapturedBranches {
  public:
-  explicit CapturedBranches(cudaStream_t s) : s_(s) { active_ = dependencies(before_); }
+  CapturedBranches(cudaStream_t s, bool wanted) : s_(s) { active_ = wanted && dependencies(before_); }
   bool active() const { return active_; }
   cudaError_t second() { return dependencies(first_) ? set(before_, cudaStreamSetCaptureDependencies) : cudaErrorUnknown; }
   cudaError_t join() { return set(first_, cudaStreamAddCaptureDependencies); }
@@ -738,7 +740,12 @@ class CapturedBranches {
 template <typename T>
 int run(b2k_ctx *ctx, Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
   int launches = 1, status = B2K_OK;
-  const bool prefix = a.prefix_splits > 0;
+  const bool prefix = a.prefix_splits > 0, several = a.own_splits + a.prefix_splits > 1;
+  CapturedBranches branches(s, several);
+  if (several && !branches.active()) {
+    a.call = ++ctx->order_calls;
+    a.ready = ctx->order_words + a.call % b2k_ctx::kOrderWords;
+  }
   auto parts = [&](Path path, bool pre, bool own, int rows, bool beside) {
     return path == kPlain ? rows_parts<T>(ctx, a, pre, own, rows, beside, s)
            : path == kMma ? paged::mma_parts(ctx, a, dtype, pre, own, rows, beside, s)
@@ -749,7 +756,7 @@ int run(b2k_ctx *ctx, Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
     status = parts(p.own_path, false, true, p.own_rows, false);
   } else if (p.own_path == p.prefix_path && p.own_path != kUmma && p.own_rows == p.prefix_rows) {
     status = parts(p.own_path, true, true, p.own_rows, false);
-  } else if (CapturedBranches branches(s); p.own_path != kUmma && branches.active()) {
+  } else if (p.own_path != kUmma && branches.active()) {
     status = parts(p.prefix_path, true, false, p.prefix_rows, false);
     cudaError_t err = status == B2K_OK ? branches.second() : cudaSuccess;
     a.pdl = false;  // the own part's and the merge's dependences are whole
@@ -758,13 +765,9 @@ int run(b2k_ctx *ctx, Args &a, const Plan &p, int32_t dtype, cudaStream_t s) {
     if (err != cudaSuccess) status = b2k::cuda_fail(ctx, err, "paged_attention capture");
     ++launches;
   } else {
-    const bool beside = p.own_path != kUmma;  // (the tensor-memory kernel waits)
-    if (beside) {
-      a.call = ++ctx->order_calls;
-      a.ready = ctx->order_words + a.call % b2k_ctx::kOrderWords;
-    }
     status = parts(p.prefix_path, true, false, p.prefix_rows, false);
-    if (status == B2K_OK) status = parts(p.own_path, false, true, p.own_rows, beside);
+    // (the tensor-memory kernel waits)
+    if (status == B2K_OK) status = parts(p.own_path, false, true, p.own_rows, p.own_path != kUmma);
     ++launches;
   }
   if (status != B2K_OK) return status;

@@ -35,8 +35,8 @@ struct Args {
   int own_splits, own_chunk, prefix_splits, prefix_chunk;
   int joined;
   int joined_keys;   // where a joined part's own keys begin in its numbering: prefix_len, or that rounded up to whole tiles
-  unsigned *ready;   // prefix and own part in two kernels side by side: the word that orders them (part_begin),
-  unsigned call;     // and this call's value of it; ready is null otherwise
+  unsigned *ready;   // several kernels, not captured: the word that orders them (part_begin), and this
+  unsigned call;     // call's value of it; ready is null otherwise
   bool pdl;          // launched with programmatic dependence on the kernel before
   float *part_o;   // [own_splits + prefix_splits][tokens * q heads][d]
   float2 *part_ml; // [own_splits + prefix_splits][tokens * q heads]: m, l
@@ -123,6 +123,7 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
 // for that and then releases the call's number to a word of the context; a
 // thread of the own part that acquires this number is ordered behind that wait.
 // One that does not find it yet waits for the prefix part itself: nothing spins.
+// The merge reads the sequences' numbers ahead of its own wait in the same way.
 // (Blocks of the prefix part let the next kernel start only behind their wait, so
 // nearly all find it.)  No number is used twice: a captured call, whose number would
 // repeat at every replay, has the two parts as parallel branches of its graph
@@ -133,11 +134,15 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
 // part's end means the prefix part's too and the merge, which waits for the own
 // part, has both.  (The last block alone: waiting blocks hold their place on an SM, and
 // with all of them waiting the two parts all but took turns.)
+__device__ __forceinline__ bool call_ready(const Args &a) {
+  if (!a.ready) return false;
+  unsigned seen;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(a.ready) : "memory");
+  return seen == a.call;
+}
 __device__ __forceinline__ void part_begin(const Args &a, bool beside) {
   if (beside) {
-    unsigned seen;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(a.ready) : "memory");
-    if (seen != a.call) grid_dependency_wait();
+    if (!call_ready(a)) grid_dependency_wait();
   } else {
     grid_dependency_wait();
     if (a.ready && blockIdx.x == 0 && threadIdx.x == 0)
