@@ -6,9 +6,11 @@
 // holds f_i / 2 pi as a 64-bit fraction of a turn, so position * turn_i in
 // wrapping 64-bit integer arithmetic IS the angle modulo one turn; its top 32
 // bits, as a signed number, give the angle in half turns for sincospif.  The
-// angle's error is 2^-33 turns plus the rounding of that number to FP32 (at
-// most 2^-25 half turns), at any position: no table of cosines is read, kept
-// or outgrown, and no FP32 product position * f loses the far positions.
+// angle's error is what those bits leave out (below 2^-32 turns), the rounding
+// of that number to FP32 (at most 2^-25 half turns) and |position| times the
+// fraction's own error (b2k_rope_plan: below 2^-62 turns, 2^-22 of a turn at
+// position 2^40): no table of cosines is read, kept or outgrown, and no FP32
+// product position * f loses the far positions.
 //
 // Bound: HBM (each element read and written once).  A warp takes a token, or
 // some of its heads where tokens are few; nothing in a block waits for another
@@ -552,8 +554,10 @@ int b2k_rope_plan(const b2k_rope_params *p, b2k_rope *out) {
   if (ramp && (!(p->context > 0) || !isfinite(p->context) || !(p->low < p->high) || !isfinite(p->low) ||
                !isfinite(p->high) || (p->scaling == B2K_ROPE_LOG_RAMP && !(p->low > 0))))
     return B2K_EINVAL;
-  // long double: 64 significant bits on this platform, so a turn is good to
-  // about 2^-63 of itself
+  // long double: 64 significant bits on this platform.  A power f = theta^-e
+  // is off by f (|ln f| + 2) 2^-64 (its exponent's rounding, its own), the turn
+  // by another two roundings and the last one to 2^-64: below 2^-63 for f <= 1,
+  // and with the scalings' sums and quotients below 2^-62.
   const long double two_pi = 2.0L * acosl(-1.0L);
   const long double s = p->factor;
   long double theta = p->theta;

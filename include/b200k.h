@@ -319,10 +319,11 @@ int b2k_attention_set_fused(int mode);
  *                      held to [0, 1], t = context * f / 2 pi: the turns the
  *                      pair makes over the trained context
  *   B2K_ROPE_LOG_RAMP  the same with log t, log low and log high
- * and g = magnitude.  Angles are exact for every 64-bit position: the plan
- * holds f_i / 2 pi as a 64-bit binary fraction of a turn, so position * turn
- * modulo 2^64 is the angle, with an error of position * 2^-65 turns, and no
- * table bounds the positions.  No counterpart in the reference. */
+ * and g = magnitude.  No table bounds the positions: the plan holds f_i / 2 pi
+ * as a 64-bit binary fraction of a turn, and position * turn modulo 2^64 is the
+ * angle.  That is off by less than |position| * 2^-62 turns (the fraction's
+ * error, with theta >= 1, factor >= 1 and, for the ramps, high >= 2 low), plus
+ * 2^-32 turns and the rounding to FP32.  No counterpart in the reference. */
 #define B2K_F32 0 /* element types of the operators below */
 #define B2K_F16 1
 #define B2K_BF16 2

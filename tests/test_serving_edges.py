@@ -1,9 +1,10 @@
-"""Host side of the serving operators' edges: which operands meet (no GPU)."""
+"""Host side of the serving operators' edges: which operands meet, what a session keeps and checks, plans, turns (no GPU)."""
 from __future__ import annotations
 
 import ctypes as C
 import importlib
 import random
+from decimal import Decimal, localcontext
 
 import pytest
 
@@ -195,3 +196,38 @@ def test_plan_tells_the_f32_kernels_apart():
     assert plan(prefix=100) == 3 and plan(prefix=100, sequences=32) == 3 and plan(prefix=100, sequences=33) == 1
     assert plan(new=32, prefix=100, sequences=1) == 3 and plan(new=33, prefix=100, sequences=1) == 0
     assert plan(d=66) == 0 and plan(at=4100) == 0 and plan(kernel=1) == 0 and plan(dtype=rt.BF16, prefix=100) == 0
+
+
+PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+def exact_turns(rot, theta, scaling="none", factor=1.0, context=0.0, low=1.0, high=32.0):
+    """f_i / 2 pi with 60 digits."""
+    theta, s, out = Decimal(theta), Decimal(factor), []
+    if scaling == "base":
+        theta *= (s.ln() * rot / (rot - 2)).exp()
+    for i in range(rot // 2):
+        f = (theta.ln() * -2 * i / rot).exp()
+        if scaling == "linear":
+            f /= s
+        if scaling in ("ramp", "log_ramp"):
+            g = (lambda x: x.ln()) if scaling == "log_ramp" else (lambda x: x)
+            t, lo, hi = Decimal(context) * f / (2 * PI), Decimal(low), Decimal(high)
+            w = min(Decimal(1), max(Decimal(0), (g(t) - g(lo)) / (g(hi) - g(lo))))
+            f = f * w + f * (1 - w) / s
+        out.append(f / (2 * PI))
+    return out
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(scaling="linear", factor=4.0), dict(scaling="base", factor=8.0),
+                                dict(scaling="ramp", factor=8.0, context=8192.0, low=1.0, high=4.0),
+                                dict(scaling="log_ramp", factor=16.0, context=4096.0, low=1.0, high=32.0),
+                                dict(scaling="log_ramp", factor=2.5, context=131072.0, low=3.0, high=6.0)])
+@pytest.mark.parametrize("rot,theta", [(128, 10000.0), (64, 500000.0), (6, 10.0), (256, 1e6), (32, 1.0), (96, 1e7)])
+def test_turns_are_good_to_their_bound(kw, rot, theta):
+    """The plan's fractions of a turn against 60 digits: within 2^-62, as b2k_rope_plan's comment derives."""
+    with localcontext() as c:
+        c.prec = 60
+        for i, exact in enumerate(exact_turns(rot, theta, **kw)):
+            off = abs(Decimal(rt.rope_plan(rot, theta=theta, **kw).turn[i]) / 2 ** 64 - exact)
+            assert min(off, 1 - off) * 2 ** 62 < 1, (i, off * 2 ** 64)
