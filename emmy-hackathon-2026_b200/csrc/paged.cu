@@ -856,7 +856,10 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
                                    size_t workspace_bytes, void *stream) {
   B2K_CHECK_CTX(ctx);
   const char *what = "paged_attention";
-  if (!(scale_div > 0.0f) || !isfinite(scale_div)) return b2k::fail(ctx, B2K_EINVAL, "%s: scale %g", what, scale_div);
+  // (a subnormal scale's reciprocal is beyond FP32)
+  const float scale_log2 = (float)(1.4426950408889634074 / scale_div);
+  if (!(scale_div > 0.0f) || !isfinite(scale_div) || !isfinite(scale_log2))
+    return b2k::fail(ctx, B2K_EINVAL, "%s: scale %g", what, scale_div);
   Plan p;
   int status = check_operands(ctx, cache, batch, q, o, ctx->sm_count, p);
   if (status == B2K_OK) status = serve::check_apart(ctx, what, "o", *o, *q, false, batch->tokens, cache->d, cache->dtype);
@@ -899,7 +902,7 @@ extern "C" int b2k_paged_attention(b2k_ctx *ctx, const b2k_paged_cache *cache, c
   a.prefix_len = batch->prefix_len;
   a.max_new = batch->max_new;
   a.max_len = batch->max_len;
-  a.scale_log2 = (float)(1.4426950408889634074 / scale_div);
+  a.scale_log2 = scale_log2;
   a.err = ctx->error_flag;
   a.pdl = b2k::pdl_enabled();
   a.own_splits = p.own_splits;

@@ -441,7 +441,7 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
 /* Attention of the new tokens over the cache, with the prefix read once for
  * all sequences: new token j of sequence b sees the whole prefix and own
  * positions up to its own,
- *   o = sum_s softmax_s(q . k_s / scale_div) v_s.
+ *   o = sum_s softmax_s(q . k_s / scale_div) v_s,   0 < scale_div < inf, 1.45 / scale_div finite in FP32.
  * Query head h reads cache head h / (q heads / cache heads).  A row that sees
  * no key is zero.  FP32 softmax and sums; f16 and bf16 operands run on the
  * tensor cores, with the probabilities rounded to the operands' type.  Rows of a

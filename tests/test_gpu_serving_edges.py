@@ -402,3 +402,22 @@ def test_f32_rows_around_the_rules(ctx, torch_cuda, rows, d):
             check(ctx, bt, q)
         finally:
             ctx.set_paged_attention_kernel(0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_at_the_ends_of_the_scales(ctx, torch_cuda, dtype):
+    """A scale whose reciprocal FP32 does not hold is refused; the largest leaves the mean of the values."""
+    bt = refs.batch([1, 2], [30, 20], heads=1, d=64, dtype=refs.DTYPES[dtype])
+    q, (cache, batch) = torch.randn(3, 2, 64, device="cuda").to(bt.dtype), call_parts(bt)
+    o = torch.zeros_like(q)
+    ws = torch.empty(max(16, ctx.paged_attention_workspace(cache, batch, 2)), dtype=torch.uint8, device="cuda")
+    for scale in (1e-39, 4e-39, 1e-45):
+        with pytest.raises(rt.B2KError) as e:
+            ctx.paged_attention(cache, batch, heads(q), heads(o), ws.data_ptr(), ws.numel(), scale=scale)
+        assert e.value.status == rt.B2K_EINVAL
+    for kernel in (0, 1, 2, 3):
+        ctx.set_paged_attention_kernel(kernel)
+        try:
+            check(ctx, bt, q, scale=3e38)
+        finally:
+            ctx.set_paged_attention_kernel(0)
