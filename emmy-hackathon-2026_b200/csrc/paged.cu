@@ -532,6 +532,11 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
 template <typename T>
 cudaError_t merge(const Args &a, int sms, cudaStream_t s) {
   const int64_t rows = (int64_t)a.max_new * a.kv_heads * a.group;
+  // A block to a row where it has more parts than one warp's loads and the rows
+  // leave SMs idle: 32 / 8 heads of 128, one sequence of 50001 keys 38.0 us, 44.6 with a
+  // warp to a row, 4 of 8000 23.9 and 26.8, 8 of 4000 22.5 and 23.4; with four parts
+  // and fewer a block to a row costs 2 us (32 of 4000: 62.0 against 60.1), and with
+  // rows for all SMs neither is faster.
   const bool shared = a.own_splits + a.prefix_splits > 4 && rows * a.sequences < (int64_t)sms * 8;
   const int64_t blocks = shared ? rows : (rows + kWarps - 1) / kWarps;
   const dim3 grid(a.sequences, (unsigned)std::min<int64_t>(blocks, 65535));
@@ -560,6 +565,10 @@ size_t ml_bytes(size_t slots, int64_t tokens, int q_heads) {
   return (slots * (size_t)tokens * q_heads * sizeof(float2) + 15) / 16 * 16;
 }
 
+// The plain kernel's block, the fewest rows that hold them all: keys are read once,
+// and rows that are not there cost what others do (40 sequences of up to 1500 keys,
+// 8 cache heads of 100, bf16: 4 rows each 303 us in blocks of 4, 424 of 8, 530 of 32;
+// 8 rows each 424 in 8 and 525 in 32; 16 rows each 527 in 32 and 679 in two of 8).
 int plain_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 32; }
 
 // Whether the cache can be read in 16-byte pieces throughout, and of what.
@@ -586,7 +595,10 @@ bool rows_pieces(const b2k_heads &x) { return serve::vec_ok(x.data, x.stride_tok
 // f32: up to 64 rows in the kernel that streams, eight to a block (42 rows of a
 // prefix of 333: 15 us a call in it, 20 in the other), more in the one whose
 // blocks hold 32 (160 rows of 1000: 64 us against 72; prompts of 430: 161
-// against 353).
+// against 353).  Up to 4 rows in blocks of 4 (40 sequences of 4 rows over up to 1500
+// keys of 128: 81 us, 151 in blocks of 8).  Above, blocks of 8 read the keys half as
+// often as two of 4, but the second of those, launched beside the first, finds them
+// in L2: 8 rows each of the same 149 us in blocks of 8 against 105.
 int g_kernel = 0;  // b2k_paged_attention_set_kernel
 
 Path pick_path(Reach reach, const b2k_paged_cache &c, int64_t rows, int64_t keys, int64_t units, double repaid) {
@@ -617,11 +629,20 @@ Plan make_plan(const b2k_paged_cache &c, const b2k_paged_batch &b, int q_heads, 
   p.own_path = pick_path(reach, c, own, (int64_t)b.max_len + b.prefix_len, (int64_t)c.heads * b.sequences, 3e6);
   p.own_rows = block_rows(p.own_path, c.d, own);
   // Sequences whose own rows fill a block read the prefix with their own keys:
-  // stacking the rows of several sequences would save no reads of it.
+  // stacking the rows of several sequences would save no reads of it, and cost a
+  // part and its merge (32 / 8 heads of 128, own up to 600 behind 2000: 8 sequences of
+  // 64 tokens 49.5 us joined and 53.9 stacked, of 32, 128 rows, 39.4 and 41.2, of 16
+  // 37.0 and 34.9; 32 of 16 behind 4000 175 and 76).  Few sequences behind a long
+  // prefix lose by it, whose splits the own keys then bound: 4 of 32 behind 8000
+  // 50.7 and 43.6.
   p.joined = b.prefix_len > 0 && own >= 128;
   // blocks that the GPU holds at once, and keys that make a block worth its start
   // (a third decode block an SM has room, but its splits cost more than it
-  // brings: one sequence of 50001 keys 38 us with two, 41 with three)
+  // brings: one sequence of 50001 keys 38 us with two, 41 with three; plain blocks,
+  // heads of 100: one of 20000 keys 160 us with four, 196 with six or eight, 40 of up
+  // to 1500 365, 303, 312).  The shortest split, plain: 8 sequences of up to 700 31 us
+  // with 64 keys, 45 with 128; f32: 9 x 2 tokens of 700 and 333 12.7 with 64, 14.8
+  // with 128, 18.5 with 256, one of 8000 or 40 of 1500 the same with each.
   auto wave = [&](Path path) { return (int64_t)sms * (path == kPlain ? 6 : path == kUmma || (path == kMma && c.d > 128) ? 1 : 2); };
   auto least = [&](Path path) { return path == kPlain ? 64 : path == kUmma ? 128 : path == kF32 ? 128 : c.d <= 64 ? 512 : 256; };
   auto tile = [](Path path) { return path == kUmma ? 128 : 64; };  // keys of a block's step

@@ -88,10 +88,12 @@ __device__ __forceinline__ void copy16(void *dst, const void *src) {
 // Many tokens of 16-byte vectors: a lane's loads wait in shared memory, kSlots
 // steps of two vectors of all the token's segments at once, and cost no
 // registers: six blocks of four warps an SM have 190 KB on the way, where four
-// heads ahead in registers were 64 (16384 tokens x 40 heads of 128, bf16: 58 ->
-// 56 us; 6001 x 32 of 64, f32: 20.6 -> 19.1; prompts into a cache: 48 -> 45.6).
+// heads ahead in registers are 64.  Calls back to back, from registers and staged:
+// 16384 tokens x 40 heads of 128, bf16 57.5 and 55.9 us; 12 prompts into a cache,
+// interleaved f16 46.6 and 43.0; but the gradient of 6001 x 32 heads of 64,
+// interleaved f32, 18.0 and 19.0.
 // Small blocks, a token a warp, keep the last wave short: blocks of eight warps
-// 57.5 us, with two tokens a warp 60, with four 71.
+// 57.3, 44.5 and 19.5 us, the first with two tokens a warp 60, with four 71.
 constexpr int kSlots = 8, kStagedWarps = 4;
 template <typename T, int V, bool FLAT>
 constexpr bool kStaged = !FLAT && V * sizeof(T) == 16;
