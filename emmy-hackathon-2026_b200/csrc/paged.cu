@@ -20,6 +20,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <new>
 #include <vector>
 #include <type_traits>
 
@@ -745,9 +746,13 @@ class CapturedBranches {
       return false;
     }
     if (status != cudaStreamCaptureStatusActive) return false;
-    out.nodes.assign(nodes, nodes + n);
-    out.edges.assign(n, cudaGraphEdgeData{});
-    if (edges) out.edges.assign(edges, edges + n);
+    try {
+      out.nodes.assign(nodes, nodes + n);
+      out.edges.assign(n, cudaGraphEdgeData{});
+      if (edges) out.edges.assign(edges, edges + n);
+    } catch (const std::bad_alloc &) {
+      return false;
+    }
     return true;
   }
   cudaError_t set(Set &deps, unsigned flags) {
