@@ -656,6 +656,8 @@ int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *
   if (k->heads != cache->heads || v->heads != cache->heads)
     return b2k::fail(ctx, B2K_EINVAL, "%s: %d key and %d value heads for a cache of %d", what, k->heads, v->heads,
                      cache->heads);
+  if (rope && cache->k == cache->v)  // (read for both, by attention, they may be one)
+    return b2k::fail(ctx, B2K_EINVAL, "%s: rotated keys and values in one place", what);
   if (!q != !q_out || (q && !rope)) return b2k::fail(ctx, B2K_EINVAL, "%s: q needs q_out and a rope", what);
   RotaryArgs a = {};
   a.d = cache->d;

@@ -434,7 +434,8 @@ int64_t b2k_paged_slot(const int32_t *table_row, int32_t table_width, int64_t pa
  * the cache.  With a rope, keys are rotated on the way to position prefix_len
  * + own position, and, when q is not NULL, q [tokens][heads][d] is rotated
  * into q_out (which may be q) by the same launch.  Without one, k is copied
- * (q must be NULL).  No two new tokens may share a cache row. */
+ * (q must be NULL).  No two new tokens may share a cache row, nor keys and
+ * values an element. */
 int b2k_paged_append(b2k_ctx *ctx, const b2k_rope *rope, const b2k_paged_cache *cache, const b2k_paged_batch *batch,
                      const b2k_heads *k, const b2k_heads *v, const b2k_heads *q, const b2k_heads *q_out,
                      void *stream);

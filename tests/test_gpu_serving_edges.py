@@ -277,6 +277,9 @@ def test_outputs_that_meet_are_refused(ctx, torch_cuda):
     ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device="cuda")
     for o in (at(0), at(0, 1), at(1), at(n, st=d)):
         refused(ctx.paged_attention, cache, batch, at(0), o, ws.data_ptr(), nbytes)
+    cache.v = cache.k  # rotated keys and values in one place
+    refused(append, at(n, h))
+    cache.v = bt.v.data_ptr()
     ctx.sync()
     assert torch.equal(buf, keep)
     # side by side in one buffer
@@ -421,3 +424,52 @@ def test_attention_at_the_ends_of_the_scales(ctx, torch_cuda, dtype):
             check(ctx, bt, q, scale=3e38)
         finally:
             ctx.set_paged_attention_kernel(0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shift", [0, 1, 4])
+@pytest.mark.parametrize("new", [[1, 1, 3], [700, 900, 800]])
+def test_append_into_a_shared_buffer(ctx, torch_cuda, dtype, shift, new):
+    """Keys and values side by side in one buffer, queries rotated in place in a fused projection; shift moves every base
+    off its 16 bytes."""
+    dt, d, h, page = refs.DTYPES[dtype], 64, 2, 16
+    bt = refs.batch(new, [n + 5 for n in new], prefix=40, page=page, heads=h, d=d, dtype=dt, extra_rows=1, poison=False)
+    both = torch.full((bt.pages * page * h * 3 * d + 8,), 7.0, device="cuda", dtype=dt)
+    view = both[shift:shift + bt.pages * page * h * 3 * d].view(bt.pages, page, h, 3, d)
+    strides = (page * h * 3 * d, h * 3 * d, 3 * d)
+    cache = rt.paged_cache(view.data_ptr(), view[:, :, :, 2].data_ptr(), CODES[dt], bt.pages, page, h, d, k_strides=strides,
+                           v_strides=strides)
+    fused = torch.randn(bt.tokens * 9 * d + 8, device="cuda").to(dt)[shift:shift + bt.tokens * 9 * d].view(bt.tokens, 9, d)
+    was = fused.clone()
+    ctx.paged_append(cache, call_parts(bt)[1], heads(fused[:, 5:7]), heads(fused[:, 7:]), q=heads(fused[:, 1:5]),
+                     q_out=heads(fused[:, 1:5]), rope=rt.rope_plan(d))
+    ctx.sync()
+    freqs, first = refs.frequencies(d), 0
+    expect = torch.full_like(view, 7.0)
+    for b, n in enumerate(new):
+        pos = 40 + torch.arange(5, n + 5, device="cuda")
+        for x, got in ((was[first:first + n, 1:5], fused[first:first + n, 1:5]),
+                       (was[first:first + n, 5:7], refs.read_rows(bt, view[:, :, :, 0], b, n + 5)[5:])):
+            want, tol = refs.rotary(x, pos, freqs, False)
+            refs.close(got, want, tol, dt, f"sequence {b}")
+        pages, rows = refs.places(bt, b, n + 5)
+        expect[pages[5:], rows[5:], :, 0] = view[pages[5:], rows[5:], :, 0]
+        expect[pages[5:], rows[5:], :, 2] = was[first:first + n, 7:]
+        first += n
+    assert torch.equal(view, expect) and (both[:shift] == 7.0).all()
+    fused[:first, 1:5] = was[:first, 1:5]
+    assert torch.equal(fused, was)
+
+
+@pytest.mark.parametrize("dtype,prefix,kernels", TWO_KERNELS)
+def test_steps_without_programmatic_launch(ctx, torch_cuda, dtype, prefix, kernels):
+    s = Steps(ctx, dtype, prefix, steps=4)
+    s.run(s.calls)
+    want = s.state()
+    ctx.lib.b2k_set_pdl(0)
+    try:
+        s.rewind()
+        s.run(s.calls)
+        assert all(torch.equal(a, b) for a, b in zip(want, s.state()))
+    finally:
+        ctx.lib.b2k_set_pdl(1)
