@@ -9,9 +9,9 @@
 // RW rows (query heads of one cache head, tokens side by side) and streams 32
 // keys at a time through shared memory as FP32.  Scores: each warp its own RW
 // rows, lane = key, or with 32 rows lane = two rows by four keys and two dims an
-// instruction (prompts of 430 over 1430 keys, 12 / 4 heads, f32: 228 -> 211 us at
-// 64 dims, 728 -> 519 at 256; FMA pipe and shared memory both near half there,
-// with 8 to 12 warps an SM).  The next tile is on its way meanwhile (asynchronous
+// instruction (prompts of 430 over 1430 keys, 12 / 4 heads, f32: 222 -> 214 us at
+// 64 dims, 355 -> 357 at 128, 822 -> 795 at 256; FMA pipe and shared memory both
+// near half there, with 4 to 12 warps an SM).  The next tile is on its way meanwhile (asynchronous
 // copies where the cache is f32 in 16-byte pieces).  P V: lane = four
 // dims, the probabilities read back four keys at a time as one broadcast
 // (shuffled one by one they took two thirds of the kernel's instructions).  In a

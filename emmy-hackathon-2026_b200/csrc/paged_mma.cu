@@ -9,7 +9,7 @@
 // until the end), two or three blocks an SM: about 96 KB on the way at any
 // time, where the copy bandwidth times the latency of HBM is about 45 KB an SM.
 // The third block is worth its tighter registers (33 sequences of 20 rows of
-// 64: 30 us with two, 25 with three).  The products are 16 x 8 x 16 warp MMAs with the probabilities
+// 64: 30 us with two, 24 with three).  The products are 16 x 8 x 16 warp MMAs with the probabilities
 // taken from the score registers as they lie; rows that are not there cost
 // nothing that the loads would not hide, so the 16-row tile is not split
 // further.  The tensor-memory instructions need 64 rows and more to one tile:
@@ -33,8 +33,8 @@ constexpr int kWarps = 4;
 constexpr int kTile = 16;  // keys of a warp's step
 
 // Tiles a warp has in its ring.  Two at head dim 128 with 16 rows leave room for
-// a third block on an SM (one sequence of 50001 keys: 42 us with three tiles
-// and two blocks, 40 with two and three).
+// a third block on an SM (128 sequences of up to 2000 keys behind 8192: 138 us, 143
+// with two blocks of two or of three tiles; one sequence of 50001: 37.8, 37.2, 39.5).
 template <int DP, int MT>
 constexpr int stages() { return DP == 64 ? 4 : DP == 128 && MT == 1 ? 2 : 3; }
 template <int DP>

@@ -284,9 +284,9 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   b2k::PhaseTimer timer(ctx, B2K_PHASE_VERIFY, s);
   const VerifyArgs a{*d, accepted, tokens};
   // A few sequences leave an SM to each CTA, which wants many loads in flight for
-  // a long row (131071: 7.2 us with 512 threads, 8.2 with 256) and fewer warps to
-  // wait for for a short one (32000: 5.7 and 5.4); a batch wants all its CTAs
-  // resident at once (64 sequences of 131071: 24 us with 512, 17 with 256).
+  // a long row (131071: 7.0 us with 512 threads, 7.9 with 256) and fewer warps to
+  // wait for for a short one (32000: 5.5 and 5.1); a batch wants all its CTAs
+  // resident at once (64 sequences of 131071: 25 us with 512, 17.6 with 256).
   const bool few = d->batch * kCluster <= ctx->sm_count && d->vocab > 65536;
   cudaError_t err = b2k::launch_kernel(b2k::pdl_enabled(), few ? verify_kernel<512> : verify_kernel<256>,
                                        dim3((unsigned)(d->batch * kCluster)), dim3(few ? 512 : 256), 0, s, a);

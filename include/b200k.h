@@ -421,7 +421,8 @@ typedef struct b2k_paged_batch {
   const int32_t *lengths;      /* [sequences] */
   const int32_t *table;        /* [sequences][table_width] */
   int64_t table_stride;        /* >= table_width */
-  int32_t max_new, max_len;    /* upper bounds of the new tokens and of lengths[b]; sizes of the launches */
+  int32_t max_new, max_len;    /* upper bounds of the new tokens and of lengths[b]; sizes of the launches.
+                                  Attention splits the keys by max_len: fastest near the longest length */
   int32_t prefix_len;
   const int32_t *prefix_table; /* [ceil(prefix_len / page_size)] */
 } b2k_paged_batch;
