@@ -30,9 +30,9 @@ struct b2k_ctx {
   bool fixed_scratch = false;
   // Device-side error word written by kernels whose bounded waits expire.
   unsigned int *error_flag = nullptr;
-  // Words by which a kernel tells the next one in its stream that what precedes
-  // both is complete (paged.cuh), one for each of the latest calls that have two
-  // such kernels, and the number of those calls.
+  // Words by which a kernel tells the next ones of its call that what precedes the
+  // call is complete (paged.cuh), one for each of the latest calls of several
+  // kernels, and the number of those calls.
   static constexpr uint32_t kOrderWords = 64;
   unsigned int *order_words = nullptr;
   uint32_t order_calls = 0;

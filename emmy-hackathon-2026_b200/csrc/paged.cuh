@@ -125,11 +125,12 @@ __device__ __forceinline__ int64_t key_page(const Args &a, bool prefix, int b, i
 // One that does not find it yet waits for the prefix part itself: nothing spins.
 // The merge reads the sequences' numbers ahead of its own wait in the same way.
 // (Blocks of the prefix part let the next kernel start only behind their wait, so
-// nearly all find it.)  No number is used twice: a captured call, whose number would
-// repeat at every replay, has the two parts as parallel branches of its graph
-// instead (paged.cu).  (128 single tokens behind 8192 shared ones: 102 us a call in
-// a stream, 92 in a graph; with no ordering of the own part's reads 102 and 90,
-// with the parts one after the other 142.)
+// nearly all find it.)  A number comes again after 2^32 calls, which have written
+// its word 2^26 times by then.  A captured call, whose number would come again at
+// every replay, has the two parts as parallel branches of its graph instead
+// (paged.cu).  128 single tokens behind 8192 shared ones: 102 us a call in a
+// stream, 92 in a graph; with no ordering of the own part's reads 102 and 90, with
+// the parts one after the other 142.
 // The own part's last block waits for the prefix part at its end, so that the own
 // part's end means the prefix part's too and the merge, which waits for the own
 // part, has both.  (The last block alone: waiting blocks hold their place on an SM, and

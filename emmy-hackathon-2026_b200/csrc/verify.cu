@@ -275,7 +275,7 @@ extern "C" int b2k_verify_drafts(b2k_ctx *ctx, const b2k_drafts *d, int32_t *acc
   for (int i = 0; i < 2; ++i)
     for (const auto &x : arrays) {
       const auto &out = arrays[i];
-      if (&x == &out || !x.p) continue;
+      if (&x == &out || !x.p || x.n == 0.0) continue;
       const double apart = (double)(reinterpret_cast<uintptr_t>(x.p) / 4) - (double)(reinterpret_cast<uintptr_t>(out.p) / 4);
       if (apart < out.n && -apart < x.n)
         return b2k::fail(ctx, B2K_EINVAL, "verify_drafts: %s overlaps another array", i ? "tokens" : "accepted");

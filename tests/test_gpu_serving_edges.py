@@ -330,7 +330,8 @@ def test_verification_refuses_outputs_in_other_arrays(ctx, torch_cuda):
     ctx.sync()
     assert not ints.any()
     for kw in (dict(), dict(tokens=i(9), accepted=i(60)), dict(tokens=i(19)), dict(accepted=i(9)), dict(accepted=i(13)), dict(accepted=i(41)),
-               dict(accepted=f(144)), dict(tokens=f(81))):
+               dict(accepted=f(144)), dict(tokens=f(81)),
+               dict(drafts=0, drafted=i(33), u_accept=i(33), draft=i(33), accepted=i(60))):  # arrays of no elements
         ctx.verify_drafts(**{**good, **kw})
     ctx.sync()
 
